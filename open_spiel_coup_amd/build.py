@@ -72,6 +72,12 @@ ARCH = os.environ.get("COUP_OFFLOAD_ARCH", "gfx950")
 # are 0.7-1% faster without it (profiles/r03/codegen/).
 NO_SLP = "-fno-slp-vectorize"
 
+# No packed 32-bit float instructions either (none is
+# made today: the kernels' assembly is the same with and without): some
+# of their forms have given wrong results on this hardware now and then.
+# hipcc's host pass warns that it does not know the feature.
+NO_PACKED_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+
 # Optimisation level per source.  -O2 measured 1% faster than -O3 for the
 # 6-player step (33.7-34.0 against 33.9-34.5 us) but 6% slower for its
 # trajectory kernel (26.3-26.5 against 24.7-24.9 us per step) and 0.5-1 us
@@ -94,7 +100,7 @@ HOST_OBJ = os.path.join(OBJ_DIR, "coup_host.o")
 def command(resource_usage=False, out=OUT, defines=()):
     """Measurement builds: one hipcc command over the HIP sources and the
     host object (build it first with host_command(HOST_OBJ))."""
-    cmd = [HIPCC, f"--offload-arch={ARCH}", "-O3", NO_SLP, "-std=c++17", "-fPIC", "-shared",
+    cmd = [HIPCC, f"--offload-arch={ARCH}", "-O3", NO_SLP, *NO_PACKED_F32, "-std=c++17", "-fPIC", "-shared",
            "-Wall", "-I", os.path.join(ROOT, "include"), "-o", out] + [f"-D{d}" for d in defines] + SOURCES + [HOST_OBJ]
     if resource_usage:
         cmd.insert(1, "-Rpass-analysis=kernel-resource-usage")
@@ -121,7 +127,7 @@ INFO_REPRO_OUT = os.path.join(ROOT, "build", "info_prefix_repro")
 def info_repro_command():
     """The uint2-prefix reproducer of round 4's k_info_sweep sighting
     (tests/test_gpu_codegen_hazard.py), with the product's device flags."""
-    return [HIPCC, f"--offload-arch={ARCH}", "-O3", NO_SLP, "-std=c++17", "-I", os.path.join(ROOT, "include"),
+    return [HIPCC, f"--offload-arch={ARCH}", "-O3", NO_SLP, *NO_PACKED_F32, "-std=c++17", "-I", os.path.join(ROOT, "include"),
             "-I", CSRC, INFO_REPRO_SRC, "-o", INFO_REPRO_OUT]
 
 
@@ -140,7 +146,7 @@ def repro_command():
     # COUP_RULES_V1: the branch-form decision transition, the form the inlined
     # k_slot miscompiles (the effect form, default since round 2, happens to
     # compile correctly inline: DESIGN.md section 12)
-    return [HIPCC, f"--offload-arch={ARCH}", "-O3", NO_SLP, "-std=c++17", "-DCOUP_RULES_V1", "-I", os.path.join(ROOT, "include"),
+    return [HIPCC, f"--offload-arch={ARCH}", "-O3", NO_SLP, *NO_PACKED_F32, "-std=c++17", "-DCOUP_RULES_V1", "-I", os.path.join(ROOT, "include"),
             "-I", CSRC, REPRO_SRC, os.path.join(CSRC, "coup_nplayer.hip"), "-o", REPRO_OUT]
 
 
@@ -183,7 +189,7 @@ def build(force=False, verbose=False, repro=False, variants=True):
         for src in SOURCES:
             obj = os.path.join(odir, os.path.basename(src) + ".o")
             objs.append(obj)
-            cmd = [HIPCC, f"--offload-arch={ARCH}", OPT[os.path.basename(src)], NO_SLP, "-std=c++17", "-fPIC", "-Wall", "-I",
+            cmd = [HIPCC, f"--offload-arch={ARCH}", OPT[os.path.basename(src)], NO_SLP, *NO_PACKED_F32, "-std=c++17", "-fPIC", "-Wall", "-I",
                    os.path.join(ROOT, "include"), "-c", src, "-o", obj] + [f"-D{d}" for d in defines]
             if verbose:
                 cmd.insert(1, "-Rpass-analysis=kernel-resource-usage")
@@ -231,7 +237,7 @@ def main():
         for src in SOURCES:
             obj = os.path.join(odir, os.path.basename(src) + ".o")
             objs.append(obj)
-            jobs.append([HIPCC, f"--offload-arch={ARCH}", OPT[os.path.basename(src)], NO_SLP, "-std=c++17", "-fPIC",
+            jobs.append([HIPCC, f"--offload-arch={ARCH}", OPT[os.path.basename(src)], NO_SLP, *NO_PACKED_F32, "-std=c++17", "-fPIC",
                          "-Wall", "-I", os.path.join(ROOT, "include"), "-c", src, "-o", obj] +
                         [f"-D{d}" for d in a.define])
         _run_all(jobs, a.verbose)
