@@ -28,7 +28,7 @@
 extern "C" {
 #endif
 
-#define COUP_ABI_VERSION 14
+#define COUP_ABI_VERSION 15
 
 #define COUP_NUM_PLAYERS 2          /* coup.h:42 */
 #define COUP_MAX_PLAYERS 6          /* N-player extension */
@@ -415,6 +415,139 @@ int coup_import_history(coup_env* env, const uint8_t* src);
 /* Number of lanes that rejected an action since the last call (resets the
  * counter).  Synchronises the env's stream. */
 int coup_error_count(coup_env* env, int64_t* out);
+
+/* --- learner-side operators --------------------------------------------- */
+
+/* What a learner computes between two trajectories, on the layouts
+ * coup_step / coup_step_trajectory write: actions drawn from a network's
+ * logits under the legal-action word (for coup_step's `actions`), advantages
+ * over [T][B] windows in which the players take turns, the clipped policy
+ * loss and the paired log-ratio preference loss with their gradients.  They
+ * take no env: every pointer is device memory of the current HIP device, the
+ * work is enqueued on `hip_stream` (NULL = default) and nothing is allocated
+ * or synchronised, so every call may be captured into a HIP graph.  The
+ * workspaces are the caller's, of at least the size the _workspace functions
+ * return, 8-byte aligned, not shared by calls (or graphs) that may run at the
+ * same time.  Results do not depend on the order blocks run in.
+ *
+ * A row is one decision: num_actions (1..31) logits, a legal-action word as
+ * coup_step writes it, an action.  A row counts where its action is legal:
+ * 0 <= action < num_actions, bit `action` of the word set, bit 31
+ * (COUP_MASK_CHANCE_FLAG) clear.  Rows that do not count -- lanes that were
+ * reset or skipped (action -1), finished games, chance nodes -- give zeros,
+ * whatever their other inputs hold (NaN included); so do logits of actions
+ * outside the word.  A NaN or +inf logit of a legal action, or -inf at every
+ * one, makes its row's results NaN.
+ *
+ * Logits may be float, half or bfloat16; all arithmetic is in 32 bits or
+ * more, a gradient is rounded once, to the logits' type. */
+#define COUP_MAX_POLICY_ACTIONS 31
+#define COUP_DTYPE_F32 0
+#define COUP_DTYPE_F16 1
+#define COUP_DTYPE_BF16 2
+
+typedef struct {
+  const void* logits;         /* [rows][num_actions], rows logits_stride elements apart */
+  int64_t logits_stride;      /* >= num_actions */
+  const void* ref_logits;     /* the reference policy's, same type; NULL: none */
+  int64_t ref_stride;
+  const int8_t* actions;      /* [rows] */
+  const uint32_t* legal_mask; /* [rows] */
+  int64_t rows;
+  int32_t num_actions;
+  int32_t dtype;              /* COUP_DTYPE_* of logits, ref_logits and the gradient */
+} coup_decisions;
+
+/* Draw one action per row from softmax(logits) over the legal actions (d's
+ * actions and ref_logits are not read): the first legal action, in ascending
+ * order, whose running probability exceeds uniform[i] in [0, 1) (compared in
+ * 64 bits where 32 could turn it).  actions [rows] int8: -1 where no action is
+ * legal or the row's results are NaN; log_probs [rows] (may be NULL) its log
+ * probability, 0 where no action is legal.  The softmax policy beside
+ * coup_step's uniform one (random_agent.py:29-42). */
+int coup_sample_actions(const coup_decisions* d, const float* uniform, int8_t* actions, float* log_probs,
+                        void* hip_stream);
+
+/* Generalised advantages and value targets of a [T][B] window of a game in
+ * which the players take turns.  A decision is a step of type MID or LAST
+ * whose acting player is one of the num_players (2..6); values [T][B] holds
+ * the acting player's value of the state it acted in.  Each player's
+ * decisions form one chain: from one to its next, the player's rewards in
+ * between (the acting step's included) and the next one's value discounted by
+ * gamma, advantages decayed by gamma * lam.  A chain ends with a LAST step, a
+ * FIRST step cuts off what follows it; past the window a player's next value
+ * is bootstrap [B][num_players] (NULL: 0).  adv and target ([T][B], target =
+ * adv + value) are 0 at steps that are no decision; their value is not read.
+ * players [T][B] is the player BEFORE the step (the cur_player output of the
+ * step before). */
+typedef struct {
+  const int8_t* rewards;    /* [T][B][num_players] */
+  const uint8_t* step_type; /* [T][B] */
+  const int8_t* players;    /* [T][B] */
+  const void* values;       /* [T][B] */
+  const void* bootstrap;    /* [B][num_players], values' type, or NULL */
+  int64_t steps;
+  int64_t lanes;
+  int32_t num_players;
+  int32_t dtype;            /* COUP_DTYPE_* of values and bootstrap */
+} coup_window;
+int coup_advantages(const coup_window* w, double gamma, double lam, float* adv, float* target, void* hip_stream);
+
+/* The clipped policy loss with a KL term, averaged over the decisions that
+ * count (and have active[i] != 0, if given):
+ *   -min(rho adv, clip(rho, 1 - clip_low, 1 + clip_high) adv)
+ *     + kl_coef KL(pi || pi_ref) - entropy_coef H(pi),
+ * rho = exp(log pi(action) - old_log_probs); KL and H over the legal actions
+ * (KL is 0 without ref_logits).  A ratio exactly on a border is not clipped. */
+typedef struct {
+  const float* old_log_probs; /* [rows] */
+  const float* advantages;    /* [rows] */
+  const uint8_t* active;      /* [rows] or NULL */
+  double clip_low, clip_high; /* 0 <= clip_low <= 1, 0 <= clip_high */
+  double kl_coef, entropy_coef;
+} coup_policy_terms;
+typedef struct {
+  float* loss;      /* [1]; 0 where nothing counts */
+  float* stats;     /* [4] means over the decisions: clipped surrogate, KL, entropy, share clipped; or NULL */
+  int64_t* count;   /* [1] decisions that count, or NULL */
+  float* log_probs; /* [rows] log pi(action), 0 where the row does not count; or NULL */
+  void* grad;       /* [rows][num_actions] of the logits, d loss / d logits; or NULL */
+} coup_policy_outputs;
+size_t coup_policy_workspace(int64_t rows);
+int coup_policy_loss(const coup_decisions* d, const coup_policy_terms* terms, const coup_policy_outputs* out,
+                     void* workspace, size_t workspace_bytes, void* hip_stream);
+
+/* The paired log-ratio loss of preferred against rejected sequences of
+ * decisions: sequence s is rows [offsets[s], offsets[s + 1]), pair i prefers
+ * sequence 2 i to 2 i + 1 (e.g. a game's winner's decisions to its loser's).
+ * A sequence's reward is beta times the sum over its decisions of
+ * log pi(action) - log pi_ref(action) (without ref_logits the second is 0);
+ * with x the difference of a pair's rewards the loss is the mean over pairs
+ * of -(1 - label_smoothing) log sigmoid(x) - label_smoothing log sigmoid(-x).
+ * offsets: 2 * pairs + 1 of int32 or int64 (offset_bytes 4 or 8), ascending,
+ * 0..rows; rows outside every sequence get zero gradients.  Offsets that do
+ * not ascend make the loss NaN; none makes the call read outside the rows. */
+typedef struct {
+  const void* offsets;
+  int32_t offset_bytes;
+  int64_t pairs;
+  double beta;
+  double label_smoothing; /* 0..0.5 */
+} coup_preference_terms;
+typedef struct {
+  float* loss;    /* [1]; 0 for no pairs */
+  float* rewards; /* [2 * pairs] or NULL */
+  void* grad;     /* [rows][num_actions] of the logits, or NULL */
+} coup_preference_outputs;
+size_t coup_preference_workspace(int64_t rows, int64_t pairs);
+int coup_preference_loss(const coup_decisions* d, const coup_preference_terms* terms,
+                         const coup_preference_outputs* out, void* workspace, size_t workspace_bytes,
+                         void* hip_stream);
+
+/* grad[0..n) *= *scale (device float): the chain rule's last factor for a
+ * gradient the calls above wrote.  Returns without touching grad where *scale
+ * is 1. */
+int coup_scale_grad(void* grad, int dtype, int64_t n, const float* scale, void* hip_stream);
 
 /* --- measurement ------------------------------------------------------- */
 

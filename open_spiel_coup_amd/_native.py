@@ -11,7 +11,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 # COUP_LIB_PATH: load another build of the same library (A/B timing of two
 # builds, tools/ab_builds.sh); there is still no fallback
 LIB_PATH = os.environ.get("COUP_LIB_PATH") or os.path.join(HERE, "libcoup_mi355x.so")
-ABI_VERSION = 14
+ABI_VERSION = 15
 FLAG_AUTO_RESET, FLAG_HISTORY, FLAG_GENERIC, FLAG_UNCHECKED = 1, 2, 4, 8
 MAX_PLAYERS = 6
 HISTORY_BYTES = 96
@@ -34,6 +34,8 @@ SYMBOLS = (
     "coup_host_state_init", "coup_host_state_apply", "coup_host_state_tensors", "coup_host_state_string",
     "coup_host_state_step",
     "coup_write_lane",
+    "coup_sample_actions", "coup_advantages", "coup_policy_workspace", "coup_policy_loss",
+    "coup_preference_workspace", "coup_preference_loss", "coup_scale_grad",
 )
 
 # coup_slot_op flags and result layout (coup_slot_result, 128 bytes)
@@ -68,6 +70,49 @@ class SlotReq(ctypes.Structure):
     """coup_slot_req (24 bytes)."""
     _fields_ = [("lane", ctypes.c_int64), ("src_lane", ctypes.c_int64), ("action", ctypes.c_int32),
                 ("flags", ctypes.c_int32)]
+
+
+# learner-side operators
+MAX_POLICY_ACTIONS = 31
+DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
+
+
+class Decisions(ctypes.Structure):
+    """coup_decisions."""
+    _fields_ = [("logits", ctypes.c_void_p), ("logits_stride", ctypes.c_int64), ("ref_logits", ctypes.c_void_p),
+                ("ref_stride", ctypes.c_int64), ("actions", ctypes.c_void_p), ("legal_mask", ctypes.c_void_p),
+                ("rows", ctypes.c_int64), ("num_actions", ctypes.c_int32), ("dtype", ctypes.c_int32)]
+
+
+class Window(ctypes.Structure):
+    """coup_window."""
+    _fields_ = [("rewards", ctypes.c_void_p), ("step_type", ctypes.c_void_p), ("players", ctypes.c_void_p),
+                ("values", ctypes.c_void_p), ("bootstrap", ctypes.c_void_p), ("steps", ctypes.c_int64),
+                ("lanes", ctypes.c_int64), ("num_players", ctypes.c_int32), ("dtype", ctypes.c_int32)]
+
+
+class PolicyTerms(ctypes.Structure):
+    """coup_policy_terms."""
+    _fields_ = [("old_log_probs", ctypes.c_void_p), ("advantages", ctypes.c_void_p), ("active", ctypes.c_void_p),
+                ("clip_low", ctypes.c_double), ("clip_high", ctypes.c_double), ("kl_coef", ctypes.c_double),
+                ("entropy_coef", ctypes.c_double)]
+
+
+class PolicyOutputs(ctypes.Structure):
+    """coup_policy_outputs."""
+    _fields_ = [("loss", ctypes.c_void_p), ("stats", ctypes.c_void_p), ("count", ctypes.c_void_p),
+                ("log_probs", ctypes.c_void_p), ("grad", ctypes.c_void_p)]
+
+
+class PreferenceTerms(ctypes.Structure):
+    """coup_preference_terms."""
+    _fields_ = [("offsets", ctypes.c_void_p), ("offset_bytes", ctypes.c_int32), ("pairs", ctypes.c_int64),
+                ("beta", ctypes.c_double), ("label_smoothing", ctypes.c_double)]
+
+
+class PreferenceOutputs(ctypes.Structure):
+    """coup_preference_outputs."""
+    _fields_ = [("loss", ctypes.c_void_p), ("rewards", ctypes.c_void_p), ("grad", ctypes.c_void_p)]
 
 
 class CoupError(RuntimeError):
@@ -132,6 +177,15 @@ def load():
         "coup_host_state_string": ([ctypes.c_char_p, i32, i32, vp, i64], i64),
         "coup_host_state_step": ([ctypes.c_char_p, i32, i32, ctypes.c_uint64, ctypes.c_uint32, vp], i32),
         "coup_write_lane": ([vp, i64, ctypes.c_char_p], i32),
+        "coup_sample_actions": ([ctypes.POINTER(Decisions), vp, vp, vp, vp], i32),
+        "coup_advantages": ([ctypes.POINTER(Window), ctypes.c_double, ctypes.c_double, vp, vp, vp], i32),
+        "coup_policy_workspace": ([i64], ctypes.c_size_t),
+        "coup_policy_loss": ([ctypes.POINTER(Decisions), ctypes.POINTER(PolicyTerms), ctypes.POINTER(PolicyOutputs), vp,
+                              ctypes.c_size_t, vp], i32),
+        "coup_preference_workspace": ([i64, i64], ctypes.c_size_t),
+        "coup_preference_loss": ([ctypes.POINTER(Decisions), ctypes.POINTER(PreferenceTerms),
+                                  ctypes.POINTER(PreferenceOutputs), vp, ctypes.c_size_t, vp], i32),
+        "coup_scale_grad": ([vp, i32, i64, vp, vp], i32),
     }
     for name, (args, res) in sig.items():
         fn = getattr(L, name)

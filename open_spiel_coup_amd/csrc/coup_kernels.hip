@@ -10,6 +10,7 @@
 
 #include <algorithm>
 #include <chrono>
+#include <cmath>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -39,6 +40,7 @@ __device__ unsigned long long g_traj_phases[7];  // coup_traj_phases.h
 #include "coup_launch_log.h"
 #include "coup_mi355x.h"
 #include "coup_np.h"
+#include "coup_policy.h"
 #include "coup_regroup.h"
 #include "coup_tensor.h"
 
@@ -4831,6 +4833,142 @@ int coup_measure_store_sweep(float* dst, int64_t n_float4, int threads, int pass
   if (threads == 1024 && passes == 8) return go(std::integral_constant<int, 1024>(), std::integral_constant<int, 8>());
 #endif
   return fail(COUP_E_INVALID, "coup_measure_store_sweep: shape not in this build");
+}
+
+// ------------------------------------------------- learner-side operators
+// (coup_policy.h)
+
+namespace {
+
+bool dtype_ok(int dtype) { return dtype == COUP_DTYPE_F32 || dtype == COUP_DTYPE_F16 || dtype == COUP_DTYPE_BF16; }
+
+// Why `d` cannot be taken by `what`, or null.
+const char* decisions_error(const coup_decisions* d, bool acted) {
+  if (!d) return "decisions is null";
+  if (d->rows < 0 || d->rows > (int64_t(1) << 38)) return "rows out of range";
+  if (d->num_actions < 1 || d->num_actions > COUP_MAX_POLICY_ACTIONS) return "num_actions must be 1..31";
+  if (!dtype_ok(d->dtype)) return "unknown dtype";
+  if (d->rows == 0) return nullptr;
+  if (!d->logits || !d->legal_mask) return "logits or legal_mask is null";
+  if (d->logits_stride < d->num_actions && d->rows > 1) return "logits_stride is below num_actions";
+  if (!acted) return nullptr;
+  if (!d->actions) return "actions is null";
+  if (d->ref_logits && d->ref_stride < d->num_actions && d->rows > 1) return "ref_stride is below num_actions";
+  return nullptr;
+}
+
+coup::policy::Rows rows_of(const coup_decisions* d, bool acted) {
+  return {d->logits,     acted ? d->ref_logits : nullptr, d->logits_stride, d->ref_stride, d->actions,
+          d->legal_mask, d->rows,                         d->num_actions};
+}
+
+}  // namespace
+
+int coup_sample_actions(const coup_decisions* d, const float* uniform, int8_t* actions, float* log_probs,
+                        void* hip_stream) {
+  if (const char* why = decisions_error(d, false)) return fail(COUP_E_INVALID, std::string("coup_sample_actions: ") + why);
+  if (d->rows == 0) return COUP_OK;
+  if (!uniform || !actions) return fail(COUP_E_INVALID, "coup_sample_actions: uniform or actions is null");
+  coup::policy::launch_sample(rows_of(d, false), d->dtype, uniform, actions, log_probs, (hipStream_t)hip_stream);
+  COUP_HIP_TRY(hipGetLastError());
+  return COUP_OK;
+}
+
+int coup_advantages(const coup_window* w, double gamma, double lam, float* adv, float* target, void* hip_stream) {
+  if (!w) return fail(COUP_E_INVALID, "coup_advantages: window is null");
+  if (w->steps < 0 || w->lanes < 0 || (w->lanes && w->steps > (int64_t(1) << 40) / w->lanes))
+    return fail(COUP_E_INVALID, "coup_advantages: steps or lanes out of range");
+  if (w->num_players < 2 || w->num_players > COUP_MAX_PLAYERS)
+    return fail(COUP_E_INVALID, "coup_advantages: num_players must be 2..6");
+  if (!dtype_ok(w->dtype)) return fail(COUP_E_INVALID, "coup_advantages: unknown dtype");
+  if (!(gamma >= 0.0 && gamma <= 1.0 && lam >= 0.0 && lam <= 1.0))
+    return fail(COUP_E_INVALID, "coup_advantages: gamma and lam must be in 0..1");
+  if (w->steps == 0 || w->lanes == 0) return COUP_OK;
+  if (!w->rewards || !w->step_type || !w->players || !w->values || !adv || !target)
+    return fail(COUP_E_INVALID, "coup_advantages: null buffer");
+  const coup::policy::AdvantageArgs q{w->rewards, w->step_type, w->players,   w->values,           w->bootstrap,
+                                      adv,        target,       w->steps,     w->lanes,            (float)gamma,
+                                      (float)(gamma * lam),     (float)(gamma * (1.0 - lam))};
+  coup::policy::launch_advantages(q, w->dtype, w->num_players, (hipStream_t)hip_stream);
+  COUP_HIP_TRY(hipGetLastError());
+  return COUP_OK;
+}
+
+size_t coup_policy_workspace(int64_t rows) { return coup::policy::policy_workspace(rows > 0 ? rows : 0); }
+
+int coup_policy_loss(const coup_decisions* d, const coup_policy_terms* terms, const coup_policy_outputs* out,
+                     void* workspace, size_t workspace_bytes, void* hip_stream) {
+  if (const char* why = decisions_error(d, true)) return fail(COUP_E_INVALID, std::string("coup_policy_loss: ") + why);
+  if (!terms || !out || !out->loss) return fail(COUP_E_INVALID, "coup_policy_loss: terms, out or its loss is null");
+  if (d->rows && (!terms->old_log_probs || !terms->advantages))
+    return fail(COUP_E_INVALID, "coup_policy_loss: old_log_probs or advantages is null");
+  if (!(terms->clip_low >= 0.0 && terms->clip_low <= 1.0 && terms->clip_high >= 0.0 && std::isfinite(terms->clip_high)))
+    return fail(COUP_E_INVALID, "coup_policy_loss: clip_low must be in 0..1 and clip_high finite and not negative");
+  if (!std::isfinite(terms->kl_coef) || !std::isfinite(terms->entropy_coef))
+    return fail(COUP_E_INVALID, "coup_policy_loss: kl_coef and entropy_coef must be finite");
+  if (!workspace || ((uintptr_t)workspace & 7) || workspace_bytes < coup_policy_workspace(d->rows))
+    return fail(COUP_E_INVALID, "coup_policy_loss: workspace is null, misaligned or too small");
+  coup::policy::PolicyArgs q{};
+  q.r = rows_of(d, true);
+  q.old = terms->old_log_probs;
+  q.adv = terms->advantages;
+  q.active = terms->active;
+  q.low = (float)(1.0 - terms->clip_low);
+  q.high = (float)(1.0 + terms->clip_high);
+  q.log_low = std::log1p(-terms->clip_low);
+  q.log_high = std::log1p(terms->clip_high);
+  q.kl = (float)terms->kl_coef;
+  q.ent = (float)terms->entropy_coef;
+  q.log_probs = out->log_probs;
+  q.grad = out->grad;
+  coup::policy::launch_policy(q, d->dtype, terms->kl_coef, terms->entropy_coef, out->loss, out->stats, out->count,
+                              workspace, (hipStream_t)hip_stream);
+  COUP_HIP_TRY(hipGetLastError());
+  return COUP_OK;
+}
+
+size_t coup_preference_workspace(int64_t rows, int64_t pairs) {
+  return coup::policy::preference_workspace(rows > 0 ? rows : 0, pairs > 0 ? pairs : 0);
+}
+
+int coup_preference_loss(const coup_decisions* d, const coup_preference_terms* terms,
+                         const coup_preference_outputs* out, void* workspace, size_t workspace_bytes,
+                         void* hip_stream) {
+  if (const char* why = decisions_error(d, true))
+    return fail(COUP_E_INVALID, std::string("coup_preference_loss: ") + why);
+  if (!terms || !out || !out->loss) return fail(COUP_E_INVALID, "coup_preference_loss: terms, out or its loss is null");
+  if (terms->pairs < 0 || terms->pairs > (int64_t(1) << 30))
+    return fail(COUP_E_INVALID, "coup_preference_loss: pairs out of range");
+  if (terms->offset_bytes != 4 && terms->offset_bytes != 8)
+    return fail(COUP_E_INVALID, "coup_preference_loss: offset_bytes must be 4 or 8");
+  if (!terms->offsets) return fail(COUP_E_INVALID, "coup_preference_loss: offsets is null");
+  if (!std::isfinite(terms->beta)) return fail(COUP_E_INVALID, "coup_preference_loss: beta must be finite");
+  if (!(terms->label_smoothing >= 0.0 && terms->label_smoothing <= 0.5))
+    return fail(COUP_E_INVALID, "coup_preference_loss: label_smoothing must be in 0..0.5");
+  if (!workspace || ((uintptr_t)workspace & 7) || workspace_bytes < coup_preference_workspace(d->rows, terms->pairs))
+    return fail(COUP_E_INVALID, "coup_preference_loss: workspace is null, misaligned or too small");
+  coup::policy::PreferenceArgs q{};
+  q.r = rows_of(d, true);
+  q.offsets = terms->offsets;
+  q.wide = terms->offset_bytes == 8;
+  q.pairs = terms->pairs;
+  q.beta = terms->beta;
+  q.eps = terms->label_smoothing;
+  q.rewards = out->rewards;
+  q.grad = out->grad;
+  coup::policy::launch_preference(q, d->dtype, out->loss, workspace, (hipStream_t)hip_stream);
+  COUP_HIP_TRY(hipGetLastError());
+  return COUP_OK;
+}
+
+int coup_scale_grad(void* grad, int dtype, int64_t n, const float* scale, void* hip_stream) {
+  if (!dtype_ok(dtype)) return fail(COUP_E_INVALID, "coup_scale_grad: unknown dtype");
+  if (n < 0) return fail(COUP_E_INVALID, "coup_scale_grad: negative n");
+  if (n == 0) return COUP_OK;
+  if (!grad || !scale) return fail(COUP_E_INVALID, "coup_scale_grad: grad or scale is null");
+  coup::policy::launch_scale(grad, dtype, n, scale, (hipStream_t)hip_stream);
+  COUP_HIP_TRY(hipGetLastError());
+  return COUP_OK;
 }
 
 }  // extern "C"

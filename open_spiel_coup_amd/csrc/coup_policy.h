@@ -1,0 +1,657 @@
+// coup_policy.h -- the learner-side operators over the env's trajectories
+// (include/coup_mi355x.h, "learner-side operators"): masked action sampling,
+// turn-based generalised advantages, the clipped policy loss and the paired
+// log-ratio preference loss, forward and gradient.
+//
+// A row is one decision: A <= 31 logits, its legal-action word, its action.
+// A row counts where the action is legal: 0 <= action < A, the word's bit
+// `action` set, bit 31 (a chance node) clear.  Rows that do not count are
+// never computed on, so whatever their logits, old log probabilities and
+// advantages hold cannot reach an output.  One thread works on one row, whose
+// logits it keeps in registers, padded to AP (an illegal or padded action is
+// -inf, which every sum below takes as 0).
+//
+// Arithmetic: logits are widened to 32 bits on load; the softmax statistics,
+// the log probabilities and the gradient are 32-bit; sums over rows are
+// 64-bit past one wave.  A gradient is rounded once, to the logits' type, at
+// its store.  Two comparisons decide whole outputs and are repeated in 64
+// bits where 32-bit rounding could turn them: which action a uniform number
+// falls on, and which side of the clip border a ratio is on.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "coup_launch_log.h"
+#include "coup_mi355x.h"
+
+namespace coup {
+namespace policy {
+
+constexpr int kRowThreads = 256;
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLowest = -3.402823466e38f;
+
+template <class T>
+__device__ __forceinline__ float widen(T v) {
+  return (float)v;
+}
+
+// The rows of a call, as the kernels take them.
+struct Rows {
+  const void* logits;
+  const void* ref;  // null: no reference policy
+  int64_t stride, ref_stride;  // elements between rows
+  const int8_t* actions;
+  const uint32_t* mask;
+  int64_t n;
+  int A;
+};
+
+// The legal actions of a mask word among A: none at a chance node.
+__device__ __forceinline__ uint32_t legal_bits(uint32_t mask, int A) {
+  return (mask >> 31) ? 0u : mask & ((1u << A) - 1u);
+}
+
+__device__ __forceinline__ bool decided(uint32_t legal, int action) {
+  return action >= 0 && action < 31 && ((legal >> action) & 1u);
+}
+
+// One row's logits, -inf at actions outside `legal`.
+template <class T, int AP>
+__device__ __forceinline__ void load_row(const T* row, int A, uint32_t legal, float (&x)[AP]) {
+#pragma unroll
+  for (int a = 0; a < AP; ++a) {
+    float v = -INFINITY;
+    if (a < A) v = widen(row[a]);
+    x[a] = ((legal >> a) & 1u) ? v : -INFINITY;
+  }
+}
+
+struct Softmax {
+  float m;     // largest logit
+  float sum;   // sum of e
+  float lse;   // log of the sum: log p_a = (x_a - m) - lse
+};
+
+// x becomes x - m and e = exp(x - m).  The sum is at least 1 (the largest
+// logit's own e); when only one e is 1, lse is taken as log1p of the others'
+// sum, so a nearly certain action's log probability keeps its precision.
+template <int AP>
+__device__ __forceinline__ Softmax softmax(float (&x)[AP], float (&e)[AP]) {
+  Softmax s;
+  s.m = x[0];
+#pragma unroll
+  for (int a = 1; a < AP; ++a) s.m = fmaxf(s.m, x[a]);
+  s.sum = 0.0f;
+  float others = 0.0f;  // the sum without the ones: fract(1) = 0
+#pragma unroll
+  for (int a = 0; a < AP; ++a) {
+    x[a] -= s.m;
+    e[a] = __builtin_amdgcn_exp2f(x[a] * kLog2e);
+    s.sum += e[a];
+    others += __builtin_amdgcn_fractf(e[a]);
+  }
+  s.lse = (s.sum - others < 1.5f) ? log1pf(others) : logf(s.sum);
+  return s;
+}
+
+// The same statistics of a row in 64 bits, for the rows next to a border.
+template <class T>
+__device__ __attribute__((noinline)) double lse64(const T* row, uint32_t legal, float m) {
+  double sum = 0.0;
+#pragma unroll 1
+  for (uint32_t b = legal; b; b &= b - 1) sum += exp((double)widen(row[__builtin_ctz(b)]) - (double)m);
+  return log(sum);
+}
+
+// The action a uniform number u falls on: the first legal a whose running
+// sum passes u * total, in 64 bits; the last with a share where rounding
+// leaves the total at or below it.
+template <class T>
+__device__ __attribute__((noinline)) int pick64(const T* row, uint32_t legal, float m, float u) {
+  double total = 0.0;
+#pragma unroll 1
+  for (uint32_t b = legal; b; b &= b - 1) total += exp((double)widen(row[__builtin_ctz(b)]) - (double)m);
+  const double t = (double)u * total;
+  double c = 0.0;
+  int last = -1;
+#pragma unroll 1
+  for (uint32_t b = legal; b; b &= b - 1) {
+    const int a = __builtin_ctz(b);
+    const double e = exp((double)widen(row[a]) - (double)m);
+    c += e;
+    if (e > 0.0) last = a;
+    if (c > t) return a;
+  }
+  return last;
+}
+
+// ------------------------------------------------------- action sampling
+
+// Row i's action is min {a : sum_{b <= a} e_b > u total} (inverse
+// distribution function over the legal actions in ascending order).  The
+// 32-bit running sums are off by less than 2^-17 of the total: the e's
+// relative error is (1 + |x - m|) 2^-23, which weighs at most 3 * 2^-23 over
+// a row, and 31 additions and the product add 16 * 2^-23 a side.  A running
+// sum that near to u * total sends the row through pick64.
+constexpr float kPickMargin = 7.62939453125e-6f;  // 2^-17
+
+template <class T, int AP>
+__global__ __launch_bounds__(kRowThreads) void k_sample(Rows r, const float* __restrict__ uniform,
+                                                         int8_t* __restrict__ actions, float* __restrict__ log_probs) {
+  const int64_t i = (int64_t)blockIdx.x * kRowThreads + threadIdx.x;
+  if (i >= r.n) return;
+  const uint32_t legal = legal_bits(r.mask[i], r.A);
+  int action = -1;
+  float logp = 0.0f;
+  if (legal) {
+    const T* row = (const T*)r.logits + i * r.stride;
+    float x[AP], e[AP];
+    load_row<T, AP>(row, r.A, legal, x);
+    const Softmax s = softmax<AP>(x, e);
+    if (s.sum == s.sum) {
+      float u = uniform[i];
+      bool near = !(u < 1.0f);  // outside [0, 1): below as 0, above (and a NaN) the last action with a share
+      u = u < 0.0f ? 0.0f : u;
+      const float t = u * s.sum, margin = kPickMargin * s.sum;
+      float c = 0.0f, xa = 0.0f;
+#pragma unroll
+      for (int a = AP - 1; a >= 0; --a) {  // from above: the sums still to come
+        const float rest = s.sum - c;      // the running sum through a
+        near |= fabsf(rest - t) <= margin;
+        if (rest > t) action = a, xa = x[a];
+        c += e[a];
+      }
+      if (near) {
+        action = pick64(row, legal, s.m, u);
+        xa = widen(row[action]) - s.m;
+      }
+      logp = xa - s.lse;
+    } else {
+      logp = s.sum;  // NaN or +inf at a legal action: no distribution, no action
+    }
+  }
+  actions[i] = (int8_t)action;
+  if (log_probs) log_probs[i] = logp;
+}
+
+// ------------------------------------------------------------ advantages
+
+// Player p's advantage at its decision in step t is, with V its value there,
+//   A = R + gamma V' - V + gamma lam A',
+// R the rewards it gets from t until its next decision, V' and A' that
+// decision's.  Back in time with z_p = R + gamma V' + gamma lam A' so far:
+// a step adds its reward to every z_p; the step's player takes A = z_p - V
+// and leaves z_p = gamma lam z_p + gamma (1 - lam) V for its earlier ones; a
+// LAST or FIRST step cuts what lies behind it (z = 0 before its reward).
+struct AdvantageArgs {
+  const int8_t* rewards;  // [T][B][P]
+  const uint8_t* step_type;
+  const int8_t* players;
+  const void* values;
+  const void* bootstrap;  // [B][P] or null
+  float *adv, *target;
+  int64_t T, B;
+  float gamma, gl, gv;  // gamma, gamma lam, gamma (1 - lam)
+};
+
+template <class T, int P>
+__global__ __launch_bounds__(64) void k_advantages(AdvantageArgs q) {
+  const int64_t b = (int64_t)blockIdx.x * 64 + threadIdx.x;
+  if (b >= q.B) return;
+  float z[P];
+#pragma unroll
+  for (int p = 0; p < P; ++p) z[p] = q.bootstrap ? q.gamma * widen(((const T*)q.bootstrap)[b * P + p]) : 0.0f;
+  for (int64_t t = q.T - 1; t >= 0; --t) {
+    const int64_t i = t * q.B + b;
+    const int st = q.step_type[i];
+    const bool step = st == COUP_STEP_MID || st == COUP_STEP_LAST;
+    const bool cut = st == COUP_STEP_FIRST || st == COUP_STEP_LAST;
+    const int player = step ? q.players[i] : -1;
+    const bool acts = player >= 0 && player < P;
+    const float v = acts ? widen(((const T*)q.values)[i]) : 0.0f;
+    float target = 0.0f;
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      if (cut) z[p] = 0.0f;
+      if (step) z[p] += (float)q.rewards[i * P + p];
+      if (p == player) {
+        target = z[p];
+        z[p] = q.gl * z[p] + q.gv * v;
+      }
+    }
+    q.adv[i] = acts ? target - v : 0.0f;
+    q.target[i] = target;
+  }
+}
+
+// ----------------------------------------------------- sums over a block
+
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+  for (int s = 32; s >= 1; s >>= 1) v += __shfl_xor(v, s, 64);
+  return v;
+}
+
+// `v` summed over the block (32-bit within a wave, 64-bit across); thread 0
+// has the result.
+template <int THREADS>
+__device__ __forceinline__ double block_sum(float v, double* lds) {
+  v = wave_sum(v);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = (double)v;
+  __syncthreads();
+  double s = 0.0;
+  if (threadIdx.x == 0)
+    for (int w = 0; w < THREADS / 64; ++w) s += lds[w];
+  return s;
+}
+
+// ----------------------------------------------------------- policy loss
+
+// A decision's terms, with l = log pi, d = l - log pi_ref, rho =
+// exp(l_action - old), the advantage Z and H = -sum p l, K = sum p d:
+//   surrogate  -min(rho Z, clip(rho, 1 - low, 1 + high) Z)
+//   loss       surrogate + kl K - ent H, averaged over the decisions.
+// Its derivative in x_b, with w = -rho Z where the clip does not hold (else 0):
+//   w ([b = action] - p_b) + p_b (kl (d_b - K) + ent (l_b + H)).
+struct PolicyArgs {
+  Rows r;
+  const float* old;
+  const float* adv;
+  const uint8_t* active;  // null: every row
+  float low, high;              // 1 - clip_low, 1 + clip_high
+  double log_low, log_high;     // their logs
+  float kl, ent;
+  float* log_probs;  // null: not wanted
+  void* grad;        // null: no gradient
+  double* partial;   // [blocks][4] sums of the terms
+  int64_t* counts;   // [count blocks] decisions
+  int count_blocks;
+};
+
+constexpr int kCountBlocks = 256;
+
+// How many decisions there are: 6 bytes a row.  The gradient needs it before
+// its first store, and a second pass over the gradient would cost 2 A e.
+__global__ __launch_bounds__(kRowThreads) void k_policy_count(PolicyArgs q) {
+  __shared__ int wave[kRowThreads / 64];
+  int n = 0;  // a wave's rows are a 1024th of the call's: below 2^31
+  for (int64_t i = (int64_t)blockIdx.x * kRowThreads + threadIdx.x; i < q.r.n; i += (int64_t)gridDim.x * kRowThreads)
+    n += decided(legal_bits(q.r.mask[i], q.r.A), q.r.actions[i]) && (!q.active || q.active[i]);
+#pragma unroll
+  for (int s = 32; s >= 1; s >>= 1) n += __shfl_xor(n, s, 64);
+  if ((threadIdx.x & 63) == 0) wave[threadIdx.x >> 6] = n;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  int64_t total = 0;
+  for (int w = 0; w < kRowThreads / 64; ++w) total += wave[w];
+  q.counts[blockIdx.x] = total;
+}
+
+template <class T, int AP>
+__global__ __launch_bounds__(kRowThreads) void k_policy_loss(PolicyArgs q) {
+  __shared__ double lds[kRowThreads / 64];
+  __shared__ int64_t total;
+  int64_t c = threadIdx.x < (uint32_t)q.count_blocks ? q.counts[threadIdx.x] : 0;
+  {
+    __shared__ int64_t wave[kRowThreads / 64];
+#pragma unroll
+    for (int s = 32; s >= 1; s >>= 1) c += __shfl_xor(c, s, 64);
+    if ((threadIdx.x & 63) == 0) wave[threadIdx.x >> 6] = c;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      int64_t n = 0;
+      for (int w = 0; w < kRowThreads / 64; ++w) n += wave[w];
+      total = n;
+    }
+    __syncthreads();
+  }
+  const float scale = 1.0f / (float)(total > 0 ? total : 1);
+
+  const int64_t i = (int64_t)blockIdx.x * kRowThreads + threadIdx.x;
+  float surrogate = 0.0f, kl = 0.0f, entropy = 0.0f, clipped = 0.0f;
+  if (i < q.r.n) {
+    const uint32_t legal = legal_bits(q.r.mask[i], q.r.A);
+    const int action = q.r.actions[i];
+    float logp = 0.0f;
+    T* grad = q.grad ? (T*)q.grad + i * q.r.A : nullptr;
+    if (decided(legal, action) && (!q.active || q.active[i])) {
+      const T* row = (const T*)q.r.logits + i * q.r.stride;
+      float x[AP], e[AP], d[AP];
+      load_row<T, AP>(row, q.r.A, legal, x);
+      const Softmax s = softmax<AP>(x, e);
+      const float inv = 1.0f / s.sum;
+      if (q.r.ref) {
+        float re[AP];
+        load_row<T, AP>((const T*)q.r.ref + i * q.r.ref_stride, q.r.A, legal, d);
+        const Softmax rs = softmax<AP>(d, re);
+#pragma unroll
+        for (int a = 0; a < AP; ++a) d[a] = ((legal >> a) & 1u) ? (fmaxf(x[a], kLowest) - s.lse) - (d[a] - rs.lse) : 0.0f;
+      }
+      float z = 0.0f, w = 0.0f;
+#pragma unroll
+      for (int a = 0; a < AP; ++a) {
+        e[a] *= inv;                            // p
+        if (a == action) z = x[a];
+        x[a] = fmaxf(x[a] - s.lse, kLowest);    // log p; finite, so that 0 log 0 is 0
+        entropy -= e[a] * x[a];
+        if (q.r.ref) kl += e[a] * d[a];
+      }
+      if (kl > 1e30f) kl = INFINITY;  // an action that the reference never takes
+      logp = z - s.lse;
+      const float old = q.old[i], adv = q.adv[i], dl = logp - old;
+      const double border = adv > 0.0f ? q.log_high : q.log_low;
+      bool over = adv > 0.0f ? dl > (float)border : dl < (float)border;
+      // 32 bits hold dl to a few 2^-23 of its terms
+      if (fabsf(dl - (float)border) <= 4.76837158e-7f * (4.0f + fabsf(z) + fabsf(old))) {
+        const double dl64 = ((double)widen(row[action]) - (double)s.m) - lse64(row, legal, s.m) - (double)old;
+        over = adv > 0.0f ? dl64 > border : dl64 < border;
+      }
+      over = over && adv != 0.0f;
+      const float rho = expf(dl);
+      surrogate = adv == 0.0f ? 0.0f : -(over ? (adv > 0.0f ? q.high : q.low) : rho) * adv;
+      clipped = over ? 1.0f : 0.0f;
+      w = (over || adv == 0.0f) ? 0.0f : -rho * adv;
+      if (grad) {
+        const float base = q.ent * entropy - (q.r.ref ? q.kl * kl : 0.0f) - w;
+#pragma unroll
+        for (int a = 0; a < AP; ++a) {
+          float g = q.ent * x[a] + base;
+          if (q.r.ref) g += q.kl * d[a];
+          g *= e[a];
+          if (a == action) g += w;
+          if (a < q.r.A) grad[a] = (T)(((legal >> a) & 1u) ? g * scale : 0.0f);
+        }
+      }
+    } else if (grad) {
+      for (int a = 0; a < q.r.A; ++a) grad[a] = (T)0.0f;
+    }
+    if (q.log_probs) q.log_probs[i] = logp;
+  }
+  const double s0 = block_sum<kRowThreads>(surrogate, lds), s1 = block_sum<kRowThreads>(kl, lds),
+               s2 = block_sum<kRowThreads>(entropy, lds), s3 = block_sum<kRowThreads>(clipped, lds);
+  if (threadIdx.x == 0) {
+    double* o = q.partial + 4 * (int64_t)blockIdx.x;
+    o[0] = s0, o[1] = s1, o[2] = s2, o[3] = s3;
+  }
+}
+
+// The blocks' sums in a fixed order: the loss and its terms' means.
+__global__ __launch_bounds__(kRowThreads) void k_policy_finish(const double* __restrict__ partial, int64_t blocks,
+                                                                const int64_t* __restrict__ counts, int count_blocks,
+                                                                double kl, double ent, float* loss, float* stats,
+                                                                int64_t* count) {
+  __shared__ double lds[5][kRowThreads / 64];
+  double s[5] = {0.0, 0.0, 0.0, 0.0, 0.0};
+  for (int64_t i = threadIdx.x; i < blocks; i += kRowThreads)
+    for (int k = 0; k < 4; ++k) s[k] += partial[4 * i + k];
+  if (threadIdx.x < (uint32_t)count_blocks) s[4] = (double)counts[threadIdx.x];
+  for (int k = 0; k < 5; ++k) {
+    for (int d = 32; d >= 1; d >>= 1) s[k] += __shfl_xor(s[k], d, 64);
+    if ((threadIdx.x & 63) == 0) lds[k][threadIdx.x >> 6] = s[k];
+  }
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  for (int k = 0; k < 5; ++k) {
+    s[k] = 0.0;
+    for (int w = 0; w < kRowThreads / 64; ++w) s[k] += lds[k][w];
+  }
+  const double n = s[4] > 0.0 ? s[4] : 1.0;
+  for (int k = 0; k < 4; ++k) s[k] /= n;
+  *loss = (float)(s[0] + (kl != 0.0 ? kl * s[1] : 0.0) - ent * s[2]);
+  for (int k = 0; k < 4; ++k)
+    if (stats) stats[k] = (float)s[k];
+  if (count) *count = (int64_t)s[4];
+}
+
+// ------------------------------------------------------- preference loss
+
+// Sequences are packed: sequence s holds rows [offsets[s], offsets[s + 1]),
+// 2 i the chosen and 2 i + 1 the rejected one of pair i.  With R_s = beta
+// times the sum of l - l_ref over its decisions and x = R_2i - R_2i+1, a pair
+// costs -(1 - eps) log sigma(x) - eps log sigma(-x); a row's derivative is
+// +-beta / pairs (eps - sigma(-x)) ([b = action] - p_b).
+struct PreferenceArgs {
+  Rows r;
+  const void* offsets;
+  int wide;  // offsets are int64 (else int32)
+  int64_t pairs;
+  double beta, eps;
+  float* ratio;     // [n] a row's l - l_ref
+  double* partial;  // [pairs] a pair's cost; NaN where its offsets are not ascending within the rows
+  float* coef;      // [2 pairs]
+  float* rewards;   // [2 pairs]
+  void* grad;
+};
+
+__device__ __forceinline__ int64_t raw_offset(const PreferenceArgs& q, int64_t s) {
+  return q.wide ? ((const int64_t*)q.offsets)[s] : (int64_t)((const int32_t*)q.offsets)[s];
+}
+
+// Held to the rows: every row read is one of the call's.
+__device__ __forceinline__ int64_t offset_at(const PreferenceArgs& q, int64_t s) {
+  const int64_t o = raw_offset(q, s);
+  return o < 0 ? 0 : o > q.r.n ? q.r.n : o;
+}
+
+template <class T, int AP>
+__global__ __launch_bounds__(kRowThreads) void k_preference_rows(PreferenceArgs q) {
+  const int64_t i = (int64_t)blockIdx.x * kRowThreads + threadIdx.x;
+  if (i >= q.r.n) return;
+  const uint32_t legal = legal_bits(q.r.mask[i], q.r.A);
+  const int action = q.r.actions[i];
+  float out = 0.0f;
+  if (decided(legal, action)) {
+    float x[AP], e[AP];
+    load_row<T, AP>((const T*)q.r.logits + i * q.r.stride, q.r.A, legal, x);
+    Softmax s = softmax<AP>(x, e);
+#pragma unroll
+    for (int a = 0; a < AP; ++a)
+      if (a == action) out = x[a];
+    out -= s.lse;
+    if (q.r.ref) {
+      load_row<T, AP>((const T*)q.r.ref + i * q.r.ref_stride, q.r.A, legal, x);
+      s = softmax<AP>(x, e);
+      float z = 0.0f;
+#pragma unroll
+      for (int a = 0; a < AP; ++a)
+        if (a == action) z = x[a];
+      out -= z - s.lse;
+    }
+  }
+  q.ratio[i] = out;
+}
+
+__device__ __forceinline__ double log1p_exp_neg(double x) {  // -log sigma(x)
+  return fmax(-x, 0.0) + log1p(exp(-fabs(x)));
+}
+
+__global__ __launch_bounds__(kRowThreads) void k_preference_pairs(PreferenceArgs q) {
+  __shared__ double lds[2][kRowThreads / 64];
+  const int64_t pair = blockIdx.x;
+  const int64_t o0 = offset_at(q, 2 * pair), o1 = offset_at(q, 2 * pair + 1), o2 = offset_at(q, 2 * pair + 2);
+  double s[2] = {0.0, 0.0};
+  for (int64_t i = o0 + threadIdx.x; i < o1; i += kRowThreads) s[0] += (double)q.ratio[i];
+  for (int64_t i = o1 + threadIdx.x; i < o2; i += kRowThreads) s[1] += (double)q.ratio[i];
+  for (int k = 0; k < 2; ++k) {
+    for (int d = 32; d >= 1; d >>= 1) s[k] += __shfl_xor(s[k], d, 64);
+    if ((threadIdx.x & 63) == 0) lds[k][threadIdx.x >> 6] = s[k];
+  }
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  for (int k = 0; k < 2; ++k) {
+    s[k] = 0.0;
+    for (int w = 0; w < kRowThreads / 64; ++w) s[k] += lds[k][w];
+    s[k] *= q.beta;
+  }
+  const double x = s[0] - s[1];
+  double cost = (1.0 - q.eps) * log1p_exp_neg(x) + q.eps * log1p_exp_neg(-x);
+  double d = (q.eps - 1.0 / (1.0 + exp(x))) * q.beta / (double)q.pairs;
+  const int64_t r0 = raw_offset(q, 2 * pair), r1 = raw_offset(q, 2 * pair + 1), r2 = raw_offset(q, 2 * pair + 2);
+  if (r0 < 0 || r1 < r0 || r2 < r1 || r2 > q.r.n) cost = d = NAN;
+  q.partial[pair] = cost;
+  q.coef[2 * pair] = (float)d;
+  q.coef[2 * pair + 1] = (float)-d;
+  if (q.rewards) q.rewards[2 * pair] = (float)s[0], q.rewards[2 * pair + 1] = (float)s[1];
+}
+
+__global__ __launch_bounds__(kRowThreads) void k_preference_finish(const double* __restrict__ partial, int64_t pairs,
+                                                                    float* loss) {
+  __shared__ double lds[kRowThreads / 64];
+  double s = 0.0;
+  for (int64_t i = threadIdx.x; i < pairs; i += kRowThreads) s += partial[i];
+  for (int d = 32; d >= 1; d >>= 1) s += __shfl_xor(s, d, 64);
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  s = 0.0;
+  for (int w = 0; w < kRowThreads / 64; ++w) s += lds[w];
+  *loss = (float)(s / (double)(pairs > 0 ? pairs : 1));
+}
+
+template <class T, int AP>
+__global__ __launch_bounds__(kRowThreads) void k_preference_grad(PreferenceArgs q) {
+  const int64_t i = (int64_t)blockIdx.x * kRowThreads + threadIdx.x;
+  if (i >= q.r.n) return;
+  const uint32_t legal = legal_bits(q.r.mask[i], q.r.A);
+  const int action = q.r.actions[i];
+  T* grad = (T*)q.grad + i * q.r.A;
+  float coef = 0.0f;
+  if (decided(legal, action)) {
+    // the last sequence that starts at or before row i (the non-empty one where several start there)
+    int64_t lo = 0, hi = 2 * q.pairs + 1;  // offsets[lo - 1] <= i < offsets[hi]
+    while (lo < hi) {
+      const int64_t mid = (lo + hi) >> 1;
+      if (offset_at(q, mid) <= i) lo = mid + 1;
+      else hi = mid;
+    }
+    if (lo >= 1 && lo <= 2 * q.pairs) coef = q.coef[lo - 1];
+  }
+  if (coef != 0.0f) {
+    float x[AP], e[AP];
+    load_row<T, AP>((const T*)q.r.logits + i * q.r.stride, q.r.A, legal, x);
+    const Softmax s = softmax<AP>(x, e);
+    const float p = -coef / s.sum;
+#pragma unroll
+    for (int a = 0; a < AP; ++a) {
+      if (a < q.r.A) grad[a] = (T)(((legal >> a) & 1u) ? p * e[a] + (a == action ? coef : 0.0f) : 0.0f);
+    }
+  } else {
+    for (int a = 0; a < q.r.A; ++a) grad[a] = (T)0.0f;
+  }
+}
+
+// ---------------------------------------------------------- grad scaling
+
+// A gradient for a loss's own derivative of 1, times the derivative that
+// came in: nothing is read or written where that is 1, as in loss.backward().
+template <class T>
+__global__ __launch_bounds__(kRowThreads) void k_scale_grad(T* grad, int64_t n, const float* __restrict__ scale) {
+  const float g = *scale;
+  if (g == 1.0f) return;
+  for (int64_t i = (int64_t)blockIdx.x * kRowThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kRowThreads)
+    grad[i] = (T)(g * (float)grad[i]);
+}
+
+// ---------------------------------------------------------------- launch
+
+inline unsigned row_blocks(int64_t n) { return (unsigned)((n + kRowThreads - 1) / kRowThreads); }
+
+template <class T>
+struct type_of {
+  using type = T;
+};
+
+// f(type_of<T>, integral AP) for a dtype code and a number of actions: rows
+// are padded to 8, 16, 20 or 32 actions (20: the game's 18).
+template <class T, class F>
+void with_actions(int A, F f) {
+  if (A <= 8) f(type_of<T>(), std::integral_constant<int, 8>());
+  else if (A <= 16) f(type_of<T>(), std::integral_constant<int, 16>());
+  else if (A <= 20) f(type_of<T>(), std::integral_constant<int, 20>());
+  else f(type_of<T>(), std::integral_constant<int, 32>());
+}
+
+template <class F>
+void with_dtype(int dtype, F f) {
+  if (dtype == COUP_DTYPE_F32) f(type_of<float>());
+  else if (dtype == COUP_DTYPE_F16) f(type_of<_Float16>());
+  else f(type_of<__bf16>());
+}
+
+template <class F>
+void with_rows(int dtype, int A, F f) {
+  with_dtype(dtype, [&](auto t) { with_actions<typename decltype(t)::type>(A, f); });
+}
+
+inline void launch_sample(const Rows& r, int dtype, const float* uniform, int8_t* actions, float* log_probs,
+                          hipStream_t s) {
+  with_rows(dtype, r.A, [&](auto t, auto ap) {
+    using T = typename decltype(t)::type;
+    k_sample<T, decltype(ap)::value><<<row_blocks(r.n), kRowThreads, 0, s>>>(r, uniform, actions, log_probs);
+  });
+}
+
+inline void launch_advantages(const AdvantageArgs& q, int dtype, int players, hipStream_t s) {
+  const unsigned grid = (unsigned)((q.B + 63) / 64);
+  with_dtype(dtype, [&](auto t) {
+    using T = typename decltype(t)::type;
+    switch (players) {
+      case 2: k_advantages<T, 2><<<grid, 64, 0, s>>>(q); break;
+      case 3: k_advantages<T, 3><<<grid, 64, 0, s>>>(q); break;
+      case 4: k_advantages<T, 4><<<grid, 64, 0, s>>>(q); break;
+      case 5: k_advantages<T, 5><<<grid, 64, 0, s>>>(q); break;
+      default: k_advantages<T, 6><<<grid, 64, 0, s>>>(q); break;
+    }
+  });
+}
+
+inline size_t policy_workspace(int64_t n) { return sizeof(int64_t) * kCountBlocks + sizeof(double) * 4 * row_blocks(n); }
+
+inline void launch_policy(PolicyArgs q, int dtype, double kl, double ent, float* loss, float* stats, int64_t* count,
+                          void* workspace, hipStream_t s) {
+  const unsigned blocks = row_blocks(q.r.n);
+  q.counts = (int64_t*)workspace;
+  q.partial = (double*)(q.counts + kCountBlocks);
+  q.count_blocks = blocks < (unsigned)kCountBlocks ? (int)blocks : kCountBlocks;
+  if (blocks) {
+    k_policy_count<<<q.count_blocks, kRowThreads, 0, s>>>(q);
+    with_rows(dtype, q.r.A, [&](auto t, auto ap) {
+      using T = typename decltype(t)::type;
+      k_policy_loss<T, decltype(ap)::value><<<blocks, kRowThreads, 0, s>>>(q);
+    });
+  }
+  k_policy_finish<<<1, kRowThreads, 0, s>>>(q.partial, blocks, q.counts, q.count_blocks, kl, ent, loss, stats, count);
+}
+
+inline size_t preference_workspace(int64_t n, int64_t pairs) {
+  return sizeof(double) * pairs + sizeof(float) * 2 * pairs + sizeof(float) * n;
+}
+
+inline void launch_preference(PreferenceArgs q, int dtype, float* loss, void* workspace, hipStream_t s) {
+  q.partial = (double*)workspace;
+  q.coef = (float*)(q.partial + q.pairs);
+  q.ratio = q.coef + 2 * q.pairs;
+  const unsigned blocks = row_blocks(q.r.n);
+  with_rows(dtype, q.r.A, [&](auto t, auto ap) {
+    using T = typename decltype(t)::type;
+    constexpr int AP = decltype(ap)::value;
+    if (blocks) k_preference_rows<T, AP><<<blocks, kRowThreads, 0, s>>>(q);
+    if (q.pairs) k_preference_pairs<<<(unsigned)q.pairs, kRowThreads, 0, s>>>(q);
+    k_preference_finish<<<1, kRowThreads, 0, s>>>(q.partial, q.pairs, loss);
+    if (blocks && q.grad) k_preference_grad<T, AP><<<blocks, kRowThreads, 0, s>>>(q);
+  });
+}
+
+inline void launch_scale(void* grad, int dtype, int64_t n, const float* scale, hipStream_t s) {
+  const int64_t blocks = (n + kRowThreads - 1) / kRowThreads;
+  with_dtype(dtype, [&](auto t) {
+    using T = typename decltype(t)::type;
+    k_scale_grad<T><<<(unsigned)(blocks < 2048 ? blocks : 2048), kRowThreads, 0, s>>>((T*)grad, n, scale);
+  });
+}
+
+}  // namespace policy
+}  // namespace coup

@@ -413,6 +413,70 @@ class BatchedCoupEnv:
             _native.check(self.lib.coup_step(self._h, None, ctypes.byref(out)))
         return buf
 
+    def policy_trajectory_buffers(self, steps, values=False):
+        """trajectory_buffers for collect_policy_trajectory: besides the step
+        outputs, what each step's decision was made on -- decision_mask int32
+        and decision_player int8 [T, B] (the legal-action word and player
+        BEFORE the step), decision_obs [T, B, P, obs_size] where the env
+        writes observations, decision_info_state likewise -- and log_probs
+        float32 [T, B], with `values` also values float32 [T, B]."""
+        buf = self.trajectory_buffers(steps)
+        T, B, dev = int(steps), self.batch, self.device
+        buf["decision_mask"] = torch.empty(T, B, dtype=torch.int32, device=dev)
+        buf["decision_player"] = torch.empty(T, B, dtype=torch.int8, device=dev)
+        buf["log_probs"] = torch.empty(T, B, dtype=torch.float32, device=dev)
+        if values:
+            buf["values"] = torch.empty(T, B, dtype=torch.float32, device=dev)
+        for k in ("obs", "info_state"):
+            if k in buf:
+                buf["decision_" + k] = torch.empty_like(buf[k])
+        return buf
+
+    def collect_policy_trajectory(self, steps, policy, buf=None, generator=None):
+        """`steps` env steps played by a policy (collect_trajectory plays the
+        uniform one): before each step policy(time_step) gets a dict of
+        legal_mask, current_player and the tensors the env writes (obs,
+        info_state), all of the state to act in, and returns logits [B, 18],
+        or (logits, values [B]); the actions are drawn from their softmax
+        over each lane's legal actions (policy.sample_actions) with uniform
+        numbers of `generator`.  Returns buf (policy_trajectory_buffers): the
+        inputs of policy.advantages and policy.policy_loss.  Lanes without a
+        legal action (a finished game of an env without auto_reset) take
+        their reset step instead: action -1, log probability 0."""
+        from . import policy as ops
+        T, dev = int(steps), self.device
+        now = self.query(obs=self.obs is not None, info_state=self.info_state is not None)
+        over = now["terminal"] != 0
+        for t in range(T):
+            given = policy({k: now[k] for k in ("legal_mask", "current_player", "obs", "info_state") if k in now})
+            logits, values = given if isinstance(given, (tuple, list)) else (given, None)
+            if buf is None:
+                buf = self.policy_trajectory_buffers(T, values is not None)
+            uniform = torch.rand(self.batch, dtype=torch.float32, device=dev, generator=generator)
+            word = now["legal_mask"].masked_fill(over, 0)
+            actions, log_probs = ops.sample_actions(logits.detach(), word, uniform)
+            buf["decision_mask"][t].copy_(word)
+            buf["decision_player"][t].copy_(now["current_player"])
+            buf["log_probs"][t].copy_(log_probs)
+            if values is not None:
+                buf["values"][t].copy_(values.detach())
+            for k in ("obs", "info_state"):
+                if k in buf:
+                    buf["decision_" + k][t].copy_(now[k])
+            # a finished lane's next step resets it whatever its action is; action 0 asks for that step
+            actions = actions.masked_fill(over, 0)
+            self._bind_stream()
+            self._ep_reserve(1)
+            out = self._slice_outputs(buf, t)
+            _native.check(self.lib.coup_step(self._h, _ptr(actions), ctypes.byref(out)))
+            self._keep_actions = actions
+            now = {"legal_mask": buf["legal_mask"][t], "current_player": buf["current_player"][t]}
+            for k in ("obs", "info_state"):
+                if k in buf:
+                    now[k] = buf[k][t]
+            over = (buf["step_type"][t] == LAST) if not self.auto_reset else torch.zeros_like(over)
+        return buf if buf is not None else self.policy_trajectory_buffers(T)
+
     def step_trajectory_launcher(self, steps, buf):
         """collect_trajectory(steps, buf) as a zero-argument callable that only
         enqueues the one coup_step_trajectory launch (timing loops)."""

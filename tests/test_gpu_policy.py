@@ -1,0 +1,581 @@
+"""The learner-side operators (open_spiel_coup_amd.policy) on the GPU against
+their definitions in 64 bits (tests/policy_oracle.py).
+
+Tolerances, with h = 2^-24 (half a step of a 32-bit value of 1):
+- a log probability (x_a - m) - lse: x_a - m is off by h |x_a - m|; lse by the
+  relative error of a sum of at most 31 exponentials, each off by at most
+  (2 + 2 |x - m|) h, whose weighted mean over a row is below (2 + 2 * 5) h,
+  plus 31 additions and the logarithm's 3: 48 h; so (48 + 2 |l|) h in all, and
+  twice that for a difference of two.
+- a gradient entry is a sum of at most 6 products of log probabilities, p and
+  the ratio, each factor within the above: 8 * (48 + 2 Z) h of the sum of its
+  terms' sizes (the oracle's `size`), Z the largest |x - m|; plus half a step
+  of its own type, and half the smallest step where it is subnormal.
+- a mean over rows adds the sums' rounding: a row's terms are summed in 32 bits
+  over a wave (6 additions), then in 64: 16 h of the mean absolute term beside
+  the row's own error.
+"""
+import ctypes
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from open_spiel_coup_amd import BatchedCoupEnv, _native, policy
+from tests import policy_oracle as oracle
+
+pytestmark = pytest.mark.gpu
+
+H = 2.0 ** -24
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+DEV = "cuda"
+
+
+def _np(t):
+    return t.detach().double().cpu().numpy()
+
+
+def _words(mask):
+    return torch.tensor(np.asarray(mask, np.int64)).to(torch.int32)  # bit 31 wraps into the sign
+
+
+def _table(gen, n, A, dtype, spread=2.0):
+    """(logits, mask words, actions): legal sets of every size, empty rows, chance nodes, strays, waste in masked places."""
+    x = spread * torch.randn(n, A, generator=gen)
+    legal = torch.rand(n, A, generator=gen) < torch.rand(n, 1, generator=gen)
+    mask, actions = [], []
+    for i in range(n):
+        bits = sum(1 << a for a in range(A) if legal[i, a])
+        kind = i % 11
+        if kind == 3:
+            bits = 0
+        elif not bits:
+            bits = 1 << (i % A)
+        if kind == 5:
+            bits |= 1 << 31
+        ok = oracle.legal_actions(bits & 0x7FFFFFFF, A)
+        act = ok[int(torch.randint(len(ok), (1,), generator=gen))] if ok else -1
+        if kind == 7:
+            act = -1
+        elif kind == 8:
+            act = (ok[-1] + 1) if ok else 3  # perhaps outside the word, perhaps past A
+        mask.append(bits | (0x7FFFFFFF & ~((1 << A) - 1)))  # bits past A mean nothing
+        actions.append(act)
+        for a in range(A):
+            if not (bits >> a) & 1:
+                x[i, a] = [math.nan, math.inf, torch.finfo(dtype).min, -math.inf][(i + a) % 4]
+    return x.to(dtype), _words(mask), torch.tensor(actions, dtype=torch.int8)
+
+
+def _reach(logits, mask):
+    """Largest |x - m| over the finite legal logits."""
+    z = 0.0
+    for row, w in zip(_np(logits), mask.numpy()):
+        v = [row[a] for a in oracle.legal_actions(w, logits.shape[1]) if math.isfinite(row[a])]
+        z = max(z, max(v) - min(v)) if v else z
+    return z
+
+
+def _close(got, want, tol, what):
+    got, want = np.asarray(got, np.float64), np.asarray(want, np.float64)
+    assert got.shape == want.shape, what
+    assert np.array_equal(np.isnan(got), np.isnan(want)), what
+    off = np.abs(got - want)
+    bad = ~(off <= tol) & ~np.isnan(want)
+    assert not bad.any(), (what, np.argwhere(bad)[:4], got[bad][:4], want[bad][:4], np.broadcast_to(tol, want.shape)[bad][:4])
+
+
+def _logp_tol(want):
+    return (48 + 2 * np.abs(np.nan_to_num(want))) * H
+
+
+def _grad_tol(o, z, dtype):
+    info = torch.finfo(dtype)
+    return 8 * (48 + 2 * z) * H * o["size"] + info.eps / 2 * np.abs(o["grad"]) + info.smallest_normal * info.eps / 2
+
+
+# ------------------------------------------------------------ sampling
+@pytest.mark.parametrize("dtype", DTYPES, ids=lambda d: str(d)[6:])
+@pytest.mark.parametrize("A", [1, 2, 7, 16, 18, 21, 31])
+@pytest.mark.parametrize("n", [1, 63, 257, 1001])
+def test_sample(n, A, dtype):
+    gen = torch.Generator().manual_seed(100 * A + n)
+    x, mask, _ = _table(gen, n, A, dtype)
+    u = torch.rand(n, generator=gen)
+    u[:: 17] = 0.0
+    u[1:: 17] = 1 - 2.0 ** -24
+    a, lp = policy.sample_actions(x.to(DEV), mask.to(DEV), u.to(DEV))
+    assert a.dtype == torch.int8 and lp.dtype == torch.float32
+    wa, wl = oracle.sample(_np(x), mask.numpy(), u.numpy())
+    assert np.array_equal(a.cpu().numpy(), wa)
+    _close(lp.cpu().numpy(), wl, _logp_tol(wl), "log_probs")
+
+
+def test_sample_on_the_borders():
+    """Uniform numbers on both sides of every border of the distribution, and on the exact borders of equal logits."""
+    gen = torch.Generator().manual_seed(5)
+    rows, us, words = [], [], []
+    for k in range(60):
+        x = torch.randn(18, generator=gen) * 3
+        legal = [a for a in range(18) if (k * 7 + a * 5) % 3] or [0]
+        p = np.exp([oracle.log_softmax(x.double().numpy(), legal)[a] for a in legal])
+        for c in np.cumsum(p)[:-1]:
+            for u in (np.float32(c), np.nextafter(np.float32(c), np.float32(0)), np.nextafter(np.float32(c), np.float32(1))):
+                rows.append(x), us.append(u), words.append(sum(1 << a for a in legal))
+    for m in (1, 2, 4, 6, 8, 16):
+        for k in range(m):
+            rows.append(torch.full((18,), -7.25)), us.append(np.float32(k / m)), words.append((1 << m) - 1)
+    x, u, mask = torch.stack(rows), torch.tensor(np.array(us)), _words(words)
+    a, lp = policy.sample_actions(x.to(DEV), mask.to(DEV), u.to(DEV))
+    wa, wl = oracle.sample(_np(x), mask.numpy(), u.numpy())
+    assert np.array_equal(a.cpu().numpy(), wa)
+    _close(lp.cpu().numpy(), wl, _logp_tol(wl), "log_probs")
+
+
+def test_sample_degenerate_rows():
+    """NaN, +inf and nothing but -inf at legal actions: no action, log probability NaN; -inf beside finite ones has no
+    share; lowest values are ordinary; numbers outside [0, 1) fall on the first or last action with a share."""
+    low, inf, nan = torch.finfo(torch.float32).min, math.inf, math.nan
+    x = torch.tensor([[nan, 0, 0], [inf, 0, 0], [-inf, -inf, -inf], [-inf, 1.0, -inf], [low, low, low], [low, 0.0, low],
+                      [0.0, 0.0, -inf], [0.0, 0.0, 0.0], [0.0, 0.0, 0.0], [1e30, -1e30, 0.0]])
+    u = torch.tensor([0.5, 0.5, 0.5, 0.0, 0.5, 0.99, 1.0, -1.0, nan, 0.999])
+    a, lp = policy.sample_actions(x.to(DEV), torch.full((10,), 7, dtype=torch.int32, device=DEV), u.to(DEV))
+    assert a.tolist() == [-1, -1, -1, 1, 1, 1, 1, 0, 2, 0]
+    want = [nan, nan, nan, 0.0, -math.log(3), 0.0, -math.log(2), -math.log(3), -math.log(3), 0.0]
+    _close(lp.cpu().numpy(), want, 50 * H, "log_probs")
+
+
+def test_sample_layouts_and_devices():
+    """Strided rows, a transposed table, leading dimensions, non-contiguous words; another stream; no rows."""
+    gen = torch.Generator().manual_seed(9)
+    x, mask, _ = _table(gen, 120, 18, torch.float32)
+    u = torch.rand(120, generator=gen)
+    want = [t.cpu() for t in policy.sample_actions(x.to(DEV), mask.to(DEV), u.to(DEV))]
+    wide = torch.full((120, 25), math.nan, device=DEV)
+    wide[:, 3:21] = x.to(DEV)
+    odd = torch.full((240, 18), math.nan, device=DEV)
+    odd[::2] = x.to(DEV)
+    words = torch.zeros(120, 3, dtype=torch.int32, device=DEV)
+    words[:, 1] = mask.to(DEV)
+    side = torch.cuda.Stream()
+    for logits in (wide[:, 3:21], odd[::2], x.to(DEV).t().contiguous().t()):
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            got = policy.sample_actions(logits, words[:, 1], u.to(DEV))
+        side.synchronize()
+        for g, w in zip(got, want):
+            assert torch.equal(g.cpu().nan_to_num(7), w.nan_to_num(7))
+    got = policy.sample_actions(x.to(DEV).view(4, 30, 18), mask.to(DEV).view(4, 30), u.to(DEV).view(4, 30))
+    assert got[0].shape == (4, 30) and torch.equal(got[0].cpu().flatten(), want[0])
+    empty = policy.sample_actions(x.to(DEV)[:0], mask.to(DEV)[:0], u.to(DEV)[:0])
+    assert empty[0].shape == (0,)
+    one = policy.sample_actions(x.to(DEV)[0], mask.to(DEV)[0], u.to(DEV)[0])
+    assert one[0].shape == () and int(one[0]) == int(want[0][0])
+
+
+# ------------------------------------------------------------ advantages
+def _window(gen, T, B, P, dtype, ends=0.1):
+    kind = torch.rand(T, B, generator=gen)
+    st = torch.full((T, B), 1, dtype=torch.uint8)
+    st[kind < ends] = 2
+    st[(kind >= ends) & (kind < ends + 0.05)] = 0
+    st[(kind >= ends + 0.05) & (kind < ends + 0.1)] = 3
+    pl = torch.randint(0, P, (T, B), generator=gen).to(torch.int8)
+    pl[torch.rand(T, B, generator=gen) < 0.05] = -4
+    rewards = torch.randint(-P, P + 1, (T, B, P), generator=gen).to(torch.int8)
+    v = torch.randn(T, B, generator=gen)
+    v[(st == 0) | (st == 3) | (pl < 0)] = math.nan
+    return rewards, st, pl, v.to(dtype), torch.randn(B, P, generator=gen).to(dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=lambda d: str(d)[6:])
+@pytest.mark.parametrize("T,B,P,gamma,lam", [(1, 1, 2, 0.99, 0.95), (2, 65, 2, 1.0, 1.0), (17, 3, 6, 0.9, 0.8),
+                                             (64, 130, 2, 0.99, 0.95), (513, 4, 3, 0.99, 0.95), (1030, 1, 2, 1.0, 0.9),
+                                             (130, 33, 5, 1.0, 0.0), (40, 257, 4, 0.0, 1.0)])
+@pytest.mark.parametrize("boot", [True, False], ids=["bootstrap", "none"])
+def test_advantages(T, B, P, gamma, lam, boot, dtype):
+    """Against every player's chain written out forwards.  A chain's advantage is a sum of at most T terms decayed by
+    gamma lam < 1 or, undecayed, cut every ten steps or so: 4 roundings a term, of sums bounded by `bound`."""
+    gen = torch.Generator().manual_seed(T * 7 + B + P)
+    r, st, pl, v, b = _window(gen, T, B, P, dtype)
+    got = policy.advantages(r.to(DEV), st.to(DEV), pl.to(DEV), v.to(DEV), b.to(DEV) if boot else None, gamma=gamma, lam=lam)
+    want = oracle.advantages(r.numpy(), st.numpy(), pl.numpy(), _np(v), _np(b) if boot else None, gamma, lam)
+    # partial sums stay below the absolute rewards and values of the steps within reach (the cuts' longest run)
+    cuts = ((st == 0) | (st == 2)).float()
+    run = max((len(s) for col in cuts.t().int().tolist() for s in "".join(map(str, col)).split("1")), default=0) + 1
+    bound = run * (P + 2 * 4.5)
+    for g, w, name in zip(got, want, ("advantages", "targets")):
+        assert g.dtype == torch.float32
+        _close(g.cpu().numpy(), w, 4 * run * H * bound, name)
+
+
+def test_advantages_no_ends_and_empty():
+    """A window without an end (every chain runs to the bootstrap), all-skipped lanes, and windows of no steps or lanes."""
+    gen = torch.Generator().manual_seed(3)
+    r, st, pl, v, b = _window(gen, 96, 70, 2, torch.float32, ends=0.0)
+    st[:] = 1
+    st[:, 7] = 3
+    v = torch.randn(96, 70, generator=gen)
+    got = policy.advantages(*(t.to(DEV) for t in (r, st, pl, v, b)), gamma=0.99, lam=0.95)
+    want = oracle.advantages(r.numpy(), st.numpy(), pl.numpy(), _np(v), _np(b), 0.99, 0.95)
+    for g, w in zip(got, want):
+        _close(g.cpu().numpy(), w, 4 * 96 * H * 96 * 11, "no ends")
+        assert not g[:, 7].any()
+    z = lambda *s, d: torch.zeros(*s, dtype=d, device=DEV)  # noqa: E731
+    for T, B in ((0, 5), (5, 0)):
+        a, t = policy.advantages(z(T, B, 2, d=torch.int8), z(T, B, d=torch.uint8), z(T, B, d=torch.int8), z(T, B, d=torch.float32))
+        assert a.shape == t.shape == (T, B)
+
+
+# ------------------------------------------------------------ policy loss
+def _policy_inputs(seed, n, A, dtype, move=0.3):
+    gen = torch.Generator().manual_seed(seed)
+    x, mask, actions = _table(gen, n, A, dtype)
+    ref = (x.float() + 0.4 * torch.randn(n, A, generator=gen)).to(dtype)
+    old, adv = torch.full((n,), math.nan), torch.full((n,), math.inf)
+    for i in range(n):
+        legal = oracle.legal_actions(mask[i], A)
+        if int(actions[i]) in legal:
+            lp = oracle.log_softmax(_np(x)[i], legal)
+            old[i] = lp[int(actions[i])] + move * float(torch.randn((), generator=gen))
+            adv[i] = float(torch.randn((), generator=gen)) if i % 5 else 0.0
+    return x, mask, actions, ref, old, adv
+
+
+def _check_policy(got, o, x, mask, dtype):
+    z = _reach(x, mask)
+    loss, stats, count, log_probs = got[:4]
+    assert int(count) == o["count"]
+    _close(log_probs.cpu().numpy(), o["log_probs"], _logp_tol(o["log_probs"]), "log_probs")
+    row = 8 * (48 + 2 * z) * H
+    tol = (row + 16 * H) * (o["mass"] + np.array([0, 2 * z, z, 0]))
+    _close(stats.cpu().numpy(), o["stats"], tol + H * np.abs(o["stats"]), "stats")
+    _close(loss.item(), o["loss"], tol.sum() + H * abs(o["loss"]), "loss")
+    if len(got) > 4:
+        assert got[4].dtype == dtype
+        _close(_np(got[4]), o["grad"], _grad_tol(o, z, dtype), "grad")
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=lambda d: str(d)[6:])
+@pytest.mark.parametrize("n,A,with_ref,with_active", [(1, 18, True, False), (2, 1, True, True), (65, 18, False, False),
+                                                      (257, 18, True, True), (300, 5, True, False), (700, 31, True, True),
+                                                      (513, 16, False, True), (4099, 18, True, False)])
+def test_policy_loss(n, A, with_ref, with_active, dtype):
+    x, mask, actions, ref, old, adv = _policy_inputs(n + A, n, A, dtype)
+    active = (torch.arange(n) % 3 != 1) if with_active else None
+    kl, ent = (0.3, 0.05) if with_ref else (0.0, 0.05)
+    o = oracle.policy(_np(x), actions.numpy(), mask.numpy(), _np(old), _np(adv), _np(ref) if with_ref else None,
+                      None if active is None else active.numpy(), 0.2, 0.3, kl, ent)
+    d = lambda t: None if t is None else t.to(DEV)  # noqa: E731
+    args = [d(t) for t in (x, actions, mask, old, adv)]
+    kw = dict(ref_logits=d(ref) if with_ref else None, active=d(active), clip_low=0.2, clip_high=0.3, kl_coef=kl,
+              entropy_coef=ent)
+    both = policy.policy_loss_and_grad(*args, **kw)
+    _check_policy(both, o, x, mask, dtype)
+    only = policy.policy_loss(*args, **kw)
+    for a, b in zip(only, both):
+        assert torch.equal(a, b)
+    # through autograd: the derivative that comes in scales the gradient
+    leaf = args[0].clone().requires_grad_()
+    out = policy.policy_loss(leaf, *args[1:], **kw)
+    grad, = torch.autograd.grad(out.loss, leaf, retain_graph=True)
+    assert torch.equal(grad, both.grad)
+    again, = torch.autograd.grad(out.loss * -4.0, leaf)
+    assert torch.equal(again, (both.grad.float() * -4.0).to(dtype)) and torch.equal(grad, both.grad)
+    with pytest.raises(RuntimeError, match="backward through the graph a second time|already been freed"):
+        torch.autograd.grad(out.loss, leaf)
+
+
+def test_policy_clip_borders():
+    """Ratios on and next to both borders, told apart in 64 bits; clip widths of 0 and a low of 1."""
+    A = 18
+    gen = torch.Generator().manual_seed(8)
+    x = torch.randn(400, A, generator=gen)
+    mask = torch.full((400,), (1 << A) - 1, dtype=torch.int32)
+    actions = (torch.arange(400) % A).to(torch.int8)
+    lp = np.array([oracle.log_softmax(_np(x)[i], list(range(A)))[int(actions[i])] for i in range(400)])
+    adv = torch.where(torch.arange(400) % 2 == 0, 1.0, -1.0)
+    for low, high in ((0.2, 0.2), (0.0, 0.0), (1.0, 0.5)):
+        edge = np.where(adv.numpy() > 0, math.log1p(high), math.log1p(-low) if low < 1 else -20.0)
+        old = torch.tensor(lp - edge).float()
+        step = torch.arange(400) // 2 % 5 - 2  # some 32-bit steps to either side
+        old = torch.tensor(np.array([np.float32(v) + np.float32(k) * np.spacing(np.float32(v)) for v, k in
+                                     zip(old.numpy(), step.numpy())]))
+        o = oracle.policy(_np(x), actions.numpy(), mask.numpy(), _np(old), _np(adv), None, None, low, high, 0.0, 0.0)
+        got = policy.policy_loss_and_grad(*(t.to(DEV) for t in (x, actions, mask, old, adv)), clip_low=low, clip_high=high)
+        assert 0 < o["stats"][3] < 1
+        assert float(got.stats[3]) == np.float32(o["stats"][3])
+        _check_policy(got, o, x, mask, torch.float32)
+
+
+def test_policy_nothing_counts_and_extremes():
+    """No decision: zeros.  A zero advantage beside an overflowing ratio: zero.  A legal -inf logit: no share and no
+    gradient.  A reference without a share: an infinite KL."""
+    n, A = 70, 18
+    x, mask, actions, ref, old, adv = (t.to(DEV) for t in _policy_inputs(4, n, A, torch.float32))
+    got = policy.policy_loss_and_grad(x, torch.full_like(actions, -1), mask, old, adv, ref_logits=ref, kl_coef=0.1)
+    assert float(got.loss) == 0 and int(got.count) == 0 and not got.stats.any() and not got.grad.any() and not got.log_probs.any()
+    none = policy.policy_loss_and_grad(x[:0], actions[:0], mask[:0], old[:0], adv[:0])
+    assert float(none.loss) == 0 and int(none.count) == 0 and none.grad.shape == (0, A)
+    y = torch.zeros(2, 3, device=DEV)
+    y[1, 2] = -math.inf
+    seven = torch.full((2,), 7, dtype=torch.int32, device=DEV)
+    acts = torch.zeros(2, dtype=torch.int8, device=DEV)
+    z = policy.policy_loss_and_grad(y, acts, seven, torch.tensor([-1000.0, math.log(0.5)], device=DEV),
+                                    torch.tensor([0.0, 1.0], device=DEV))
+    want = oracle.policy(_np(y), acts.cpu().numpy(), [7, 7], [-700.0, math.log(0.5)], [0.0, 1.0], None, None, 0.2, 0.2, 0, 0)
+    _close(_np(z.grad), want["grad"], 500 * H, "grad")
+    _close(float(z.loss), want["loss"], 100 * H, "loss")
+    assert not z.grad[0].any() and float(z.grad[1, 2]) == 0
+    r = torch.zeros(2, 3, device=DEV)
+    r[0, 1] = -math.inf
+    k = policy.policy_loss(torch.zeros(2, 3, device=DEV), acts, seven, torch.zeros(2, device=DEV), torch.ones(2, device=DEV),
+                           ref_logits=r, kl_coef=0.1)
+    assert float(k.stats[1]) == math.inf and float(k.loss) == math.inf
+
+
+def test_policy_layouts():
+    """Strided and expanded logits, 3-d leading shapes, uint8 and strided `active`: the contiguous call's results."""
+    n, A = 128, 18
+    x, mask, actions, ref, old, adv = (t.to(DEV) for t in _policy_inputs(6, n, A, torch.bfloat16))
+    active = (torch.arange(n, device=DEV) % 4 != 0)
+    base = policy.policy_loss_and_grad(x, actions, mask, old, adv, ref_logits=ref, active=active, kl_coef=0.1)
+    wide = torch.full((n, 2, 40), math.nan, dtype=x.dtype, device=DEV)
+    wide[:, 0, 1:19], wide[:, 1, 5:23] = x, ref
+    pair = torch.zeros(n, 2, dtype=torch.uint8, device=DEV)
+    pair[:, 1] = active
+    got = policy.policy_loss_and_grad(wide[:, 0, 1:19], actions, mask, old, adv, ref_logits=wide[:, 1, 5:23],
+                                      active=pair[:, 1], kl_coef=0.1)
+    for a, b in zip(got, base):
+        assert torch.equal(a, b)
+    lead = [t.view(8, 16, *t.shape[1:]) for t in (x, actions, mask, old, adv)]
+    got = policy.policy_loss_and_grad(*lead, ref_logits=ref.view(8, 16, A), active=active.view(8, 16), kl_coef=0.1)
+    assert got.grad.shape == (8, 16, A) and torch.equal(got.grad.view(n, A), base.grad) and torch.equal(got.loss, base.loss)
+    # one row of logits for every decision: its gradient is the rows' sum
+    row = torch.randn(A, device=DEV, requires_grad=True)
+    words = torch.full((n,), (1 << A) - 1, dtype=torch.int32, device=DEV)
+    acts = (torch.arange(n, device=DEV) % A).to(torch.int8)
+    flat = torch.full((n,), -2.0, device=DEV)
+    policy.policy_loss(row.expand(n, A), acts, words, flat, torch.ones(n, device=DEV)).loss.backward()
+    each = policy.policy_loss_and_grad(row.detach().expand(n, A).contiguous(), acts, words, flat, torch.ones(n, device=DEV))
+    assert torch.allclose(row.grad, each.grad.sum(0), atol=1e-6)
+
+
+def test_policy_refusals():
+    n, A = 8, 18
+    x, mask, actions, ref, old, adv = (t.to(DEV) for t in _policy_inputs(1, n, A, torch.float32))
+    ok = dict(logits=x, actions=actions, legal_mask=mask, old_log_probs=old, advantages=adv)
+    for kw, why in ((dict(logits=x.double()), "float32"), (dict(logits=torch.zeros(n, 32, device=DEV)), "1..31"),
+                    (dict(actions=actions.long()), "int8"), (dict(actions=actions[:3]), "shape"),
+                    (dict(legal_mask=mask.long()), "int32"), (dict(old_log_probs=old.half()), "float32"),
+                    (dict(advantages=adv.cpu()), "is on cpu"), (dict(ref_logits=ref.half()), "type and shape"),
+                    (dict(ref_logits=ref[:2]), "type and shape"), (dict(active=actions), "bool"),
+                    (dict(clip_low=1.5), "clip_low"), (dict(clip_high=-0.1), "clip"), (dict(kl_coef=math.inf), "finite"),
+                    (dict(entropy_coef=math.nan), "finite"),
+                    (dict(old_log_probs=old.clone().requires_grad_()), "held constant"),
+                    (dict(ref_logits=ref.clone().requires_grad_()), "held constant")):
+        with pytest.raises(ValueError, match=why):
+            policy.policy_loss(**{**ok, **kw})
+    with pytest.raises(ValueError, match="held constant"):
+        policy.advantages(torch.zeros(1, 1, 2, dtype=torch.int8, device=DEV), torch.zeros(1, 1, dtype=torch.uint8, device=DEV),
+                          torch.zeros(1, 1, dtype=torch.int8, device=DEV), torch.zeros(1, 1, device=DEV),
+                          torch.zeros(1, 2, device=DEV, requires_grad=True))
+
+
+# ------------------------------------------------------------ preference loss
+def _check_preference(got, o, x, mask, beta, dtype):
+    z = _reach(x, mask)
+    each = 2 * (48 + 4 * z) * H  # a row's log ratio
+    tol = abs(beta) * each * o["length"]
+    _close(got[1].cpu().numpy(), o["rewards"], tol + H * np.abs(o["rewards"]), "rewards")
+    # a pair's cost changes by less than its difference's error
+    _close(got[0].item(), o["loss"], 2 * tol.max(initial=0.0) + H * abs(o["loss"]), "loss")
+    if len(got) > 2:
+        # so does its derivative, relative to sigma's own slope (at most itself): size (x error + softmax error)
+        info = torch.finfo(dtype)
+        lim = (8 * (48 + 2 * z) * H + 2 * tol.max(initial=0.0)) * o["size"] + info.eps / 2 * np.abs(o["grad"])
+        _close(_np(got[2]), o["grad"], lim + info.smallest_normal * info.eps / 2, "grad")
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=lambda d: str(d)[6:])
+@pytest.mark.parametrize("offsets,n,A", [([0, 1, 2], 2, 18), ([0, 0, 0], 3, 18), ([2, 30, 64, 64, 97], 101, 18),
+                                         ([0, 300, 1300], 1300, 18), ([0] + [7 * k + k % 3 for k in range(1, 129)], 930, 5),
+                                         ([0, 0, 900, 900, 1800], 1803, 31), ([0], 4, 18)], ids=lambda v: str(v)[:18])
+@pytest.mark.parametrize("with_ref,eps", [(True, 0.0), (False, 0.2)])
+def test_preference_loss(offsets, n, A, with_ref, eps, dtype):
+    gen = torch.Generator().manual_seed(n + A)
+    x, mask, actions = _table(gen, n, A, dtype)
+    ref = (x.float() + 0.5 * torch.randn(n, A, generator=gen)).to(dtype) if with_ref else None
+    beta = 0.3 if with_ref else 0.02
+    o = oracle.preference(_np(x), actions.numpy(), mask.numpy(), offsets, None if ref is None else _np(ref), beta, eps)
+    kw = dict(ref_logits=None if ref is None else ref.to(DEV), beta=beta, label_smoothing=eps)
+    for itype in (torch.int32, torch.int64):
+        args = [x.to(DEV), actions.to(DEV), mask.to(DEV), torch.tensor(offsets, dtype=itype, device=DEV)]
+        both = policy.preference_loss_and_grad(*args, **kw)
+        _check_preference(both, o, x, mask, beta, dtype)
+        for a, b in zip(policy.preference_loss(*args, **kw), both):
+            assert torch.equal(a, b)
+    leaf = args[0].clone().requires_grad_()
+    out = policy.preference_loss(leaf, *args[1:], **kw)
+    grad, = torch.autograd.grad(out.loss, leaf, retain_graph=True)
+    assert torch.equal(grad, both.grad)
+    again, = torch.autograd.grad(out.loss * 2.0, leaf)
+    assert torch.equal(again, (both.grad.float() * 2.0).to(dtype))
+
+
+def test_preference_extreme_margins_and_bad_offsets():
+    """Margins far past exp's range keep a finite loss; offsets that run backwards or out of the rows make the loss NaN
+    and read nothing outside (the kernels clamp every offset to the rows)."""
+    A, n = 18, 400
+    gen = torch.Generator().manual_seed(2)
+    x, mask, actions = _table(gen, n, A, torch.float32)
+    for beta in (50.0, -50.0):
+        o = oracle.preference(_np(x), actions.numpy(), mask.numpy(), [0, 100, 400], None, beta, 0.1)
+        got = policy.preference_loss_and_grad(x.to(DEV), actions.to(DEV), mask.to(DEV),
+                                              torch.tensor([0, 100, 400], device=DEV), beta=beta, label_smoothing=0.1)
+        assert abs(o["rewards"][0] - o["rewards"][1]) > 800
+        _check_preference(got, o, x, mask, beta, torch.float32)
+    for bad in ([0, 300, 200], [0, 100, 500], [-5, 100, 200], [0, 1 << 30, 400]):
+        got = policy.preference_loss_and_grad(x.to(DEV), actions.to(DEV), mask.to(DEV), torch.tensor(bad, device=DEV))
+        assert math.isnan(float(got.loss)), bad
+
+
+def test_preference_refusals():
+    x = torch.zeros(6, 18, device=DEV)
+    m, a = torch.zeros(6, dtype=torch.int32, device=DEV), torch.zeros(6, dtype=torch.int8, device=DEV)
+    off = torch.tensor([0, 3, 6], device=DEV)
+    for args, kw, why in (((x.view(2, 3, 18), a, m, off), {}, "rows, A"), ((x, a, m, off[:2]), {}, "2 \\* pairs"),
+                          ((x, a, m, off.float()), {}, "int32"), ((x, a, m, off.cpu()), {}, "is on cpu"),
+                          ((x, a, m, off), dict(beta=math.inf), "beta"),
+                          ((x, a, m, off), dict(label_smoothing=0.7), "label_smoothing")):
+        with pytest.raises(ValueError, match=why):
+            policy.preference_loss(*args, **kw)
+
+
+# ------------------------------------------------------------ graphs
+def test_graph_replays_of_every_call():
+    """Each call captured once and replayed over new inputs, eager work and synchronisations in between: every replay
+    equals the eager call."""
+    n, A, T, B = 3000, 18, 96, 40
+    fresh = []
+    for seed in range(4):
+        x, mask, actions, ref, old, adv = (t.to(DEV) for t in _policy_inputs(seed, n, A, torch.float32))
+        gen = torch.Generator().manual_seed(seed)
+        win = [t.to(DEV) for t in _window(gen, T, B, 2, torch.float32)]
+        u = torch.rand(n, generator=gen).to(DEV)
+        off = torch.randint(0, n + 1, (9,), generator=gen).sort().values.to(DEV)
+        fresh.append([x, mask, actions, ref, old, adv, u, off, *win])
+    held = [t.clone() for t in fresh[0]]
+
+    def everything(x, mask, actions, ref, old, adv, u, off, *win):
+        return [*policy.sample_actions(x, mask, u), *policy.advantages(*win, gamma=0.99, lam=0.9),
+                *policy.policy_loss_and_grad(x, actions, mask, old, adv, ref_logits=ref, kl_coef=0.1, entropy_coef=0.01),
+                *policy.policy_loss(x, actions, mask, old, adv),
+                *policy.preference_loss_and_grad(x, actions, mask, off, ref_logits=ref)]
+
+    everything(*held)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        outs = everything(*held)
+    for k in (0, 1, 2, 3, 1):
+        for h, f in zip(held, fresh[k]):
+            h.copy_(f)
+        g.replay()
+        got = [o.clone() for o in outs]
+        torch.cuda.synchronize()
+        want = everything(*fresh[k])
+        for i, (a, b) in enumerate(zip(got, want)):
+            assert torch.equal(a.nan_to_num(3), b.nan_to_num(3)), (k, i)
+
+
+def test_captured_autograd_is_refused():
+    """A loss whose logits require a gradient raises under capture, before anything is enqueued; so does the captured
+    backward of an eager loss."""
+    n, A = 64, 18
+    x, mask, actions, ref, old, adv = (t.to(DEV) for t in _policy_inputs(3, n, A, torch.float32))
+    leaf = x.clone().requires_grad_()
+    policy.policy_loss(x, actions, mask, old, adv)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    said = None
+    with torch.cuda.graph(g):
+        y = x * 1.0
+        try:
+            policy.policy_loss(leaf, actions, mask, old, adv)
+        except RuntimeError as e:
+            said = str(e)
+        with torch.no_grad():
+            kept = policy.policy_loss(leaf, actions, mask, old, adv)
+    assert said and "_and_grad" in said
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(kept.loss, policy.policy_loss(x, actions, mask, old, adv).loss) and torch.equal(y.nan_to_num(2), x.nan_to_num(2))
+
+
+# ------------------------------------------------------------ a run of them
+@pytest.mark.parametrize("players", [2, 4])
+def test_a_learners_round(players):
+    """Trajectories played by a policy, advantages over them, policy updates on their rows, and the finished games'
+    winners against losers -- every number checked against the oracle."""
+    B, T = 96, 40
+    env = BatchedCoupEnv(B, seed=11, auto_reset=True, obs=True, num_players=players)
+    torch.manual_seed(0)
+    net = torch.nn.Linear(env.obs_size, 18 + 1, device=DEV)
+
+    def act(ts):
+        seat = ts["current_player"].long()
+        seen = ts["obs"][torch.arange(B, device=DEV), seat]
+        out = net(seen).detach()
+        return out[:, :18], out[:, 18]
+
+    gen = torch.Generator(DEV).manual_seed(1)
+    buf = env.collect_policy_trajectory(T, act, generator=gen)
+    assert env.error_count() == 0
+    mask, actions, old = buf["decision_mask"], buf["actions"], buf["log_probs"]
+    assert ((mask >> actions.int()) & 1).all()
+    seat = buf["decision_player"].long()
+    seen = buf["decision_obs"].gather(2, seat[:, :, None, None].expand(T, B, 1, env.obs_size))[:, :, 0]
+    logits = net(seen)[:, :, :18]
+    adv, target = policy.advantages(buf["rewards"], buf["step_type"], buf["decision_player"], buf["values"], gamma=0.99)
+    wa, wt = oracle.advantages(*(buf[k].cpu().numpy() for k in ("rewards", "step_type", "decision_player")),
+                               _np(buf["values"]), None, 0.99, 0.95)
+    _close(adv.cpu().numpy(), wa, 4 * T * H * T * 10, "advantages")
+    ref = (logits.detach() + 0.1 * torch.randn(T, B, 18, device=DEV))
+    out = policy.policy_loss(logits, actions, mask, old, adv, ref_logits=ref, kl_coef=0.1, entropy_coef=0.01)
+    out.loss.backward()
+    assert int(out.count) == T * B
+    flat = lambda t: _np(t.detach()).reshape(T * B, -1)  # noqa: E731
+    o = oracle.policy(flat(logits), actions.flatten().cpu().numpy(), mask.flatten().cpu().numpy(), _np(old).ravel(),
+                      _np(adv).ravel(), flat(ref), None, 0.2, 0.2, 0.1, 0.01)
+    z = _reach(logits.detach().reshape(T * B, 18).cpu(), mask.flatten().cpu())
+    assert abs(float(out.loss.detach()) - o["loss"]) <= 8 * (48 + 2 * z) * H * (o["mass"].sum() + 3 * z)
+    want = torch.tensor(o["grad"].T @ flat(seen))  # d loss / d weight
+    size = torch.tensor(o["size"].T @ np.abs(flat(seen)))
+    got = net.weight.grad[:18].double().cpu()
+    # a product over T B rows of 32-bit numbers
+    assert ((got - want).abs() <= (8 * (48 + 2 * z) * H + T * B * H) * size + 1e-12).all()
+    # the finished games' winners against losers
+    last = (buf["step_type"] == 2).cpu()
+    rows, offsets, start = [], [0], torch.zeros(B, dtype=torch.long)
+    p_of, r_of = buf["decision_player"].cpu(), buf["rewards"].cpu().long()
+    for b in range(B):
+        begin = 0
+        for t in torch.nonzero(last[:, b]).flatten().tolist():
+            gain = r_of[begin:t + 1, b].sum(0)
+            best, worst = int(gain.argmax()), int(gain.argmin())
+            for who in (best, worst):
+                rows += [s * B + b for s in range(begin, t + 1) if int(p_of[s, b]) == who]
+                offsets.append(len(rows))
+            begin = t + 1
+    assert len(offsets) > 5
+    pick = torch.tensor(rows, device=DEV)
+    packed = net(seen.reshape(T * B, -1)[pick])[:, :18]
+    chosen = [t.flatten()[pick] for t in (actions, mask)]
+    pr = policy.preference_loss(packed, *chosen, torch.tensor(offsets, device=DEV), beta=0.2)
+    po = oracle.preference(_np(packed), chosen[0].cpu().numpy(), chosen[1].cpu().numpy(), offsets, None, 0.2, 0.0)
+    _check_preference(pr, po, packed.detach().cpu(), chosen[1].cpu(), 0.2, torch.float32)
+    net.zero_grad()
+    pr.loss.backward()
+    assert torch.isfinite(net.weight.grad).all() and net.weight.grad.abs().sum() > 0

@@ -1,0 +1,191 @@
+"""The learner-side operators without a GPU: the oracle's gradients against
+differences of its losses, and what the C entry points refuse before they
+make any HIP call."""
+import ctypes
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from open_spiel_coup_amd import _native, policy
+from tests import policy_oracle as oracle
+
+
+def _rows(rng, n, A):
+    logits = rng.normal(size=(n, A)) * 2
+    mask = np.array([int(sum(1 << a for a in range(A) if rng.random() < 0.5)) | (1 << int(rng.integers(A)))
+                     for _ in range(n)], np.int64)
+    actions = np.array([rng.choice(oracle.legal_actions(m, A)) for m in mask], np.int8)
+    return logits, mask, actions
+
+
+def test_policy_oracle_gradient_is_its_losss_difference():
+    rng = np.random.default_rng(0)
+    n, A = 9, 5
+    logits, mask, actions = _rows(rng, n, A)
+    mask[2], actions[3] = 0, -1
+    ref = logits + rng.normal(size=logits.shape)
+    old, adv = rng.normal(size=n) * 0.2 - 1.0, rng.normal(size=n)
+    args = (actions, mask, old, adv, ref, None, 0.2, 0.3, 0.7, 0.4)
+    got = oracle.policy(logits, *args)
+    assert got["count"] == 7 and 0 < got["stats"][3] < 1
+    h = 1e-6
+    for i in range(n):
+        for a in range(A):
+            up, down = logits.copy(), logits.copy()
+            up[i, a] += h
+            down[i, a] -= h
+            slope = (oracle.policy(up, *args)["loss"] - oracle.policy(down, *args)["loss"]) / (2 * h)
+            # second derivatives stay below ~1 and 64-bit loss values carry ~1e-16 / h
+            assert abs(slope - got["grad"][i, a]) < 1e-8, (i, a)
+
+
+def test_preference_oracle_gradient_is_its_losss_difference():
+    rng = np.random.default_rng(1)
+    n, A = 11, 4
+    logits, mask, actions = _rows(rng, n, A)
+    mask[1] = 0
+    ref = logits + rng.normal(size=logits.shape)
+    args = (actions, mask, [0, 3, 3, 6, 9], ref, 0.6, 0.1)
+    got = oracle.preference(logits, *args)
+    h = 1e-6
+    for i in range(n):
+        for a in range(A):
+            up, down = logits.copy(), logits.copy()
+            up[i, a] += h
+            down[i, a] -= h
+            slope = (oracle.preference(up, *args)["loss"] - oracle.preference(down, *args)["loss"]) / (2 * h)
+            assert abs(slope - got["grad"][i, a]) < 1e-8, (i, a)
+    assert not got["grad"][9:].any()
+
+
+def test_advantage_oracle_on_a_written_out_game():
+    """Two players, three decisions: player 0 at steps 0 and 2, player 1 at 1;
+    step 2 ends the game."""
+    rewards = np.array([[[0, 0]], [[-1, 1]], [[1, -1]]], np.int8)
+    v = np.array([[0.5], [0.25], [-0.5]])
+    adv, target = oracle.advantages(rewards, np.array([[1], [1], [2]]), np.array([[0], [1], [0]]), v, None, 0.9, 0.5)
+    a2 = 1 - (-0.5)
+    a1 = (1 - 1) - 0.25
+    a0 = (0 - 1) + 0.9 * -0.5 - 0.5 + 0.45 * a2
+    assert np.allclose(adv[:, 0], [a0, a1, a2]) and np.allclose(target, adv + v)
+
+
+F = ctypes.c_void_p(4096)  # never dereferenced: every call below fails first
+
+
+def _decisions(**kw):
+    d = dict(logits=F, logits_stride=18, ref_logits=None, ref_stride=0, actions=F, legal_mask=F, rows=4, num_actions=18,
+             dtype=_native.DTYPE_F32)
+    d.update(kw)
+    return _native.Decisions(*d.values())
+
+
+BAD_DECISIONS = [(dict(rows=-1), b"rows"), (dict(num_actions=0), b"num_actions"), (dict(num_actions=32), b"num_actions"),
+                 (dict(dtype=3), b"dtype"), (dict(logits=None), b"null"), (dict(legal_mask=None), b"null"),
+                 (dict(logits_stride=17), b"stride")]
+
+
+def _terms(**kw):
+    t = dict(old_log_probs=F, advantages=F, active=None, clip_low=0.2, clip_high=0.2, kl_coef=0.0, entropy_coef=0.0)
+    t.update(kw)
+    return _native.PolicyTerms(*t.values())
+
+
+def _refused(rc, what):
+    L = _native.load()
+    assert rc == _native.COUP_E_INVALID and what in L.coup_last_error(), L.coup_last_error()
+
+
+@pytest.mark.parametrize("bad,why", BAD_DECISIONS, ids=lambda x: str(x))
+def test_decisions_are_checked_by_every_entry(bad, why):
+    L = _native.load()
+    d = _decisions(**bad)
+    _refused(L.coup_sample_actions(ctypes.byref(d), F, F, F, None), why)
+    out = _native.PolicyOutputs(F, None, None, None, None)
+    _refused(L.coup_policy_loss(ctypes.byref(d), ctypes.byref(_terms()), ctypes.byref(out), F, 1 << 20, None), why)
+    pt, po = _native.PreferenceTerms(F, 4, 1, 0.1, 0.0), _native.PreferenceOutputs(F, None, None)
+    _refused(L.coup_preference_loss(ctypes.byref(d), ctypes.byref(pt), ctypes.byref(po), F, 1 << 20, None), why)
+
+
+def test_sample_refusals():
+    L = _native.load()
+    _refused(L.coup_sample_actions(None, F, F, F, None), b"null")
+    d = _decisions()
+    _refused(L.coup_sample_actions(ctypes.byref(d), None, F, F, None), b"uniform")
+    _refused(L.coup_sample_actions(ctypes.byref(d), F, None, F, None), b"actions")
+    assert L.coup_sample_actions(ctypes.byref(_decisions(rows=0, logits=None)), None, None, None, None) == _native.COUP_OK
+
+
+def test_advantage_refusals():
+    L = _native.load()
+
+    def call(gamma=0.9, lam=0.9, adv=F, target=F, **kw):
+        w = dict(rewards=F, step_type=F, players=F, values=F, bootstrap=None, steps=2, lanes=3, num_players=2, dtype=0)
+        w.update(kw)
+        return L.coup_advantages(ctypes.byref(_native.Window(*w.values())), gamma, lam, adv, target, None)
+
+    for kw, why in ((dict(steps=-1), b"steps"), (dict(lanes=-1), b"lanes"), (dict(steps=1 << 30, lanes=1 << 30), b"range"),
+                    (dict(num_players=1), b"num_players"), (dict(num_players=7), b"num_players"), (dict(dtype=9), b"dtype"),
+                    (dict(gamma=1.5), b"gamma"), (dict(lam=-0.1), b"gamma"), (dict(gamma=math.nan), b"gamma"),
+                    (dict(rewards=None), b"null"), (dict(values=None), b"null"), (dict(adv=None), b"null"),
+                    (dict(target=None), b"null")):
+        _refused(call(**kw), why)
+    assert call(steps=0, rewards=None) == _native.COUP_OK and call(lanes=0) == _native.COUP_OK
+
+
+def test_policy_refusals():
+    L = _native.load()
+
+    def call(d=None, out=None, ws=F, nbytes=1 << 20, **kw):
+        d, out = d or _decisions(), out or _native.PolicyOutputs(F, None, None, None, None)
+        return L.coup_policy_loss(ctypes.byref(d), ctypes.byref(_terms(**kw)), ctypes.byref(out), ws, nbytes, None)
+
+    for kw, why in ((dict(old_log_probs=None), b"old_log_probs"), (dict(advantages=None), b"advantages"),
+                    (dict(clip_low=-0.1), b"clip"), (dict(clip_low=1.1), b"clip"), (dict(clip_high=math.inf), b"clip"),
+                    (dict(clip_high=-1.0), b"clip"), (dict(kl_coef=math.nan), b"kl_coef"),
+                    (dict(entropy_coef=math.inf), b"entropy_coef"), (dict(ws=None), b"workspace"),
+                    (dict(ws=ctypes.c_void_p(4100)), b"workspace"), (dict(nbytes=8), b"workspace"),
+                    (dict(d=_decisions(actions=None)), b"actions"),
+                    (dict(d=_decisions(ref_logits=F, ref_stride=3)), b"ref_stride"),
+                    (dict(out=_native.PolicyOutputs(None, None, None, None, None)), b"loss")):
+        _refused(call(**kw), why)
+
+
+def test_preference_refusals():
+    L = _native.load()
+
+    def call(ws=F, nbytes=1 << 20, loss=F, **kw):
+        t = dict(offsets=F, offset_bytes=4, pairs=1, beta=0.1, label_smoothing=0.0)
+        t.update(kw)
+        return L.coup_preference_loss(ctypes.byref(_decisions()), ctypes.byref(_native.PreferenceTerms(*t.values())),
+                                      ctypes.byref(_native.PreferenceOutputs(loss, None, None)), ws, nbytes, None)
+
+    for kw, why in ((dict(offsets=None), b"offsets"), (dict(offset_bytes=2), b"offset_bytes"), (dict(pairs=-1), b"pairs"),
+                    (dict(beta=math.nan), b"beta"), (dict(label_smoothing=0.6), b"label_smoothing"),
+                    (dict(label_smoothing=-0.1), b"label_smoothing"), (dict(nbytes=8), b"workspace"),
+                    (dict(ws=None), b"workspace"), (dict(loss=None), b"loss")):
+        _refused(call(**kw), why)
+
+
+def test_scale_refusals():
+    L = _native.load()
+    _refused(L.coup_scale_grad(F, 7, 1, F, None), b"dtype")
+    _refused(L.coup_scale_grad(F, 0, -1, F, None), b"negative")
+    _refused(L.coup_scale_grad(None, 0, 1, F, None), b"null")
+    assert L.coup_scale_grad(None, 0, 0, None, None) == _native.COUP_OK
+
+
+def test_python_refuses_host_tensors():
+    x, m = torch.zeros(3, 18), torch.zeros(3, dtype=torch.int32)
+    a = torch.zeros(3, dtype=torch.int8)
+    with pytest.raises(ValueError, match="HIP device"):
+        policy.sample_actions(x, m, torch.zeros(3))
+    with pytest.raises(ValueError, match="HIP device"):
+        policy.policy_loss(x, a, m, torch.zeros(3), torch.zeros(3))
+    with pytest.raises(ValueError, match="HIP device"):
+        policy.preference_loss(x, a, m, torch.zeros(3, dtype=torch.int32))
+    with pytest.raises(ValueError, match="HIP device"):
+        policy.advantages(torch.zeros(2, 3, 2, dtype=torch.int8), torch.zeros(2, 3, dtype=torch.uint8),
+                          torch.zeros(2, 3, dtype=torch.int8), torch.zeros(2, 3))
