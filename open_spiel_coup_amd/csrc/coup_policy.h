@@ -9,7 +9,7 @@
 // never computed on, so whatever their logits, old log probabilities and
 // advantages hold cannot reach an output.  One thread works on one row, whose
 // logits it keeps in registers, padded to AP (an illegal or padded action is
-// -inf, which every sum below takes as 0).
+// -inf, which every sum below takes as 0); a block's 256 rows go through LDS.
 //
 // Arithmetic: logits are widened to 32 bits on load; the softmax statistics,
 // the log probabilities and the gradient are 32-bit; sums over rows are
@@ -27,6 +27,8 @@
 
 namespace coup {
 namespace policy {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kRowThreads = 256;
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -57,14 +59,199 @@ __device__ __forceinline__ bool decided(uint32_t legal, int action) {
   return action >= 0 && action < 31 && ((legal >> action) & 1u);
 }
 
-// One row's logits, -inf at actions outside `legal`.
+// ------------------------------------------------- rows through the LDS
+//
+// A block's 256 rows are one run of memory when the table is contiguous, so
+// its threads copy it in 16-byte pieces, all of them issued before the first
+// is used, into LDS, and each thread then reads its own row from there (72
+// bytes apart for the game's 18 float logits; read straight from memory those
+// loads touch 64 lines an instruction: the 4 x 2^20-row loss took 461 us that
+// way).  A gradient goes the same way back.  Strided or unaligned tables are
+// copied by elements.
+//
+// LDS: element j of row r is at byte (r A + j) sizeof(T), so a wave's lanes
+// read words A sizeof(T) / 4 apart: for odd multiples of 4 or 8 bytes at most
+// two lanes meet in a bank.  Rows that are multiples of 16 bytes (8, 16, 24
+// float logits...) would meet 8 or 16 deep; they are read in 16-byte pieces,
+// and piece k of the tile stands at place k ^ (k / 16 mod 16), which spreads
+// one column of pieces over the 16 places.
 template <class T, int AP>
-__device__ __forceinline__ void load_row(const T* row, int A, uint32_t legal, float (&x)[AP]) {
+struct Tile {
+  static constexpr int kPieces = (AP * (int)sizeof(T) + 15) / 16;  // 16-byte pieces a thread, at most
+  static constexpr int kBytes = kRowThreads * kPieces * 16 + 256;  // reads past a tile's last row stay inside
+  typedef T vec __attribute__((ext_vector_type(16 / sizeof(T))));
+
+  // 16-byte pieces (else elements) in memory; rows in whole pieces in LDS
+  static __device__ __forceinline__ bool in_pieces(const void* p, int64_t stride, int A) {
+    return stride == A && ((uintptr_t)p & 15) == 0;
+  }
+  static __device__ __forceinline__ bool whole(int A) { return (A * (int)sizeof(T)) % 16 == 0; }
+  static __device__ __forceinline__ int place(int k) { return k ^ ((k >> 4) & 15); }
+
+  // The block's rows [row0, row0 + rows) in flight to registers.
+  struct Flight {
+    u32x4 piece[kPieces];
+  };
+
+  static __device__ __forceinline__ void fetch(Flight& f, const T* base, int64_t row0, int rows, int A) {
+    const char* src = (const char*)(base + row0 * A);
+    const int bytes = rows * A * (int)sizeof(T);
 #pragma unroll
-  for (int a = 0; a < AP; ++a) {
-    float v = -INFINITY;
-    if (a < A) v = widen(row[a]);
-    x[a] = ((legal >> a) & 1u) ? v : -INFINITY;
+    for (int c = 0; c < kPieces; ++c) {
+      const int at = (c * kRowThreads + (int)threadIdx.x) * 16;
+      f.piece[c] = u32x4{0, 0, 0, 0};
+      if (at + 16 <= bytes) f.piece[c] = *(const u32x4*)(src + at);
+    }
+  }
+
+  static __device__ __forceinline__ void land(const Flight& f, char* lds, const T* base, int64_t row0, int rows, int A) {
+    const int bytes = rows * A * (int)sizeof(T);
+    const bool w = whole(A);
+#pragma unroll
+    for (int c = 0; c < kPieces; ++c) {
+      const int k = c * kRowThreads + (int)threadIdx.x;
+      if (k * 16 + 16 <= bytes) *(u32x4*)(lds + (w ? place(k) : k) * 16) = f.piece[c];
+    }
+    if (!w) {  // what is left of the last piece (whole rows leave none)
+      const int k = bytes / 16 * 16 / (int)sizeof(T) + (int)threadIdx.x;
+      if (k < rows * A) ((T*)lds)[k] = base[row0 * A + k];
+    }
+  }
+
+  // LDS byte of element e of the tile
+  static __device__ __forceinline__ int at_element(int e, int A) {
+    const int b = e * (int)sizeof(T);
+    return whole(A) ? place(b >> 4) * 16 + (b & 15) : b;
+  }
+
+  // The same through elements, for strided rows.
+  static __device__ __forceinline__ void copy_in(char* lds, const T* base, int64_t stride, int64_t row0, int rows, int A) {
+    const uint32_t inv = ((1u << 20) + A - 1) / A;  // e / A = e inv >> 20: e < 256 A, and e (A - 1) < 2^20
+    for (int e = (int)threadIdx.x; e < rows * A; e += kRowThreads) {
+      const int r = (int)((uint32_t)e * inv >> 20);
+      *(T*)(lds + at_element(e, A)) = base[(row0 + r) * stride + (e - r * A)];
+    }
+  }
+
+  // This thread's row, widened; -inf at actions outside `legal`.
+  static __device__ __forceinline__ void read(const char* lds, int A, uint32_t legal, float (&x)[AP]) {
+    const int r = (int)threadIdx.x;
+    if (whole(A)) {
+      const int k0 = r * A * (int)sizeof(T) / 16;
+#pragma unroll
+      for (int c = 0; c < kPieces; ++c) {
+        const vec v = *(const vec*)(lds + place(k0 + c) * 16);
+#pragma unroll
+        for (int j = 0; j < (int)(16 / sizeof(T)); ++j) {
+          const int a = c * (int)(16 / sizeof(T)) + j;
+          if (a < AP) x[a] = widen((T)v[j]);
+        }
+      }
+    } else if (sizeof(T) == 2 && !(A & 1)) {
+      typedef T two __attribute__((ext_vector_type(2)));
+      const two* row = (const two*)(lds + r * A * (int)sizeof(T));
+#pragma unroll
+      for (int a = 0; a < AP; a += 2) {
+        const two v = row[a / 2];
+        x[a] = widen((T)v[0]);
+        x[a + 1] = widen((T)v[1]);
+      }
+    } else {
+      const T* row = (const T*)lds + r * A;
+#pragma unroll
+      for (int a = 0; a < AP; ++a) x[a] = widen(row[a]);
+    }
+#pragma unroll
+    for (int a = 0; a < AP; ++a) x[a] = ((legal >> a) & 1u) ? x[a] : -INFINITY;
+  }
+
+  // This thread's row of results, rounded, over its row.
+  static __device__ __forceinline__ void write(char* lds, int A, const float (&g)[AP]) {
+    const int r = (int)threadIdx.x;
+    if (whole(A)) {
+      const int k0 = r * A * (int)sizeof(T) / 16;
+#pragma unroll
+      for (int c = 0; c < kPieces; ++c) {
+        vec v;
+#pragma unroll
+        for (int j = 0; j < (int)(16 / sizeof(T)); ++j) {
+          const int a = c * (int)(16 / sizeof(T)) + j;
+          v[j] = (T)(a < AP ? g[a < AP ? a : 0] : 0.0f);
+        }
+        if (c * (int)(16 / sizeof(T)) < A) *(vec*)(lds + place(k0 + c) * 16) = v;
+      }
+    } else if (sizeof(T) == 2 && !(A & 1)) {
+      typedef T two __attribute__((ext_vector_type(2)));
+      two* row = (two*)(lds + r * A * (int)sizeof(T));
+#pragma unroll
+      for (int a = 0; a < AP; a += 2)
+        if (a < A) row[a / 2] = two{(T)g[a], (T)g[a + 1]};
+    } else {
+      T* row = (T*)lds + r * A;
+#pragma unroll
+      for (int a = 0; a < AP; ++a)
+        if (a < A) row[a] = (T)g[a];
+    }
+  }
+
+  // The tile's rows out to a contiguous table.
+  static __device__ __forceinline__ void copy_out(const char* lds, T* base, int64_t row0, int rows, int A) {
+    const int n = rows * A, bytes = n * (int)sizeof(T);
+    T* dst = base + row0 * A;
+    int done = 0;
+    if (((uintptr_t)base & 15) == 0) {
+      const bool w = whole(A);
+#pragma unroll
+      for (int c = 0; c < kPieces; ++c) {
+        const int k = c * kRowThreads + (int)threadIdx.x;
+        if (k * 16 + 16 <= bytes) ((u32x4*)dst)[k] = *(const u32x4*)(lds + (w ? place(k) : k) * 16);
+      }
+      done = bytes / 16 * 16 / (int)sizeof(T);
+    }
+    for (int e = done + (int)threadIdx.x; e < n; e += kRowThreads) dst[e] = *(const T*)(lds + at_element(e, A));
+  }
+};
+
+// A block's rows of a table into LDS (its own: the caller keeps other
+// threads' uses of it apart with barriers).
+template <class T, int AP>
+__device__ __forceinline__ void stage(char* lds, const void* base, int64_t stride, int64_t row0, int rows, int A) {
+  using Tl = Tile<T, AP>;
+  if (Tl::in_pieces(base, stride, A)) {
+    typename Tl::Flight f;
+    Tl::fetch(f, (const T*)base, row0, rows, A);
+    Tl::land(f, lds, (const T*)base, row0, rows, A);
+  } else {
+    Tl::copy_in(lds, (const T*)base, stride, row0, rows, A);
+  }
+}
+
+// Two tables' rows through one tile: x, then (where `ref`) d.  Both are in
+// flight before the first is waited for.
+template <class T, int AP>
+__device__ __forceinline__ void stage_two(char* lds, const Rows& q, int64_t row0, int rows, uint32_t legal,
+                                          float (&x)[AP], float (&d)[AP]) {
+  using Tl = Tile<T, AP>;
+  const bool pieces = Tl::in_pieces(q.logits, q.stride, q.A) && Tl::in_pieces(q.ref, q.ref_stride, q.A);
+  if (pieces) {
+    typename Tl::Flight f, g;
+    Tl::fetch(f, (const T*)q.logits, row0, rows, q.A);
+    Tl::fetch(g, (const T*)q.ref, row0, rows, q.A);
+    Tl::land(f, lds, (const T*)q.logits, row0, rows, q.A);
+    __syncthreads();
+    Tl::read(lds, q.A, legal, x);
+    __syncthreads();
+    Tl::land(g, lds, (const T*)q.ref, row0, rows, q.A);
+    __syncthreads();
+    Tl::read(lds, q.A, legal, d);
+  } else {
+    Tl::copy_in(lds, (const T*)q.logits, q.stride, row0, rows, q.A);
+    __syncthreads();
+    Tl::read(lds, q.A, legal, x);
+    __syncthreads();
+    Tl::copy_in(lds, (const T*)q.ref, q.ref_stride, row0, rows, q.A);
+    __syncthreads();
+    Tl::read(lds, q.A, legal, d);
   }
 }
 
@@ -98,7 +285,7 @@ __device__ __forceinline__ Softmax softmax(float (&x)[AP], float (&e)[AP]) {
 
 // The same statistics of a row in 64 bits, for the rows next to a border.
 template <class T>
-__device__ __attribute__((noinline)) double lse64(const T* row, uint32_t legal, float m) {
+__device__ __forceinline__ double lse64(const T* row, uint32_t legal, float m) {
   double sum = 0.0;
 #pragma unroll 1
   for (uint32_t b = legal; b; b &= b - 1) sum += exp((double)widen(row[__builtin_ctz(b)]) - (double)m);
@@ -109,7 +296,7 @@ __device__ __attribute__((noinline)) double lse64(const T* row, uint32_t legal, 
 // sum passes u * total, in 64 bits; the last with a share where rounding
 // leaves the total at or below it.
 template <class T>
-__device__ __attribute__((noinline)) int pick64(const T* row, uint32_t legal, float m, float u) {
+__device__ __forceinline__ int pick64(const T* row, uint32_t legal, float m, float u) {
   double total = 0.0;
 #pragma unroll 1
   for (uint32_t b = legal; b; b &= b - 1) total += exp((double)widen(row[__builtin_ctz(b)]) - (double)m);
@@ -140,30 +327,35 @@ constexpr float kPickMargin = 7.62939453125e-6f;  // 2^-17
 template <class T, int AP>
 __global__ __launch_bounds__(kRowThreads) void k_sample(Rows r, const float* __restrict__ uniform,
                                                          int8_t* __restrict__ actions, float* __restrict__ log_probs) {
-  const int64_t i = (int64_t)blockIdx.x * kRowThreads + threadIdx.x;
-  if (i >= r.n) return;
-  const uint32_t legal = legal_bits(r.mask[i], r.A);
+  __shared__ __align__(16) char lds[Tile<T, AP>::kBytes];
+  const int64_t row0 = (int64_t)blockIdx.x * kRowThreads, i = row0 + threadIdx.x;
+  const int rows = (int)(r.n - row0 < kRowThreads ? r.n - row0 : kRowThreads);
+  const bool mine = (int)threadIdx.x < rows;
+  const uint32_t legal = mine ? legal_bits(r.mask[i], r.A) : 0u;
+  float u = mine ? uniform[i] : 0.0f;
+  stage<T, AP>(lds, r.logits, r.stride, row0, rows, r.A);
+  __syncthreads();
   int action = -1;
   float logp = 0.0f;
   if (legal) {
-    const T* row = (const T*)r.logits + i * r.stride;
     float x[AP], e[AP];
-    load_row<T, AP>(row, r.A, legal, x);
+    Tile<T, AP>::read(lds, r.A, legal, x);
     const Softmax s = softmax<AP>(x, e);
     if (s.sum == s.sum) {
-      float u = uniform[i];
       bool near = !(u < 1.0f);  // outside [0, 1): below as 0, above (and a NaN) the last action with a share
       u = u < 0.0f ? 0.0f : u;
-      const float t = u * s.sum, margin = kPickMargin * s.sum;
-      float c = 0.0f, xa = 0.0f;
+      const float t = u * s.sum;
+      float c = 0.0f, xa = 0.0f, gap = INFINITY;
 #pragma unroll
       for (int a = AP - 1; a >= 0; --a) {  // from above: the sums still to come
-        const float rest = s.sum - c;      // the running sum through a
-        near |= fabsf(rest - t) <= margin;
-        if (rest > t) action = a, xa = x[a];
+        const float rest = (s.sum - c) - t;  // the running sum through a, less u total
+        gap = fminf(gap, fabsf(rest));
+        if (rest > 0.0f) action = a, xa = x[a];
         c += e[a];
       }
+      near |= gap <= kPickMargin * s.sum;
       if (near) {
+        const T* row = (const T*)r.logits + i * r.stride;
         action = pick64(row, legal, s.m, u);
         xa = widen(row[action]) - s.m;
       }
@@ -172,8 +364,10 @@ __global__ __launch_bounds__(kRowThreads) void k_sample(Rows r, const float* __r
       logp = s.sum;  // NaN or +inf at a legal action: no distribution, no action
     }
   }
-  actions[i] = (int8_t)action;
-  if (log_probs) log_probs[i] = logp;
+  if (mine) {
+    actions[i] = (int8_t)action;
+    if (log_probs) log_probs[i] = logp;
+  }
 }
 
 // ------------------------------------------------------------ advantages
@@ -293,6 +487,7 @@ __global__ __launch_bounds__(kRowThreads) void k_policy_count(PolicyArgs q) {
 template <class T, int AP>
 __global__ __launch_bounds__(kRowThreads) void k_policy_loss(PolicyArgs q) {
   __shared__ double lds[kRowThreads / 64];
+  __shared__ __align__(16) char tile[Tile<T, AP>::kBytes];
   __shared__ int64_t total;
   int64_t c = threadIdx.x < (uint32_t)q.count_blocks ? q.counts[threadIdx.x] : 0;
   {
@@ -310,65 +505,83 @@ __global__ __launch_bounds__(kRowThreads) void k_policy_loss(PolicyArgs q) {
   }
   const float scale = 1.0f / (float)(total > 0 ? total : 1);
 
-  const int64_t i = (int64_t)blockIdx.x * kRowThreads + threadIdx.x;
-  float surrogate = 0.0f, kl = 0.0f, entropy = 0.0f, clipped = 0.0f;
-  if (i < q.r.n) {
-    const uint32_t legal = legal_bits(q.r.mask[i], q.r.A);
-    const int action = q.r.actions[i];
-    float logp = 0.0f;
-    T* grad = q.grad ? (T*)q.grad + i * q.r.A : nullptr;
-    if (decided(legal, action) && (!q.active || q.active[i])) {
-      const T* row = (const T*)q.r.logits + i * q.r.stride;
-      float x[AP], e[AP], d[AP];
-      load_row<T, AP>(row, q.r.A, legal, x);
-      const Softmax s = softmax<AP>(x, e);
-      const float inv = 1.0f / s.sum;
-      if (q.r.ref) {
-        float re[AP];
-        load_row<T, AP>((const T*)q.r.ref + i * q.r.ref_stride, q.r.A, legal, d);
-        const Softmax rs = softmax<AP>(d, re);
+  const int64_t row0 = (int64_t)blockIdx.x * kRowThreads, i = row0 + threadIdx.x;
+  const int rows = (int)(q.r.n - row0 < kRowThreads ? q.r.n - row0 : kRowThreads);
+  const bool mine = (int)threadIdx.x < rows;
+  uint32_t legal = 0;
+  int action = -1;
+  float old = 0.0f, adv = 0.0f;
+  if (mine) {
+    legal = legal_bits(q.r.mask[i], q.r.A);
+    action = q.r.actions[i];
+    if (!decided(legal, action) || (q.active && !q.active[i])) legal = 0;
+    old = q.old[i];
+    adv = q.adv[i];
+  }
+  float x[AP], e[AP], d[AP];
+  if (q.r.ref) {
+    stage_two<T, AP>(tile, q.r, row0, rows, legal, x, d);
+  } else {
+    stage<T, AP>(tile, q.r.logits, q.r.stride, row0, rows, q.r.A);
+    __syncthreads();
+    Tile<T, AP>::read(tile, q.r.A, legal, x);
+  }
+  float surrogate = 0.0f, kl = 0.0f, entropy = 0.0f, clipped = 0.0f, logp = 0.0f;
+  if (legal) {
+    float rlse = 0.0f;
+    if (q.r.ref) {
+      rlse = softmax<AP>(d, e).lse;
+    }
+    const Softmax s = softmax<AP>(x, e);
+    const float inv = 1.0f / s.sum;
+    float z = 0.0f;
 #pragma unroll
-        for (int a = 0; a < AP; ++a) d[a] = ((legal >> a) & 1u) ? (fmaxf(x[a], kLowest) - s.lse) - (d[a] - rs.lse) : 0.0f;
+    for (int a = 0; a < AP; ++a) {
+      e[a] *= inv;  // p
+      if (a == action) z = x[a];
+      x[a] = fmaxf(x[a] - s.lse, kLowest);  // log p; finite, so that 0 log 0 is 0
+      entropy -= e[a] * x[a];
+      if (q.r.ref) {
+        d[a] = ((legal >> a) & 1u) ? x[a] - (d[a] - rlse) : 0.0f;
+        kl += e[a] * d[a];
       }
-      float z = 0.0f, w = 0.0f;
+    }
+    if (kl > 1e30f) kl = INFINITY;  // an action that the reference never takes
+    logp = z - s.lse;
+    const float dl = logp - old;
+    const double border = adv > 0.0f ? q.log_high : q.log_low;
+    bool over = adv > 0.0f ? dl > (float)border : dl < (float)border;
+    // 32 bits hold dl to a few 2^-23 of its terms
+    if (fabsf(dl - (float)border) <= 4.76837158e-7f * (4.0f + fabsf(z) + fabsf(old))) {
+      const T* row = (const T*)q.r.logits + i * q.r.stride;
+      const double dl64 = ((double)widen(row[action]) - (double)s.m) - lse64(row, legal, s.m) - (double)old;
+      over = adv > 0.0f ? dl64 > border : dl64 < border;
+    }
+    over = over && adv != 0.0f;
+    const float rho = expf(dl);
+    surrogate = adv == 0.0f ? 0.0f : -(over ? (adv > 0.0f ? q.high : q.low) : rho) * adv;
+    clipped = over ? 1.0f : 0.0f;
+    if (q.grad) {
+      const float w = (over || adv == 0.0f) ? 0.0f : -rho * adv;
+      const float base = q.ent * entropy - (q.r.ref ? q.kl * kl : 0.0f) - w;
 #pragma unroll
       for (int a = 0; a < AP; ++a) {
-        e[a] *= inv;                            // p
-        if (a == action) z = x[a];
-        x[a] = fmaxf(x[a] - s.lse, kLowest);    // log p; finite, so that 0 log 0 is 0
-        entropy -= e[a] * x[a];
-        if (q.r.ref) kl += e[a] * d[a];
+        float g = q.ent * x[a] + base;
+        if (q.r.ref) g += q.kl * d[a];
+        g *= e[a];
+        if (a == action) g += w;
+        x[a] = ((legal >> a) & 1u) ? g * scale : 0.0f;
       }
-      if (kl > 1e30f) kl = INFINITY;  // an action that the reference never takes
-      logp = z - s.lse;
-      const float old = q.old[i], adv = q.adv[i], dl = logp - old;
-      const double border = adv > 0.0f ? q.log_high : q.log_low;
-      bool over = adv > 0.0f ? dl > (float)border : dl < (float)border;
-      // 32 bits hold dl to a few 2^-23 of its terms
-      if (fabsf(dl - (float)border) <= 4.76837158e-7f * (4.0f + fabsf(z) + fabsf(old))) {
-        const double dl64 = ((double)widen(row[action]) - (double)s.m) - lse64(row, legal, s.m) - (double)old;
-        over = adv > 0.0f ? dl64 > border : dl64 < border;
-      }
-      over = over && adv != 0.0f;
-      const float rho = expf(dl);
-      surrogate = adv == 0.0f ? 0.0f : -(over ? (adv > 0.0f ? q.high : q.low) : rho) * adv;
-      clipped = over ? 1.0f : 0.0f;
-      w = (over || adv == 0.0f) ? 0.0f : -rho * adv;
-      if (grad) {
-        const float base = q.ent * entropy - (q.r.ref ? q.kl * kl : 0.0f) - w;
-#pragma unroll
-        for (int a = 0; a < AP; ++a) {
-          float g = q.ent * x[a] + base;
-          if (q.r.ref) g += q.kl * d[a];
-          g *= e[a];
-          if (a == action) g += w;
-          if (a < q.r.A) grad[a] = (T)(((legal >> a) & 1u) ? g * scale : 0.0f);
-        }
-      }
-    } else if (grad) {
-      for (int a = 0; a < q.r.A; ++a) grad[a] = (T)0.0f;
     }
-    if (q.log_probs) q.log_probs[i] = logp;
+  } else {
+#pragma unroll
+    for (int a = 0; a < AP; ++a) x[a] = 0.0f;
+  }
+  if (mine && q.log_probs) q.log_probs[i] = logp;
+  if (q.grad) {
+    Tile<T, AP>::write(tile, q.r.A, x);
+    __syncthreads();
+    Tile<T, AP>::copy_out(tile, (T*)q.grad, row0, rows, q.r.A);
   }
   const double s0 = block_sum<kRowThreads>(surrogate, lds), s1 = block_sum<kRowThreads>(kl, lds),
                s2 = block_sum<kRowThreads>(entropy, lds), s3 = block_sum<kRowThreads>(clipped, lds);
@@ -438,26 +651,35 @@ __device__ __forceinline__ int64_t offset_at(const PreferenceArgs& q, int64_t s)
 
 template <class T, int AP>
 __global__ __launch_bounds__(kRowThreads) void k_preference_rows(PreferenceArgs q) {
-  const int64_t i = (int64_t)blockIdx.x * kRowThreads + threadIdx.x;
-  if (i >= q.r.n) return;
-  const uint32_t legal = legal_bits(q.r.mask[i], q.r.A);
-  const int action = q.r.actions[i];
+  __shared__ __align__(16) char tile[Tile<T, AP>::kBytes];
+  const int64_t row0 = (int64_t)blockIdx.x * kRowThreads, i = row0 + threadIdx.x;
+  const int rows = (int)(q.r.n - row0 < kRowThreads ? q.r.n - row0 : kRowThreads);
+  const bool mine = (int)threadIdx.x < rows;
+  uint32_t legal = mine ? legal_bits(q.r.mask[i], q.r.A) : 0u;
+  const int action = mine ? q.r.actions[i] : -1;
+  if (!decided(legal, action)) legal = 0;
+  float x[AP], d[AP], e[AP];
+  if (q.r.ref) {
+    stage_two<T, AP>(tile, q.r, row0, rows, legal, x, d);
+  } else {
+    stage<T, AP>(tile, q.r.logits, q.r.stride, row0, rows, q.r.A);
+    __syncthreads();
+    Tile<T, AP>::read(tile, q.r.A, legal, x);
+  }
+  if (!mine) return;
   float out = 0.0f;
-  if (decided(legal, action)) {
-    float x[AP], e[AP];
-    load_row<T, AP>((const T*)q.r.logits + i * q.r.stride, q.r.A, legal, x);
+  if (legal) {
     Softmax s = softmax<AP>(x, e);
 #pragma unroll
     for (int a = 0; a < AP; ++a)
       if (a == action) out = x[a];
     out -= s.lse;
     if (q.r.ref) {
-      load_row<T, AP>((const T*)q.r.ref + i * q.r.ref_stride, q.r.A, legal, x);
-      s = softmax<AP>(x, e);
+      s = softmax<AP>(d, e);
       float z = 0.0f;
 #pragma unroll
       for (int a = 0; a < AP; ++a)
-        if (a == action) z = x[a];
+        if (a == action) z = d[a];
       out -= z - s.lse;
     }
   }
@@ -513,11 +735,12 @@ __global__ __launch_bounds__(kRowThreads) void k_preference_finish(const double*
 
 template <class T, int AP>
 __global__ __launch_bounds__(kRowThreads) void k_preference_grad(PreferenceArgs q) {
-  const int64_t i = (int64_t)blockIdx.x * kRowThreads + threadIdx.x;
-  if (i >= q.r.n) return;
-  const uint32_t legal = legal_bits(q.r.mask[i], q.r.A);
-  const int action = q.r.actions[i];
-  T* grad = (T*)q.grad + i * q.r.A;
+  __shared__ __align__(16) char tile[Tile<T, AP>::kBytes];
+  const int64_t row0 = (int64_t)blockIdx.x * kRowThreads, i = row0 + threadIdx.x;
+  const int rows = (int)(q.r.n - row0 < kRowThreads ? q.r.n - row0 : kRowThreads);
+  const bool mine = (int)threadIdx.x < rows;
+  uint32_t legal = mine ? legal_bits(q.r.mask[i], q.r.A) : 0u;
+  const int action = mine ? q.r.actions[i] : -1;
   float coef = 0.0f;
   if (decided(legal, action)) {
     // the last sequence that starts at or before row i (the non-empty one where several start there)
@@ -529,18 +752,23 @@ __global__ __launch_bounds__(kRowThreads) void k_preference_grad(PreferenceArgs 
     }
     if (lo >= 1 && lo <= 2 * q.pairs) coef = q.coef[lo - 1];
   }
-  if (coef != 0.0f) {
-    float x[AP], e[AP];
-    load_row<T, AP>((const T*)q.r.logits + i * q.r.stride, q.r.A, legal, x);
+  if (coef == 0.0f) legal = 0;
+  stage<T, AP>(tile, q.r.logits, q.r.stride, row0, rows, q.r.A);
+  __syncthreads();
+  float x[AP], e[AP];
+  Tile<T, AP>::read(tile, q.r.A, legal, x);
+  if (legal) {
     const Softmax s = softmax<AP>(x, e);
     const float p = -coef / s.sum;
 #pragma unroll
-    for (int a = 0; a < AP; ++a) {
-      if (a < q.r.A) grad[a] = (T)(((legal >> a) & 1u) ? p * e[a] + (a == action ? coef : 0.0f) : 0.0f);
-    }
+    for (int a = 0; a < AP; ++a) x[a] = ((legal >> a) & 1u) ? p * e[a] + (a == action ? coef : 0.0f) : 0.0f;
   } else {
-    for (int a = 0; a < q.r.A; ++a) grad[a] = (T)0.0f;
+#pragma unroll
+    for (int a = 0; a < AP; ++a) x[a] = 0.0f;
   }
+  Tile<T, AP>::write(tile, q.r.A, x);
+  __syncthreads();
+  Tile<T, AP>::copy_out(tile, (T*)q.grad, row0, rows, q.r.A);
 }
 
 // ---------------------------------------------------------- grad scaling
