@@ -4876,7 +4876,7 @@ int coup_sample_actions(const coup_decisions* d, const float* uniform, int8_t* a
 
 int coup_advantages(const coup_window* w, double gamma, double lam, float* adv, float* target, void* hip_stream) {
   if (!w) return fail(COUP_E_INVALID, "coup_advantages: window is null");
-  if (w->steps < 0 || w->lanes < 0 || (w->lanes && w->steps > (int64_t(1) << 40) / w->lanes))
+  if (w->steps < 0 || w->lanes < 0 || w->lanes > (int64_t(1) << 38) || (w->lanes && w->steps > (int64_t(1) << 40) / w->lanes))
     return fail(COUP_E_INVALID, "coup_advantages: steps or lanes out of range");
   if (w->num_players < 2 || w->num_players > COUP_MAX_PLAYERS)
     return fail(COUP_E_INVALID, "coup_advantages: num_players must be 2..6");
@@ -4886,10 +4886,21 @@ int coup_advantages(const coup_window* w, double gamma, double lam, float* adv, 
   if (w->steps == 0 || w->lanes == 0) return COUP_OK;
   if (!w->rewards || !w->step_type || !w->players || !w->values || !adv || !target)
     return fail(COUP_E_INVALID, "coup_advantages: null buffer");
-  const coup::policy::AdvantageArgs q{w->rewards, w->step_type, w->players,   w->values,           w->bootstrap,
-                                      adv,        target,       w->steps,     w->lanes,            (float)gamma,
-                                      (float)(gamma * lam),     (float)(gamma * (1.0 - lam))};
-  coup::policy::launch_advantages(q, w->dtype, w->num_players, (hipStream_t)hip_stream);
+  coup::policy::AdvantageArgs q{};
+  q.rewards = w->rewards;
+  q.step_type = w->step_type;
+  q.players = w->players;
+  q.values = w->values;
+  q.bootstrap = w->bootstrap;
+  q.adv = adv;
+  q.target = target;
+  q.T = w->steps;
+  q.B = w->lanes;
+  q.dtype = w->dtype;
+  q.gamma = (float)gamma;
+  q.gl = (float)(gamma * lam);
+  q.gv = (float)(gamma * (1.0 - lam));
+  coup::policy::launch_advantages(q, w->num_players, (hipStream_t)hip_stream);
   COUP_HIP_TRY(hipGetLastError());
   return COUP_OK;
 }

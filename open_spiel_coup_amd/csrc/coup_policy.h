@@ -379,6 +379,13 @@ __global__ __launch_bounds__(kRowThreads) void k_sample(Rows r, const float* __r
 // a step adds its reward to every z_p; the step's player takes A = z_p - V
 // and leaves z_p = gamma lam z_p + gamma (1 - lam) V for its earlier ones; a
 // LAST or FIRST step cuts what lies behind it (z = 0 before its reward).
+//
+// A step's map of z_p is affine with factors of at most 1, so a stretch of
+// steps is one pair (f, g), z -> f z + g, per player, and stretches compose.
+// A block holds L lanes; its NT / L threads of a lane take kStretch steps
+// each, latest first, all loaded before the first is used (the window is read
+// once); a scan over the stretches' pairs gives each its z, and the block
+// goes on to the next NT / L * kStretch steps.
 struct AdvantageArgs {
   const int8_t* rewards;  // [T][B][P]
   const uint8_t* step_type;
@@ -387,36 +394,197 @@ struct AdvantageArgs {
   const void* bootstrap;  // [B][P] or null
   float *adv, *target;
   int64_t T, B;
+  int dtype;
   float gamma, gl, gv;  // gamma, gamma lam, gamma (1 - lam)
 };
 
-template <class T, int P>
-__global__ __launch_bounds__(64) void k_advantages(AdvantageArgs q) {
-  const int64_t b = (int64_t)blockIdx.x * 64 + threadIdx.x;
-  if (b >= q.B) return;
-  float z[P];
+constexpr int kStretch = 8;
+
+// A value as it is stored (16 or 32 bits), and widened.
+__device__ __forceinline__ uint32_t load_bits(const void* p, int64_t i, int dtype) {
+  return dtype == COUP_DTYPE_F32 ? ((const uint32_t*)p)[i] : (uint32_t)((const uint16_t*)p)[i];
+}
+__device__ __forceinline__ float widen_bits(uint32_t v, int dtype) {
+  if (dtype == COUP_DTYPE_F32) return __uint_as_float(v);
+  if (dtype == COUP_DTYPE_BF16) return __uint_as_float(v << 16);
+  return (float)__builtin_bit_cast(_Float16, (uint16_t)v);
+}
+
+// P reward bytes of one step and lane, at any alignment.
+template <int P>
+struct Rewards {
+  struct __attribute__((packed, aligned(1))) U32 { uint32_t v; };
+  struct __attribute__((packed, aligned(1))) U16 { uint16_t v; };
+  uint32_t lo = 0, hi = 0;
+  __device__ __forceinline__ void load(const int8_t* p) {
+    if (P >= 4) lo = ((const U32*)p)->v;
+    if (P == 6) hi = ((const U16*)(p + 4))->v;
+    if (P == 5) hi = (uint8_t)p[4];
+    if (P == 2 || P == 3) lo = ((const U16*)p)->v;
+    if (P == 3) hi = (uint8_t)p[2];
+  }
+  __device__ __forceinline__ float of(int p) const {
+    const uint32_t w = (P == 3) ? (p < 2 ? lo : hi) : (p < 4 ? lo : hi);
+    const int at = (P == 3) ? (p & 1) * (p < 2) : (p & 3);
+    return (float)(int8_t)(w >> (8 * at));
+  }
+};
+
+// A thread's steps in memory: step k of lane l is at uniform element `base[k]`
+// plus `off[k]`.  With one stretch a lane the step is the block's, so the
+// offset is the lane; with more, it is the lane and the stretch's steps from
+// the window's first, below 2^27 bytes of any array (launch_advantages).
+template <int C>
+struct Steps {
+  int64_t base[C == 1 ? kStretch : 1];
+  uint32_t off[C == 1 ? 1 : kStretch];
+  template <class V>
+  __device__ __forceinline__ V* at(V* p, int k, int scale = 1) const {
+    const int64_t u = base[C == 1 ? k : 0] * scale;
+    const uint32_t v = off[C == 1 ? 0 : k] * (uint32_t)(scale * sizeof(V));
+    return (V*)((char*)(p + u) + v);
+  }
+};
+
+// One stretch from its z: the outputs, and z after it.
+template <int P, int C>
+__device__ __forceinline__ void advance(const AdvantageArgs& q, const Steps<C>& at, const int (&st)[kStretch],
+                                        const int (&pl)[kStretch], const Rewards<P> (&r)[kStretch],
+                                        const float (&v)[kStretch], float (&z)[P], int steps) {
 #pragma unroll
-  for (int p = 0; p < P; ++p) z[p] = q.bootstrap ? q.gamma * widen(((const T*)q.bootstrap)[b * P + p]) : 0.0f;
-  for (int64_t t = q.T - 1; t >= 0; --t) {
-    const int64_t i = t * q.B + b;
-    const int st = q.step_type[i];
-    const bool step = st == COUP_STEP_MID || st == COUP_STEP_LAST;
-    const bool cut = st == COUP_STEP_FIRST || st == COUP_STEP_LAST;
-    const int player = step ? q.players[i] : -1;
-    const bool acts = player >= 0 && player < P;
-    const float v = acts ? widen(((const T*)q.values)[i]) : 0.0f;
+  for (int k = 0; k < kStretch; ++k) {
+    const bool step = st[k] == COUP_STEP_MID || st[k] == COUP_STEP_LAST;
+    const bool cut = st[k] == COUP_STEP_FIRST || st[k] == COUP_STEP_LAST;
     float target = 0.0f;
 #pragma unroll
     for (int p = 0; p < P; ++p) {
       if (cut) z[p] = 0.0f;
-      if (step) z[p] += (float)q.rewards[i * P + p];
-      if (p == player) {
+      if (step) z[p] += r[k].of(p);
+      if (p == pl[k]) {
         target = z[p];
-        z[p] = q.gl * z[p] + q.gv * v;
+        z[p] = q.gl * z[p] + q.gv * v[k];
       }
     }
-    q.adv[i] = acts ? target - v : 0.0f;
-    q.target[i] = target;
+    if (k < steps) {
+      *at.at(q.adv, k) = pl[k] >= 0 ? target - v[k] : 0.0f;
+      *at.at(q.target, k) = target;
+    }
+  }
+}
+
+template <int P, int L, int NT>
+__global__ __launch_bounds__(NT) void k_advantages(AdvantageArgs q) {
+  constexpr int C = NT / L;                // stretches of a lane in flight
+  constexpr int CW = L < 64 ? 64 / L : 1;  // of them in a wave
+  constexpr int NW = C / CW;               // waves a lane's stretches span
+  constexpr int LW = L < 64 ? L : 64;
+  static_assert(C == 1 || L <= 64, "a wave's threads are of one run of lanes");
+  __shared__ float totals[C > 1 ? NW * LW * P * 2 : 1];
+  const int64_t b0 = (int64_t)blockIdx.x * L;
+  const int lanes = (int)(q.B - b0 < L ? q.B - b0 : L);
+  const int l = (int)threadIdx.x % L, c = (int)threadIdx.x / L;
+  const int lane = l < lanes ? l : lanes - 1;  // lanes past the last load its steps and store nothing
+  float z[P];
+#pragma unroll
+  for (int p = 0; p < P; ++p)
+    z[p] = q.bootstrap ? q.gamma * widen_bits(load_bits(q.bootstrap, (b0 + lane) * P + p, q.dtype), q.dtype) : 0.0f;
+
+  for (int64_t end = q.T; end > 0; end -= C * kStretch) {
+    // this thread's steps: kStretch back from the window's step `top`; ones before the first load it and are skipped
+    const int64_t first = end > C * kStretch ? end - C * kStretch : 0;
+    const int top = (int)(end - first) - 1 - c * kStretch;
+    const int steps = l < lanes ? top + 1 : 0;
+    Steps<C> at;
+#pragma unroll
+    for (int k = 0; k < kStretch; ++k) {
+      const int rel = top - k > 0 ? top - k : 0;
+      if (C == 1) at.base[k < (int)(sizeof(at.base) / 8) ? k : 0] = (first + rel) * q.B + b0;
+      else at.off[k < (int)(sizeof(at.off) / 4) ? k : 0] = (uint32_t)rel * (uint32_t)q.B + lane;
+    }
+    if (C == 1) at.off[0] = lane;
+    else at.base[0] = first * q.B + b0;
+    int st[kStretch], pl[kStretch];
+    uint32_t bits[kStretch];
+    Rewards<P> r[kStretch];
+#pragma unroll
+    for (int k = 0; k < kStretch; ++k) {
+      st[k] = *at.at(q.step_type, k);
+      pl[k] = *at.at(q.players, k);
+      r[k].load(at.at(q.rewards, k, P));
+    }
+    if (q.dtype == COUP_DTYPE_F32) {
+#pragma unroll
+      for (int k = 0; k < kStretch; ++k) bits[k] = *at.at((const uint32_t*)q.values, k);
+    } else {
+#pragma unroll
+      for (int k = 0; k < kStretch; ++k) bits[k] = *at.at((const uint16_t*)q.values, k);
+    }
+    float v[kStretch];
+#pragma unroll
+    for (int k = 0; k < kStretch; ++k) {
+      if (k > top) st[k] = COUP_STEP_SKIPPED;
+      const bool step = st[k] == COUP_STEP_MID || st[k] == COUP_STEP_LAST;
+      if (!step || pl[k] >= P) pl[k] = -1;
+      v[k] = pl[k] >= 0 ? widen_bits(bits[k], q.dtype) : 0.0f;
+    }
+    if (C == 1) {
+      advance<P, C>(q, at, st, pl, r, v, z, steps);
+    } else {
+      float f[P], g[P];
+#pragma unroll
+      for (int p = 0; p < P; ++p) f[p] = 1.0f, g[p] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < kStretch; ++k) {
+        const bool step = st[k] == COUP_STEP_MID || st[k] == COUP_STEP_LAST;
+        const bool cut = st[k] == COUP_STEP_FIRST || st[k] == COUP_STEP_LAST;
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+          if (cut) f[p] = 0.0f, g[p] = 0.0f;
+          if (step) g[p] += r[k].of(p);
+          if (p == pl[k]) {
+            f[p] *= q.gl;
+            g[p] = q.gl * g[p] + q.gv * v[k];
+          }
+        }
+      }
+      // the wave's stretches up to each, a lower index (a later time) first
+      const int cw = c % CW, wave = c / CW;
+#pragma unroll
+      for (int d = 1; d < CW; d *= 2) {
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+          const float f0 = __shfl_up(f[p], d * L, 64), g0 = __shfl_up(g[p], d * L, 64);
+          if (cw >= d) {
+            g[p] = f[p] * g0 + g[p];
+            f[p] *= f0;
+          }
+        }
+      }
+      // the wave's whole, then what stands before this stretch in its wave
+      float* mine = totals + (wave * LW + (l & (LW - 1))) * P * 2;
+      if (cw == CW - 1) {
+#pragma unroll
+        for (int p = 0; p < P; ++p) mine[2 * p] = f[p], mine[2 * p + 1] = g[p];
+      }
+#pragma unroll
+      for (int p = 0; p < P; ++p) {
+        f[p] = CW > 1 ? __shfl_up(f[p], L, 64) : 1.0f;
+        g[p] = CW > 1 ? __shfl_up(g[p], L, 64) : 0.0f;
+        if (cw == 0) f[p] = 1.0f, g[p] = 0.0f;
+      }
+      __syncthreads();
+      float here[P];
+      for (int w = 0; w < NW; ++w) {
+        const float* o = totals + (w * LW + (l & (LW - 1))) * P * 2;
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+          if (w == wave) here[p] = f[p] * z[p] + g[p];  // z runs through the waves: here it stands before this one
+          z[p] = o[2 * p] * z[p] + o[2 * p + 1];
+        }
+      }
+      __syncthreads();  // the next window writes the totals again
+      advance<P, C>(q, at, st, pl, r, v, here, steps);
+    }
   }
 }
 
@@ -822,18 +990,27 @@ inline void launch_sample(const Rows& r, int dtype, const float* uniform, int8_t
   });
 }
 
-inline void launch_advantages(const AdvantageArgs& q, int dtype, int players, hipStream_t s) {
-  const unsigned grid = (unsigned)((q.B + 63) / 64);
-  with_dtype(dtype, [&](auto t) {
-    using T = typename decltype(t)::type;
-    switch (players) {
-      case 2: k_advantages<T, 2><<<grid, 64, 0, s>>>(q); break;
-      case 3: k_advantages<T, 3><<<grid, 64, 0, s>>>(q); break;
-      case 4: k_advantages<T, 4><<<grid, 64, 0, s>>>(q); break;
-      case 5: k_advantages<T, 5><<<grid, 64, 0, s>>>(q); break;
-      default: k_advantages<T, 6><<<grid, 64, 0, s>>>(q); break;
-    }
-  });
+// How a window is split: enough threads to fill the chip (2^17), but no more
+// stretches than the window has.  C = 1, 4, 16, 128 or 512 of a lane's at a time.
+template <int P>
+void launch_advantages_of(const AdvantageArgs& q, hipStream_t s) {
+  const auto enough = [&](int c) { return q.B * c >= (1 << 17) || (int64_t)c * kStretch >= q.T; };
+  const auto grid = [&](int lanes) { return (unsigned)((q.B + lanes - 1) / lanes); };
+  if (enough(1)) k_advantages<P, 256, 256><<<grid(256), 256, 0, s>>>(q);
+  else if (enough(4)) k_advantages<P, 64, 256><<<grid(64), 256, 0, s>>>(q);
+  else if (enough(16)) k_advantages<P, 16, 256><<<grid(16), 256, 0, s>>>(q);
+  else if (enough(128)) k_advantages<P, 4, 512><<<grid(4), 512, 0, s>>>(q);
+  else k_advantages<P, 1, 512><<<grid(1), 512, 0, s>>>(q);
+}
+
+inline void launch_advantages(const AdvantageArgs& q, int players, hipStream_t s) {
+  switch (players) {
+    case 2: return launch_advantages_of<2>(q, s);
+    case 3: return launch_advantages_of<3>(q, s);
+    case 4: return launch_advantages_of<4>(q, s);
+    case 5: return launch_advantages_of<5>(q, s);
+    default: return launch_advantages_of<6>(q, s);
+  }
 }
 
 inline size_t policy_workspace(int64_t n) { return sizeof(int64_t) * kCountBlocks + sizeof(double) * 4 * row_blocks(n); }

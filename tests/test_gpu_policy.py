@@ -210,6 +210,25 @@ def test_advantages(T, B, P, gamma, lam, boot, dtype):
         _close(g.cpu().numpy(), w, 4 * run * H * bound, name)
 
 
+@pytest.mark.parametrize("B,players", [(131075, 2), (40001, 3), (9001, 6)])
+def test_advantages_of_many_lanes(B, players):
+    """Windows of many lanes (a lane's stretches 1, 4 or 16 at a time over several rounds): some lanes against the oracle."""
+    T = 200
+    gen = torch.Generator(DEV).manual_seed(B)
+    kind = torch.rand(T, B, generator=gen, device=DEV)
+    st = torch.where(kind < 0.05, 2, torch.where(kind < 0.07, 0, torch.where(kind < 0.1, 3, 1))).to(torch.uint8)
+    pl = torch.randint(-1, players, (T, B), generator=gen, device=DEV).to(torch.int8)
+    r = torch.randint(-players, players + 1, (T, B, players), generator=gen, device=DEV).to(torch.int8)
+    v = torch.randn(T, B, generator=gen, device=DEV)
+    b = torch.randn(B, players, generator=gen, device=DEV)
+    got = policy.advantages(r, st, pl, v, b, gamma=0.99, lam=0.95)
+    lanes = torch.tensor([0, 1, 255, 256, B // 2, B - 258, B - 2, B - 1], device=DEV)
+    pick = [t[:, lanes].cpu().numpy() for t in (r, st, pl)]
+    want = oracle.advantages(*pick, _np(v[:, lanes]), _np(b[lanes]), 0.99, 0.95)
+    for g, w in zip(got, want):  # chains here run for at most T steps: 4 roundings a term, of sums below T (P + 9)
+        _close(g[:, lanes].cpu().numpy(), w, 4 * T * H * T * (players + 9) * 0.1, "advantages")
+
+
 def test_advantages_no_ends_and_empty():
     """A window without an end (every chain runs to the bootstrap), all-skipped lanes, and windows of no steps or lanes."""
     gen = torch.Generator().manual_seed(3)
