@@ -427,7 +427,7 @@ int coup_error_count(coup_env* env, int64_t* out);
  * work is enqueued on `hip_stream` (NULL = default) and nothing is allocated
  * or synchronised, so every call may be captured into a HIP graph.  The
  * workspaces are the caller's, of at least the size the _workspace functions
- * return, 8-byte aligned, not shared by calls (or graphs) that may run at the
+ * return, 16-byte aligned, not shared by calls (or graphs) that may run at the
  * same time.  Results do not depend on the order blocks run in.
  *
  * A row is one decision: num_actions (1..31) logits, a legal-action word as

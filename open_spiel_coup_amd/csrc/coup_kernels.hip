@@ -4917,7 +4917,7 @@ int coup_policy_loss(const coup_decisions* d, const coup_policy_terms* terms, co
     return fail(COUP_E_INVALID, "coup_policy_loss: clip_low must be in 0..1 and clip_high finite and not negative");
   if (!std::isfinite(terms->kl_coef) || !std::isfinite(terms->entropy_coef))
     return fail(COUP_E_INVALID, "coup_policy_loss: kl_coef and entropy_coef must be finite");
-  if (!workspace || ((uintptr_t)workspace & 7) || workspace_bytes < coup_policy_workspace(d->rows))
+  if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < coup_policy_workspace(d->rows))
     return fail(COUP_E_INVALID, "coup_policy_loss: workspace is null, misaligned or too small");
   coup::policy::PolicyArgs q{};
   q.r = rows_of(d, true);
@@ -4956,7 +4956,7 @@ int coup_preference_loss(const coup_decisions* d, const coup_preference_terms* t
   if (!std::isfinite(terms->beta)) return fail(COUP_E_INVALID, "coup_preference_loss: beta must be finite");
   if (!(terms->label_smoothing >= 0.0 && terms->label_smoothing <= 0.5))
     return fail(COUP_E_INVALID, "coup_preference_loss: label_smoothing must be in 0..0.5");
-  if (!workspace || ((uintptr_t)workspace & 7) || workspace_bytes < coup_preference_workspace(d->rows, terms->pairs))
+  if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < coup_preference_workspace(d->rows, terms->pairs))
     return fail(COUP_E_INVALID, "coup_preference_loss: workspace is null, misaligned or too small");
   coup::policy::PreferenceArgs q{};
   q.r = rows_of(d, true);
@@ -4967,7 +4967,8 @@ int coup_preference_loss(const coup_decisions* d, const coup_preference_terms* t
   q.eps = terms->label_smoothing;
   q.rewards = out->rewards;
   q.grad = out->grad;
-  coup::policy::launch_preference(q, d->dtype, out->loss, workspace, (hipStream_t)hip_stream);
+  q.loss = out->loss;
+  coup::policy::launch_preference(q, d->dtype, workspace, (hipStream_t)hip_stream);
   COUP_HIP_TRY(hipGetLastError());
   return COUP_OK;
 }

@@ -29,6 +29,7 @@ namespace coup {
 namespace policy {
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kRowThreads = 256;
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -66,8 +67,8 @@ __device__ __forceinline__ bool decided(uint32_t legal, int action) {
 // is used, into LDS, and each thread then reads its own row from there (72
 // bytes apart for the game's 18 float logits; read straight from memory those
 // loads touch 64 lines an instruction: the 4 x 2^20-row loss took 461 us that
-// way).  A gradient goes the same way back.  Strided or unaligned tables are
-// copied by elements.
+// way).  A gradient goes the same way back.  Strided tables are copied
+// by elements.
 //
 // LDS: element j of row r is at byte (r A + j) sizeof(T), so a wave's lanes
 // read words A sizeof(T) / 4 apart: for odd multiples of 4 or 8 bytes at most
@@ -80,11 +81,10 @@ struct Tile {
   static constexpr int kPieces = (AP * (int)sizeof(T) + 15) / 16;  // 16-byte pieces a thread, at most
   static constexpr int kBytes = kRowThreads * kPieces * 16 + 256;  // reads past a tile's last row stay inside
   typedef T vec __attribute__((ext_vector_type(16 / sizeof(T))));
+  // a piece in memory: at any element (gfx950's 16-byte accesses need no alignment)
+  typedef uint32_t piece_at __attribute__((ext_vector_type(4), aligned(2)));
 
-  // 16-byte pieces (else elements) in memory; rows in whole pieces in LDS
-  static __device__ __forceinline__ bool in_pieces(const void* p, int64_t stride, int A) {
-    return stride == A && ((uintptr_t)p & 15) == 0;
-  }
+  // rows in whole pieces
   static __device__ __forceinline__ bool whole(int A) { return (A * (int)sizeof(T)) % 16 == 0; }
   static __device__ __forceinline__ int place(int k) { return k ^ ((k >> 4) & 15); }
 
@@ -100,7 +100,7 @@ struct Tile {
     for (int c = 0; c < kPieces; ++c) {
       const int at = (c * kRowThreads + (int)threadIdx.x) * 16;
       f.piece[c] = u32x4{0, 0, 0, 0};
-      if (at + 16 <= bytes) f.piece[c] = *(const u32x4*)(src + at);
+      if (at + 16 <= bytes) f.piece[c] = *(const piece_at*)(src + at);
     }
   }
 
@@ -198,17 +198,14 @@ struct Tile {
   static __device__ __forceinline__ void copy_out(const char* lds, T* base, int64_t row0, int rows, int A) {
     const int n = rows * A, bytes = n * (int)sizeof(T);
     T* dst = base + row0 * A;
-    int done = 0;
-    if (((uintptr_t)base & 15) == 0) {
-      const bool w = whole(A);
+    const bool w = whole(A);
 #pragma unroll
-      for (int c = 0; c < kPieces; ++c) {
-        const int k = c * kRowThreads + (int)threadIdx.x;
-        if (k * 16 + 16 <= bytes) ((u32x4*)dst)[k] = *(const u32x4*)(lds + (w ? place(k) : k) * 16);
-      }
-      done = bytes / 16 * 16 / (int)sizeof(T);
+    for (int c = 0; c < kPieces; ++c) {
+      const int k = c * kRowThreads + (int)threadIdx.x;
+      if (k * 16 + 16 <= bytes) ((piece_at*)dst)[k] = *(const u32x4*)(lds + (w ? place(k) : k) * 16);
     }
-    for (int e = done + (int)threadIdx.x; e < n; e += kRowThreads) dst[e] = *(const T*)(lds + at_element(e, A));
+    const int e = bytes / 16 * 16 / (int)sizeof(T) + (int)threadIdx.x;  // the last piece's rest (none of whole rows)
+    if (e < n) dst[e] = ((const T*)lds)[e];
   }
 };
 
@@ -217,7 +214,7 @@ struct Tile {
 template <class T, int AP>
 __device__ __forceinline__ void stage(char* lds, const void* base, int64_t stride, int64_t row0, int rows, int A) {
   using Tl = Tile<T, AP>;
-  if (Tl::in_pieces(base, stride, A)) {
+  if (stride == A) {
     typename Tl::Flight f;
     Tl::fetch(f, (const T*)base, row0, rows, A);
     Tl::land(f, lds, (const T*)base, row0, rows, A);
@@ -232,8 +229,7 @@ template <class T, int AP>
 __device__ __forceinline__ void stage_two(char* lds, const Rows& q, int64_t row0, int rows, uint32_t legal,
                                           float (&x)[AP], float (&d)[AP]) {
   using Tl = Tile<T, AP>;
-  const bool pieces = Tl::in_pieces(q.logits, q.stride, q.A) && Tl::in_pieces(q.ref, q.ref_stride, q.A);
-  if (pieces) {
+  if (q.stride == q.A && q.ref_stride == q.A) {
     typename Tl::Flight f, g;
     Tl::fetch(f, (const T*)q.logits, row0, rows, q.A);
     Tl::fetch(g, (const T*)q.ref, row0, rows, q.A);
@@ -590,24 +586,23 @@ __global__ __launch_bounds__(NT) void k_advantages(AdvantageArgs q) {
 
 // ----------------------------------------------------- sums over a block
 
-__device__ __forceinline__ float wave_sum(float v) {
+// Each of v[0..K) summed over the block, in a fixed order; thread 0 has the
+// sums.  lds: K THREADS / 64 values.
+template <int THREADS, int K, class V>
+__device__ __forceinline__ void block_sum(V (&v)[K], V* lds) {
 #pragma unroll
-  for (int s = 32; s >= 1; s >>= 1) v += __shfl_xor(v, s, 64);
-  return v;
-}
-
-// `v` summed over the block (32-bit within a wave, 64-bit across); thread 0
-// has the result.
-template <int THREADS>
-__device__ __forceinline__ double block_sum(float v, double* lds) {
-  v = wave_sum(v);
+  for (int k = 0; k < K; ++k) {
+#pragma unroll
+    for (int s = 32; s >= 1; s >>= 1) v[k] += __shfl_xor(v[k], s, 64);
+    if ((threadIdx.x & 63) == 0) lds[k * (THREADS / 64) + (threadIdx.x >> 6)] = v[k];
+  }
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = (double)v;
-  __syncthreads();
-  double s = 0.0;
-  if (threadIdx.x == 0)
-    for (int w = 0; w < THREADS / 64; ++w) s += lds[w];
-  return s;
+  if (threadIdx.x == 0) {
+    for (int k = 0; k < K; ++k) {
+      v[k] = 0;
+      for (int w = 0; w < THREADS / 64; ++w) v[k] += lds[k * (THREADS / 64) + w];
+    }
+  }
 }
 
 // ----------------------------------------------------------- policy loss
@@ -628,19 +623,32 @@ struct PolicyArgs {
   float kl, ent;
   float* log_probs;  // null: not wanted
   void* grad;        // null: no gradient
-  double* partial;   // [blocks][4] sums of the terms
+  f32x4* partial;    // [blocks] sums of the terms over a block's rows
   int64_t* counts;   // [count blocks] decisions
   int count_blocks;
 };
 
-constexpr int kCountBlocks = 256;
+constexpr int kCountBlocks = 256, kCountThreads = 1024, kFinishThreads = 1024;
 
-// How many decisions there are: 6 bytes a row.  The gradient needs it before
-// its first store, and a second pass over the gradient would cost 2 A e.
-__global__ __launch_bounds__(kRowThreads) void k_policy_count(PolicyArgs q) {
-  __shared__ int wave[kRowThreads / 64];
-  int n = 0;  // a wave's rows are a 1024th of the call's: below 2^31
-  for (int64_t i = (int64_t)blockIdx.x * kRowThreads + threadIdx.x; i < q.r.n; i += (int64_t)gridDim.x * kRowThreads)
+// How many decisions there are: 6 bytes a row, four rows a thread at a time.
+// The gradient needs it before its first store, and a second pass over the
+// gradient would cost 2 A sizeof(T) a row.
+__global__ __launch_bounds__(kCountThreads) void k_policy_count(PolicyArgs q) {
+  __shared__ int wave[kCountThreads / 64];
+  int n = 0;  // a thread's rows: below 2^31 for any call
+  const int64_t first = (int64_t)blockIdx.x * kCountThreads + threadIdx.x, step = (int64_t)gridDim.x * kCountThreads;
+  const bool fours = ((uintptr_t)q.r.mask & 15) == 0 && ((uintptr_t)q.r.actions & 3) == 0 &&
+                     ((uintptr_t)q.active & 3) == 0;
+  const int64_t quads = fours ? q.r.n / 4 : 0;
+  for (int64_t i = first; i < quads; i += step) {
+    const u32x4 m = ((const u32x4*)q.r.mask)[i];
+    const uint32_t a = ((const uint32_t*)q.r.actions)[i];
+    const uint32_t on = q.active ? ((const uint32_t*)q.active)[i] : ~0u;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      n += decided(legal_bits(m[k], q.r.A), (int8_t)(a >> (8 * k))) && ((on >> (8 * k)) & 0xFF);
+  }
+  for (int64_t i = 4 * quads + first; i < q.r.n; i += step)
     n += decided(legal_bits(q.r.mask[i], q.r.A), q.r.actions[i]) && (!q.active || q.active[i]);
 #pragma unroll
   for (int s = 32; s >= 1; s >>= 1) n += __shfl_xor(n, s, 64);
@@ -648,13 +656,13 @@ __global__ __launch_bounds__(kRowThreads) void k_policy_count(PolicyArgs q) {
   __syncthreads();
   if (threadIdx.x != 0) return;
   int64_t total = 0;
-  for (int w = 0; w < kRowThreads / 64; ++w) total += wave[w];
+  for (int w = 0; w < kCountThreads / 64; ++w) total += wave[w];
   q.counts[blockIdx.x] = total;
 }
 
 template <class T, int AP>
 __global__ __launch_bounds__(kRowThreads) void k_policy_loss(PolicyArgs q) {
-  __shared__ double lds[kRowThreads / 64];
+  __shared__ float lds[4 * (kRowThreads / 64)];
   __shared__ __align__(16) char tile[Tile<T, AP>::kBytes];
   __shared__ int64_t total;
   int64_t c = threadIdx.x < (uint32_t)q.count_blocks ? q.counts[threadIdx.x] : 0;
@@ -751,34 +759,27 @@ __global__ __launch_bounds__(kRowThreads) void k_policy_loss(PolicyArgs q) {
     __syncthreads();
     Tile<T, AP>::copy_out(tile, (T*)q.grad, row0, rows, q.r.A);
   }
-  const double s0 = block_sum<kRowThreads>(surrogate, lds), s1 = block_sum<kRowThreads>(kl, lds),
-               s2 = block_sum<kRowThreads>(entropy, lds), s3 = block_sum<kRowThreads>(clipped, lds);
-  if (threadIdx.x == 0) {
-    double* o = q.partial + 4 * (int64_t)blockIdx.x;
-    o[0] = s0, o[1] = s1, o[2] = s2, o[3] = s3;
-  }
+  float sums[4] = {surrogate, kl, entropy, clipped};
+  block_sum<kRowThreads, 4>(sums, lds);
+  if (threadIdx.x == 0) q.partial[blockIdx.x] = f32x4{sums[0], sums[1], sums[2], sums[3]};
 }
 
-// The blocks' sums in a fixed order: the loss and its terms' means.
-__global__ __launch_bounds__(kRowThreads) void k_policy_finish(const double* __restrict__ partial, int64_t blocks,
-                                                                const int64_t* __restrict__ counts, int count_blocks,
-                                                                double kl, double ent, float* loss, float* stats,
-                                                                int64_t* count) {
-  __shared__ double lds[5][kRowThreads / 64];
+// The blocks' sums in a fixed order, in 64 bits: the loss and its terms'
+// means.  One block: the 16,384 sums of 4 x 2^20 rows are 256 KiB.
+__global__ __launch_bounds__(kFinishThreads) void k_policy_finish(const f32x4* __restrict__ partial, int64_t blocks,
+                                                                   const int64_t* __restrict__ counts, int count_blocks,
+                                                                   double kl, double ent, float* loss, float* stats,
+                                                                   int64_t* count) {
+  __shared__ double lds[5 * (kFinishThreads / 64)];
   double s[5] = {0.0, 0.0, 0.0, 0.0, 0.0};
-  for (int64_t i = threadIdx.x; i < blocks; i += kRowThreads)
-    for (int k = 0; k < 4; ++k) s[k] += partial[4 * i + k];
+#pragma unroll 4
+  for (int64_t i = threadIdx.x; i < blocks; i += kFinishThreads) {
+    const f32x4 v = partial[i];
+    for (int k = 0; k < 4; ++k) s[k] += (double)v[k];
+  }
   if (threadIdx.x < (uint32_t)count_blocks) s[4] = (double)counts[threadIdx.x];
-  for (int k = 0; k < 5; ++k) {
-    for (int d = 32; d >= 1; d >>= 1) s[k] += __shfl_xor(s[k], d, 64);
-    if ((threadIdx.x & 63) == 0) lds[k][threadIdx.x >> 6] = s[k];
-  }
-  __syncthreads();
+  block_sum<kFinishThreads, 5>(s, lds);
   if (threadIdx.x != 0) return;
-  for (int k = 0; k < 5; ++k) {
-    s[k] = 0.0;
-    for (int w = 0; w < kRowThreads / 64; ++w) s[k] += lds[k][w];
-  }
   const double n = s[4] > 0.0 ? s[4] : 1.0;
   for (int k = 0; k < 4; ++k) s[k] /= n;
   *loss = (float)(s[0] + (kl != 0.0 ? kl * s[1] : 0.0) - ent * s[2]);
@@ -800,11 +801,16 @@ struct PreferenceArgs {
   int wide;  // offsets are int64 (else int32)
   int64_t pairs;
   double beta, eps;
-  float* ratio;     // [n] a row's l - l_ref
-  double* partial;  // [pairs] a pair's cost; NaN where its offsets are not ascending within the rows
-  float* coef;      // [2 pairs]
-  float* rewards;   // [2 pairs]
-  void* grad;
+  float* loss;
+  float* rewards;   // [2 pairs] or null
+  void* grad;       // or null
+  double* partial;  // [blocks] a block's pairs' costs
+  int group;        // the short form: pairs a block
+  // the long form
+  int slices;     // of a sequence, summed by a block each
+  float* ratio;   // [n] a row's l - l_ref
+  double* sums;   // [2 pairs][slices]
+  float* coef;    // [2 pairs]
 };
 
 __device__ __forceinline__ int64_t raw_offset(const PreferenceArgs& q, int64_t s) {
@@ -812,21 +818,41 @@ __device__ __forceinline__ int64_t raw_offset(const PreferenceArgs& q, int64_t s
 }
 
 // Held to the rows: every row read is one of the call's.
-__device__ __forceinline__ int64_t offset_at(const PreferenceArgs& q, int64_t s) {
-  const int64_t o = raw_offset(q, s);
-  return o < 0 ? 0 : o > q.r.n ? q.r.n : o;
+__device__ __forceinline__ int64_t held(int64_t o, int64_t n) { return o < 0 ? 0 : o > n ? n : o; }
+__device__ __forceinline__ int64_t offset_at(const PreferenceArgs& q, int64_t s) { return held(raw_offset(q, s), q.r.n); }
+
+__device__ __forceinline__ double log1p_exp_neg(double x) {  // -log sigma(x)
+  return fmax(-x, 0.0) + log1p(exp(-fabs(x)));
 }
 
+// A pair from its sequences' summed log ratios: its cost, and coef, the
+// derivative in a chosen row's log ratio (a rejected row's is -coef).  NaN
+// where its offsets do not ascend within the rows.
+__device__ __forceinline__ double pair_cost(const PreferenceArgs& q, int64_t pair, double chosen, double rejected,
+                                            float* coef) {
+  chosen *= q.beta, rejected *= q.beta;
+  const double x = chosen - rejected;
+  double cost = (1.0 - q.eps) * log1p_exp_neg(x) + q.eps * log1p_exp_neg(-x);
+  double d = (q.eps - 1.0 / (1.0 + exp(x))) * q.beta / (double)q.pairs;
+  const int64_t r0 = raw_offset(q, 2 * pair), r1 = raw_offset(q, 2 * pair + 1), r2 = raw_offset(q, 2 * pair + 2);
+  if (r0 < 0 || r1 < r0 || r2 < r1 || r2 > q.r.n) cost = d = NAN;
+  if (q.rewards) q.rewards[2 * pair] = (float)chosen, q.rewards[2 * pair + 1] = (float)rejected;
+  *coef = (float)d;
+  return cost;
+}
+
+// One row's legal word and action: no legal action where it does not count.
+__device__ __forceinline__ uint32_t row_of(const Rows& r, int64_t i, bool mine, int& action) {
+  const uint32_t legal = mine ? legal_bits(r.mask[i], r.A) : 0u;
+  action = mine ? r.actions[i] : -1;
+  return decided(legal, action) ? legal : 0u;
+}
+
+// A tile's rows: this thread's log ratio, its e and their sum (x is spent).
 template <class T, int AP>
-__global__ __launch_bounds__(kRowThreads) void k_preference_rows(PreferenceArgs q) {
-  __shared__ __align__(16) char tile[Tile<T, AP>::kBytes];
-  const int64_t row0 = (int64_t)blockIdx.x * kRowThreads, i = row0 + threadIdx.x;
-  const int rows = (int)(q.r.n - row0 < kRowThreads ? q.r.n - row0 : kRowThreads);
-  const bool mine = (int)threadIdx.x < rows;
-  uint32_t legal = mine ? legal_bits(q.r.mask[i], q.r.A) : 0u;
-  const int action = mine ? q.r.actions[i] : -1;
-  if (!decided(legal, action)) legal = 0;
-  float x[AP], d[AP], e[AP];
+__device__ __forceinline__ float row_ratio(char* tile, const PreferenceArgs& q, int64_t row0, int rows, uint32_t legal,
+                                           int action, float (&e)[AP], float& sum) {
+  float x[AP], d[AP];
   if (q.r.ref) {
     stage_two<T, AP>(tile, q.r, row0, rows, legal, x, d);
   } else {
@@ -834,71 +860,185 @@ __global__ __launch_bounds__(kRowThreads) void k_preference_rows(PreferenceArgs 
     __syncthreads();
     Tile<T, AP>::read(tile, q.r.A, legal, x);
   }
-  if (!mine) return;
   float out = 0.0f;
+  sum = 1.0f;
   if (legal) {
-    Softmax s = softmax<AP>(x, e);
-#pragma unroll
-    for (int a = 0; a < AP; ++a)
-      if (a == action) out = x[a];
-    out -= s.lse;
     if (q.r.ref) {
-      s = softmax<AP>(d, e);
-      float z = 0.0f;
+      const Softmax s = softmax<AP>(d, e);
 #pragma unroll
       for (int a = 0; a < AP; ++a)
-        if (a == action) z = d[a];
-      out -= z - s.lse;
+        if (a == action) out = d[a];
+      out -= s.lse;
+    }
+    const Softmax s = softmax<AP>(x, e);
+    float z = 0.0f;
+#pragma unroll
+    for (int a = 0; a < AP; ++a)
+      if (a == action) z = x[a];
+    out = (z - s.lse) - out;
+    sum = s.sum;
+  }
+  return out;
+}
+
+// The gradient of a tile's rows, out of this thread's e, sum and coef.
+template <class T, int AP>
+__device__ __forceinline__ void row_grad(char* tile, const PreferenceArgs& q, int64_t row0, int rows, uint32_t legal,
+                                         int action, float (&e)[AP], float sum, float coef) {
+  const float p = -coef / sum;
+#pragma unroll
+  for (int a = 0; a < AP; ++a) e[a] = ((legal >> a) & 1u) ? p * e[a] + (a == action ? coef : 0.0f) : 0.0f;
+  Tile<T, AP>::write(tile, q.r.A, e);
+  __syncthreads();
+  Tile<T, AP>::copy_out(tile, (T*)q.grad, row0, rows, q.r.A);
+}
+
+// Short sequences (a game's decisions): a block takes `group` consecutive
+// pairs, whose rows are one run, mostly of one tile.  The tile is read once:
+// its rows' log ratios go to LDS, a wave sums each sequence's, the pairs'
+// costs follow, and the gradient is written from the e still in registers.
+// A group of more rows goes through its tiles twice.  Blocks past the groups
+// write the zero gradients of the rows outside every sequence.
+constexpr int kMaxGroup = 32, kZeroBlocks = 64;
+
+template <class T, int AP>
+__global__ __launch_bounds__(kRowThreads) void k_preference_short(PreferenceArgs q) {
+  __shared__ __align__(16) char tile[Tile<T, AP>::kBytes];
+  __shared__ float ratio[kRowThreads];
+  __shared__ int64_t edge[2 * kMaxGroup + 1];
+  __shared__ double sum[2 * kMaxGroup];
+  __shared__ float coef[2 * kMaxGroup];
+  __shared__ double lds[kRowThreads / 64];
+  const int64_t groups = (q.pairs + q.group - 1) / q.group;
+  if ((int64_t)blockIdx.x >= groups) {
+    if (!q.grad) return;
+    // rows before the first sequence and behind the last, by elements
+    const int64_t head = offset_at(q, 0) * q.r.A, tail = offset_at(q, 2 * q.pairs) * q.r.A, n = q.r.n * q.r.A;
+    const int64_t first = ((int64_t)blockIdx.x - groups) * kRowThreads + threadIdx.x;
+    for (int64_t k = first; k < head; k += (int64_t)kZeroBlocks * kRowThreads) ((T*)q.grad)[k] = (T)0.0f;
+    for (int64_t k = tail + first; k < n; k += (int64_t)kZeroBlocks * kRowThreads) ((T*)q.grad)[k] = (T)0.0f;
+    return;
+  }
+  const int64_t pair0 = (int64_t)blockIdx.x * q.group;
+  const int pairs = (int)(q.pairs - pair0 < q.group ? q.pairs - pair0 : q.group);
+  const int wave = (int)threadIdx.x >> 6, seqs = 2 * pairs;
+  if ((int)threadIdx.x <= seqs) edge[threadIdx.x] = offset_at(q, 2 * pair0 + threadIdx.x);
+  if ((int)threadIdx.x < seqs) sum[threadIdx.x] = 0.0;
+  __syncthreads();
+  const int64_t begin = edge[0], end = edge[seqs];
+  float e[AP], total = 1.0f;
+  uint32_t legal = 0;
+  int action = -1, rows = 0;
+  for (int64_t row0 = begin; row0 < end; row0 += kRowThreads) {
+    const int64_t i = row0 + threadIdx.x;
+    rows = (int)(end - row0 < kRowThreads ? end - row0 : kRowThreads);
+    legal = row_of(q.r, i, (int)threadIdx.x < rows, action);
+    ratio[threadIdx.x] = row_ratio<T, AP>(tile, q, row0, rows, legal, action, e, total);
+    __syncthreads();
+    for (int s = wave; s < seqs; s += kRowThreads / 64) {
+      const int64_t lo = edge[s] - row0, hi = edge[s + 1] - row0;
+      const int to = hi < rows ? (int)hi : rows;
+      double v = 0.0;
+      for (int k = (lo > 0 ? (int)lo : 0) + ((int)threadIdx.x & 63); k < to; k += 64) v += (double)ratio[k];
+#pragma unroll
+      for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d, 64);
+      if ((threadIdx.x & 63) == 0) sum[s] += v;
+    }
+    __syncthreads();
+  }
+  double cost[1] = {0.0};
+  if ((int)threadIdx.x < pairs) {
+    const int s = 2 * threadIdx.x;
+    cost[0] = pair_cost(q, pair0 + threadIdx.x, sum[s], sum[s + 1], &coef[s]);
+    coef[s + 1] = -coef[s];
+  }
+  block_sum<kRowThreads, 1>(cost, lds);  // its barrier also shows the coefs
+  if (threadIdx.x == 0) {
+    q.partial[blockIdx.x] = cost[0];
+    if (groups == 1) *q.loss = (float)(cost[0] / (double)q.pairs);
+  }
+  if (!q.grad) return;
+  const bool once = end - begin <= kRowThreads;
+  for (int64_t row0 = begin; row0 < end; row0 += kRowThreads) {
+    const int64_t i = row0 + threadIdx.x;
+    if (!once) {
+      rows = (int)(end - row0 < kRowThreads ? end - row0 : kRowThreads);
+      legal = row_of(q.r, i, (int)threadIdx.x < rows, action);
+      stage<T, AP>(tile, q.r.logits, q.r.stride, row0, rows, q.r.A);
+      __syncthreads();
+      float x[AP];
+      Tile<T, AP>::read(tile, q.r.A, legal, x);
+      total = softmax<AP>(x, e).sum;
+    }
+    int lo = 0, hi = seqs;  // the last sequence that starts at or before row i
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (edge[mid + 1] <= i) lo = mid + 1;
+      else hi = mid;
+    }
+    row_grad<T, AP>(tile, q, row0, rows, legal, action, e, total, lo < seqs ? coef[lo] : 0.0f);
+    __syncthreads();
+  }
+}
+
+// Long sequences: every row's log ratio to memory, the sequences' sums from
+// slices of them, the pairs, then the gradient with the logits read again
+// (A sizeof(T) of a row's 3 A sizeof(T) + 5 bytes).
+template <class T, int AP>
+__global__ __launch_bounds__(kRowThreads) void k_preference_rows(PreferenceArgs q) {
+  __shared__ __align__(16) char tile[Tile<T, AP>::kBytes];
+  const int64_t row0 = (int64_t)blockIdx.x * kRowThreads, i = row0 + threadIdx.x;
+  const int rows = (int)(q.r.n - row0 < kRowThreads ? q.r.n - row0 : kRowThreads);
+  const bool mine = (int)threadIdx.x < rows;
+  int action;
+  const uint32_t legal = row_of(q.r, i, mine, action);
+  float e[AP], total;
+  const float out = row_ratio<T, AP>(tile, q, row0, rows, legal, action, e, total);
+  if (mine) q.ratio[i] = out;
+}
+
+__global__ __launch_bounds__(kRowThreads) void k_preference_sums(PreferenceArgs q) {
+  __shared__ double lds[kRowThreads / 64];
+  const int64_t seq = (int64_t)blockIdx.x / q.slices;
+  const int slice = (int)((int64_t)blockIdx.x % q.slices);
+  const int64_t lo = offset_at(q, seq), hi = offset_at(q, seq + 1), len = hi > lo ? hi - lo : 0;
+  const int64_t from = lo + len / q.slices * slice + (len % q.slices) * slice / q.slices;
+  const int64_t to = lo + len / q.slices * (slice + 1) + (len % q.slices) * (slice + 1) / q.slices;
+  double s[1] = {0.0};
+#pragma unroll 4
+  for (int64_t i = from + threadIdx.x; i < to; i += kRowThreads) s[0] += (double)q.ratio[i];
+  block_sum<kRowThreads, 1>(s, lds);
+  if (threadIdx.x == 0) q.sums[blockIdx.x] = s[0];
+}
+
+constexpr int kPairThreads = 1024, kPairsABlock = 64;
+
+// A wave a pair: its slices' sums, its cost and coefs.
+__global__ __launch_bounds__(kPairThreads) void k_preference_pairs(PreferenceArgs q) {
+  __shared__ double lds[kPairThreads / 64];
+  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+  double cost[1] = {0.0};
+  for (int k = wave; k < kPairsABlock; k += kPairThreads / 64) {
+    const int64_t pair = (int64_t)blockIdx.x * kPairsABlock + k;
+    if (pair >= q.pairs) break;
+    double s[2] = {0.0, 0.0};
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      for (int j = lane; j < q.slices; j += 64) s[h] += q.sums[(2 * pair + h) * q.slices + j];
+#pragma unroll
+      for (int d = 32; d >= 1; d >>= 1) s[h] += __shfl_xor(s[h], d, 64);
+    }
+    if (lane == 0) {
+      float d;
+      cost[0] += pair_cost(q, pair, s[0], s[1], &d);
+      q.coef[2 * pair] = d, q.coef[2 * pair + 1] = -d;
     }
   }
-  q.ratio[i] = out;
-}
-
-__device__ __forceinline__ double log1p_exp_neg(double x) {  // -log sigma(x)
-  return fmax(-x, 0.0) + log1p(exp(-fabs(x)));
-}
-
-__global__ __launch_bounds__(kRowThreads) void k_preference_pairs(PreferenceArgs q) {
-  __shared__ double lds[2][kRowThreads / 64];
-  const int64_t pair = blockIdx.x;
-  const int64_t o0 = offset_at(q, 2 * pair), o1 = offset_at(q, 2 * pair + 1), o2 = offset_at(q, 2 * pair + 2);
-  double s[2] = {0.0, 0.0};
-  for (int64_t i = o0 + threadIdx.x; i < o1; i += kRowThreads) s[0] += (double)q.ratio[i];
-  for (int64_t i = o1 + threadIdx.x; i < o2; i += kRowThreads) s[1] += (double)q.ratio[i];
-  for (int k = 0; k < 2; ++k) {
-    for (int d = 32; d >= 1; d >>= 1) s[k] += __shfl_xor(s[k], d, 64);
-    if ((threadIdx.x & 63) == 0) lds[k][threadIdx.x >> 6] = s[k];
+  block_sum<kPairThreads, 1>(cost, lds);
+  if (threadIdx.x == 0) {
+    q.partial[blockIdx.x] = cost[0];
+    if (gridDim.x == 1) *q.loss = (float)(cost[0] / (double)q.pairs);
   }
-  __syncthreads();
-  if (threadIdx.x != 0) return;
-  for (int k = 0; k < 2; ++k) {
-    s[k] = 0.0;
-    for (int w = 0; w < kRowThreads / 64; ++w) s[k] += lds[k][w];
-    s[k] *= q.beta;
-  }
-  const double x = s[0] - s[1];
-  double cost = (1.0 - q.eps) * log1p_exp_neg(x) + q.eps * log1p_exp_neg(-x);
-  double d = (q.eps - 1.0 / (1.0 + exp(x))) * q.beta / (double)q.pairs;
-  const int64_t r0 = raw_offset(q, 2 * pair), r1 = raw_offset(q, 2 * pair + 1), r2 = raw_offset(q, 2 * pair + 2);
-  if (r0 < 0 || r1 < r0 || r2 < r1 || r2 > q.r.n) cost = d = NAN;
-  q.partial[pair] = cost;
-  q.coef[2 * pair] = (float)d;
-  q.coef[2 * pair + 1] = (float)-d;
-  if (q.rewards) q.rewards[2 * pair] = (float)s[0], q.rewards[2 * pair + 1] = (float)s[1];
-}
-
-__global__ __launch_bounds__(kRowThreads) void k_preference_finish(const double* __restrict__ partial, int64_t pairs,
-                                                                    float* loss) {
-  __shared__ double lds[kRowThreads / 64];
-  double s = 0.0;
-  for (int64_t i = threadIdx.x; i < pairs; i += kRowThreads) s += partial[i];
-  for (int d = 32; d >= 1; d >>= 1) s += __shfl_xor(s, d, 64);
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = s;
-  __syncthreads();
-  if (threadIdx.x != 0) return;
-  s = 0.0;
-  for (int w = 0; w < kRowThreads / 64; ++w) s += lds[w];
-  *loss = (float)(s / (double)(pairs > 0 ? pairs : 1));
 }
 
 template <class T, int AP>
@@ -906,11 +1046,10 @@ __global__ __launch_bounds__(kRowThreads) void k_preference_grad(PreferenceArgs 
   __shared__ __align__(16) char tile[Tile<T, AP>::kBytes];
   const int64_t row0 = (int64_t)blockIdx.x * kRowThreads, i = row0 + threadIdx.x;
   const int rows = (int)(q.r.n - row0 < kRowThreads ? q.r.n - row0 : kRowThreads);
-  const bool mine = (int)threadIdx.x < rows;
-  uint32_t legal = mine ? legal_bits(q.r.mask[i], q.r.A) : 0u;
-  const int action = mine ? q.r.actions[i] : -1;
+  int action;
+  const uint32_t legal = row_of(q.r, i, (int)threadIdx.x < rows, action);
   float coef = 0.0f;
-  if (decided(legal, action)) {
+  if (legal) {
     // the last sequence that starts at or before row i (the non-empty one where several start there)
     int64_t lo = 0, hi = 2 * q.pairs + 1;  // offsets[lo - 1] <= i < offsets[hi]
     while (lo < hi) {
@@ -920,23 +1059,28 @@ __global__ __launch_bounds__(kRowThreads) void k_preference_grad(PreferenceArgs 
     }
     if (lo >= 1 && lo <= 2 * q.pairs) coef = q.coef[lo - 1];
   }
-  if (coef == 0.0f) legal = 0;
   stage<T, AP>(tile, q.r.logits, q.r.stride, row0, rows, q.r.A);
   __syncthreads();
-  float x[AP], e[AP];
-  Tile<T, AP>::read(tile, q.r.A, legal, x);
-  if (legal) {
-    const Softmax s = softmax<AP>(x, e);
-    const float p = -coef / s.sum;
-#pragma unroll
-    for (int a = 0; a < AP; ++a) x[a] = ((legal >> a) & 1u) ? p * e[a] + (a == action ? coef : 0.0f) : 0.0f;
+  float x[AP], e[AP], total = 1.0f;
+  Tile<T, AP>::read(tile, q.r.A, coef == 0.0f ? 0u : legal, x);
+  if (coef != 0.0f) {
+    total = softmax<AP>(x, e).sum;
   } else {
 #pragma unroll
-    for (int a = 0; a < AP; ++a) x[a] = 0.0f;
+    for (int a = 0; a < AP; ++a) e[a] = 0.0f;
   }
-  Tile<T, AP>::write(tile, q.r.A, x);
-  __syncthreads();
-  Tile<T, AP>::copy_out(tile, (T*)q.grad, row0, rows, q.r.A);
+  row_grad<T, AP>(tile, q, row0, rows, legal, action, e, total, coef);
+}
+
+// The blocks' costs in a fixed order.
+__global__ __launch_bounds__(kFinishThreads) void k_preference_finish(const double* __restrict__ partial, int64_t blocks,
+                                                                       int64_t pairs, float* loss) {
+  __shared__ double lds[kFinishThreads / 64];
+  double s[1] = {0.0};
+#pragma unroll 4
+  for (int64_t i = threadIdx.x; i < blocks; i += kFinishThreads) s[0] += partial[i];
+  block_sum<kFinishThreads, 1>(s, lds);
+  if (threadIdx.x == 0) *loss = (float)(s[0] / (double)(pairs > 0 ? pairs : 1));
 }
 
 // ---------------------------------------------------------- grad scaling
@@ -1013,40 +1157,82 @@ inline void launch_advantages(const AdvantageArgs& q, int players, hipStream_t s
   }
 }
 
-inline size_t policy_workspace(int64_t n) { return sizeof(int64_t) * kCountBlocks + sizeof(double) * 4 * row_blocks(n); }
+inline size_t policy_workspace(int64_t n) { return sizeof(int64_t) * kCountBlocks + sizeof(f32x4) * row_blocks(n); }
 
 inline void launch_policy(PolicyArgs q, int dtype, double kl, double ent, float* loss, float* stats, int64_t* count,
                           void* workspace, hipStream_t s) {
   const unsigned blocks = row_blocks(q.r.n);
-  q.counts = (int64_t*)workspace;
-  q.partial = (double*)(q.counts + kCountBlocks);
-  q.count_blocks = blocks < (unsigned)kCountBlocks ? (int)blocks : kCountBlocks;
+  const int64_t counters = (q.r.n + 4 * kCountThreads - 1) / (4 * kCountThreads);
+  q.partial = (f32x4*)workspace;
+  q.counts = (int64_t*)(q.partial + blocks);
+  q.count_blocks = (int)(counters < kCountBlocks ? counters : kCountBlocks);
   if (blocks) {
-    k_policy_count<<<q.count_blocks, kRowThreads, 0, s>>>(q);
+    k_policy_count<<<q.count_blocks, kCountThreads, 0, s>>>(q);
     with_rows(dtype, q.r.A, [&](auto t, auto ap) {
       using T = typename decltype(t)::type;
       k_policy_loss<T, decltype(ap)::value><<<blocks, kRowThreads, 0, s>>>(q);
     });
   }
-  k_policy_finish<<<1, kRowThreads, 0, s>>>(q.partial, blocks, q.counts, q.count_blocks, kl, ent, loss, stats, count);
+  k_policy_finish<<<1, kFinishThreads, 0, s>>>(q.partial, blocks, q.counts, q.count_blocks, kl, ent, loss, stats, count);
+}
+
+// How a preference call is split.  Short where a pair has at most kShortRows
+// rows on average: `group` pairs a block, some 5 / 8 of a tile so that few
+// groups spill into a second; else a sequence's sum takes a block per 4096
+// rows of the average one.
+constexpr int kShortRows = 160;
+
+struct PreferencePlan {
+  bool is_short;
+  int group, slices;
+  int64_t blocks;  // that leave a partial sum
+};
+
+inline PreferencePlan preference_plan(int64_t n, int64_t pairs) {
+  PreferencePlan p{};
+  const int64_t each = pairs ? n / pairs : 0;
+  p.is_short = each <= kShortRows;
+  if (p.is_short) {
+    const int64_t g = kShortRows / (each > 0 ? each : 1);
+    p.group = (int)(g < kMaxGroup ? g : kMaxGroup);
+    p.blocks = (pairs + p.group - 1) / p.group;
+  } else {
+    const int64_t sl = each / 2 / 4096;
+    p.slices = (int)(sl < 1 ? 1 : sl > 256 ? 256 : sl);
+    p.blocks = (pairs + kPairsABlock - 1) / kPairsABlock;
+  }
+  return p;
 }
 
 inline size_t preference_workspace(int64_t n, int64_t pairs) {
-  return sizeof(double) * pairs + sizeof(float) * 2 * pairs + sizeof(float) * n;
+  const PreferencePlan p = preference_plan(n, pairs);
+  const size_t partial = sizeof(double) * (p.blocks + 1);
+  if (p.is_short) return partial;
+  return partial + sizeof(double) * 2 * pairs * p.slices + sizeof(float) * (2 * pairs + n);
 }
 
-inline void launch_preference(PreferenceArgs q, int dtype, float* loss, void* workspace, hipStream_t s) {
+inline void launch_preference(PreferenceArgs q, int dtype, void* workspace, hipStream_t s) {
+  const PreferencePlan p = preference_plan(q.r.n, q.pairs);
   q.partial = (double*)workspace;
-  q.coef = (float*)(q.partial + q.pairs);
-  q.ratio = q.coef + 2 * q.pairs;
-  const unsigned blocks = row_blocks(q.r.n);
+  q.group = p.group;
+  q.slices = p.slices;
+  const unsigned tiles = row_blocks(q.r.n);
   with_rows(dtype, q.r.A, [&](auto t, auto ap) {
     using T = typename decltype(t)::type;
     constexpr int AP = decltype(ap)::value;
-    if (blocks) k_preference_rows<T, AP><<<blocks, kRowThreads, 0, s>>>(q);
-    if (q.pairs) k_preference_pairs<<<(unsigned)q.pairs, kRowThreads, 0, s>>>(q);
-    k_preference_finish<<<1, kRowThreads, 0, s>>>(q.partial, q.pairs, loss);
-    if (blocks && q.grad) k_preference_grad<T, AP><<<blocks, kRowThreads, 0, s>>>(q);
+    if (p.is_short) {
+      const int64_t grid = p.blocks + (q.grad && q.r.n ? kZeroBlocks : 0);
+      if (grid) k_preference_short<T, AP><<<(unsigned)grid, kRowThreads, 0, s>>>(q);
+    } else {
+      q.sums = q.partial + p.blocks + 1;
+      q.coef = (float*)(q.sums + 2 * q.pairs * p.slices);
+      q.ratio = q.coef + 2 * q.pairs;
+      k_preference_rows<T, AP><<<tiles, kRowThreads, 0, s>>>(q);
+      k_preference_sums<<<(unsigned)(2 * q.pairs * p.slices), kRowThreads, 0, s>>>(q);
+      k_preference_pairs<<<(unsigned)p.blocks, kPairThreads, 0, s>>>(q);
+      if (q.grad) k_preference_grad<T, AP><<<tiles, kRowThreads, 0, s>>>(q);
+    }
+    if (p.blocks != 1) k_preference_finish<<<1, kFinishThreads, 0, s>>>(q.partial, p.blocks, q.pairs, q.loss);
   });
 }
 

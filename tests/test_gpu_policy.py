@@ -420,7 +420,11 @@ def _check_preference(got, o, x, mask, beta, dtype):
 @pytest.mark.parametrize("dtype", DTYPES, ids=lambda d: str(d)[6:])
 @pytest.mark.parametrize("offsets,n,A", [([0, 1, 2], 2, 18), ([0, 0, 0], 3, 18), ([2, 30, 64, 64, 97], 101, 18),
                                          ([0, 300, 1300], 1300, 18), ([0] + [7 * k + k % 3 for k in range(1, 129)], 930, 5),
-                                         ([0, 0, 900, 900, 1800], 1803, 31), ([0], 4, 18)], ids=lambda v: str(v)[:18])
+                                         ([0, 0, 900, 900, 1800], 1803, 31), ([0], 4, 18),
+                                         # short sequences but for one of several tiles; and 70 pairs of long ones
+                                         ([0] + [3 + 21 * k + 700 * (k > 11) for k in range(1, 81)], 2400, 18),
+                                         ([5 + 90 * k + k % 7 for k in range(141)], 12700, 3)],
+                         ids=lambda v: str(v)[:18])
 @pytest.mark.parametrize("with_ref,eps", [(True, 0.0), (False, 0.2)])
 def test_preference_loss(offsets, n, A, with_ref, eps, dtype):
     gen = torch.Generator().manual_seed(n + A)
