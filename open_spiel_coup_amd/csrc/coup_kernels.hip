@@ -4924,10 +4924,10 @@ int coup_policy_loss(const coup_decisions* d, const coup_policy_terms* terms, co
   q.old = terms->old_log_probs;
   q.adv = terms->advantages;
   q.active = terms->active;
-  q.low = (float)(1.0 - terms->clip_low);
-  q.high = (float)(1.0 + terms->clip_high);
-  q.log_low = std::log1p(-terms->clip_low);
-  q.log_high = std::log1p(terms->clip_high);
+  q.low = 1.0 - terms->clip_low;
+  q.high = 1.0 + terms->clip_high;
+  q.log_low = (float)std::log1p(-terms->clip_low);
+  q.log_high = (float)std::log1p(terms->clip_high);
   q.kl = (float)terms->kl_coef;
   q.ent = (float)terms->entropy_coef;
   q.log_probs = out->log_probs;

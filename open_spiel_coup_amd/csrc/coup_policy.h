@@ -32,7 +32,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kRowThreads = 256;
-constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 constexpr float kLowest = -3.402823466e38f;
 
 template <class T>
@@ -58,6 +58,25 @@ __device__ __forceinline__ uint32_t legal_bits(uint32_t mask, int A) {
 
 __device__ __forceinline__ bool decided(uint32_t legal, int action) {
   return action >= 0 && action < 31 && ((legal >> action) & 1u);
+}
+
+// v where bit a of `legal` is set, else `other`: a field extract and a bit
+// select (the compiler, seeing what m is, would make a test, a comparison and
+// a conditional move of it).
+__device__ __forceinline__ float keep(uint32_t legal, int a, float v, float other) {
+  uint32_t m = (uint32_t)__builtin_amdgcn_sbfe((int)legal, a, 1);
+  asm("" : "+v"(m));
+  return __uint_as_float((__float_as_uint(v) & m) | (__float_as_uint(other) & ~m));
+}
+
+// One row's legal word and action: no legal action, and action 0, where it
+// does not count.
+__device__ __forceinline__ uint32_t row_of(const Rows& r, int64_t i, bool mine, int& action) {
+  const uint32_t legal = mine ? legal_bits(r.mask[i], r.A) : 0u;
+  action = mine ? r.actions[i] : 0;
+  if (decided(legal, action)) return legal;
+  action = 0;
+  return 0u;
 }
 
 // ------------------------------------------------- rows through the LDS
@@ -98,9 +117,9 @@ struct Tile {
     const int bytes = rows * A * (int)sizeof(T);
 #pragma unroll
     for (int c = 0; c < kPieces; ++c) {
-      const int at = (c * kRowThreads + (int)threadIdx.x) * 16;
+      const uint32_t at = (c * kRowThreads + threadIdx.x) * 16;
       f.piece[c] = u32x4{0, 0, 0, 0};
-      if (at + 16 <= bytes) f.piece[c] = *(const piece_at*)(src + at);
+      if ((int)at + 16 <= bytes) f.piece[c] = *(const piece_at*)(src + at);
     }
   }
 
@@ -127,10 +146,19 @@ struct Tile {
   // The same through elements, for strided rows.
   static __device__ __forceinline__ void copy_in(char* lds, const T* base, int64_t stride, int64_t row0, int rows, int A) {
     const uint32_t inv = ((1u << 20) + A - 1) / A;  // e / A = e inv >> 20: e < 256 A, and e (A - 1) < 2^20
+#pragma unroll 1
     for (int e = (int)threadIdx.x; e < rows * A; e += kRowThreads) {
       const int r = (int)((uint32_t)e * inv >> 20);
       *(T*)(lds + at_element(e, A)) = base[(row0 + r) * stride + (e - r * A)];
     }
+  }
+
+  // This thread's logit of one action.
+  static __device__ __forceinline__ float read_one(const char* lds, int A, int action) {
+    return widen(*(const T*)(lds + at_element((int)threadIdx.x * A + action, A)));
+  }
+  static __device__ __forceinline__ void write_one(char* lds, int A, int action, float g) {
+    *(T*)(lds + at_element((int)threadIdx.x * A + action, A)) = (T)g;
   }
 
   // This thread's row, widened; -inf at actions outside `legal`.
@@ -161,8 +189,14 @@ struct Tile {
 #pragma unroll
       for (int a = 0; a < AP; ++a) x[a] = widen(row[a]);
     }
+    // The masks are made here, not kept from another table's, and used here,
+    // not carried beside the raw logits to where x is.
+    asm volatile("" : "+v"(legal));
 #pragma unroll
-    for (int a = 0; a < AP; ++a) x[a] = ((legal >> a) & 1u) ? x[a] : -INFINITY;
+    for (int a = 0; a < AP; ++a) {
+      x[a] = keep(legal, a, x[a], -INFINITY);
+      asm volatile("" : "+v"(x[a]));
+    }
   }
 
   // This thread's row of results, rounded, over its row.
@@ -202,7 +236,7 @@ struct Tile {
 #pragma unroll
     for (int c = 0; c < kPieces; ++c) {
       const int k = c * kRowThreads + (int)threadIdx.x;
-      if (k * 16 + 16 <= bytes) ((piece_at*)dst)[k] = *(const u32x4*)(lds + (w ? place(k) : k) * 16);
+      if (k * 16 + 16 <= bytes) *(piece_at*)((char*)dst + (uint32_t)k * 16) = *(const u32x4*)(lds + (w ? place(k) : k) * 16);
     }
     const int e = bytes / 16 * 16 / (int)sizeof(T) + (int)threadIdx.x;  // the last piece's rest (none of whole rows)
     if (e < n) dst[e] = ((const T*)lds)[e];
@@ -223,69 +257,116 @@ __device__ __forceinline__ void stage(char* lds, const void* base, int64_t strid
   }
 }
 
-// Two tables' rows through one tile: x, then (where `ref`) d.  Both are in
-// flight before the first is waited for.
+// Two tables' rows through one tile: x, then d, and both's logits of `action`.
+// Both are in flight before the first is waited for.
 template <class T, int AP>
-__device__ __forceinline__ void stage_two(char* lds, const Rows& q, int64_t row0, int rows, uint32_t legal,
-                                          float (&x)[AP], float (&d)[AP]) {
+__device__ __forceinline__ void stage_two(char* lds, const Rows& q, int64_t row0, int rows, uint32_t legal, int action,
+                                          float (&x)[AP], float& xa, float (&d)[AP], float& da) {
   using Tl = Tile<T, AP>;
-  if (q.stride == q.A && q.ref_stride == q.A) {
-    typename Tl::Flight f, g;
+  typename Tl::Flight g;
+  const bool pieces = q.stride == q.A && q.ref_stride == q.A;
+  if (pieces) {
+    typename Tl::Flight f;
     Tl::fetch(f, (const T*)q.logits, row0, rows, q.A);
     Tl::fetch(g, (const T*)q.ref, row0, rows, q.A);
     Tl::land(f, lds, (const T*)q.logits, row0, rows, q.A);
-    __syncthreads();
-    Tl::read(lds, q.A, legal, x);
-    __syncthreads();
-    Tl::land(g, lds, (const T*)q.ref, row0, rows, q.A);
-    __syncthreads();
-    Tl::read(lds, q.A, legal, d);
   } else {
     Tl::copy_in(lds, (const T*)q.logits, q.stride, row0, rows, q.A);
-    __syncthreads();
-    Tl::read(lds, q.A, legal, x);
-    __syncthreads();
-    Tl::copy_in(lds, (const T*)q.ref, q.ref_stride, row0, rows, q.A);
-    __syncthreads();
-    Tl::read(lds, q.A, legal, d);
   }
+  __syncthreads();
+  Tl::read(lds, q.A, legal, x);
+  xa = Tl::read_one(lds, q.A, action);
+  __syncthreads();
+  if (pieces) Tl::land(g, lds, (const T*)q.ref, row0, rows, q.A);
+  else Tl::copy_in(lds, (const T*)q.ref, q.ref_stride, row0, rows, q.A);
+  __syncthreads();
+  Tl::read(lds, q.A, legal, d);
+  da = Tl::read_one(lds, q.A, action);
+}
+
+// The logits' rows alone, or (REF) both.  `action` must be one of the A (0 for rows that do not count).
+template <class T, int AP, bool REF>
+__device__ __forceinline__ void stage_rows(char* lds, const Rows& q, int64_t row0, int rows, uint32_t legal, int action,
+                                           float (&x)[AP], float& xa, float (&d)[AP], float& da) {
+  if (REF) {
+    stage_two<T, AP>(lds, q, row0, rows, legal, action, x, xa, d, da);
+  } else {
+    stage<T, AP>(lds, q.logits, q.stride, row0, rows, q.A);
+    __syncthreads();
+    Tile<T, AP>::read(lds, q.A, legal, x);
+    xa = Tile<T, AP>::read_one(lds, q.A, action);
+    da = 0.0f;
+  }
+}
+
+// The larger; NaN where either is (one instruction, and for three values too).
+__device__ __forceinline__ float max_of(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
+// The hardware's base-2 logarithm, exponential and reciprocal, each good to
+// a unit in the last place.
+__device__ __forceinline__ float log_of(float v) { return __builtin_amdgcn_logf(v) * kLn2; }  // v >= 1, or of a ratio
+__device__ __forceinline__ float exp_of(float v) {  // the product's rounding is made good
+  const float hi = v * kLog2e, lo = __builtin_fmaf(v, kLog2e, -hi);
+  const float e = __builtin_amdgcn_exp2f(hi);
+  return lo == lo ? __builtin_fmaf(e * lo, kLn2, e) : e;
+}
+// log(1 + v), 0 <= v: the rounding of w = 1 + v is made good by v / (w - 1),
+// along which log(w) / (w - 1) hardly changes.
+__device__ __forceinline__ float log1p_of(float v) {
+  const float w = 1.0f + v, d = w - 1.0f;
+  return d == 0.0f ? v : log_of(w) * (v * __builtin_amdgcn_rcpf(d));
 }
 
 struct Softmax {
-  float m;     // largest logit
-  float sum;   // sum of e
-  float lse;   // log of the sum: log p_a = (x_a - m) - lse
+  float m;    // largest logit
+  float sum;  // sum of e
+  float lse;  // log of the sum (precise only): log p_a = (x_a - m) - lse
+  __device__ __forceinline__ float e(float logit) const { return __builtin_amdgcn_exp2f((logit - m) * kLog2e); }
+  __device__ __forceinline__ float t(float logit) const { return max_of(logit - m, kLowest); }
 };
 
-// x becomes x - m and e = exp(x - m).  The sum is at least 1 (the largest
-// logit's own e); when only one e is 1, lse is taken as log1p of the others'
-// sum, so a nearly certain action's log probability keeps its precision.
 template <int AP>
+__device__ __forceinline__ float row_max(const float (&x)[AP]) {
+  float m = x[0];
+#pragma unroll
+  for (int a = 1; a < AP; ++a) m = max_of(m, x[a]);
+  return m;
+}
+
+// The log of a row's sum of e, `others` the sum of the e's fractions, that is
+// without the ones: log1p of it while only one e is 1, so that a nearly
+// certain action's log probability keeps its precision.
+__device__ __forceinline__ float lse_of(float sum, float others) {
+  return sum - others < 1.5f ? log1p_of(others) : log_of(sum);
+}
+
+// e = exp(x - m), and x becomes t = x - m held above -inf, so that e t is 0
+// where e is; a NaN or +inf logit makes the sum NaN.  The sum is at least 1,
+// the largest logit's own e.  PRECISE: also lse.
+template <bool PRECISE, int AP>
 __device__ __forceinline__ Softmax softmax(float (&x)[AP], float (&e)[AP]) {
   Softmax s;
-  s.m = x[0];
-#pragma unroll
-  for (int a = 1; a < AP; ++a) s.m = fmaxf(s.m, x[a]);
+  s.m = row_max<AP>(x);
   s.sum = 0.0f;
-  float others = 0.0f;  // the sum without the ones: fract(1) = 0
+  float others = 0.0f;
 #pragma unroll
   for (int a = 0; a < AP; ++a) {
-    x[a] -= s.m;
-    e[a] = __builtin_amdgcn_exp2f(x[a] * kLog2e);
+    e[a] = s.e(x[a]);
+    x[a] = s.t(x[a]);
     s.sum += e[a];
-    others += __builtin_amdgcn_fractf(e[a]);
+    if (PRECISE) others += __builtin_amdgcn_fractf(e[a]);
   }
-  s.lse = (s.sum - others < 1.5f) ? log1pf(others) : logf(s.sum);
+  s.lse = PRECISE ? lse_of(s.sum, others) : 0.0f;
   return s;
 }
 
-// The same statistics of a row in 64 bits, for the rows next to a border.
+// A row's sum of e in 64 bits, for the rows next to a border.
 template <class T>
-__device__ __forceinline__ double lse64(const T* row, uint32_t legal, float m) {
+__device__ __forceinline__ double sum64(const T* row, uint32_t legal, float m) {
   double sum = 0.0;
 #pragma unroll 1
   for (uint32_t b = legal; b; b &= b - 1) sum += exp((double)widen(row[__builtin_ctz(b)]) - (double)m);
-  return log(sum);
+  return sum;
 }
 
 // The action a uniform number u falls on: the first legal a whose running
@@ -293,10 +374,7 @@ __device__ __forceinline__ double lse64(const T* row, uint32_t legal, float m) {
 // leaves the total at or below it.
 template <class T>
 __device__ __forceinline__ int pick64(const T* row, uint32_t legal, float m, float u) {
-  double total = 0.0;
-#pragma unroll 1
-  for (uint32_t b = legal; b; b &= b - 1) total += exp((double)widen(row[__builtin_ctz(b)]) - (double)m);
-  const double t = (double)u * total;
+  const double t = (double)u * sum64(row, legal, m);
   double c = 0.0;
   int last = -1;
 #pragma unroll 1
@@ -336,26 +414,22 @@ __global__ __launch_bounds__(kRowThreads) void k_sample(Rows r, const float* __r
   if (legal) {
     float x[AP], e[AP];
     Tile<T, AP>::read(lds, r.A, legal, x);
-    const Softmax s = softmax<AP>(x, e);
+    const Softmax s = softmax<true, AP>(x, e);
     if (s.sum == s.sum) {
       bool near = !(u < 1.0f);  // outside [0, 1): below as 0, above (and a NaN) the last action with a share
       u = u < 0.0f ? 0.0f : u;
       const float t = u * s.sum;
-      float c = 0.0f, xa = 0.0f, gap = INFINITY;
+      float c = 0.0f, gap = INFINITY;
+      action = 0;  // the actions whose running sums are no more than t
 #pragma unroll
-      for (int a = AP - 1; a >= 0; --a) {  // from above: the sums still to come
-        const float rest = (s.sum - c) - t;  // the running sum through a, less u total
-        gap = fminf(gap, fabsf(rest));
-        if (rest > 0.0f) action = a, xa = x[a];
+      for (int a = 0; a < AP; ++a) {
         c += e[a];
+        gap = fminf(gap, fabsf(c - t));
+        action += c <= t;
       }
       near |= gap <= kPickMargin * s.sum;
-      if (near) {
-        const T* row = (const T*)r.logits + i * r.stride;
-        action = pick64(row, legal, s.m, u);
-        xa = widen(row[action]) - s.m;
-      }
-      logp = xa - s.lse;
+      if (near) action = pick64((const T*)r.logits + i * r.stride, legal, s.m, u);
+      logp = (Tile<T, AP>::read_one(lds, r.A, action) - s.m) - s.lse;
     } else {
       logp = s.sum;  // NaN or +inf at a legal action: no distribution, no action
     }
@@ -586,6 +660,24 @@ __global__ __launch_bounds__(NT) void k_advantages(AdvantageArgs q) {
 
 // ----------------------------------------------------- sums over a block
 
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+  for (int s = 32; s >= 1; s >>= 1) v += __shfl_xor(v, s, 64);
+  return v;
+}
+
+// Four values summed over the wave at once: the sum of value k is lane k's (7
+// exchanges for 24: each of the first two halves what a lane still holds).
+__device__ __forceinline__ float wave_sum_four(const float (&v)[4]) {
+  const bool odd = threadIdx.x & 1, upper = threadIdx.x & 2;
+  const float a = (odd ? v[1] : v[0]) + __shfl_xor(odd ? v[0] : v[1], 1, 64);
+  const float b = (odd ? v[3] : v[2]) + __shfl_xor(odd ? v[2] : v[3], 1, 64);
+  float s = (upper ? b : a) + __shfl_xor(upper ? a : b, 2, 64);
+#pragma unroll
+  for (int d = 4; d < 64; d *= 2) s += __shfl_xor(s, d, 64);
+  return s;
+}
+
 // Each of v[0..K) summed over the block, in a fixed order; thread 0 has the
 // sums.  lds: K THREADS / 64 values.
 template <int THREADS, int K, class V>
@@ -618,13 +710,14 @@ struct PolicyArgs {
   const float* old;
   const float* adv;
   const uint8_t* active;  // null: every row
-  float low, high;              // 1 - clip_low, 1 + clip_high
-  double log_low, log_high;     // their logs
+  double low, high;           // 1 - clip_low, 1 + clip_high
+  float log_low, log_high;    // their logs
   float kl, ent;
   float* log_probs;  // null: not wanted
   void* grad;        // null: no gradient
   f32x4* partial;    // [blocks] sums of the terms over a block's rows
-  int64_t* counts;   // [count blocks] decisions
+  int32_t* decided;  // [blocks] its decisions
+  int64_t* counts;   // [count blocks] the call's decisions, for the gradient
   int count_blocks;
 };
 
@@ -660,93 +753,91 @@ __global__ __launch_bounds__(kCountThreads) void k_policy_count(PolicyArgs q) {
   q.counts[blockIdx.x] = total;
 }
 
-template <class T, int AP>
-__global__ __launch_bounds__(kRowThreads) void k_policy_loss(PolicyArgs q) {
+template <class T, int AP, bool REF>
+__global__ __launch_bounds__(kRowThreads, AP <= 20 ? 4 : 2) void k_policy_loss(PolicyArgs q) {
   __shared__ float lds[4 * (kRowThreads / 64)];
+  __shared__ int decisions[kRowThreads / 64];
   __shared__ __align__(16) char tile[Tile<T, AP>::kBytes];
-  __shared__ int64_t total;
-  int64_t c = threadIdx.x < (uint32_t)q.count_blocks ? q.counts[threadIdx.x] : 0;
-  {
-    __shared__ int64_t wave[kRowThreads / 64];
-#pragma unroll
-    for (int s = 32; s >= 1; s >>= 1) c += __shfl_xor(c, s, 64);
-    if ((threadIdx.x & 63) == 0) wave[threadIdx.x >> 6] = c;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      int64_t n = 0;
-      for (int w = 0; w < kRowThreads / 64; ++w) n += wave[w];
-      total = n;
-    }
-    __syncthreads();
-  }
-  const float scale = 1.0f / (float)(total > 0 ? total : 1);
-
   const int64_t row0 = (int64_t)blockIdx.x * kRowThreads, i = row0 + threadIdx.x;
   const int rows = (int)(q.r.n - row0 < kRowThreads ? q.r.n - row0 : kRowThreads);
   const bool mine = (int)threadIdx.x < rows;
-  uint32_t legal = 0;
-  int action = -1;
+  // the decisions of the call: every wave adds the counting blocks' numbers
+  // (as 32-bit floats: they scale the gradient)
+  float count = 0.0f;
+  if (q.grad) {
+#pragma unroll
+    for (int k = 0; k < kCountBlocks; k += 64) {
+      const int at = k + ((int)threadIdx.x & 63);
+      if (at < q.count_blocks) count += (float)q.counts[at];
+    }
+  }
+  int action;
+  uint32_t legal = row_of(q.r, i, mine, action);
   float old = 0.0f, adv = 0.0f;
   if (mine) {
-    legal = legal_bits(q.r.mask[i], q.r.A);
-    action = q.r.actions[i];
-    if (!decided(legal, action) || (q.active && !q.active[i])) legal = 0;
+    if (q.active && !q.active[i]) legal = 0;
     old = q.old[i];
     adv = q.adv[i];
   }
-  float x[AP], e[AP], d[AP];
-  if (q.r.ref) {
-    stage_two<T, AP>(tile, q.r, row0, rows, legal, x, d);
-  } else {
-    stage<T, AP>(tile, q.r.logits, q.r.stride, row0, rows, q.r.A);
-    __syncthreads();
-    Tile<T, AP>::read(tile, q.r.A, legal, x);
-  }
-  float surrogate = 0.0f, kl = 0.0f, entropy = 0.0f, clipped = 0.0f, logp = 0.0f;
+  float x[AP], d[AP], xa, da;
+  stage_rows<T, AP, REF>(tile, q.r, row0, rows, legal, action, x, xa, d, da);
+  const float n = wave_sum(count), scale = 1.0f / (n > 0.0f ? n : 1.0f);
+  float surrogate = 0.0f, kl = 0.0f, entropy = 0.0f, clipped = 0.0f, logp = 0.0f, ga = 0.0f;
   if (legal) {
-    float rlse = 0.0f;
-    if (q.r.ref) {
-      rlse = softmax<AP>(d, e).lse;
+    Softmax rs{0.0f, 1.0f, 0.0f};
+    if (REF) {
+      float e[AP];
+      rs = softmax<false, AP>(d, e);
     }
-    const Softmax s = softmax<AP>(x, e);
-    const float inv = 1.0f / s.sum;
-    float z = 0.0f;
+    // x becomes e; d becomes the part of w_b (below) that is known by now
+    Softmax s;
+    s.m = row_max<AP>(x);
+    s.sum = 0.0f;
+    float others = 0.0f, et = 0.0f, ed = 0.0f;  // sums of e t and, with d = t - t_ref, of e d
 #pragma unroll
     for (int a = 0; a < AP; ++a) {
-      e[a] *= inv;  // p
-      if (a == action) z = x[a];
-      x[a] = fmaxf(x[a] - s.lse, kLowest);  // log p; finite, so that 0 log 0 is 0
-      entropy -= e[a] * x[a];
-      if (q.r.ref) {
-        d[a] = ((legal >> a) & 1u) ? x[a] - (d[a] - rlse) : 0.0f;
-        kl += e[a] * d[a];
-      }
+      const float t = s.t(x[a]), ea = s.e(x[a]);
+      s.sum += ea;
+      others += __builtin_amdgcn_fractf(ea);
+      et += ea * t;
+      const float dt = REF ? t - d[a] : 0.0f;
+      if (REF) ed += ea * dt;
+      d[a] = REF ? q.ent * t + q.kl * dt : q.ent * t;
+      x[a] = ea;
     }
-    if (kl > 1e30f) kl = INFINITY;  // an action that the reference never takes
-    logp = z - s.lse;
+    s.lse = lse_of(s.sum, others);
+    const float inv = __builtin_amdgcn_rcpf(s.sum);
+    et *= inv, ed *= inv;
+    entropy = s.lse - et;
+    if (REF) {
+      kl = ed - log_of(s.sum * __builtin_amdgcn_rcpf(rs.sum));
+      if (kl > 1e25f) kl = INFINITY;  // an action that the reference never takes
+    }
+    logp = (xa - s.m) - s.lse;
     const float dl = logp - old;
-    const double border = adv > 0.0f ? q.log_high : q.log_low;
-    bool over = adv > 0.0f ? dl > (float)border : dl < (float)border;
+    const float border = adv > 0.0f ? q.log_high : q.log_low;
+    bool over = adv > 0.0f ? dl > border : dl < border;
     // 32 bits hold dl to a few 2^-23 of its terms
-    if (fabsf(dl - (float)border) <= 4.76837158e-7f * (4.0f + fabsf(z) + fabsf(old))) {
-      const T* row = (const T*)q.r.logits + i * q.r.stride;
-      const double dl64 = ((double)widen(row[action]) - (double)s.m) - lse64(row, legal, s.m) - (double)old;
-      over = adv > 0.0f ? dl64 > border : dl64 < border;
+    if (fabsf(dl - border) <= 4.76837158e-7f * (4.0f + fabsf(xa - s.m) + fabsf(old))) {
+      const double lhs = exp((double)xa - (double)s.m - (double)old);  // rho, times the sum
+      const double sum = sum64((const T*)q.r.logits + i * q.r.stride, legal, s.m);
+      over = adv > 0.0f ? lhs > q.high * sum : lhs < q.low * sum;
     }
     over = over && adv != 0.0f;
-    const float rho = expf(dl);
-    surrogate = adv == 0.0f ? 0.0f : -(over ? (adv > 0.0f ? q.high : q.low) : rho) * adv;
+    const float rho = exp_of(dl);
+    surrogate = adv == 0.0f ? 0.0f : -(over ? (float)(adv > 0.0f ? q.high : q.low) : rho) * adv;
     clipped = over ? 1.0f : 0.0f;
     if (q.grad) {
+      // p_b w_b, w_b = ent (l_b + H) + kl (d_b - K) - w, in which the lse's cancel
       const float w = (over || adv == 0.0f) ? 0.0f : -rho * adv;
-      const float base = q.ent * entropy - (q.r.ref ? q.kl * kl : 0.0f) - w;
+      const float share = inv * scale, base = -q.ent * et - (REF ? q.kl * ed : 0.0f) - w;
 #pragma unroll
-      for (int a = 0; a < AP; ++a) {
-        float g = q.ent * x[a] + base;
-        if (q.r.ref) g += q.kl * d[a];
-        g *= e[a];
-        if (a == action) g += w;
-        x[a] = ((legal >> a) & 1u) ? g * scale : 0.0f;
+      for (int a = 0; a < AP; ++a) x[a] = (d[a] + base) * (x[a] * share);
+      const float ta = s.t(xa), dta = REF ? ta - rs.t(da) : 0.0f;
+      ga = (q.ent * ta + (REF ? q.kl * dta : 0.0f) + base) * (s.e(xa) * share) + w * scale;
+      if (!(fabsf(base) < 1e30f)) {  // else 0 times it is 0 at the actions outside the word
+#pragma unroll
+        for (int a = 0; a < AP; ++a) x[a] = keep(legal, a, x[a], 0.0f);
       }
     }
   } else {
@@ -756,18 +847,32 @@ __global__ __launch_bounds__(kRowThreads) void k_policy_loss(PolicyArgs q) {
   if (mine && q.log_probs) q.log_probs[i] = logp;
   if (q.grad) {
     Tile<T, AP>::write(tile, q.r.A, x);
+    if (legal) Tile<T, AP>::write_one(tile, q.r.A, action, ga);
     __syncthreads();
     Tile<T, AP>::copy_out(tile, (T*)q.grad, row0, rows, q.r.A);
   }
-  float sums[4] = {surrogate, kl, entropy, clipped};
-  block_sum<kRowThreads, 4>(sums, lds);
-  if (threadIdx.x == 0) q.partial[blockIdx.x] = f32x4{sums[0], sums[1], sums[2], sums[3]};
+  const float sums[4] = {surrogate, kl, entropy, clipped};
+  const float v = wave_sum_four(sums);
+  if ((threadIdx.x & 63) < 4) lds[(threadIdx.x >> 6) * 4 + (threadIdx.x & 63)] = v;
+  const int here = (int)__popcll(__ballot(legal != 0));
+  if ((threadIdx.x & 63) == 0) decisions[threadIdx.x >> 6] = here;
+  __syncthreads();
+  if (threadIdx.x < 4) {
+    float total = 0.0f;
+    for (int w = 0; w < kRowThreads / 64; ++w) total += lds[4 * w + threadIdx.x];
+    ((float*)(q.partial + blockIdx.x))[threadIdx.x] = total;
+  }
+  if (threadIdx.x == 4) {
+    int total = 0;
+    for (int w = 0; w < kRowThreads / 64; ++w) total += decisions[w];
+    q.decided[blockIdx.x] = total;
+  }
 }
 
 // The blocks' sums in a fixed order, in 64 bits: the loss and its terms'
-// means.  One block: the 16,384 sums of 4 x 2^20 rows are 256 KiB.
-__global__ __launch_bounds__(kFinishThreads) void k_policy_finish(const f32x4* __restrict__ partial, int64_t blocks,
-                                                                   const int64_t* __restrict__ counts, int count_blocks,
+// means.  One block: the 16,384 blocks of 4 x 2^20 rows left 320 KiB.
+__global__ __launch_bounds__(kFinishThreads) void k_policy_finish(const f32x4* __restrict__ partial,
+                                                                   const int32_t* __restrict__ decided, int64_t blocks,
                                                                    double kl, double ent, float* loss, float* stats,
                                                                    int64_t* count) {
   __shared__ double lds[5 * (kFinishThreads / 64)];
@@ -776,8 +881,8 @@ __global__ __launch_bounds__(kFinishThreads) void k_policy_finish(const f32x4* _
   for (int64_t i = threadIdx.x; i < blocks; i += kFinishThreads) {
     const f32x4 v = partial[i];
     for (int k = 0; k < 4; ++k) s[k] += (double)v[k];
+    s[4] += (double)decided[i];
   }
-  if (threadIdx.x < (uint32_t)count_blocks) s[4] = (double)counts[threadIdx.x];
   block_sum<kFinishThreads, 5>(s, lds);
   if (threadIdx.x != 0) return;
   const double n = s[4] > 0.0 ? s[4] : 1.0;
@@ -821,74 +926,57 @@ __device__ __forceinline__ int64_t raw_offset(const PreferenceArgs& q, int64_t s
 __device__ __forceinline__ int64_t held(int64_t o, int64_t n) { return o < 0 ? 0 : o > n ? n : o; }
 __device__ __forceinline__ int64_t offset_at(const PreferenceArgs& q, int64_t s) { return held(raw_offset(q, s), q.r.n); }
 
-__device__ __forceinline__ double log1p_exp_neg(double x) {  // -log sigma(x)
-  return fmax(-x, 0.0) + log1p(exp(-fabs(x)));
-}
-
 // A pair from its sequences' summed log ratios: its cost, and coef, the
 // derivative in a chosen row's log ratio (a rejected row's is -coef).  NaN
-// where its offsets do not ascend within the rows.
-__device__ __forceinline__ double pair_cost(const PreferenceArgs& q, int64_t pair, double chosen, double rejected,
-                                            float* coef) {
+// where `ok` is false: its offsets do not ascend within the rows.  With
+// y = exp(-|x|), -log sigma(+-x) is log(1 + y) and for the wrong sign |x| more,
+// and sigma(-|x|) is y / (1 + y): 32 bits hold both to a few units.
+__device__ __forceinline__ float pair_cost(const PreferenceArgs& q, int64_t pair, double chosen, double rejected, bool ok,
+                                           float* coef) {
   chosen *= q.beta, rejected *= q.beta;
-  const double x = chosen - rejected;
-  double cost = (1.0 - q.eps) * log1p_exp_neg(x) + q.eps * log1p_exp_neg(-x);
-  double d = (q.eps - 1.0 / (1.0 + exp(x))) * q.beta / (double)q.pairs;
-  const int64_t r0 = raw_offset(q, 2 * pair), r1 = raw_offset(q, 2 * pair + 1), r2 = raw_offset(q, 2 * pair + 2);
-  if (r0 < 0 || r1 < r0 || r2 < r1 || r2 > q.r.n) cost = d = NAN;
   if (q.rewards) q.rewards[2 * pair] = (float)chosen, q.rewards[2 * pair + 1] = (float)rejected;
-  *coef = (float)d;
-  return cost;
+  const float x = (float)(chosen - rejected), size = fabsf(x), eps = (float)q.eps;
+  const float y = exp_of(-size), part = __builtin_amdgcn_rcpf(1.0f + y);
+  const float miss = x > 0.0f ? y * part : part;  // sigma(-x)
+  *coef = ok ? (eps - miss) * (float)(q.beta / (double)q.pairs) : NAN;
+  return ok ? log1p_of(y) + size * (x > 0.0f ? eps : 1.0f - eps) : NAN;
 }
 
-// One row's legal word and action: no legal action where it does not count.
-__device__ __forceinline__ uint32_t row_of(const Rows& r, int64_t i, bool mine, int& action) {
-  const uint32_t legal = mine ? legal_bits(r.mask[i], r.A) : 0u;
-  action = mine ? r.actions[i] : -1;
-  return decided(legal, action) ? legal : 0u;
+__device__ __forceinline__ bool ascending(int64_t a, int64_t b, int64_t c, int64_t n) {
+  return a >= 0 && b >= a && c >= b && c <= n;
 }
 
-// A tile's rows: this thread's log ratio, its e and their sum (x is spent).
-template <class T, int AP>
+// A tile's rows: this thread's log ratio, its e, the action's and their sum.
+template <class T, int AP, bool REF>
 __device__ __forceinline__ float row_ratio(char* tile, const PreferenceArgs& q, int64_t row0, int rows, uint32_t legal,
-                                           int action, float (&e)[AP], float& sum) {
-  float x[AP], d[AP];
-  if (q.r.ref) {
-    stage_two<T, AP>(tile, q.r, row0, rows, legal, x, d);
-  } else {
-    stage<T, AP>(tile, q.r.logits, q.r.stride, row0, rows, q.r.A);
-    __syncthreads();
-    Tile<T, AP>::read(tile, q.r.A, legal, x);
-  }
+                                           int action, float (&e)[AP], float& ea, float& sum) {
+  float x[AP], d[AP], xa, da;
+  stage_rows<T, AP, REF>(tile, q.r, row0, rows, legal, action, x, xa, d, da);
   float out = 0.0f;
   sum = 1.0f;
+  ea = 0.0f;
   if (legal) {
-    if (q.r.ref) {
-      const Softmax s = softmax<AP>(d, e);
-#pragma unroll
-      for (int a = 0; a < AP; ++a)
-        if (a == action) out = d[a];
-      out -= s.lse;
+    if (REF) {
+      const Softmax s = softmax<false, AP>(d, e);
+      out = (da - s.m) - log_of(s.sum);
     }
-    const Softmax s = softmax<AP>(x, e);
-    float z = 0.0f;
-#pragma unroll
-    for (int a = 0; a < AP; ++a)
-      if (a == action) z = x[a];
-    out = (z - s.lse) - out;
+    const Softmax s = softmax<true, AP>(x, e);
+    out = (xa - s.m) - s.lse - out;
+    ea = s.e(xa);
     sum = s.sum;
   }
   return out;
 }
 
-// The gradient of a tile's rows, out of this thread's e, sum and coef.
+// The gradient of a tile's rows: coef ([b = action] - e_b / sum).
 template <class T, int AP>
 __device__ __forceinline__ void row_grad(char* tile, const PreferenceArgs& q, int64_t row0, int rows, uint32_t legal,
-                                         int action, float (&e)[AP], float sum, float coef) {
+                                         int action, float (&e)[AP], float ea, float sum, float coef) {
   const float p = -coef / sum;
 #pragma unroll
-  for (int a = 0; a < AP; ++a) e[a] = ((legal >> a) & 1u) ? p * e[a] + (a == action ? coef : 0.0f) : 0.0f;
+  for (int a = 0; a < AP; ++a) e[a] = keep(legal, a, p * e[a], 0.0f);
   Tile<T, AP>::write(tile, q.r.A, e);
+  if (legal) Tile<T, AP>::write_one(tile, q.r.A, action, p * ea + coef);
   __syncthreads();
   Tile<T, AP>::copy_out(tile, (T*)q.grad, row0, rows, q.r.A);
 }
@@ -901,14 +989,13 @@ __device__ __forceinline__ void row_grad(char* tile, const PreferenceArgs& q, in
 // write the zero gradients of the rows outside every sequence.
 constexpr int kMaxGroup = 32, kZeroBlocks = 64;
 
-template <class T, int AP>
-__global__ __launch_bounds__(kRowThreads) void k_preference_short(PreferenceArgs q) {
+template <class T, int AP, bool REF>
+__global__ __launch_bounds__(kRowThreads, AP <= 20 ? 4 : 2) void k_preference_short(PreferenceArgs q) {
   __shared__ __align__(16) char tile[Tile<T, AP>::kBytes];
   __shared__ float ratio[kRowThreads];
   __shared__ int64_t edge[2 * kMaxGroup + 1];
   __shared__ double sum[2 * kMaxGroup];
   __shared__ float coef[2 * kMaxGroup];
-  __shared__ double lds[kRowThreads / 64];
   const int64_t groups = (q.pairs + q.group - 1) / q.group;
   if ((int64_t)blockIdx.x >= groups) {
     if (!q.grad) return;
@@ -922,40 +1009,55 @@ __global__ __launch_bounds__(kRowThreads) void k_preference_short(PreferenceArgs
   const int64_t pair0 = (int64_t)blockIdx.x * q.group;
   const int pairs = (int)(q.pairs - pair0 < q.group ? q.pairs - pair0 : q.group);
   const int wave = (int)threadIdx.x >> 6, seqs = 2 * pairs;
-  if ((int)threadIdx.x <= seqs) edge[threadIdx.x] = offset_at(q, 2 * pair0 + threadIdx.x);
+  int64_t raw = 0;
+  if ((int)threadIdx.x <= seqs) {
+    raw = raw_offset(q, 2 * pair0 + threadIdx.x);
+    edge[threadIdx.x] = raw;
+  }
   if ((int)threadIdx.x < seqs) sum[threadIdx.x] = 0.0;
   __syncthreads();
+  bool ok = true;
+  if ((int)threadIdx.x < pairs) {
+    const int64_t* o = edge + 2 * threadIdx.x;
+    ok = ascending(o[0], o[1], o[2], q.r.n);
+  }
+  __syncthreads();
+  if ((int)threadIdx.x <= seqs) edge[threadIdx.x] = held(raw, q.r.n);
+  __syncthreads();
   const int64_t begin = edge[0], end = edge[seqs];
-  float e[AP], total = 1.0f;
+  float e[AP], ea = 0.0f, total = 1.0f;
   uint32_t legal = 0;
   int action = -1, rows = 0;
   for (int64_t row0 = begin; row0 < end; row0 += kRowThreads) {
     const int64_t i = row0 + threadIdx.x;
     rows = (int)(end - row0 < kRowThreads ? end - row0 : kRowThreads);
     legal = row_of(q.r, i, (int)threadIdx.x < rows, action);
-    ratio[threadIdx.x] = row_ratio<T, AP>(tile, q, row0, rows, legal, action, e, total);
+    ratio[threadIdx.x] = row_ratio<T, AP, REF>(tile, q, row0, rows, legal, action, e, ea, total);
     __syncthreads();
     for (int s = wave; s < seqs; s += kRowThreads / 64) {
       const int64_t lo = edge[s] - row0, hi = edge[s + 1] - row0;
       const int to = hi < rows ? (int)hi : rows;
-      double v = 0.0;
-      for (int k = (lo > 0 ? (int)lo : 0) + ((int)threadIdx.x & 63); k < to; k += 64) v += (double)ratio[k];
-#pragma unroll
-      for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d, 64);
-      if ((threadIdx.x & 63) == 0) sum[s] += v;
+      float v = 0.0f;  // a tile's rows in 32 bits, tiles in 64
+      for (int k = (lo > 0 ? (lo < rows ? (int)lo : rows) : 0) + ((int)threadIdx.x & 63); k < to; k += 64) v += ratio[k];
+      v = wave_sum(v);
+      if ((threadIdx.x & 63) == 0) sum[s] += (double)v;
     }
     __syncthreads();
   }
   double cost[1] = {0.0};
   if ((int)threadIdx.x < pairs) {
     const int s = 2 * threadIdx.x;
-    cost[0] = pair_cost(q, pair0 + threadIdx.x, sum[s], sum[s + 1], &coef[s]);
+    cost[0] = (double)pair_cost(q, pair0 + threadIdx.x, sum[s], sum[s + 1], ok, &coef[s]);
     coef[s + 1] = -coef[s];
   }
-  block_sum<kRowThreads, 1>(cost, lds);  // its barrier also shows the coefs
-  if (threadIdx.x == 0) {
-    q.partial[blockIdx.x] = cost[0];
-    if (groups == 1) *q.loss = (float)(cost[0] / (double)q.pairs);
+  __syncthreads();
+  if (wave == 0) {  // the group's pairs are lanes of one wave
+#pragma unroll
+    for (int d = kMaxGroup / 2; d >= 1; d >>= 1) cost[0] += __shfl_xor(cost[0], d, 64);
+    if (threadIdx.x == 0) {
+      q.partial[blockIdx.x] = cost[0];
+      if (groups == 1) *q.loss = (float)(cost[0] / (double)q.pairs);
+    }
   }
   if (!q.grad) return;
   const bool once = end - begin <= kRowThreads;
@@ -968,7 +1070,10 @@ __global__ __launch_bounds__(kRowThreads) void k_preference_short(PreferenceArgs
       __syncthreads();
       float x[AP];
       Tile<T, AP>::read(tile, q.r.A, legal, x);
-      total = softmax<AP>(x, e).sum;
+      const float xa = Tile<T, AP>::read_one(tile, q.r.A, action);
+      const Softmax sm = softmax<false, AP>(x, e);
+      ea = sm.e(xa);
+      total = sm.sum;
     }
     int lo = 0, hi = seqs;  // the last sequence that starts at or before row i
     while (lo < hi) {
@@ -976,7 +1081,7 @@ __global__ __launch_bounds__(kRowThreads) void k_preference_short(PreferenceArgs
       if (edge[mid + 1] <= i) lo = mid + 1;
       else hi = mid;
     }
-    row_grad<T, AP>(tile, q, row0, rows, legal, action, e, total, lo < seqs ? coef[lo] : 0.0f);
+    row_grad<T, AP>(tile, q, row0, rows, legal, action, e, ea, total, lo < seqs ? coef[lo] : 0.0f);
     __syncthreads();
   }
 }
@@ -984,7 +1089,7 @@ __global__ __launch_bounds__(kRowThreads) void k_preference_short(PreferenceArgs
 // Long sequences: every row's log ratio to memory, the sequences' sums from
 // slices of them, the pairs, then the gradient with the logits read again
 // (A sizeof(T) of a row's 3 A sizeof(T) + 5 bytes).
-template <class T, int AP>
+template <class T, int AP, bool REF>
 __global__ __launch_bounds__(kRowThreads) void k_preference_rows(PreferenceArgs q) {
   __shared__ __align__(16) char tile[Tile<T, AP>::kBytes];
   const int64_t row0 = (int64_t)blockIdx.x * kRowThreads, i = row0 + threadIdx.x;
@@ -992,8 +1097,8 @@ __global__ __launch_bounds__(kRowThreads) void k_preference_rows(PreferenceArgs 
   const bool mine = (int)threadIdx.x < rows;
   int action;
   const uint32_t legal = row_of(q.r, i, mine, action);
-  float e[AP], total;
-  const float out = row_ratio<T, AP>(tile, q, row0, rows, legal, action, e, total);
+  float e[AP], ea, total;
+  const float out = row_ratio<T, AP, REF>(tile, q, row0, rows, legal, action, e, ea, total);
   if (mine) q.ratio[i] = out;
 }
 
@@ -1029,8 +1134,9 @@ __global__ __launch_bounds__(kPairThreads) void k_preference_pairs(PreferenceArg
       for (int d = 32; d >= 1; d >>= 1) s[h] += __shfl_xor(s[h], d, 64);
     }
     if (lane == 0) {
+      const bool ok = ascending(raw_offset(q, 2 * pair), raw_offset(q, 2 * pair + 1), raw_offset(q, 2 * pair + 2), q.r.n);
       float d;
-      cost[0] += pair_cost(q, pair, s[0], s[1], &d);
+      cost[0] += (double)pair_cost(q, pair, s[0], s[1], ok, &d);
       q.coef[2 * pair] = d, q.coef[2 * pair + 1] = -d;
     }
   }
@@ -1047,7 +1153,7 @@ __global__ __launch_bounds__(kRowThreads) void k_preference_grad(PreferenceArgs 
   const int64_t row0 = (int64_t)blockIdx.x * kRowThreads, i = row0 + threadIdx.x;
   const int rows = (int)(q.r.n - row0 < kRowThreads ? q.r.n - row0 : kRowThreads);
   int action;
-  const uint32_t legal = row_of(q.r, i, (int)threadIdx.x < rows, action);
+  uint32_t legal = row_of(q.r, i, (int)threadIdx.x < rows, action);
   float coef = 0.0f;
   if (legal) {
     // the last sequence that starts at or before row i (the non-empty one where several start there)
@@ -1058,18 +1164,15 @@ __global__ __launch_bounds__(kRowThreads) void k_preference_grad(PreferenceArgs 
       else hi = mid;
     }
     if (lo >= 1 && lo <= 2 * q.pairs) coef = q.coef[lo - 1];
+    else legal = 0;
   }
   stage<T, AP>(tile, q.r.logits, q.r.stride, row0, rows, q.r.A);
   __syncthreads();
-  float x[AP], e[AP], total = 1.0f;
-  Tile<T, AP>::read(tile, q.r.A, coef == 0.0f ? 0u : legal, x);
-  if (coef != 0.0f) {
-    total = softmax<AP>(x, e).sum;
-  } else {
-#pragma unroll
-    for (int a = 0; a < AP; ++a) e[a] = 0.0f;
-  }
-  row_grad<T, AP>(tile, q, row0, rows, legal, action, e, total, coef);
+  float x[AP], e[AP];
+  Tile<T, AP>::read(tile, q.r.A, legal, x);
+  const float xa = Tile<T, AP>::read_one(tile, q.r.A, action);
+  const Softmax sm = softmax<false, AP>(x, e);
+  row_grad<T, AP>(tile, q, row0, rows, legal, action, e, sm.e(xa), sm.sum, coef);
 }
 
 // The blocks' costs in a fixed order.
@@ -1157,7 +1260,9 @@ inline void launch_advantages(const AdvantageArgs& q, int players, hipStream_t s
   }
 }
 
-inline size_t policy_workspace(int64_t n) { return sizeof(int64_t) * kCountBlocks + sizeof(f32x4) * row_blocks(n); }
+inline size_t policy_workspace(int64_t n) {
+  return sizeof(int64_t) * kCountBlocks + (sizeof(f32x4) + sizeof(int32_t)) * row_blocks(n);
+}
 
 inline void launch_policy(PolicyArgs q, int dtype, double kl, double ent, float* loss, float* stats, int64_t* count,
                           void* workspace, hipStream_t s) {
@@ -1165,15 +1270,18 @@ inline void launch_policy(PolicyArgs q, int dtype, double kl, double ent, float*
   const int64_t counters = (q.r.n + 4 * kCountThreads - 1) / (4 * kCountThreads);
   q.partial = (f32x4*)workspace;
   q.counts = (int64_t*)(q.partial + blocks);
+  q.decided = (int32_t*)(q.counts + kCountBlocks);
   q.count_blocks = (int)(counters < kCountBlocks ? counters : kCountBlocks);
   if (blocks) {
-    k_policy_count<<<q.count_blocks, kCountThreads, 0, s>>>(q);
+    if (q.grad) k_policy_count<<<q.count_blocks, kCountThreads, 0, s>>>(q);
     with_rows(dtype, q.r.A, [&](auto t, auto ap) {
       using T = typename decltype(t)::type;
-      k_policy_loss<T, decltype(ap)::value><<<blocks, kRowThreads, 0, s>>>(q);
+      constexpr int AP = decltype(ap)::value;
+      if (q.r.ref) k_policy_loss<T, AP, true><<<blocks, kRowThreads, 0, s>>>(q);
+      else k_policy_loss<T, AP, false><<<blocks, kRowThreads, 0, s>>>(q);
     });
   }
-  k_policy_finish<<<1, kFinishThreads, 0, s>>>(q.partial, blocks, q.counts, q.count_blocks, kl, ent, loss, stats, count);
+  k_policy_finish<<<1, kFinishThreads, 0, s>>>(q.partial, q.decided, blocks, kl, ent, loss, stats, count);
 }
 
 // How a preference call is split.  Short where a pair has at most kShortRows
@@ -1222,12 +1330,14 @@ inline void launch_preference(PreferenceArgs q, int dtype, void* workspace, hipS
     constexpr int AP = decltype(ap)::value;
     if (p.is_short) {
       const int64_t grid = p.blocks + (q.grad && q.r.n ? kZeroBlocks : 0);
-      if (grid) k_preference_short<T, AP><<<(unsigned)grid, kRowThreads, 0, s>>>(q);
+      if (grid && q.r.ref) k_preference_short<T, AP, true><<<(unsigned)grid, kRowThreads, 0, s>>>(q);
+      else if (grid) k_preference_short<T, AP, false><<<(unsigned)grid, kRowThreads, 0, s>>>(q);
     } else {
       q.sums = q.partial + p.blocks + 1;
       q.coef = (float*)(q.sums + 2 * q.pairs * p.slices);
       q.ratio = q.coef + 2 * q.pairs;
-      k_preference_rows<T, AP><<<tiles, kRowThreads, 0, s>>>(q);
+      if (q.r.ref) k_preference_rows<T, AP, true><<<tiles, kRowThreads, 0, s>>>(q);
+      else k_preference_rows<T, AP, false><<<tiles, kRowThreads, 0, s>>>(q);
       k_preference_sums<<<(unsigned)(2 * q.pairs * p.slices), kRowThreads, 0, s>>>(q);
       k_preference_pairs<<<(unsigned)p.blocks, kPairThreads, 0, s>>>(q);
       if (q.grad) k_preference_grad<T, AP><<<tiles, kRowThreads, 0, s>>>(q);
