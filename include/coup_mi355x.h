@@ -504,7 +504,7 @@ typedef struct {
   const float* advantages;    /* [rows] */
   const uint8_t* active;      /* [rows] or NULL */
   double clip_low, clip_high; /* 0 <= clip_low <= 1, 0 <= clip_high */
-  double kl_coef, entropy_coef;
+  double kl_coef, entropy_coef; /* within -1e4..1e4 */
 } coup_policy_terms;
 typedef struct {
   float* loss;      /* [1]; 0 where nothing counts */

@@ -4915,8 +4915,8 @@ int coup_policy_loss(const coup_decisions* d, const coup_policy_terms* terms, co
     return fail(COUP_E_INVALID, "coup_policy_loss: old_log_probs or advantages is null");
   if (!(terms->clip_low >= 0.0 && terms->clip_low <= 1.0 && terms->clip_high >= 0.0 && std::isfinite(terms->clip_high)))
     return fail(COUP_E_INVALID, "coup_policy_loss: clip_low must be in 0..1 and clip_high finite and not negative");
-  if (!std::isfinite(terms->kl_coef) || !std::isfinite(terms->entropy_coef))
-    return fail(COUP_E_INVALID, "coup_policy_loss: kl_coef and entropy_coef must be finite");
+  if (!(std::fabs(terms->kl_coef) <= 1e4 && std::fabs(terms->entropy_coef) <= 1e4))
+    return fail(COUP_E_INVALID, "coup_policy_loss: kl_coef and entropy_coef must be finite, within 1e4");
   if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < coup_policy_workspace(d->rows))
     return fail(COUP_E_INVALID, "coup_policy_loss: workspace is null, misaligned or too small");
   coup::policy::PolicyArgs q{};

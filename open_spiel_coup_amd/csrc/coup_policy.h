@@ -33,7 +33,9 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kRowThreads = 256;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
-constexpr float kLowest = -3.402823466e38f;
+// Stands for -inf in products with a 0 share.  Far below any logit's distance,
+// and 1e4 (the largest coefficient of the loss) times it is still finite.
+constexpr float kLowest = -1e33f;
 
 template <class T>
 __device__ __forceinline__ float widen(T v) {
@@ -523,17 +525,15 @@ __device__ __forceinline__ void advance(const AdvantageArgs& q, const Steps<C>& 
                                         const float (&v)[kStretch], float (&z)[P], int steps) {
 #pragma unroll
   for (int k = 0; k < kStretch; ++k) {
-    const bool step = st[k] == COUP_STEP_MID || st[k] == COUP_STEP_LAST;
-    const bool cut = st[k] == COUP_STEP_FIRST || st[k] == COUP_STEP_LAST;
+    const bool cut = !(st[k] & 1);
+    const float gvv = q.gv * v[k];
     float target = 0.0f;
 #pragma unroll
     for (int p = 0; p < P; ++p) {
-      if (cut) z[p] = 0.0f;
-      if (step) z[p] += r[k].of(p);
-      if (p == pl[k]) {
-        target = z[p];
-        z[p] = q.gl * z[p] + q.gv * v[k];
-      }
+      const float here = (cut ? 0.0f : z[p]) + r[k].of(p), after = q.gl * here + gvv;
+      const bool acts = p == pl[k];
+      target = acts ? here : target;
+      z[p] = acts ? after : here;
     }
     if (k < steps) {
       *at.at(q.adv, k) = pl[k] >= 0 ? target - v[k] : 0.0f;
@@ -592,9 +592,12 @@ __global__ __launch_bounds__(NT) void k_advantages(AdvantageArgs q) {
     float v[kStretch];
 #pragma unroll
     for (int k = 0; k < kStretch; ++k) {
-      if (k > top) st[k] = COUP_STEP_SKIPPED;
+      // FIRST 0 and LAST 2 cut, MID 1 and LAST 2 are steps; the rest is skipped, as 3
+      st[k] = k > top || st[k] > COUP_STEP_SKIPPED ? COUP_STEP_SKIPPED : st[k];
       const bool step = st[k] == COUP_STEP_MID || st[k] == COUP_STEP_LAST;
-      if (!step || pl[k] >= P) pl[k] = -1;
+      r[k].lo = step ? r[k].lo : 0u;
+      r[k].hi = step ? r[k].hi : 0u;
+      pl[k] = step && pl[k] < P ? pl[k] : -1;
       v[k] = pl[k] >= 0 ? widen_bits(bits[k], q.dtype) : 0.0f;
     }
     if (C == 1) {
@@ -605,16 +608,15 @@ __global__ __launch_bounds__(NT) void k_advantages(AdvantageArgs q) {
       for (int p = 0; p < P; ++p) f[p] = 1.0f, g[p] = 0.0f;
 #pragma unroll
       for (int k = 0; k < kStretch; ++k) {
-        const bool step = st[k] == COUP_STEP_MID || st[k] == COUP_STEP_LAST;
-        const bool cut = st[k] == COUP_STEP_FIRST || st[k] == COUP_STEP_LAST;
+        const bool cut = !(st[k] & 1);
+        const float gvv = q.gv * v[k];
 #pragma unroll
         for (int p = 0; p < P; ++p) {
-          if (cut) f[p] = 0.0f, g[p] = 0.0f;
-          if (step) g[p] += r[k].of(p);
-          if (p == pl[k]) {
-            f[p] *= q.gl;
-            g[p] = q.gl * g[p] + q.gv * v[k];
-          }
+          const float here = (cut ? 0.0f : g[p]) + r[k].of(p), after = q.gl * here + gvv;
+          const bool acts = p == pl[k];
+          const float kept = cut ? 0.0f : f[p];
+          f[p] = acts ? q.gl * kept : kept;
+          g[p] = acts ? after : here;
         }
       }
       // the wave's stretches up to each, a lower index (a later time) first
@@ -660,10 +662,20 @@ __global__ __launch_bounds__(NT) void k_advantages(AdvantageArgs q) {
 
 // ----------------------------------------------------- sums over a block
 
+// v summed over the wave, in every lane: row shifts, then row broadcasts
+// leave the sum in the last lane (no LDS traffic, six additions).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float add_moved(float v) {
+  return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, ROWS, 0xf, true));
+}
 __device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int s = 32; s >= 1; s >>= 1) v += __shfl_xor(v, s, 64);
-  return v;
+  v = add_moved<0x111, 0xf>(v);  // row_shr 1, 2, 4, 8
+  v = add_moved<0x112, 0xf>(v);
+  v = add_moved<0x114, 0xf>(v);
+  v = add_moved<0x118, 0xf>(v);
+  v = add_moved<0x142, 0xa>(v);  // row_bcast 15 to rows 1 and 3, 31 to rows 2 and 3
+  v = add_moved<0x143, 0xc>(v);
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 
 // Four values summed over the wave at once: the sum of value k is lane k's (7
@@ -717,7 +729,7 @@ struct PolicyArgs {
   void* grad;        // null: no gradient
   f32x4* partial;    // [blocks] sums of the terms over a block's rows
   int32_t* decided;  // [blocks] its decisions
-  int64_t* counts;   // [count blocks] the call's decisions, for the gradient
+  float* counts;     // [count blocks] the call's decisions, for the gradient
   int count_blocks;
 };
 
@@ -750,7 +762,7 @@ __global__ __launch_bounds__(kCountThreads) void k_policy_count(PolicyArgs q) {
   if (threadIdx.x != 0) return;
   int64_t total = 0;
   for (int w = 0; w < kCountThreads / 64; ++w) total += wave[w];
-  q.counts[blockIdx.x] = total;
+  q.counts[blockIdx.x] = (float)total;
 }
 
 template <class T, int AP, bool REF>
@@ -768,7 +780,7 @@ __global__ __launch_bounds__(kRowThreads, AP <= 20 ? 4 : 2) void k_policy_loss(P
 #pragma unroll
     for (int k = 0; k < kCountBlocks; k += 64) {
       const int at = k + ((int)threadIdx.x & 63);
-      if (at < q.count_blocks) count += (float)q.counts[at];
+      if (at < q.count_blocks) count += q.counts[at];
     }
   }
   int action;
@@ -786,34 +798,26 @@ __global__ __launch_bounds__(kRowThreads, AP <= 20 ? 4 : 2) void k_policy_loss(P
   if (legal) {
     Softmax rs{0.0f, 1.0f, 0.0f};
     if (REF) {
-      float e[AP];
-      rs = softmax<false, AP>(d, e);
+      float unused[AP];
+      rs = softmax<false, AP>(d, unused);
     }
-    // x becomes e; d becomes the part of w_b (below) that is known by now
-    Softmax s;
-    s.m = row_max<AP>(x);
-    s.sum = 0.0f;
-    float others = 0.0f, et = 0.0f, ed = 0.0f;  // sums of e t and, with d = t - t_ref, of e d
+    // x becomes t, d is the reference's
+    float e[AP];
+    const Softmax s = softmax<false, AP>(x, e);
+    float et = 0.0f, er = 0.0f;  // sums of e t and e t_ref
 #pragma unroll
     for (int a = 0; a < AP; ++a) {
-      const float t = s.t(x[a]), ea = s.e(x[a]);
-      s.sum += ea;
-      others += __builtin_amdgcn_fractf(ea);
-      et += ea * t;
-      const float dt = REF ? t - d[a] : 0.0f;
-      if (REF) ed += ea * dt;
-      d[a] = REF ? q.ent * t + q.kl * dt : q.ent * t;
-      x[a] = ea;
+      et += e[a] * x[a];
+      if (REF) er += e[a] * d[a];
     }
-    s.lse = lse_of(s.sum, others);
-    const float inv = __builtin_amdgcn_rcpf(s.sum);
-    et *= inv, ed *= inv;
-    entropy = s.lse - et;
+    const float inv = __builtin_amdgcn_rcpf(s.sum), lse = log_of(s.sum);
+    et *= inv, er *= inv;
+    entropy = lse - et;
     if (REF) {
-      kl = ed - log_of(s.sum * __builtin_amdgcn_rcpf(rs.sum));
-      if (kl > 1e25f) kl = INFINITY;  // an action that the reference never takes
+      kl = (et - er) - log_of(s.sum * __builtin_amdgcn_rcpf(rs.sum));
+      if (kl > 1e24f) kl = INFINITY;  // an action that the reference never takes
     }
-    logp = (xa - s.m) - s.lse;
+    logp = (xa - s.m) - lse;
     const float dl = logp - old;
     const float border = adv > 0.0f ? q.log_high : q.log_low;
     bool over = adv > 0.0f ? dl > border : dl < border;
@@ -828,13 +832,14 @@ __global__ __launch_bounds__(kRowThreads, AP <= 20 ? 4 : 2) void k_policy_loss(P
     surrogate = adv == 0.0f ? 0.0f : -(over ? (float)(adv > 0.0f ? q.high : q.low) : rho) * adv;
     clipped = over ? 1.0f : 0.0f;
     if (q.grad) {
-      // p_b w_b, w_b = ent (l_b + H) + kl (d_b - K) - w, in which the lse's cancel
+      // p_b w_b, w_b = ent (l_b + H) + kl (d_b - K) - w, in which the lse's
+      // cancel: (ent + kl) (t_b - E t) - kl (tr_b - E tr) - w
       const float w = (over || adv == 0.0f) ? 0.0f : -rho * adv;
-      const float share = inv * scale, base = -q.ent * et - (REF ? q.kl * ed : 0.0f) - w;
+      const float share = inv * scale, ct = (REF ? q.ent + q.kl : q.ent) * share, cr = REF ? q.kl * share : 0.0f;
+      const float base = cr * er - ct * et - w * share;
 #pragma unroll
-      for (int a = 0; a < AP; ++a) x[a] = (d[a] + base) * (x[a] * share);
-      const float ta = s.t(xa), dta = REF ? ta - rs.t(da) : 0.0f;
-      ga = (q.ent * ta + (REF ? q.kl * dta : 0.0f) + base) * (s.e(xa) * share) + w * scale;
+      for (int a = 0; a < AP; ++a) x[a] = e[a] * (ct * x[a] + (REF ? base - cr * d[a] : base));
+      ga = s.e(xa) * (ct * s.t(xa) + (REF ? base - cr * rs.t(da) : base)) + w * scale;
       if (!(fabsf(base) < 1e30f)) {  // else 0 times it is 0 at the actions outside the word
 #pragma unroll
         for (int a = 0; a < AP; ++a) x[a] = keep(legal, a, x[a], 0.0f);
@@ -960,8 +965,8 @@ __device__ __forceinline__ float row_ratio(char* tile, const PreferenceArgs& q, 
       const Softmax s = softmax<false, AP>(d, e);
       out = (da - s.m) - log_of(s.sum);
     }
-    const Softmax s = softmax<true, AP>(x, e);
-    out = (xa - s.m) - s.lse - out;
+    const Softmax s = softmax<false, AP>(x, e);
+    out = (xa - s.m) - log_of(s.sum) - out;
     ea = s.e(xa);
     sum = s.sum;
   }
@@ -1261,7 +1266,7 @@ inline void launch_advantages(const AdvantageArgs& q, int players, hipStream_t s
 }
 
 inline size_t policy_workspace(int64_t n) {
-  return sizeof(int64_t) * kCountBlocks + (sizeof(f32x4) + sizeof(int32_t)) * row_blocks(n);
+  return sizeof(float) * kCountBlocks + (sizeof(f32x4) + sizeof(int32_t)) * row_blocks(n);
 }
 
 inline void launch_policy(PolicyArgs q, int dtype, double kl, double ent, float* loss, float* stats, int64_t* count,
@@ -1269,7 +1274,7 @@ inline void launch_policy(PolicyArgs q, int dtype, double kl, double ent, float*
   const unsigned blocks = row_blocks(q.r.n);
   const int64_t counters = (q.r.n + 4 * kCountThreads - 1) / (4 * kCountThreads);
   q.partial = (f32x4*)workspace;
-  q.counts = (int64_t*)(q.partial + blocks);
+  q.counts = (float*)(q.partial + blocks);
   q.decided = (int32_t*)(q.counts + kCountBlocks);
   q.count_blocks = (int)(counters < kCountBlocks ? counters : kCountBlocks);
   if (blocks) {

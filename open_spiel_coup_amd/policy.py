@@ -276,8 +276,8 @@ def _policy_call(logits, actions, legal_mask, old_log_probs, advantages, ref_log
     clip_low, clip_high, kl_coef, entropy_coef = float(clip_low), float(clip_high), float(kl_coef), float(entropy_coef)
     if not (0.0 <= clip_low <= 1.0 and 0.0 <= clip_high < float("inf")):
         raise ValueError("clip_low must be in 0..1, clip_high finite and not negative")
-    if kl_coef - kl_coef != 0.0 or entropy_coef - entropy_coef != 0.0:
-        raise ValueError("kl_coef and entropy_coef must be finite")
+    if not (-1e4 <= kl_coef <= 1e4 and -1e4 <= entropy_coef <= 1e4):
+        raise ValueError("kl_coef and entropy_coef must be finite, within 1e4")
     terms = _native.PolicyTerms(old.data_ptr(), adv.data_ptr(), None if act is None else act.data_ptr(), clip_low,
                                 clip_high, kl_coef, entropy_coef)
     lib = _native.load()

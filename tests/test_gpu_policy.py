@@ -390,7 +390,7 @@ def test_policy_refusals():
                     (dict(legal_mask=mask.long()), "int32"), (dict(old_log_probs=old.half()), "float32"),
                     (dict(advantages=adv.cpu()), "is on cpu"), (dict(ref_logits=ref.half()), "type and shape"),
                     (dict(ref_logits=ref[:2]), "type and shape"), (dict(active=actions), "bool"),
-                    (dict(clip_low=1.5), "clip_low"), (dict(clip_high=-0.1), "clip"), (dict(kl_coef=math.inf), "finite"),
+                    (dict(clip_low=1.5), "clip_low"), (dict(clip_high=-0.1), "clip"), (dict(kl_coef=math.inf), "finite"), (dict(entropy_coef=2e4), "1e4"),
                     (dict(entropy_coef=math.nan), "finite"),
                     (dict(old_log_probs=old.clone().requires_grad_()), "held constant"),
                     (dict(ref_logits=ref.clone().requires_grad_()), "held constant")):
