@@ -259,46 +259,38 @@ __device__ __forceinline__ void stage(char* lds, const void* base, int64_t strid
   }
 }
 
-// Two tables' rows through one tile: x, then d, and both's logits of `action`.
-// Both are in flight before the first is waited for.
-template <class T, int AP>
-__device__ __forceinline__ void stage_two(char* lds, const Rows& q, int64_t row0, int rows, uint32_t legal, int action,
-                                          float (&x)[AP], float& xa, float (&d)[AP], float& da) {
+// A block's rows, and (REF) its reference's before them, through one tile:
+// both are in flight before the first is waited for, and `reference`, called
+// on the reference's row d and its logit of `action`, works while the other
+// still flies.  Then x and xa are the logits' own.  `action` must be one of
+// the A (0 for rows that do not count).
+template <class T, int AP, bool REF, class F>
+__device__ __forceinline__ void stage_rows(char* lds, const Rows& q, int64_t row0, int rows, uint32_t legal, int action,
+                                           float (&d)[AP], F reference, float (&x)[AP], float& xa) {
   using Tl = Tile<T, AP>;
-  typename Tl::Flight g;
-  const bool pieces = q.stride == q.A && q.ref_stride == q.A;
-  if (pieces) {
+  if (REF) {
     typename Tl::Flight f;
-    Tl::fetch(f, (const T*)q.logits, row0, rows, q.A);
-    Tl::fetch(g, (const T*)q.ref, row0, rows, q.A);
-    Tl::land(f, lds, (const T*)q.logits, row0, rows, q.A);
+    const bool pieces = q.stride == q.A && q.ref_stride == q.A;
+    if (pieces) {
+      typename Tl::Flight g;
+      Tl::fetch(g, (const T*)q.ref, row0, rows, q.A);
+      Tl::fetch(f, (const T*)q.logits, row0, rows, q.A);
+      Tl::land(g, lds, (const T*)q.ref, row0, rows, q.A);
+    } else {
+      Tl::copy_in(lds, (const T*)q.ref, q.ref_stride, row0, rows, q.A);
+    }
+    __syncthreads();
+    Tl::read(lds, q.A, legal, d);
+    reference(d, Tl::read_one(lds, q.A, action));
+    __syncthreads();
+    if (pieces) Tl::land(f, lds, (const T*)q.logits, row0, rows, q.A);
+    else Tl::copy_in(lds, (const T*)q.logits, q.stride, row0, rows, q.A);
   } else {
-    Tl::copy_in(lds, (const T*)q.logits, q.stride, row0, rows, q.A);
+    stage<T, AP>(lds, q.logits, q.stride, row0, rows, q.A);
   }
   __syncthreads();
   Tl::read(lds, q.A, legal, x);
   xa = Tl::read_one(lds, q.A, action);
-  __syncthreads();
-  if (pieces) Tl::land(g, lds, (const T*)q.ref, row0, rows, q.A);
-  else Tl::copy_in(lds, (const T*)q.ref, q.ref_stride, row0, rows, q.A);
-  __syncthreads();
-  Tl::read(lds, q.A, legal, d);
-  da = Tl::read_one(lds, q.A, action);
-}
-
-// The logits' rows alone, or (REF) both.  `action` must be one of the A (0 for rows that do not count).
-template <class T, int AP, bool REF>
-__device__ __forceinline__ void stage_rows(char* lds, const Rows& q, int64_t row0, int rows, uint32_t legal, int action,
-                                           float (&x)[AP], float& xa, float (&d)[AP], float& da) {
-  if (REF) {
-    stage_two<T, AP>(lds, q, row0, rows, legal, action, x, xa, d, da);
-  } else {
-    stage<T, AP>(lds, q.logits, q.stride, row0, rows, q.A);
-    __syncthreads();
-    Tile<T, AP>::read(lds, q.A, legal, x);
-    xa = Tile<T, AP>::read_one(lds, q.A, action);
-    da = 0.0f;
-  }
 }
 
 // The larger; NaN where either is (one instruction, and for three values too).
@@ -791,17 +783,20 @@ __global__ __launch_bounds__(kRowThreads, AP <= 20 ? 4 : 2) void k_policy_loss(P
     old = q.old[i];
     adv = q.adv[i];
   }
-  float x[AP], d[AP], xa, da;
-  stage_rows<T, AP, REF>(tile, q.r, row0, rows, legal, action, x, xa, d, da);
+  float x[AP], d[AP], xa, rta = 0.0f;  // d: the reference's t, rta the action's
+  Softmax rs{0.0f, 1.0f, 0.0f};
+  stage_rows<T, AP, REF>(
+      tile, q.r, row0, rows, legal, action, d,
+      [&](float(&row)[AP], float one) {
+        float unused[AP];
+        rs = softmax<false, AP>(row, unused);
+        rta = rs.t(one);
+      },
+      x, xa);
   const float n = wave_sum(count), scale = 1.0f / (n > 0.0f ? n : 1.0f);
   float surrogate = 0.0f, kl = 0.0f, entropy = 0.0f, clipped = 0.0f, logp = 0.0f, ga = 0.0f;
   if (legal) {
-    Softmax rs{0.0f, 1.0f, 0.0f};
-    if (REF) {
-      float unused[AP];
-      rs = softmax<false, AP>(d, unused);
-    }
-    // x becomes t, d is the reference's
+    // x becomes t
     float e[AP];
     const Softmax s = softmax<false, AP>(x, e);
     float et = 0.0f, er = 0.0f;  // sums of e t and e t_ref
@@ -839,7 +834,7 @@ __global__ __launch_bounds__(kRowThreads, AP <= 20 ? 4 : 2) void k_policy_loss(P
       const float base = cr * er - ct * et - w * share;
 #pragma unroll
       for (int a = 0; a < AP; ++a) x[a] = e[a] * (ct * x[a] + (REF ? base - cr * d[a] : base));
-      ga = s.e(xa) * (ct * s.t(xa) + (REF ? base - cr * rs.t(da) : base)) + w * scale;
+      ga = s.e(xa) * (ct * s.t(xa) + (REF ? base - cr * rta : base)) + w * scale;
       if (!(fabsf(base) < 1e30f)) {  // else 0 times it is 0 at the actions outside the word
 #pragma unroll
         for (int a = 0; a < AP; ++a) x[a] = keep(legal, a, x[a], 0.0f);
@@ -955,16 +950,18 @@ __device__ __forceinline__ bool ascending(int64_t a, int64_t b, int64_t c, int64
 template <class T, int AP, bool REF>
 __device__ __forceinline__ float row_ratio(char* tile, const PreferenceArgs& q, int64_t row0, int rows, uint32_t legal,
                                            int action, float (&e)[AP], float& ea, float& sum) {
-  float x[AP], d[AP], xa, da;
-  stage_rows<T, AP, REF>(tile, q.r, row0, rows, legal, action, x, xa, d, da);
-  float out = 0.0f;
+  float x[AP], d[AP], xa, out = 0.0f;
+  stage_rows<T, AP, REF>(
+      tile, q.r, row0, rows, legal, action, d,
+      [&](float(&row)[AP], float one) {
+        float unused[AP];
+        const Softmax s = softmax<false, AP>(row, unused);
+        out = legal ? (one - s.m) - log_of(s.sum) : 0.0f;
+      },
+      x, xa);
   sum = 1.0f;
   ea = 0.0f;
   if (legal) {
-    if (REF) {
-      const Softmax s = softmax<false, AP>(d, e);
-      out = (da - s.m) - log_of(s.sum);
-    }
     const Softmax s = softmax<false, AP>(x, e);
     out = (xa - s.m) - log_of(s.sum) - out;
     ea = s.e(xa);
@@ -995,7 +992,7 @@ __device__ __forceinline__ void row_grad(char* tile, const PreferenceArgs& q, in
 constexpr int kMaxGroup = 32, kZeroBlocks = 64;
 
 template <class T, int AP, bool REF>
-__global__ __launch_bounds__(kRowThreads, AP <= 20 ? 4 : 2) void k_preference_short(PreferenceArgs q) {
+__global__ __launch_bounds__(kRowThreads, AP > 20 ? 2 : sizeof(T) == 2 ? 6 : 5) void k_preference_short(PreferenceArgs q) {
   __shared__ __align__(16) char tile[Tile<T, AP>::kBytes];
   __shared__ float ratio[kRowThreads];
   __shared__ int64_t edge[2 * kMaxGroup + 1];
@@ -1030,63 +1027,79 @@ __global__ __launch_bounds__(kRowThreads, AP <= 20 ? 4 : 2) void k_preference_sh
   if ((int)threadIdx.x <= seqs) edge[threadIdx.x] = held(raw, q.r.n);
   __syncthreads();
   const int64_t begin = edge[0], end = edge[seqs];
-  float e[AP], ea = 0.0f, total = 1.0f;
-  uint32_t legal = 0;
-  int action = -1, rows = 0;
-  for (int64_t row0 = begin; row0 < end; row0 += kRowThreads) {
-    const int64_t i = row0 + threadIdx.x;
-    rows = (int)(end - row0 < kRowThreads ? end - row0 : kRowThreads);
-    legal = row_of(q.r, i, (int)threadIdx.x < rows, action);
-    ratio[threadIdx.x] = row_ratio<T, AP, REF>(tile, q, row0, rows, legal, action, e, ea, total);
+
+  // a tile's log ratios to its sequences' sums (32 bits within a tile, 64 across)
+  const auto add_tile = [&](int64_t row0, int rows) {
     __syncthreads();
     for (int s = wave; s < seqs; s += kRowThreads / 64) {
       const int64_t lo = edge[s] - row0, hi = edge[s + 1] - row0;
       const int to = hi < rows ? (int)hi : rows;
-      float v = 0.0f;  // a tile's rows in 32 bits, tiles in 64
+      float v = 0.0f;
       for (int k = (lo > 0 ? (lo < rows ? (int)lo : rows) : 0) + ((int)threadIdx.x & 63); k < to; k += 64) v += ratio[k];
       v = wave_sum(v);
       if ((threadIdx.x & 63) == 0) sum[s] += (double)v;
     }
     __syncthreads();
-  }
-  double cost[1] = {0.0};
-  if ((int)threadIdx.x < pairs) {
-    const int s = 2 * threadIdx.x;
-    cost[0] = (double)pair_cost(q, pair0 + threadIdx.x, sum[s], sum[s + 1], ok, &coef[s]);
-    coef[s + 1] = -coef[s];
-  }
-  __syncthreads();
-  if (wave == 0) {  // the group's pairs are lanes of one wave
+  };
+  // the pairs, lanes of one wave
+  const auto close_pairs = [&]() {
+    double cost = 0.0;
+    if ((int)threadIdx.x < pairs) {
+      const int s = 2 * threadIdx.x;
+      cost = (double)pair_cost(q, pair0 + threadIdx.x, sum[s], sum[s + 1], ok, &coef[s]);
+      coef[s + 1] = -coef[s];
+    }
+    __syncthreads();
+    if (wave != 0) return;
 #pragma unroll
-    for (int d = kMaxGroup / 2; d >= 1; d >>= 1) cost[0] += __shfl_xor(cost[0], d, 64);
+    for (int d = kMaxGroup / 2; d >= 1; d >>= 1) cost += __shfl_xor(cost, d, 64);
     if (threadIdx.x == 0) {
-      q.partial[blockIdx.x] = cost[0];
-      if (groups == 1) *q.loss = (float)(cost[0] / (double)q.pairs);
+      q.partial[blockIdx.x] = cost;
+      if (groups == 1) *q.loss = (float)(cost / (double)q.pairs);
     }
-  }
-  if (!q.grad) return;
-  const bool once = end - begin <= kRowThreads;
-  for (int64_t row0 = begin; row0 < end; row0 += kRowThreads) {
-    const int64_t i = row0 + threadIdx.x;
-    if (!once) {
-      rows = (int)(end - row0 < kRowThreads ? end - row0 : kRowThreads);
-      legal = row_of(q.r, i, (int)threadIdx.x < rows, action);
-      stage<T, AP>(tile, q.r.logits, q.r.stride, row0, rows, q.r.A);
-      __syncthreads();
-      float x[AP];
-      Tile<T, AP>::read(tile, q.r.A, legal, x);
-      const float xa = Tile<T, AP>::read_one(tile, q.r.A, action);
-      const Softmax sm = softmax<false, AP>(x, e);
-      ea = sm.e(xa);
-      total = sm.sum;
-    }
-    int lo = 0, hi = seqs;  // the last sequence that starts at or before row i
+  };
+  // the coef of row i: its sequence is the last that starts at or before it
+  const auto coef_of = [&](int64_t i) {
+    int lo = 0, hi = seqs;
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
       if (edge[mid + 1] <= i) lo = mid + 1;
       else hi = mid;
     }
-    row_grad<T, AP>(tile, q, row0, rows, legal, action, e, ea, total, lo < seqs ? coef[lo] : 0.0f);
+    return lo < seqs ? coef[lo] : 0.0f;
+  };
+
+  float e[AP], ea, total;
+  int action;
+  if (end - begin <= kRowThreads) {
+    const int64_t i = begin + threadIdx.x;
+    const int rows = end > begin ? (int)(end - begin) : 0;
+    const uint32_t legal = row_of(q.r, i, (int)threadIdx.x < rows, action);
+    ratio[threadIdx.x] = row_ratio<T, AP, REF>(tile, q, begin, rows, legal, action, e, ea, total);
+    add_tile(begin, rows);
+    close_pairs();
+    if (q.grad) row_grad<T, AP>(tile, q, begin, rows, legal, action, e, ea, total, coef_of(i));
+    return;
+  }
+  for (int64_t row0 = begin; row0 < end; row0 += kRowThreads) {
+    const int rows = (int)(end - row0 < kRowThreads ? end - row0 : kRowThreads);
+    const uint32_t legal = row_of(q.r, row0 + threadIdx.x, (int)threadIdx.x < rows, action);
+    ratio[threadIdx.x] = row_ratio<T, AP, REF>(tile, q, row0, rows, legal, action, e, ea, total);
+    add_tile(row0, rows);
+  }
+  close_pairs();
+  if (!q.grad) return;
+  for (int64_t row0 = begin; row0 < end; row0 += kRowThreads) {
+    const int64_t i = row0 + threadIdx.x;
+    const int rows = (int)(end - row0 < kRowThreads ? end - row0 : kRowThreads);
+    const uint32_t legal = row_of(q.r, i, (int)threadIdx.x < rows, action);
+    stage<T, AP>(tile, q.r.logits, q.r.stride, row0, rows, q.r.A);
+    __syncthreads();
+    float x[AP];
+    Tile<T, AP>::read(tile, q.r.A, legal, x);
+    const float xa = Tile<T, AP>::read_one(tile, q.r.A, action);
+    const Softmax sm = softmax<false, AP>(x, e);
+    row_grad<T, AP>(tile, q, row0, rows, legal, action, e, sm.e(xa), sm.sum, coef_of(i));
     __syncthreads();
   }
 }

@@ -30,7 +30,7 @@ gradient, which raise there: capture the *_and_grad form and hand its gradient
 on (`logits.backward(grad)`).
 """
 import ctypes
-from typing import NamedTuple, Optional
+from typing import NamedTuple
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -76,48 +76,59 @@ class PreferenceLossAndGrad(NamedTuple):
 
 
 # ------------------------------------------------------------ arguments
-class _on:
-    """The device of `t` current (a no-op where it is); .stream is torch's
-    current stream of it."""
-
-    def __init__(self, t):
-        self.index = t.device.index
-        self.before = torch.cuda.current_device()
-
-    def __enter__(self):
-        if self.before != self.index:
-            torch.cuda.set_device(self.index)
-        return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(self.index))
-
-    def __exit__(self, *exc):
-        if self.before != self.index:
-            torch.cuda.set_device(self.before)
+_lib = None
 
 
-def _arg(t, name, like, shape, *dtypes):
-    """`t` checked and contiguous."""
+def _enqueue(name, device, *args):
+    """Call the library's `name` with the device current and torch's current
+    stream of it as the last argument."""
+    global _lib
+    if _lib is None:
+        _lib = _native.load()
+    index, before = device.index, torch._C._cuda_getDevice()
+    if before != index:
+        torch.cuda.set_device(index)
+    try:
+        rc = getattr(_lib, name)(*args, torch._C._cuda_getCurrentRawStream(index))
+    finally:
+        if before != index:
+            torch.cuda.set_device(before)
+    if rc != _native.COUP_OK:
+        _native.check(rc)
+
+
+def _wrong(t, name, device, shape, dtypes):
+    """What is wrong with an argument, as an exception."""
     if not isinstance(t, torch.Tensor):
-        raise ValueError(f"{name} must be a tensor")
+        return ValueError(f"{name} must be a tensor")
     if t.dtype not in dtypes:
-        raise ValueError(f"{name} must be {' or '.join(str(d)[6:] for d in dtypes)}, not {str(t.dtype)[6:]}")
-    if t.device != like.device:
-        raise ValueError(f"{name} is on {t.device}, not on {like.device}")
+        return ValueError(f"{name} must be {' or '.join(str(d)[6:] for d in dtypes)}, not {str(t.dtype)[6:]}")
+    if t.device != device:
+        return ValueError(f"{name} is on {t.device}, not on {device}")
     if t.shape != shape:
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, not {tuple(shape)}")
-    if t.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{name} is held constant: detach() it")
-    return t.contiguous()
+        return ValueError(f"{name} has shape {tuple(t.shape)}, not {tuple(shape)}")
+    return ValueError(f"{name} is held constant: detach() it")
+
+
+def _arg(t, name, device, shape, dtypes):
+    """`t` checked and contiguous."""
+    if (not isinstance(t, torch.Tensor) or t.dtype not in dtypes or t.device != device or t.shape != shape
+            or (t.requires_grad and torch.is_grad_enabled())):
+        raise _wrong(t, name, device, shape, dtypes)
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _table(t, name):
     """(the rows of a [..., A] tensor of logits, their stride in elements)"""
     if not isinstance(t, torch.Tensor) or t.dtype not in _DTYPES:
         raise ValueError(f"{name} must be a float32, float16 or bfloat16 tensor")
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         raise ValueError(f"{name} must be on a HIP device")
     A = t.shape[-1] if t.dim() else 0
     if not 1 <= A <= _native.MAX_POLICY_ACTIONS:
         raise ValueError(f"{name} must have 1..{_native.MAX_POLICY_ACTIONS} actions in the last dimension")
+    if t.is_contiguous():
+        return t, A
     rows = t.detach()
     if rows.dim() != 2:
         rows = rows.reshape(-1, A)
@@ -126,33 +137,36 @@ def _table(t, name):
     return rows, max(rows.stride(0), A)
 
 
+_INT8, _INT32, _FLOAT32 = (torch.int8,), (torch.int32, torch.uint32), (torch.float32,)
+_BOOL, _OFFSET, _BYTE = (torch.bool, torch.uint8), (torch.int32, torch.int64), (torch.uint8,)
+
+
 def _decisions(logits, legal_mask, actions=None, ref_logits=None):
     """A coup_decisions of the arguments, and the tensors it points into."""
     rows, stride = _table(logits, "logits")
-    lead = logits.shape[:-1]
-    mask = _arg(legal_mask, "legal_mask", logits, lead, torch.int32, torch.uint32)
-    keep = [rows, mask]
-    ref, ref_stride, acts = None, 0, None
+    lead, device = logits.shape[:-1], logits.device
+    A = logits.shape[-1]
+    mask = _arg(legal_mask, "legal_mask", device, lead, _INT32)
+    ref = acts = None
+    ref_stride = 0
     if actions is not None:
-        acts = _arg(actions, "actions", logits, lead, torch.int8)
-        keep.append(acts)
+        acts = _arg(actions, "actions", device, lead, _INT8)
     if ref_logits is not None:
-        _arg_ref(ref_logits, logits)
+        if not isinstance(ref_logits, torch.Tensor) or ref_logits.dtype != logits.dtype or ref_logits.shape != logits.shape:
+            raise ValueError("ref_logits must have the type and shape of logits")
+        _arg_held(ref_logits, "ref_logits", device)
         ref, ref_stride = _table(ref_logits, "ref_logits")
-        keep.append(ref)
-    d = _native.Decisions(rows.data_ptr(), stride, ref.data_ptr() if ref is not None else None, ref_stride,
-                          acts.data_ptr() if acts is not None else None, mask.data_ptr(), rows.shape[0], rows.shape[1],
-                          _DTYPES[rows.dtype])
-    return d, keep
+    d = _native.Decisions(rows.data_ptr(), stride, None if ref is None else ref.data_ptr(), ref_stride,
+                          None if acts is None else acts.data_ptr(), mask.data_ptr(), logits.numel() // A, A,
+                          _DTYPES[logits.dtype])
+    return d, (rows, mask, acts, ref)
 
 
-def _arg_ref(ref, logits):
-    if not isinstance(ref, torch.Tensor) or ref.dtype != logits.dtype or ref.shape != logits.shape:
-        raise ValueError("ref_logits must have the type and shape of logits")
-    if ref.device != logits.device:
-        raise ValueError(f"ref_logits is on {ref.device}, not on {logits.device}")
-    if ref.requires_grad and torch.is_grad_enabled():
-        raise ValueError("ref_logits is held constant: detach() it")
+def _arg_held(t, name, device):
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, not on {device}")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} is held constant: detach() it")
 
 
 # ------------------------------------------------------------ acting
@@ -167,13 +181,11 @@ def sample_actions(logits, legal_mask, uniform):
     action gives -1 (which `BatchedCoupEnv.step` skips) and 0; one with a NaN
     or +inf logit at a legal action, or only -inf ones, gives -1 and NaN."""
     d, keep = _decisions(logits, legal_mask)
-    u = _arg(uniform, "uniform", logits, logits.shape[:-1], torch.float32)
-    lib = _native.load()
-    actions = torch.empty(u.shape, dtype=torch.int8, device=u.device)
-    log_probs = torch.empty(u.shape, dtype=torch.float32, device=u.device)
-    with _on(u) as stream:
-        _native.check(lib.coup_sample_actions(ctypes.byref(d), u.data_ptr(), actions.data_ptr(), log_probs.data_ptr(),
-                                              stream))
+    device = logits.device
+    u = _arg(uniform, "uniform", device, logits.shape[:-1], _FLOAT32)
+    actions = torch.empty(u.shape, dtype=torch.int8, device=device)
+    log_probs = torch.empty_like(u)
+    _enqueue("coup_sample_actions", device, ctypes.byref(d), u.data_ptr(), actions.data_ptr(), log_probs.data_ptr())
     return actions, log_probs
 
 
@@ -194,10 +206,10 @@ def advantages(rewards, step_type, players, values, bootstrap=None, gamma=1.0, l
     steps that are no decision (FIRST, SKIPPED, no acting player)."""
     if not isinstance(values, torch.Tensor) or values.dtype not in _DTYPES:
         raise ValueError("values must be a float32, float16 or bfloat16 tensor")
-    if values.device.type != "cuda":
+    device = values.device
+    if device.type != "cuda":
         raise ValueError("values must be on a HIP device")
-    if values.requires_grad and torch.is_grad_enabled():
-        raise ValueError("values is held constant: detach() it")
+    _arg_held(values, "values", device)
     if values.dim() != 2:
         raise ValueError("values must be [T, B]")
     T, B = values.shape
@@ -207,18 +219,16 @@ def advantages(rewards, step_type, players, values, bootstrap=None, gamma=1.0, l
     gamma, lam = float(gamma), float(lam)
     if not (0.0 <= gamma <= 1.0 and 0.0 <= lam <= 1.0):
         raise ValueError("gamma and lam must be in 0..1")
-    r = _arg(rewards, "rewards", values, (T, B, P), torch.int8)
-    st = _arg(step_type, "step_type", values, (T, B), torch.uint8)
-    pl = _arg(players, "players", values, (T, B), torch.int8)
+    r = _arg(rewards, "rewards", device, (T, B, P), _INT8)
+    st = _arg(step_type, "step_type", device, (T, B), _BYTE)
+    pl = _arg(players, "players", device, (T, B), _INT8)
     v = values.contiguous()
-    boot = None if bootstrap is None else _arg(bootstrap, "bootstrap", values, (B, P), values.dtype)
-    lib = _native.load()
-    adv = torch.empty(T, B, dtype=torch.float32, device=v.device)
-    target = torch.empty(T, B, dtype=torch.float32, device=v.device)
+    boot = None if bootstrap is None else _arg(bootstrap, "bootstrap", device, (B, P), (values.dtype,))
+    adv = torch.empty(T, B, dtype=torch.float32, device=device)
+    target = torch.empty_like(adv)
     w = _native.Window(r.data_ptr(), st.data_ptr(), pl.data_ptr(), v.data_ptr(),
                        None if boot is None else boot.data_ptr(), T, B, P, _DTYPES[v.dtype])
-    with _on(v) as stream:
-        _native.check(lib.coup_advantages(ctypes.byref(w), gamma, lam, adv.data_ptr(), target.data_ptr(), stream))
+    _enqueue("coup_advantages", device, ctypes.byref(w), gamma, lam, adv.data_ptr(), target.data_ptr())
     return adv, target
 
 
@@ -229,10 +239,12 @@ class _LossOf(torch.autograd.Function):
     is 1).  A second backward over a retained graph makes the call again."""
 
     @staticmethod
-    def forward(ctx, logits, call, *inputs):
-        out, grad = call(True)
-        ctx.save_for_backward(logits, *inputs)  # their versions are checked where a second backward reads them
+    def forward(ctx, logits, call, args):
+        out, grad = call(True, logits, *args)
+        # for a second backward, which reads them: torch checks their versions there
+        ctx.save_for_backward(logits, *[t for t in args if isinstance(t, torch.Tensor)])
         ctx.call, ctx.grad = call, grad
+        ctx.args = [None if isinstance(t, torch.Tensor) else (t,) for t in args]
         ctx.mark_non_differentiable(*out[1:])
         return out
 
@@ -244,35 +256,31 @@ class _LossOf(torch.autograd.Function):
                                "_and_grad form and hand the gradient on")
         grad, ctx.grad = ctx.grad, None
         if grad is None:
-            ctx.saved_tensors
-            grad = ctx.call(True)[1]
+            logits, *tensors = ctx.saved_tensors
+            tensors = iter(tensors)
+            grad = ctx.call(True, logits, *[next(tensors) if a is None else a[0] for a in ctx.args])[1]
         scale = incoming.contiguous()
-        lib = _native.load()
-        with _on(grad) as stream:
-            _native.check(lib.coup_scale_grad(grad.data_ptr(), _DTYPES[grad.dtype], grad.numel(), scale.data_ptr(), stream))
-        return (grad,) + (None,) * (len(ctx.needs_input_grad) - 1)
+        _enqueue("coup_scale_grad", grad.device, grad.data_ptr(), _DTYPES[grad.dtype], grad.numel(), scale.data_ptr())
+        return grad, None, None
 
 
-def _loss(logits, call, inputs):
-    if not (logits.requires_grad and torch.is_grad_enabled()):
-        return call(False)[0]
+def _loss(call, logits, *args):
+    if not (isinstance(logits, torch.Tensor) and logits.requires_grad and torch.is_grad_enabled()):
+        return call(False, logits, *args)[0]
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError("a loss whose logits require a gradient cannot be captured into a graph: capture its "
                            "_and_grad form and hand the gradient on")
-    return _LossOf.apply(logits, call, *[t for t in inputs if t is not None])
+    return _LossOf.apply(logits, call, args)
 
 
-def _scratch(nbytes, device):
-    return torch.empty((nbytes + 7) // 8, dtype=torch.int64, device=device)
-
-
-def _policy_call(logits, actions, legal_mask, old_log_probs, advantages, ref_logits, active, clip_low, clip_high, kl_coef,
-                 entropy_coef):
+def _policy(want_grad, logits, actions, legal_mask, old_log_probs, advantages, ref_logits, active, clip_low, clip_high,
+            kl_coef, entropy_coef):
+    """((loss, stats, count, log_probs), gradient or None)"""
     d, keep = _decisions(logits, legal_mask, actions, ref_logits)
-    lead, dev = logits.shape[:-1], logits.device
-    old = _arg(old_log_probs, "old_log_probs", logits, lead, torch.float32)
-    adv = _arg(advantages, "advantages", logits, lead, torch.float32)
-    act = None if active is None else _arg(active, "active", logits, lead, torch.bool, torch.uint8)
+    lead, device = logits.shape[:-1], logits.device
+    old = _arg(old_log_probs, "old_log_probs", device, lead, _FLOAT32)
+    adv = _arg(advantages, "advantages", device, lead, _FLOAT32)
+    act = None if active is None else _arg(active, "active", device, lead, _BOOL)
     clip_low, clip_high, kl_coef, entropy_coef = float(clip_low), float(clip_high), float(kl_coef), float(entropy_coef)
     if not (0.0 <= clip_low <= 1.0 and 0.0 <= clip_high < float("inf")):
         raise ValueError("clip_low must be in 0..1, clip_high finite and not negative")
@@ -280,25 +288,18 @@ def _policy_call(logits, actions, legal_mask, old_log_probs, advantages, ref_log
         raise ValueError("kl_coef and entropy_coef must be finite, within 1e4")
     terms = _native.PolicyTerms(old.data_ptr(), adv.data_ptr(), None if act is None else act.data_ptr(), clip_low,
                                 clip_high, kl_coef, entropy_coef)
-    lib = _native.load()
-
-    def call(want_grad):
-        loss = torch.empty((), dtype=torch.float32, device=dev)
-        stats = torch.empty(4, dtype=torch.float32, device=dev)
-        count = torch.empty((), dtype=torch.int64, device=dev)
-        log_probs = torch.empty(lead, dtype=torch.float32, device=dev)
-        grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev) if want_grad else None
-        nbytes = lib.coup_policy_workspace(d.rows)
-        scratch = _scratch(nbytes, dev)
-        out = _native.PolicyOutputs(loss.data_ptr(), stats.data_ptr(), count.data_ptr(), log_probs.data_ptr(),
-                                    None if grad is None else grad.data_ptr())
-        with _on(logits) as stream:
-            _native.check(lib.coup_policy_loss(ctypes.byref(d), ctypes.byref(terms), ctypes.byref(out),
-                                               scratch.data_ptr(), nbytes, stream))
-        return (loss, stats, count, log_probs), grad
-
-    call.keep = (keep, old, adv, act)  # what d and terms point into
-    return call
+    loss = torch.empty((), dtype=torch.float32, device=device)
+    stats = torch.empty(4, dtype=torch.float32, device=device)
+    count = torch.empty((), dtype=torch.int64, device=device)
+    log_probs = torch.empty_like(old)
+    grad = torch.empty(logits.shape, dtype=logits.dtype, device=device) if want_grad else None
+    nbytes = _native.load().coup_policy_workspace(d.rows)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    out = _native.PolicyOutputs(loss.data_ptr(), stats.data_ptr(), count.data_ptr(), log_probs.data_ptr(),
+                                None if grad is None else grad.data_ptr())
+    _enqueue("coup_policy_loss", device, ctypes.byref(d), ctypes.byref(terms), ctypes.byref(out), scratch.data_ptr(),
+             nbytes)
+    return (loss, stats, count, log_probs), grad
 
 
 def policy_loss(logits, actions, legal_mask, old_log_probs, advantages, ref_logits=None, active=None, clip_low=0.2,
@@ -318,28 +319,28 @@ def policy_loss(logits, actions, legal_mask, old_log_probs, advantages, ref_logi
     The loss is 0, with zero gradients, where nothing counts.  A ratio exactly
     on a border is not clipped.  A legal action that the reference gives no
     probability makes the KL infinite."""
-    call = _policy_call(logits, actions, legal_mask, old_log_probs, advantages, ref_logits, active, clip_low, clip_high,
-                        kl_coef, entropy_coef)
-    return PolicyLoss(*_loss(logits, call, (actions, legal_mask, old_log_probs, advantages, ref_logits, active)))
+    return PolicyLoss(*_loss(_policy, logits, actions, legal_mask, old_log_probs, advantages, ref_logits, active,
+                             clip_low, clip_high, kl_coef, entropy_coef))
 
 
 def policy_loss_and_grad(logits, actions, legal_mask, old_log_probs, advantages, ref_logits=None, active=None,
                          clip_low=0.2, clip_high=0.2, kl_coef=0.0, entropy_coef=0.0) -> PolicyLossAndGrad:
     """policy_loss and its gradient in the logits in one pass, outside
     autograd (hand the gradient on with logits.backward(grad))."""
-    out, grad = _policy_call(logits, actions, legal_mask, old_log_probs, advantages, ref_logits, active, clip_low,
-                             clip_high, kl_coef, entropy_coef)(True)
+    out, grad = _policy(True, logits, actions, legal_mask, old_log_probs, advantages, ref_logits, active, clip_low,
+                        clip_high, kl_coef, entropy_coef)
     return PolicyLossAndGrad(*out, grad)
 
 
-def _preference_call(logits, actions, legal_mask, offsets, ref_logits, beta, label_smoothing):
+def _preference(want_grad, logits, actions, legal_mask, offsets, ref_logits, beta, label_smoothing):
+    """((loss, rewards), gradient or None)"""
     if not isinstance(logits, torch.Tensor) or logits.dim() != 2:
         raise ValueError("logits must be [rows, A]: the sequences' decisions one after another")
     d, keep = _decisions(logits, legal_mask, actions, ref_logits)
-    dev = logits.device
+    device = logits.device
     if not isinstance(offsets, torch.Tensor) or offsets.dim() != 1 or offsets.numel() % 2 == 0:
         raise ValueError("offsets must be [2 * pairs + 1]")
-    off = _arg(offsets, "offsets", logits, offsets.shape, torch.int32, torch.int64)
+    off = _arg(offsets, "offsets", device, offsets.shape, _OFFSET)
     pairs = off.numel() // 2
     beta, label_smoothing = float(beta), float(label_smoothing)
     if beta - beta != 0.0:
@@ -347,22 +348,15 @@ def _preference_call(logits, actions, legal_mask, offsets, ref_logits, beta, lab
     if not 0.0 <= label_smoothing <= 0.5:
         raise ValueError("label_smoothing must be in 0..0.5")
     terms = _native.PreferenceTerms(off.data_ptr(), off.element_size(), pairs, beta, label_smoothing)
-    lib = _native.load()
-
-    def call(want_grad):
-        loss = torch.empty((), dtype=torch.float32, device=dev)
-        rewards = torch.empty(2 * pairs, dtype=torch.float32, device=dev)
-        grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev) if want_grad else None
-        nbytes = lib.coup_preference_workspace(d.rows, pairs)
-        scratch = _scratch(max(nbytes, 8), dev)
-        out = _native.PreferenceOutputs(loss.data_ptr(), rewards.data_ptr(), None if grad is None else grad.data_ptr())
-        with _on(logits) as stream:
-            _native.check(lib.coup_preference_loss(ctypes.byref(d), ctypes.byref(terms), ctypes.byref(out),
-                                                   scratch.data_ptr(), nbytes, stream))
-        return (loss, rewards), grad
-
-    call.keep = (keep, off)  # what d and terms point into
-    return call
+    loss = torch.empty((), dtype=torch.float32, device=device)
+    rewards = torch.empty(2 * pairs, dtype=torch.float32, device=device)
+    grad = torch.empty(logits.shape, dtype=logits.dtype, device=device) if want_grad else None
+    nbytes = _native.load().coup_preference_workspace(d.rows, pairs)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    out = _native.PreferenceOutputs(loss.data_ptr(), rewards.data_ptr(), None if grad is None else grad.data_ptr())
+    _enqueue("coup_preference_loss", device, ctypes.byref(d), ctypes.byref(terms), ctypes.byref(out),
+             scratch.data_ptr(), nbytes)
+    return (loss, rewards), grad
 
 
 def preference_loss(logits, actions, legal_mask, offsets, ref_logits=None, beta=0.1,
@@ -380,13 +374,12 @@ def preference_loss(logits, actions, legal_mask, offsets, ref_logits=None, beta=
         -(1 - label_smoothing) log sigmoid(x) - label_smoothing log sigmoid(-x).
     Sequences may be empty; rows outside every sequence get zero gradients.
     Offsets that do not ascend from 0..rows make the loss NaN."""
-    call = _preference_call(logits, actions, legal_mask, offsets, ref_logits, beta, label_smoothing)
-    return PreferenceLoss(*_loss(logits, call, (actions, legal_mask, offsets, ref_logits)))
+    return PreferenceLoss(*_loss(_preference, logits, actions, legal_mask, offsets, ref_logits, beta, label_smoothing))
 
 
-def preference_loss_and_grad(logits, actions, legal_mask, offsets, ref_logits: Optional[torch.Tensor] = None, beta=0.1,
+def preference_loss_and_grad(logits, actions, legal_mask, offsets, ref_logits=None, beta=0.1,
                              label_smoothing=0.0) -> PreferenceLossAndGrad:
     """preference_loss and its gradient in the logits in one call, outside
     autograd (hand the gradient on with logits.backward(grad))."""
-    out, grad = _preference_call(logits, actions, legal_mask, offsets, ref_logits, beta, label_smoothing)(True)
+    out, grad = _preference(True, logits, actions, legal_mask, offsets, ref_logits, beta, label_smoothing)
     return PreferenceLossAndGrad(*out, grad)
