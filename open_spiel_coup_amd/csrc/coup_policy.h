@@ -22,6 +22,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "coup_launch_log.h"
 #include "coup_mi355x.h"
 
@@ -29,7 +31,6 @@ namespace coup {
 namespace policy {
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kRowThreads = 256;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
@@ -304,12 +305,16 @@ __device__ __forceinline__ float exp_of(float v) {  // the product's rounding is
   const float e = __builtin_amdgcn_exp2f(hi);
   return lo == lo ? __builtin_fmaf(e * lo, kLn2, e) : e;
 }
-// log(1 + v), 0 <= v: the rounding of w = 1 + v is made good by v / (w - 1),
+// log(1 + v), v > -1 / 2: the rounding of w = 1 + v is made good by v / (w - 1),
 // along which log(w) / (w - 1) hardly changes.
 __device__ __forceinline__ float log1p_of(float v) {
   const float w = 1.0f + v, d = w - 1.0f;
   return d == 0.0f ? v : log_of(w) * (v * __builtin_amdgcn_rcpf(d));
 }
+
+// log(1 + v) for any v > -1, and the log of a ratio near 1.
+__device__ __forceinline__ float log1p_any(float v) { return v > -0.5f ? log1p_of(v) : log_of(1.0f + v); }
+__device__ __forceinline__ float log_ratio(float a, float b) { return log1p_any((a - b) / b); }
 
 struct Softmax {
   float m;    // largest logit
@@ -328,7 +333,7 @@ __device__ __forceinline__ float row_max(const float (&x)[AP]) {
 }
 
 // The log of a row's sum of e, `others` the sum of the e's fractions, that is
-// without the ones: log1p of it while only one e is 1, so that a nearly
+// without the ones: log1p of it while only one e is (near) 1, so that a nearly
 // certain action's log probability keeps its precision.
 __device__ __forceinline__ float lse_of(float sum, float others) {
   return sum - others < 1.5f ? log1p_of(others) : log_of(sum);
@@ -670,13 +675,13 @@ __device__ __forceinline__ float wave_sum(float v) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 
-// Four values summed over the wave at once: the sum of value k is lane k's (7
-// exchanges for 24: each of the first two halves what a lane still holds).
-__device__ __forceinline__ float wave_sum_four(const float (&v)[4]) {
+// Four values summed over the wave at once, in 64 bits (a loss's terms nearly
+// cancel): the sum of value k is lane k's (7 exchanges for 24: each of the first two halves what a lane still holds).
+__device__ __forceinline__ double wave_sum_four(const float (&v)[4]) {
   const bool odd = threadIdx.x & 1, upper = threadIdx.x & 2;
-  const float a = (odd ? v[1] : v[0]) + __shfl_xor(odd ? v[0] : v[1], 1, 64);
-  const float b = (odd ? v[3] : v[2]) + __shfl_xor(odd ? v[2] : v[3], 1, 64);
-  float s = (upper ? b : a) + __shfl_xor(upper ? a : b, 2, 64);
+  const double a = (double)(odd ? v[1] : v[0]) + (double)__shfl_xor(odd ? v[0] : v[1], 1, 64);
+  const double b = (double)(odd ? v[3] : v[2]) + (double)__shfl_xor(odd ? v[2] : v[3], 1, 64);
+  double s = (upper ? b : a) + __shfl_xor(upper ? a : b, 2, 64);
 #pragma unroll
   for (int d = 4; d < 64; d *= 2) s += __shfl_xor(s, d, 64);
   return s;
@@ -717,14 +722,21 @@ struct PolicyArgs {
   double low, high;           // 1 - clip_low, 1 + clip_high
   float log_low, log_high;    // their logs
   float kl, ent;
+  int few;  // ratios and log probabilities from 64-bit sums in every row (kFewRows)
   float* log_probs;  // null: not wanted
   void* grad;        // null: no gradient
-  f32x4* partial;    // [blocks] sums of the terms over a block's rows
+  double* partial;   // [blocks][4] sums of the terms over a block's rows
   int32_t* decided;  // [blocks] its decisions
   float* counts;     // [count blocks] the call's decisions, for the gradient
+  uint32_t* ticket;  // of the folds that follow
   int count_blocks;
 };
 
+// Up to this many rows every row's ratio is taken in 64 bits, not only those
+// by a border: a loss of few terms that nearly cancel keeps its digits (over
+// many rows the 32-bit roundings average out), and a block a CU or less hides
+// the 18 exponentials a row.
+constexpr int64_t kFewRows = 65536;
 constexpr int kCountBlocks = 256, kCountThreads = 1024, kFinishThreads = 1024;
 
 // How many decisions there are: 6 bytes a row, four rows a thread at a time.
@@ -759,7 +771,7 @@ __global__ __launch_bounds__(kCountThreads) void k_policy_count(PolicyArgs q) {
 
 template <class T, int AP, bool REF>
 __global__ __launch_bounds__(kRowThreads, AP <= 20 ? 4 : 2) void k_policy_loss(PolicyArgs q) {
-  __shared__ float lds[4 * (kRowThreads / 64)];
+  __shared__ double lds[4 * (kRowThreads / 64)];
   __shared__ int decisions[kRowThreads / 64];
   __shared__ __align__(16) char tile[Tile<T, AP>::kBytes];
   const int64_t row0 = (int64_t)blockIdx.x * kRowThreads, i = row0 + threadIdx.x;
@@ -799,31 +811,32 @@ __global__ __launch_bounds__(kRowThreads, AP <= 20 ? 4 : 2) void k_policy_loss(P
     // x becomes t
     float e[AP];
     const Softmax s = softmax<false, AP>(x, e);
-    float et = 0.0f, er = 0.0f;  // sums of e t and e t_ref
+    float et = 0.0f, ed = 0.0f;  // sums of e t and e (t - t_ref)
 #pragma unroll
     for (int a = 0; a < AP; ++a) {
       et += e[a] * x[a];
-      if (REF) er += e[a] * d[a];
+      if (REF) ed += e[a] * (x[a] - d[a]);
     }
     const float inv = __builtin_amdgcn_rcpf(s.sum), lse = log_of(s.sum);
-    et *= inv, er *= inv;
+    et *= inv, ed *= inv;
     entropy = lse - et;
     if (REF) {
-      kl = (et - er) - log_of(s.sum * __builtin_amdgcn_rcpf(rs.sum));
+      kl = ed - log_ratio(s.sum, rs.sum);
       if (kl > 1e24f) kl = INFINITY;  // an action that the reference never takes
     }
     logp = (xa - s.m) - lse;
-    const float dl = logp - old;
-    const float border = adv > 0.0f ? q.log_high : q.log_low;
+    const float dl = logp - old, border = adv > 0.0f ? q.log_high : q.log_low;
     bool over = adv > 0.0f ? dl > border : dl < border;
+    float rho = exp_of(dl);
     // 32 bits hold dl to a few 2^-23 of its terms
-    if (fabsf(dl - border) <= 4.76837158e-7f * (4.0f + fabsf(xa - s.m) + fabsf(old))) {
-      const double lhs = exp((double)xa - (double)s.m - (double)old);  // rho, times the sum
-      const double sum = sum64((const T*)q.r.logits + i * q.r.stride, legal, s.m);
-      over = adv > 0.0f ? lhs > q.high * sum : lhs < q.low * sum;
+    if (q.few || fabsf(dl - border) <= 4.76837158e-7f * (4.0f + fabsf(xa - s.m) + fabsf(old))) {
+      const double whole = sum64((const T*)q.r.logits + i * q.r.stride, legal, s.m);
+      const double top = exp((double)xa - (double)s.m - (double)old);
+      over = adv > 0.0f ? top > q.high * whole : top < q.low * whole;
+      rho = (float)(top / whole);
+      if (q.few) logp = (xa - s.m) - lse_of((float)whole, (float)(whole - 1.0));
     }
     over = over && adv != 0.0f;
-    const float rho = exp_of(dl);
     surrogate = adv == 0.0f ? 0.0f : -(over ? (float)(adv > 0.0f ? q.high : q.low) : rho) * adv;
     clipped = over ? 1.0f : 0.0f;
     if (q.grad) {
@@ -831,7 +844,7 @@ __global__ __launch_bounds__(kRowThreads, AP <= 20 ? 4 : 2) void k_policy_loss(P
       // cancel: (ent + kl) (t_b - E t) - kl (tr_b - E tr) - w
       const float w = (over || adv == 0.0f) ? 0.0f : -rho * adv;
       const float share = inv * scale, ct = (REF ? q.ent + q.kl : q.ent) * share, cr = REF ? q.kl * share : 0.0f;
-      const float base = cr * er - ct * et - w * share;
+      const float base = cr * (et - ed) - ct * et - w * share;
 #pragma unroll
       for (int a = 0; a < AP; ++a) x[a] = e[a] * (ct * x[a] + (REF ? base - cr * d[a] : base));
       ga = s.e(xa) * (ct * s.t(xa) + (REF ? base - cr * rta : base)) + w * scale;
@@ -852,16 +865,17 @@ __global__ __launch_bounds__(kRowThreads, AP <= 20 ? 4 : 2) void k_policy_loss(P
     Tile<T, AP>::copy_out(tile, (T*)q.grad, row0, rows, q.r.A);
   }
   const float sums[4] = {surrogate, kl, entropy, clipped};
-  const float v = wave_sum_four(sums);
+  const double v = wave_sum_four(sums);
   if ((threadIdx.x & 63) < 4) lds[(threadIdx.x >> 6) * 4 + (threadIdx.x & 63)] = v;
   const int here = (int)__popcll(__ballot(legal != 0));
   if ((threadIdx.x & 63) == 0) decisions[threadIdx.x >> 6] = here;
   __syncthreads();
   if (threadIdx.x < 4) {
-    float total = 0.0f;
+    double total = 0.0;
     for (int w = 0; w < kRowThreads / 64; ++w) total += lds[4 * w + threadIdx.x];
-    ((float*)(q.partial + blockIdx.x))[threadIdx.x] = total;
+    q.partial[4 * (int64_t)blockIdx.x + threadIdx.x] = total;
   }
+  if (blockIdx.x == 0 && threadIdx.x == 5) *q.ticket = 0;
   if (threadIdx.x == 4) {
     int total = 0;
     for (int w = 0; w < kRowThreads / 64; ++w) total += decisions[w];
@@ -870,20 +884,39 @@ __global__ __launch_bounds__(kRowThreads, AP <= 20 ? 4 : 2) void k_policy_loss(P
 }
 
 // The blocks' sums in a fixed order, in 64 bits: the loss and its terms'
-// means.  One block: the 16,384 blocks of 4 x 2^20 rows left 320 KiB.
-__global__ __launch_bounds__(kFinishThreads) void k_policy_finish(const f32x4* __restrict__ partial,
-                                                                   const int32_t* __restrict__ decided, int64_t blocks,
-                                                                   double kl, double ent, float* loss, float* stats,
-                                                                   int64_t* count) {
-  __shared__ double lds[5 * (kFinishThreads / 64)];
+// means.  16,384 blocks (4 x 2^20 rows) leave 576 KiB, which one block takes
+// 13 us to read; so kFoldBlocks of them fold a stretch each, and the one that
+// is done last (by a ticket that the loss kernel reset) folds those.
+constexpr int kFoldBlocks = 64, kFoldStretch = 256;
+
+__global__ __launch_bounds__(kRowThreads) void k_policy_finish(const double* __restrict__ partial,
+                                                                const int32_t* __restrict__ decided, int64_t blocks,
+                                                                double* fold, uint32_t* ticket, double kl, double ent,
+                                                                float* loss, float* stats, int64_t* count) {
+  __shared__ double lds[5 * (kRowThreads / 64)];
+  __shared__ bool last;
   double s[5] = {0.0, 0.0, 0.0, 0.0, 0.0};
-#pragma unroll 4
-  for (int64_t i = threadIdx.x; i < blocks; i += kFinishThreads) {
-    const f32x4 v = partial[i];
-    for (int k = 0; k < 4; ++k) s[k] += (double)v[k];
+  const int64_t from = blocks * blockIdx.x / gridDim.x, to = blocks * (blockIdx.x + 1) / gridDim.x;
+  for (int64_t i = from + threadIdx.x; i < to; i += kRowThreads) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) s[k] += partial[4 * i + k];
     s[4] += (double)decided[i];
   }
-  block_sum<kFinishThreads, 5>(s, lds);
+  block_sum<kRowThreads, 5>(s, lds);
+  if (gridDim.x > 1) {
+    if (threadIdx.x == 0) {
+      for (int k = 0; k < 5; ++k) fold[5 * blockIdx.x + k] = s[k];
+      __threadfence();  // the fold before the ticket, and the ticket before the others' folds
+      last = atomicAdd(ticket, 1u) == gridDim.x - 1;
+      __threadfence();
+    }
+    __syncthreads();
+    if (!last) return;
+#pragma unroll
+    for (int k = 0; k < 5; ++k) s[k] = threadIdx.x < gridDim.x ? fold[5 * threadIdx.x + k] : 0.0;
+    __syncthreads();
+    block_sum<kRowThreads, 5>(s, lds);
+  }
   if (threadIdx.x != 0) return;
   const double n = s[4] > 0.0 ? s[4] : 1.0;
   for (int k = 0; k < 4; ++k) s[k] /= n;
@@ -947,23 +980,33 @@ __device__ __forceinline__ bool ascending(int64_t a, int64_t b, int64_t c, int64
 }
 
 // A tile's rows: this thread's log ratio, its e, the action's and their sum.
-template <class T, int AP, bool REF>
+template <class T, int AP, bool REF, bool FEW>
 __device__ __forceinline__ float row_ratio(char* tile, const PreferenceArgs& q, int64_t row0, int rows, uint32_t legal,
                                            int action, float (&e)[AP], float& ea, float& sum) {
-  float x[AP], d[AP], xa, out = 0.0f;
+  float x[AP], d[AP], xa, out = 0.0f, one = 0.0f;
+  Softmax rs{0.0f, 1.0f, 0.0f};
   stage_rows<T, AP, REF>(
       tile, q.r, row0, rows, legal, action, d,
-      [&](float(&row)[AP], float one) {
+      [&](float(&row)[AP], float taken) {
         float unused[AP];
-        const Softmax s = softmax<false, AP>(row, unused);
-        out = legal ? (one - s.m) - log_of(s.sum) : 0.0f;
+        rs = softmax<false, AP>(row, unused);
+        one = taken;
       },
       x, xa);
   sum = 1.0f;
   ea = 0.0f;
   if (legal) {
     const Softmax s = softmax<false, AP>(x, e);
-    out = (xa - s.m) - log_of(s.sum) - out;
+    // the two sums' logs as one, of a ratio near 1
+    out = REF ? (xa - s.m) - (one - rs.m) : xa - s.m;
+    if (FEW) {
+      const int64_t i = row0 + threadIdx.x;
+      double ratio = sum64((const T*)q.r.logits + i * q.r.stride, legal, s.m);
+      if (REF) ratio /= sum64((const T*)q.r.ref + i * q.r.ref_stride, legal, rs.m);
+      out -= log1p_any((float)(ratio - 1.0));
+    } else {
+      out -= REF ? log_ratio(s.sum, rs.sum) : log_of(s.sum);
+    }
     ea = s.e(xa);
     sum = s.sum;
   }
@@ -991,8 +1034,8 @@ __device__ __forceinline__ void row_grad(char* tile, const PreferenceArgs& q, in
 // write the zero gradients of the rows outside every sequence.
 constexpr int kMaxGroup = 32, kZeroBlocks = 64;
 
-template <class T, int AP, bool REF>
-__global__ __launch_bounds__(kRowThreads, AP > 20 ? 2 : sizeof(T) == 2 ? 6 : 5) void k_preference_short(PreferenceArgs q) {
+template <class T, int AP, bool REF, bool FEW>
+__global__ __launch_bounds__(kRowThreads, AP > 20 ? 2 : FEW ? 4 : sizeof(T) == 2 ? 6 : 5) void k_preference_short(PreferenceArgs q) {
   __shared__ __align__(16) char tile[Tile<T, AP>::kBytes];
   __shared__ float ratio[kRowThreads];
   __shared__ int64_t edge[2 * kMaxGroup + 1];
@@ -1075,7 +1118,7 @@ __global__ __launch_bounds__(kRowThreads, AP > 20 ? 2 : sizeof(T) == 2 ? 6 : 5) 
     const int64_t i = begin + threadIdx.x;
     const int rows = end > begin ? (int)(end - begin) : 0;
     const uint32_t legal = row_of(q.r, i, (int)threadIdx.x < rows, action);
-    ratio[threadIdx.x] = row_ratio<T, AP, REF>(tile, q, begin, rows, legal, action, e, ea, total);
+    ratio[threadIdx.x] = row_ratio<T, AP, REF, FEW>(tile, q, begin, rows, legal, action, e, ea, total);
     add_tile(begin, rows);
     close_pairs();
     if (q.grad) row_grad<T, AP>(tile, q, begin, rows, legal, action, e, ea, total, coef_of(i));
@@ -1084,7 +1127,7 @@ __global__ __launch_bounds__(kRowThreads, AP > 20 ? 2 : sizeof(T) == 2 ? 6 : 5) 
   for (int64_t row0 = begin; row0 < end; row0 += kRowThreads) {
     const int rows = (int)(end - row0 < kRowThreads ? end - row0 : kRowThreads);
     const uint32_t legal = row_of(q.r, row0 + threadIdx.x, (int)threadIdx.x < rows, action);
-    ratio[threadIdx.x] = row_ratio<T, AP, REF>(tile, q, row0, rows, legal, action, e, ea, total);
+    ratio[threadIdx.x] = row_ratio<T, AP, REF, FEW>(tile, q, row0, rows, legal, action, e, ea, total);
     add_tile(row0, rows);
   }
   close_pairs();
@@ -1107,7 +1150,7 @@ __global__ __launch_bounds__(kRowThreads, AP > 20 ? 2 : sizeof(T) == 2 ? 6 : 5) 
 // Long sequences: every row's log ratio to memory, the sequences' sums from
 // slices of them, the pairs, then the gradient with the logits read again
 // (A sizeof(T) of a row's 3 A sizeof(T) + 5 bytes).
-template <class T, int AP, bool REF>
+template <class T, int AP, bool REF, bool FEW>
 __global__ __launch_bounds__(kRowThreads) void k_preference_rows(PreferenceArgs q) {
   __shared__ __align__(16) char tile[Tile<T, AP>::kBytes];
   const int64_t row0 = (int64_t)blockIdx.x * kRowThreads, i = row0 + threadIdx.x;
@@ -1116,7 +1159,7 @@ __global__ __launch_bounds__(kRowThreads) void k_preference_rows(PreferenceArgs 
   int action;
   const uint32_t legal = row_of(q.r, i, mine, action);
   float e[AP], ea, total;
-  const float out = row_ratio<T, AP, REF>(tile, q, row0, rows, legal, action, e, ea, total);
+  const float out = row_ratio<T, AP, REF, FEW>(tile, q, row0, rows, legal, action, e, ea, total);
   if (mine) q.ratio[i] = out;
 }
 
@@ -1247,6 +1290,15 @@ void with_rows(int dtype, int A, F f) {
   with_dtype(dtype, [&](auto t) { with_actions<typename decltype(t)::type>(A, f); });
 }
 
+// f(bool constant, bool constant)
+template <class F>
+void with_flags(bool a, bool b, F f) {
+  if (a && b) f(std::true_type(), std::true_type());
+  else if (a) f(std::true_type(), std::false_type());
+  else if (b) f(std::false_type(), std::true_type());
+  else f(std::false_type(), std::false_type());
+}
+
 inline void launch_sample(const Rows& r, int dtype, const float* uniform, int8_t* actions, float* log_probs,
                           hipStream_t s) {
   with_rows(dtype, r.A, [&](auto t, auto ap) {
@@ -1279,16 +1331,20 @@ inline void launch_advantages(const AdvantageArgs& q, int players, hipStream_t s
 }
 
 inline size_t policy_workspace(int64_t n) {
-  return sizeof(float) * kCountBlocks + (sizeof(f32x4) + sizeof(int32_t)) * row_blocks(n);
+  return sizeof(double) * (4 * (size_t)row_blocks(n) + 5 * kFoldBlocks) + sizeof(float) * (kCountBlocks + 1) +
+         sizeof(int32_t) * row_blocks(n);
 }
 
 inline void launch_policy(PolicyArgs q, int dtype, double kl, double ent, float* loss, float* stats, int64_t* count,
                           void* workspace, hipStream_t s) {
   const unsigned blocks = row_blocks(q.r.n);
   const int64_t counters = (q.r.n + 4 * kCountThreads - 1) / (4 * kCountThreads);
-  q.partial = (f32x4*)workspace;
-  q.counts = (float*)(q.partial + blocks);
-  q.decided = (int32_t*)(q.counts + kCountBlocks);
+  q.partial = (double*)workspace;
+  double* fold = q.partial + 4 * (int64_t)blocks;
+  q.counts = (float*)(fold + 5 * kFoldBlocks);
+  q.ticket = (uint32_t*)(q.counts + kCountBlocks);
+  q.decided = (int32_t*)(q.ticket + 1);
+  q.few = q.r.n <= kFewRows;
   q.count_blocks = (int)(counters < kCountBlocks ? counters : kCountBlocks);
   if (blocks) {
     if (q.grad) k_policy_count<<<q.count_blocks, kCountThreads, 0, s>>>(q);
@@ -1299,7 +1355,8 @@ inline void launch_policy(PolicyArgs q, int dtype, double kl, double ent, float*
       else k_policy_loss<T, AP, false><<<blocks, kRowThreads, 0, s>>>(q);
     });
   }
-  k_policy_finish<<<1, kFinishThreads, 0, s>>>(q.partial, q.decided, blocks, kl, ent, loss, stats, count);
+  const unsigned folds = blocks / kFoldStretch < 1 ? 1 : blocks / kFoldStretch < kFoldBlocks ? blocks / kFoldStretch : kFoldBlocks;
+  k_policy_finish<<<folds, kRowThreads, 0, s>>>(q.partial, q.decided, blocks, fold, q.ticket, kl, ent, loss, stats, count);
 }
 
 // How a preference call is split.  Short where a pair has at most kShortRows
@@ -1348,14 +1405,19 @@ inline void launch_preference(PreferenceArgs q, int dtype, void* workspace, hipS
     constexpr int AP = decltype(ap)::value;
     if (p.is_short) {
       const int64_t grid = p.blocks + (q.grad && q.r.n ? kZeroBlocks : 0);
-      if (grid && q.r.ref) k_preference_short<T, AP, true><<<(unsigned)grid, kRowThreads, 0, s>>>(q);
-      else if (grid) k_preference_short<T, AP, false><<<(unsigned)grid, kRowThreads, 0, s>>>(q);
+      if (grid) {
+        with_flags(q.r.ref != nullptr, q.r.n <= kFewRows, [&](auto ref, auto few) {
+          k_preference_short<T, AP, decltype(ref)::value, decltype(few)::value>
+              <<<(unsigned)grid, kRowThreads, 0, s>>>(q);
+        });
+      }
     } else {
       q.sums = q.partial + p.blocks + 1;
       q.coef = (float*)(q.sums + 2 * q.pairs * p.slices);
       q.ratio = q.coef + 2 * q.pairs;
-      if (q.r.ref) k_preference_rows<T, AP, true><<<tiles, kRowThreads, 0, s>>>(q);
-      else k_preference_rows<T, AP, false><<<tiles, kRowThreads, 0, s>>>(q);
+      with_flags(q.r.ref != nullptr, q.r.n <= kFewRows, [&](auto ref, auto few) {
+        k_preference_rows<T, AP, decltype(ref)::value, decltype(few)::value><<<tiles, kRowThreads, 0, s>>>(q);
+      });
       k_preference_sums<<<(unsigned)(2 * q.pairs * p.slices), kRowThreads, 0, s>>>(q);
       k_preference_pairs<<<(unsigned)p.blocks, kPairThreads, 0, s>>>(q);
       if (q.grad) k_preference_grad<T, AP><<<tiles, kRowThreads, 0, s>>>(q);
