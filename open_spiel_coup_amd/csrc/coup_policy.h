@@ -24,7 +24,6 @@
 
 #include <type_traits>
 
-#include "coup_launch_log.h"
 #include "coup_mi355x.h"
 
 namespace coup {
@@ -303,7 +302,7 @@ __device__ __forceinline__ float log_of(float v) { return __builtin_amdgcn_logf(
 __device__ __forceinline__ float exp_of(float v) {  // the product's rounding is made good
   const float hi = v * kLog2e, lo = __builtin_fmaf(v, kLog2e, -hi);
   const float e = __builtin_amdgcn_exp2f(hi);
-  return lo == lo ? __builtin_fmaf(e * lo, kLn2, e) : e;
+  return e < INFINITY && lo == lo ? __builtin_fmaf(e * lo, kLn2, e) : e;  // 0 and inf as they are
 }
 // log(1 + v), v > -1 / 2: the rounding of w = 1 + v is made good by v / (w - 1),
 // along which log(w) / (w - 1) hardly changes.
@@ -967,6 +966,7 @@ __device__ __forceinline__ int64_t offset_at(const PreferenceArgs& q, int64_t s)
 __device__ __forceinline__ float pair_cost(const PreferenceArgs& q, int64_t pair, double chosen, double rejected, bool ok,
                                            float* coef) {
   chosen *= q.beta, rejected *= q.beta;
+  if (!ok) chosen = rejected = NAN;
   if (q.rewards) q.rewards[2 * pair] = (float)chosen, q.rewards[2 * pair + 1] = (float)rejected;
   const float x = (float)(chosen - rejected), size = fabsf(x), eps = (float)q.eps;
   const float y = exp_of(-size), part = __builtin_amdgcn_rcpf(1.0f + y);
@@ -1054,11 +1054,7 @@ __global__ __launch_bounds__(kRowThreads, AP > 20 ? 2 : FEW ? 4 : sizeof(T) == 2
   const int64_t pair0 = (int64_t)blockIdx.x * q.group;
   const int pairs = (int)(q.pairs - pair0 < q.group ? q.pairs - pair0 : q.group);
   const int wave = (int)threadIdx.x >> 6, seqs = 2 * pairs;
-  int64_t raw = 0;
-  if ((int)threadIdx.x <= seqs) {
-    raw = raw_offset(q, 2 * pair0 + threadIdx.x);
-    edge[threadIdx.x] = raw;
-  }
+  if ((int)threadIdx.x <= seqs) edge[threadIdx.x] = raw_offset(q, 2 * pair0 + threadIdx.x);
   if ((int)threadIdx.x < seqs) sum[threadIdx.x] = 0.0;
   __syncthreads();
   bool ok = true;
@@ -1066,17 +1062,16 @@ __global__ __launch_bounds__(kRowThreads, AP > 20 ? 2 : FEW ? 4 : sizeof(T) == 2
     const int64_t* o = edge + 2 * threadIdx.x;
     ok = ascending(o[0], o[1], o[2], q.r.n);
   }
-  __syncthreads();
-  if ((int)threadIdx.x <= seqs) edge[threadIdx.x] = held(raw, q.r.n);
-  __syncthreads();
-  const int64_t begin = edge[0], end = edge[seqs];
+  // a group of bad offsets is not walked: the groups' rows are never more than the call's
+  const bool good = __syncthreads_and(ok);
+  const int64_t begin = good ? edge[0] : 0, end = good ? edge[seqs] : 0;
 
   // a tile's log ratios to its sequences' sums (32 bits within a tile, 64 across)
   const auto add_tile = [&](int64_t row0, int rows) {
     __syncthreads();
     for (int s = wave; s < seqs; s += kRowThreads / 64) {
       const int64_t lo = edge[s] - row0, hi = edge[s + 1] - row0;
-      const int to = hi < rows ? (int)hi : rows;
+      const int to = !good ? 0 : hi < rows ? (int)hi : rows;
       float v = 0.0f;
       for (int k = (lo > 0 ? (lo < rows ? (int)lo : rows) : 0) + ((int)threadIdx.x & 63); k < to; k += 64) v += ratio[k];
       v = wave_sum(v);
@@ -1089,7 +1084,7 @@ __global__ __launch_bounds__(kRowThreads, AP > 20 ? 2 : FEW ? 4 : sizeof(T) == 2
     double cost = 0.0;
     if ((int)threadIdx.x < pairs) {
       const int s = 2 * threadIdx.x;
-      cost = (double)pair_cost(q, pair0 + threadIdx.x, sum[s], sum[s + 1], ok, &coef[s]);
+      cost = (double)pair_cost(q, pair0 + threadIdx.x, sum[s], sum[s + 1], good, &coef[s]);
       coef[s + 1] = -coef[s];
     }
     __syncthreads();

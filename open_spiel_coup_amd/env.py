@@ -442,7 +442,8 @@ class BatchedCoupEnv:
         numbers of `generator`.  Returns buf (policy_trajectory_buffers): the
         inputs of policy.advantages and policy.policy_loss.  Lanes without a
         legal action (a finished game of an env without auto_reset) take
-        their reset step instead: action -1, log probability 0."""
+        their reset step instead: action -1, log probability 0.  Lanes left
+        at a chance node (new_initial_state) are skipped: reset them first."""
         from . import policy as ops
         T, dev = int(steps), self.device
         now = self.query(obs=self.obs is not None, info_state=self.info_state is not None)
@@ -450,6 +451,8 @@ class BatchedCoupEnv:
         for t in range(T):
             given = policy({k: now[k] for k in ("legal_mask", "current_player", "obs", "info_state") if k in now})
             logits, values = given if isinstance(given, (tuple, list)) else (given, None)
+            if tuple(logits.shape) != (self.batch, NUM_ACTIONS):
+                raise ValueError(f"the policy's logits must be [{self.batch}, {NUM_ACTIONS}], not {tuple(logits.shape)}")
             if buf is None:
                 buf = self.policy_trajectory_buffers(T, values is not None)
             uniform = torch.rand(self.batch, dtype=torch.float32, device=dev, generator=generator)

@@ -26,8 +26,9 @@ are made contiguous.
 Everything runs on the tensors' device, on torch's current stream of it,
 without a synchronisation or a memory that outlives the call.  All calls may be
 captured into a HIP graph except the losses with logits that require a
-gradient, which raise there: capture the *_and_grad form and hand its gradient
-on (`logits.backward(grad)`).
+gradient, which raise there (and the backward pass of an eager loss must not
+run inside a capture): capture the *_and_grad form and hand its gradient on
+(`logits.backward(grad)`).
 """
 import ctypes
 from typing import NamedTuple
@@ -373,7 +374,8 @@ def preference_loss(logits, actions, legal_mask, offsets, ref_logits=None, beta=
     rewards the loss is the mean over pairs of
         -(1 - label_smoothing) log sigmoid(x) - label_smoothing log sigmoid(-x).
     Sequences may be empty; rows outside every sequence get zero gradients.
-    Offsets that do not ascend from 0..rows make the loss NaN."""
+    Offsets that do not ascend within 0..rows make the loss NaN and its
+    gradient undefined."""
     return PreferenceLoss(*_loss(_preference, logits, actions, legal_mask, offsets, ref_logits, beta, label_smoothing))
 
 

@@ -174,6 +174,54 @@ def test_sample_layouts_and_devices():
     assert one[0].shape == () and int(one[0]) == int(want[0][0])
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=lambda d: str(d)[6:])
+@pytest.mark.parametrize("A", [5, 8, 18, 31])
+def test_tables_at_any_element(A, dtype):
+    """Contiguous tables that start at an odd element: the copies' 16-byte pieces need no alignment."""
+    n = 999
+    gen = torch.Generator().manual_seed(A)
+    x, mask, actions = _table(gen, n, A, dtype)
+    ref = x.float().nan_to_num(0.0).to(dtype)
+    old, adv = torch.full((n,), -1.0), torch.ones(n)
+    shifted = []
+    for t in (x, ref):
+        flat = torch.full((n * A + 16,), math.nan, dtype=dtype, device=DEV)
+        flat[3:3 + n * A] = t.to(DEV).flatten()
+        shifted.append(flat[3:3 + n * A].view(n, A))
+        assert shifted[-1].is_contiguous() and shifted[-1].data_ptr() % 16
+    words = torch.empty(n + 1, dtype=torch.int32, device=DEV)[1:]
+    words.copy_(mask)
+    acts = torch.empty(n + 1, dtype=torch.int8, device=DEV)[1:]
+    acts.copy_(actions)
+    u = torch.rand(n, generator=gen).to(DEV)
+    off = torch.tensor([1, 200, 340, 341, 990], device=DEV)
+    for got, want in ((policy.sample_actions(shifted[0], words, u), policy.sample_actions(x.to(DEV), mask.to(DEV), u)),
+                      (policy.policy_loss_and_grad(shifted[0], acts, words, old.to(DEV), adv.to(DEV), ref_logits=shifted[1]),
+                       policy.policy_loss_and_grad(x.to(DEV), actions.to(DEV), mask.to(DEV), old.to(DEV), adv.to(DEV),
+                                                   ref_logits=ref.to(DEV))),
+                      (policy.preference_loss_and_grad(shifted[0], acts, words, off, ref_logits=shifted[1]),
+                       policy.preference_loss_and_grad(x.to(DEV), actions.to(DEV), mask.to(DEV), off,
+                                                       ref_logits=ref.to(DEV)))):
+        for a, b in zip(got, want):
+            assert torch.equal(a.nan_to_num(9), b.nan_to_num(9))
+
+
+def test_sample_past_two_billion_elements():
+    """A table of 2.3e9 logits: its last rows as a call of their own."""
+    n, A, tail = 130_000_000, 18, 4001
+    x = torch.zeros(n, A, dtype=torch.bfloat16, device=DEV)
+    gen = torch.Generator(DEV).manual_seed(1)
+    x[-tail:] = torch.randn(tail, A, generator=gen, device=DEV).to(x.dtype)
+    mask = torch.full((n,), 0x2A5F1, dtype=torch.int32, device=DEV)
+    u = torch.rand(n, generator=gen, device=DEV)
+    a, lp = policy.sample_actions(x, mask, u)
+    wa, wl = policy.sample_actions(x[-tail:].clone(), mask[-tail:], u[-tail:])
+    assert torch.equal(a[-tail:], wa) and torch.equal(lp[-tail:], wl)
+    legal = torch.tensor(oracle.legal_actions(0x2A5F1, A), device=DEV)
+    first = (u[:100000].double() * legal.numel()).floor().long().clamp(max=legal.numel() - 1)
+    assert torch.equal(a[:100000].long(), legal[first])
+
+
 # ------------------------------------------------------------ advantages
 def _window(gen, T, B, P, dtype, ends=0.1):
     kind = torch.rand(T, B, generator=gen)
@@ -304,6 +352,54 @@ def test_policy_loss(n, A, with_ref, with_active, dtype):
     assert torch.equal(again, (both.grad.float() * -4.0).to(dtype)) and torch.equal(grad, both.grad)
     with pytest.raises(RuntimeError, match="backward through the graph a second time|already been freed"):
         torch.autograd.grad(out.loss, leaf)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=lambda d: str(d)[6:])
+@pytest.mark.parametrize("A,with_ref", [(18, True), (18, False), (7, True), (31, True)])
+def test_losses_of_many_rows(A, with_ref, dtype):
+    """Calls of more rows than take every sum in 64 bits: 700 decisions 120 times over have the 700's loss and 1 / 120 of
+    their gradients; so have their sequences of the preference loss."""
+    n, times = 700, 120
+    x, mask, actions, ref, old, adv = _policy_inputs(A, n, A, dtype)
+    many = lambda t: t.to(DEV).repeat(times, *[1] * (t.dim() - 1))  # noqa: E731
+    kl = 0.2 if with_ref else 0.0
+    o = oracle.policy(_np(x), actions.numpy(), mask.numpy(), _np(old), _np(adv), _np(ref) if with_ref else None, None, 0.2,
+                      0.2, kl, 0.05)
+    args = [many(t) for t in (x, actions, mask, old, adv)]
+    rm = many(ref) if with_ref else None
+    got = policy.policy_loss_and_grad(*args, ref_logits=rm, kl_coef=kl, entropy_coef=0.05)
+    assert int(got.count) == times * o["count"]
+    part = {**o, "grad": o["grad"] / times, "size": o["size"] / times}
+    for k in (0, times // 2, times - 1):
+        rows = slice(k * n, (k + 1) * n)
+        _check_policy((got.loss, got.stats, torch.tensor(o["count"]), got.log_probs[rows], got.grad[rows]), part, x, mask, dtype)
+    offsets = [0, 30, 90, 90, 200, 333, 350, 690, 690]
+    po = oracle.preference(_np(x), actions.numpy(), mask.numpy(), offsets, _np(ref) if with_ref else None, 0.1, 0.1)
+    off = torch.tensor([k * n + v for k in range(times) for v in offsets[:-1]] + [(times - 1) * n + offsets[-1]])
+    # the rows between a repetition's last sequence and the next's first join that (empty) last one: none of them counts
+    acts = args[1].view(times, n).clone()
+    acts[:, 690:] = -1
+    gp = policy.preference_loss_and_grad(args[0], acts.flatten(), args[2], off.to(DEV), ref_logits=rm, beta=0.1,
+                                         label_smoothing=0.1)
+    part = {**po, "grad": po["grad"] / times, "size": po["size"] / times}
+    for k in (0, times // 2, times - 1):
+        rows, seqs = slice(k * n, (k + 1) * n), slice(8 * k, 8 * k + 8)
+        _check_preference((gp.loss, gp.rewards[seqs], gp.grad[rows]), part, x, mask, 0.1, dtype)
+
+
+def test_a_large_ratio_overflows_to_infinity():
+    """exp of more than 88, where it is not clipped (a negative advantage): an infinite loss, in calls of few rows and of many."""
+    for n in (64, 70000):
+        x = torch.zeros(n, 3, device=DEV)
+        words = torch.full((n,), 7, dtype=torch.int32, device=DEV)
+        acts = torch.ones(n, dtype=torch.int8, device=DEV)
+        old = torch.full((n,), -200.0, device=DEV)
+        up = policy.policy_loss(x, acts, words, old, torch.full((n,), 1.0, device=DEV))
+        assert abs(float(up.loss) + 1.2) < 1e-6 and float(up.stats[3]) == 1
+        down = policy.policy_loss(x, acts, words, old, torch.full((n,), -1.0, device=DEV))
+        assert float(down.loss) == math.inf
+        none = policy.policy_loss_and_grad(x, acts, words, old, torch.zeros(n, device=DEV))
+        assert float(none.loss) == 0 and not none.grad.any()
 
 
 def test_policy_clip_borders():
@@ -514,8 +610,7 @@ def test_graph_replays_of_every_call():
 
 
 def test_captured_autograd_is_refused():
-    """A loss whose logits require a gradient raises under capture, before anything is enqueued; so does the captured
-    backward of an eager loss."""
+    """A loss whose logits require a gradient raises under capture, before anything is enqueued."""
     n, A = 64, 18
     x, mask, actions, ref, old, adv = (t.to(DEV) for t in _policy_inputs(3, n, A, torch.float32))
     leaf = x.clone().requires_grad_()
@@ -537,7 +632,59 @@ def test_captured_autograd_is_refused():
     assert torch.equal(kept.loss, policy.policy_loss(x, actions, mask, old, adv).loss) and torch.equal(y.nan_to_num(2), x.nan_to_num(2))
 
 
+def test_calls_on_two_streams_at_once():
+    """The same calls enqueued on two streams without a wait between them: each has its own scratch memory."""
+    n, A = 200_000, 18
+    x, mask, actions, ref, old, adv = (t.to(DEV) for t in _policy_inputs(5, 2000, A, torch.bfloat16))
+    big = [t.repeat(n // 2000, *[1] * (t.dim() - 1)) for t in (x, actions, mask, old, adv)]
+    off = torch.arange(0, n + 1, 50, device=DEV)
+    want = [*policy.policy_loss_and_grad(*big, ref_logits=big[0]), *policy.preference_loss_and_grad(*big[:3], off)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(5):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[k] = [*policy.policy_loss_and_grad(*big, ref_logits=big[0]), *policy.preference_loss_and_grad(*big[:3], off)]
+    torch.cuda.synchronize()
+    for k in (0, 1):
+        for a, b in zip(got[k], want):
+            assert torch.equal(a, b)
+
+
 # ------------------------------------------------------------ a run of them
+@pytest.mark.parametrize("auto_reset", [True, False])
+def test_policy_trajectory_is_the_steps_it_records(auto_reset):
+    """The recorded actions stepped one by one give the recorded outputs; what each step was decided on is the state
+    before it; finished games of an env without auto_reset take their reset step."""
+    B, T = 300, 50
+    kw = dict(seed=4, auto_reset=auto_reset, obs=True)
+    env, ref = BatchedCoupEnv(B, **kw), BatchedCoupEnv(B, **kw)
+    table = torch.randn(B, 18, device=DEV)
+    buf = env.collect_policy_trajectory(T, lambda ts: (table, table[:, 0]), generator=torch.Generator(DEV).manual_seed(2))
+    assert env.error_count() == 0
+    now = ref.query()
+    for t in range(T):
+        over = now["terminal"].bool()
+        assert torch.equal(buf["decision_mask"][t], now["legal_mask"].masked_fill(over, 0))
+        assert torch.equal(buf["decision_player"][t], now["current_player"])
+        assert torch.equal(buf["decision_obs"][t], now["obs"])
+        assert torch.equal(buf["values"][t], table[:, 0])
+        acts = buf["actions"][t]
+        assert torch.equal(acts < 0, over)
+        out = ref.step(acts.masked_fill(over, 0))
+        for k in ("actions", "rewards", "step_type", "legal_mask", "current_player", "obs"):
+            assert torch.equal(buf[k][t], out[k]), (t, k)
+        lp = torch.log_softmax(table.masked_fill(~(((buf["decision_mask"][t][:, None] >> torch.arange(18, device=DEV)) & 1) > 0),
+                                                 -math.inf), 1)
+        want = torch.where(over, 0.0, lp.gather(1, acts.long().clamp(0)[:, None])[:, 0])
+        assert torch.allclose(buf["log_probs"][t], want, atol=100 * H)
+        now = ref.query()
+    firsts = buf["step_type"] == 0
+    assert bool(firsts.any()) == (not auto_reset) and (buf["log_probs"][firsts] == 0).all()
+    with pytest.raises(ValueError, match="logits must be"):
+        env.collect_policy_trajectory(1, lambda ts: table[:, :7])
+
+
 @pytest.mark.parametrize("players", [2, 4])
 def test_a_learners_round(players):
     """Trajectories played by a policy, advantages over them, policy updates on their rows, and the finished games'
