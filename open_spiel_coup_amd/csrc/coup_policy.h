@@ -501,7 +501,8 @@ struct Rewards {
 // A thread's steps in memory: step k of lane l is at uniform element `base[k]`
 // plus `off[k]`.  With one stretch a lane the step is the block's, so the
 // offset is the lane; with more, it is the lane and the stretch's steps from
-// the window's first, below 2^27 bytes of any array (launch_advantages).
+// the window's first: below 2^17 lanes x 32 steps, or 2^14 x 128, 2^11 x 512,
+// 2^7 x 4096, x 24 bytes of any array (launch_advantages_of).
 template <int C>
 struct Steps {
   int64_t base[C == 1 ? kStretch : 1];
@@ -1302,16 +1303,20 @@ inline void launch_sample(const Rows& r, int dtype, const float* uniform, int8_t
   });
 }
 
-// How a window is split: enough threads to fill the chip (2^17), but no more
-// stretches than the window has.  C = 1, 4, 16, 128 or 512 of a lane's at a time.
+// How a window is split: C = 1, 4, 16, 64 or 512 of a lane's stretches at a
+// time, by the lanes there are to fill the chip with (few lanes a block read
+// short runs of memory), and no more of them than the window has.  Either side
+// of the borders, 2 players, us: 256 steps x 65,536 lanes C = 4 52, 1 77;
+// 256 x 131,072 C = 1 117, 4 122; 1024 x 16,384 C = 4 85, 16 109; 1024 x 4096
+// C = 16 33, 128 70; 256 x 1024 C = 64 5.9, 16 7.1; 4096 x 33 C = 512 17, 128 23.
 template <int P>
 void launch_advantages_of(const AdvantageArgs& q, hipStream_t s) {
-  const auto enough = [&](int c) { return q.B * c >= (1 << 17) || (int64_t)c * kStretch >= q.T; };
+  const auto enough = [&](int c, int64_t lanes) { return q.B >= lanes || (int64_t)c * kStretch >= q.T; };
   const auto grid = [&](int lanes) { return (unsigned)((q.B + lanes - 1) / lanes); };
-  if (enough(1)) k_advantages<P, 256, 256><<<grid(256), 256, 0, s>>>(q);
-  else if (enough(4)) k_advantages<P, 64, 256><<<grid(64), 256, 0, s>>>(q);
-  else if (enough(16)) k_advantages<P, 16, 256><<<grid(16), 256, 0, s>>>(q);
-  else if (enough(128)) k_advantages<P, 4, 512><<<grid(4), 512, 0, s>>>(q);
+  if (enough(1, 1 << 17)) k_advantages<P, 256, 256><<<grid(256), 256, 0, s>>>(q);
+  else if (enough(4, 1 << 14)) k_advantages<P, 64, 256><<<grid(64), 256, 0, s>>>(q);
+  else if (enough(16, 1 << 11)) k_advantages<P, 32, 512><<<grid(32), 512, 0, s>>>(q);
+  else if (enough(64, 1 << 7)) k_advantages<P, 8, 512><<<grid(8), 512, 0, s>>>(q);
   else k_advantages<P, 1, 512><<<grid(1), 512, 0, s>>>(q);
 }
 
