@@ -358,27 +358,29 @@ __device__ __forceinline__ Softmax softmax(float (&x)[AP], float (&e)[AP]) {
   return s;
 }
 
-// A row's sum of e in 64 bits, for the rows next to a border.
-template <class T>
-__device__ __forceinline__ double sum64(const T* row, uint32_t legal, float m) {
+// This thread's row's sum of e in 64 bits, from its logits in the tile, for
+// rows next to a border and for calls of few rows.
+template <class T, int AP>
+__device__ __forceinline__ double sum64(const char* tile, int A, uint32_t legal, float m) {
   double sum = 0.0;
 #pragma unroll 1
-  for (uint32_t b = legal; b; b &= b - 1) sum += exp((double)widen(row[__builtin_ctz(b)]) - (double)m);
+  for (uint32_t b = legal; b; b &= b - 1)
+    sum += exp((double)Tile<T, AP>::read_one(tile, A, __builtin_ctz(b)) - (double)m);
   return sum;
 }
 
 // The action a uniform number u falls on: the first legal a whose running
 // sum passes u * total, in 64 bits; the last with a share where rounding
 // leaves the total at or below it.
-template <class T>
-__device__ __forceinline__ int pick64(const T* row, uint32_t legal, float m, float u) {
-  const double t = (double)u * sum64(row, legal, m);
+template <class T, int AP>
+__device__ __forceinline__ int pick64(const char* tile, int A, uint32_t legal, float m, float u) {
+  const double t = (double)u * sum64<T, AP>(tile, A, legal, m);
   double c = 0.0;
   int last = -1;
 #pragma unroll 1
   for (uint32_t b = legal; b; b &= b - 1) {
     const int a = __builtin_ctz(b);
-    const double e = exp((double)widen(row[a]) - (double)m);
+    const double e = exp((double)Tile<T, AP>::read_one(tile, A, a) - (double)m);
     c += e;
     if (e > 0.0) last = a;
     if (c > t) return a;
@@ -426,7 +428,7 @@ __global__ __launch_bounds__(kRowThreads) void k_sample(Rows r, const float* __r
         action += c <= t;
       }
       near |= gap <= kPickMargin * s.sum;
-      if (near) action = pick64((const T*)r.logits + i * r.stride, legal, s.m, u);
+      if (near) action = pick64<T, AP>(lds, r.A, legal, s.m, u);
       logp = (Tile<T, AP>::read_one(lds, r.A, action) - s.m) - s.lse;
     } else {
       logp = s.sum;  // NaN or +inf at a legal action: no distribution, no action
@@ -734,8 +736,8 @@ struct PolicyArgs {
 
 // Up to this many rows every row's ratio is taken in 64 bits, not only those
 // by a border: a loss of few terms that nearly cancel keeps its digits (over
-// many rows the 32-bit roundings average out), and a block a CU or less hides
-// the 18 exponentials a row.
+// many rows the 32-bit roundings average out).  A call of 65,536 float rows
+// takes 14.0 us, one of 65,537 13.0.
 constexpr int64_t kFewRows = 65536;
 constexpr int kCountBlocks = 256, kCountThreads = 1024, kFinishThreads = 1024;
 
@@ -830,7 +832,7 @@ __global__ __launch_bounds__(kRowThreads, AP <= 20 ? 4 : 2) void k_policy_loss(P
     float rho = exp_of(dl);
     // 32 bits hold dl to a few 2^-23 of its terms
     if (q.few || fabsf(dl - border) <= 4.76837158e-7f * (4.0f + fabsf(xa - s.m) + fabsf(old))) {
-      const double whole = sum64((const T*)q.r.logits + i * q.r.stride, legal, s.m);
+      const double whole = sum64<T, AP>(tile, q.r.A, legal, s.m);
       const double top = exp((double)xa - (double)s.m - (double)old);
       over = adv > 0.0f ? top > q.high * whole : top < q.low * whole;
       rho = (float)(top / whole);
@@ -985,6 +987,7 @@ template <class T, int AP, bool REF, bool FEW>
 __device__ __forceinline__ float row_ratio(char* tile, const PreferenceArgs& q, int64_t row0, int rows, uint32_t legal,
                                            int action, float (&e)[AP], float& ea, float& sum) {
   float x[AP], d[AP], xa, out = 0.0f, one = 0.0f;
+  double whole = 1.0;
   Softmax rs{0.0f, 1.0f, 0.0f};
   stage_rows<T, AP, REF>(
       tile, q.r, row0, rows, legal, action, d,
@@ -992,6 +995,7 @@ __device__ __forceinline__ float row_ratio(char* tile, const PreferenceArgs& q, 
         float unused[AP];
         rs = softmax<false, AP>(row, unused);
         one = taken;
+        if (FEW) whole = sum64<T, AP>(tile, q.r.A, legal, rs.m);  // the tile holds the reference's rows here
       },
       x, xa);
   sum = 1.0f;
@@ -1001,10 +1005,7 @@ __device__ __forceinline__ float row_ratio(char* tile, const PreferenceArgs& q, 
     // the two sums' logs as one, of a ratio near 1
     out = REF ? (xa - s.m) - (one - rs.m) : xa - s.m;
     if (FEW) {
-      const int64_t i = row0 + threadIdx.x;
-      double ratio = sum64((const T*)q.r.logits + i * q.r.stride, legal, s.m);
-      if (REF) ratio /= sum64((const T*)q.r.ref + i * q.r.ref_stride, legal, rs.m);
-      out -= log1p_any((float)(ratio - 1.0));
+      out -= log1p_any((float)(sum64<T, AP>(tile, q.r.A, legal, s.m) / whole - 1.0));
     } else {
       out -= REF ? log_ratio(s.sum, rs.sum) : log_of(s.sum);
     }
@@ -1363,10 +1364,15 @@ inline void launch_policy(PolicyArgs q, int dtype, double kl, double ent, float*
 // rows on average: `group` pairs a block, some 5 / 8 of a tile so that few
 // groups spill into a second; else a sequence's sum takes a block per 4096
 // rows of the average one.
+// Few rows' sums are taken in 64 bits, as the policy loss's (kFewRows): the
+// short form's up to a quarter of them (16,384 rows 18.3 us, 16,385 13.8; at
+// 65,536 it would be 22 for 15), the long form's up to all (19.6, 17.2).
+// On either side of kShortRows, 2^19 bf16 rows, us: 40 rows a pair short 34,
+// long 66; 150 41, 44; 300 39, 40; 1000 98, 37.
 constexpr int kShortRows = 160;
 
 struct PreferencePlan {
-  bool is_short;
+  bool is_short, few;
   int group, slices;
   int64_t blocks;  // that leave a partial sum
 };
@@ -1375,6 +1381,7 @@ inline PreferencePlan preference_plan(int64_t n, int64_t pairs) {
   PreferencePlan p{};
   const int64_t each = pairs ? n / pairs : 0;
   p.is_short = each <= kShortRows;
+  p.few = n <= (p.is_short ? kFewRows / 4 : kFewRows);
   if (p.is_short) {
     const int64_t g = kShortRows / (each > 0 ? each : 1);
     p.group = (int)(g < kMaxGroup ? g : kMaxGroup);
@@ -1406,7 +1413,7 @@ inline void launch_preference(PreferenceArgs q, int dtype, void* workspace, hipS
     if (p.is_short) {
       const int64_t grid = p.blocks + (q.grad && q.r.n ? kZeroBlocks : 0);
       if (grid) {
-        with_flags(q.r.ref != nullptr, q.r.n <= kFewRows, [&](auto ref, auto few) {
+        with_flags(q.r.ref != nullptr, p.few, [&](auto ref, auto few) {
           k_preference_short<T, AP, decltype(ref)::value, decltype(few)::value>
               <<<(unsigned)grid, kRowThreads, 0, s>>>(q);
         });
@@ -1415,7 +1422,7 @@ inline void launch_preference(PreferenceArgs q, int dtype, void* workspace, hipS
       q.sums = q.partial + p.blocks + 1;
       q.coef = (float*)(q.sums + 2 * q.pairs * p.slices);
       q.ratio = q.coef + 2 * q.pairs;
-      with_flags(q.r.ref != nullptr, q.r.n <= kFewRows, [&](auto ref, auto few) {
+      with_flags(q.r.ref != nullptr, p.few, [&](auto ref, auto few) {
         k_preference_rows<T, AP, decltype(ref)::value, decltype(few)::value><<<tiles, kRowThreads, 0, s>>>(q);
       });
       k_preference_sums<<<(unsigned)(2 * q.pairs * p.slices), kRowThreads, 0, s>>>(q);
