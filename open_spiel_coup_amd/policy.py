@@ -268,6 +268,8 @@ class _LossOf(torch.autograd.Function):
 def _loss(call, logits, *args):
     if not (isinstance(logits, torch.Tensor) and logits.requires_grad and torch.is_grad_enabled()):
         return call(False, logits, *args)[0]
+    if any(isinstance(t, torch.Tensor) and t.requires_grad for t in args):  # unseen inside the function below
+        raise ValueError("every argument but logits is held constant: detach() those that require a gradient")
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError("a loss whose logits require a gradient cannot be captured into a graph: capture its "
                            "_and_grad form and hand the gradient on")

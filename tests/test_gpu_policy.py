@@ -498,6 +498,25 @@ def test_policy_refusals():
                           torch.zeros(1, 2, device=DEV, requires_grad=True))
 
 
+def test_arguments_held_constant_are_refused_beside_logits_with_a_gradient():
+    """An argument that requires a gradient raises also where the logits do: its gradient would be lost without a word."""
+    n, A = 8, 18
+    x, mask, actions, ref, old, adv = (t.to(DEV) for t in _policy_inputs(1, n, A, torch.float32))
+    leaf = x.clone().requires_grad_()
+    for name in ("old_log_probs", "advantages", "ref_logits"):
+        kw = dict(old_log_probs=old, advantages=adv, ref_logits=ref)
+        kw[name] = kw[name].clone().requires_grad_()
+        with pytest.raises(ValueError, match="held constant"):
+            policy.policy_loss(leaf, actions, mask, **kw)
+    with pytest.raises(ValueError, match="held constant"):
+        policy.policy_loss(leaf, actions, mask, old, adv, ref_logits=leaf)
+    off = torch.tensor([0, 4, 8], device=DEV)
+    with pytest.raises(ValueError, match="held constant"):
+        policy.preference_loss(leaf, actions, mask, off, ref_logits=ref.clone().requires_grad_())
+    policy.policy_loss(leaf, actions, mask, old, adv, ref_logits=leaf.detach()).loss.backward()
+    assert leaf.grad is not None
+
+
 # ------------------------------------------------------------ preference loss
 def _check_preference(got, o, x, mask, beta, dtype):
     z = _reach(x, mask)
