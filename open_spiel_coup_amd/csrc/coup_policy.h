@@ -459,6 +459,7 @@ __global__ __launch_bounds__(kRowThreads) void k_sample(Rows r, const float* __r
 //
 // A step's map of z_p is affine with factors of at most 1, so a stretch of
 // steps is one pair (f, g), z -> f z + g, per player, and stretches compose.
+// A factor of 0 (a cut) takes nothing of z, be it infinite or NaN.
 // A block holds L lanes; its NT / L threads of a lane take kStretch steps
 // each, latest first, all loaded before the first is used (the window is read
 // once); a scan over the stretches' pairs gives each its z, and the block
@@ -523,6 +524,9 @@ struct Steps {
     return (V*)((char*)(p + u) + v);
   }
 };
+
+// f z + g, and g where f is 0, whatever z.
+__device__ __forceinline__ float join(float f, float z, float g) { return __builtin_fmaf(f, f != 0.0f ? z : 0.0f, g); }
 
 // One stretch from its z: the outputs, and z after it.
 template <int P, int C>
@@ -633,7 +637,7 @@ __global__ __launch_bounds__(NT) void k_advantages(AdvantageArgs q) {
         for (int p = 0; p < P; ++p) {
           const float f0 = __shfl_up(f[p], d * L, 64), g0 = __shfl_up(g[p], d * L, 64);
           if (cw >= d) {
-            g[p] = f[p] * g0 + g[p];
+            g[p] = join(f[p], g0, g[p]);
             f[p] *= f0;
           }
         }
@@ -656,8 +660,8 @@ __global__ __launch_bounds__(NT) void k_advantages(AdvantageArgs q) {
         const float* o = totals + (w * LW + (l & (LW - 1))) * P * 2;
 #pragma unroll
         for (int p = 0; p < P; ++p) {
-          if (w == wave) here[p] = f[p] * z[p] + g[p];  // z runs through the waves: here it stands before this one
-          z[p] = o[2 * p] * z[p] + o[2 * p + 1];
+          if (w == wave) here[p] = join(f[p], z[p], g[p]);  // z runs through the waves: here it stands before this one
+          z[p] = join(o[2 * p], z[p], o[2 * p + 1]);
         }
       }
       __syncthreads();  // the next window writes the totals again

@@ -295,6 +295,27 @@ def test_advantages_no_ends_and_empty():
         assert a.shape == t.shape == (T, B)
 
 
+@pytest.mark.parametrize("T,B,P", [(6, 40, 2), (40, 20000, 2), (200, 3000, 3), (300, 300, 2), (700, 5, 6), (5000, 2, 2)])
+@pytest.mark.parametrize("junk", [math.nan, math.inf, -math.inf])
+def test_nothing_crosses_a_cut(T, B, P, junk):
+    """A value or bootstrap that is no number, behind a game's end, leaves the games before it as they were, in every
+    way of splitting a window."""
+    gen = torch.Generator().manual_seed(T + B)
+    r, st, pl, v, b = _window(gen, T, B, P, torch.float32, ends=0.02)
+    lane = torch.arange(B)
+    end = torch.randint(0, T, (B,), generator=gen)
+    end[:2] = torch.tensor([T - 1, T // 2])
+    st[end, lane], v[end, lane] = 2, 0.5  # a decision whatever the step was before
+    behind = torch.arange(T)[:, None] > end
+    wild, boot = v.clone(), torch.full_like(b, junk)
+    wild[behind] = junk
+    got = policy.advantages(*(t.to(DEV) for t in (r, st, pl, wild, boot)), gamma=0.99, lam=0.95)
+    want = policy.advantages(*(t.to(DEV) for t in (r, st, pl, v, b)), gamma=0.99, lam=0.95)
+    for g, w in zip(got, want):
+        g, w = g.cpu()[~behind], w.cpu()[~behind]
+        assert torch.isfinite(w).all() and torch.equal(g, w)
+
+
 # ------------------------------------------------------------ policy loss
 def _policy_inputs(seed, n, A, dtype, move=0.3):
     gen = torch.Generator().manual_seed(seed)
