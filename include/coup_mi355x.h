@@ -442,6 +442,8 @@ int coup_error_count(coup_env* env, int64_t* out);
  * Logits may be float, half or bfloat16; all arithmetic is in 32 bits or
  * more, a gradient is rounded once, to the logits' type. */
 #define COUP_MAX_POLICY_ACTIONS 31
+#define COUP_MAX_DECISIONS (INT64_C(1) << 30) /* rows (coup_advantages: lanes) of a call: its launches stay below 2^32 threads */
+#define COUP_MAX_PAIRS (INT64_C(1) << 28)
 #define COUP_DTYPE_F32 0
 #define COUP_DTYPE_F16 1
 #define COUP_DTYPE_BF16 2

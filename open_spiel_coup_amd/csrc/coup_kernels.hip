@@ -4845,7 +4845,7 @@ bool dtype_ok(int dtype) { return dtype == COUP_DTYPE_F32 || dtype == COUP_DTYPE
 // Why `d` cannot be taken by `what`, or null.
 const char* decisions_error(const coup_decisions* d, bool acted) {
   if (!d) return "decisions is null";
-  if (d->rows < 0 || d->rows > (int64_t(1) << 38)) return "rows out of range";
+  if (d->rows < 0 || d->rows > COUP_MAX_DECISIONS) return "rows out of range";
   if (d->num_actions < 1 || d->num_actions > COUP_MAX_POLICY_ACTIONS) return "num_actions must be 1..31";
   if (!dtype_ok(d->dtype)) return "unknown dtype";
   if (d->rows == 0) return nullptr;
@@ -4876,7 +4876,7 @@ int coup_sample_actions(const coup_decisions* d, const float* uniform, int8_t* a
 
 int coup_advantages(const coup_window* w, double gamma, double lam, float* adv, float* target, void* hip_stream) {
   if (!w) return fail(COUP_E_INVALID, "coup_advantages: window is null");
-  if (w->steps < 0 || w->lanes < 0 || w->lanes > (int64_t(1) << 38) || (w->lanes && w->steps > (int64_t(1) << 40) / w->lanes))
+  if (w->steps < 0 || w->lanes < 0 || w->lanes > COUP_MAX_DECISIONS || (w->lanes && w->steps > (int64_t(1) << 40) / w->lanes))
     return fail(COUP_E_INVALID, "coup_advantages: steps or lanes out of range");
   if (w->num_players < 2 || w->num_players > COUP_MAX_PLAYERS)
     return fail(COUP_E_INVALID, "coup_advantages: num_players must be 2..6");
@@ -4948,7 +4948,7 @@ int coup_preference_loss(const coup_decisions* d, const coup_preference_terms* t
   if (const char* why = decisions_error(d, true))
     return fail(COUP_E_INVALID, std::string("coup_preference_loss: ") + why);
   if (!terms || !out || !out->loss) return fail(COUP_E_INVALID, "coup_preference_loss: terms, out or its loss is null");
-  if (terms->pairs < 0 || terms->pairs > (int64_t(1) << 30))
+  if (terms->pairs < 0 || terms->pairs > COUP_MAX_PAIRS)
     return fail(COUP_E_INVALID, "coup_preference_loss: pairs out of range");
   if (terms->offset_bytes != 4 && terms->offset_bytes != 8)
     return fail(COUP_E_INVALID, "coup_preference_loss: offset_bytes must be 4 or 8");

@@ -1390,6 +1390,10 @@ inline void launch_policy(PolicyArgs q, int dtype, double kl, double ent, float*
 // Few rows' sums are taken in 64 bits, as the policy loss's (kFewRows): the
 // short form's up to a quarter of them (16,384 rows 18.3 us, 16,385 13.8; at
 // 65,536 it would be 22 for 15), the long form's up to all (19.6, 17.2).
+// A short block has 32 pairs or 81 rows and more on average, a long sequence
+// more than 80, so the calls the entries take (COUP_MAX_DECISIONS,
+// COUP_MAX_PAIRS) launch fewer than 2^32 threads.  One sequence far longer than
+// its call's average keeps one block busy, 256 of its rows at a time.
 // On either side of kShortRows, 2^19 bf16 rows, us: 40 rows a pair short 34,
 // long 66; 150 41, 44; 300 39, 40; 1000 98, 37.
 constexpr int kShortRows = 160;

@@ -109,6 +109,21 @@ def test_decisions_are_checked_by_every_entry(bad, why):
     _refused(L.coup_preference_loss(ctypes.byref(d), ctypes.byref(pt), ctypes.byref(po), F, 1 << 20, None), why)
 
 
+def test_calls_whose_launches_would_pass_32_bits_are_refused():
+    """A grid of 2^32 threads is no launch: rows, lanes and pairs beyond what keeps every kernel's below are refused."""
+    L = _native.load()
+    d = _decisions(rows=(1 << 30) + 1)
+    out = _native.PolicyOutputs(F, None, None, None, None)
+    po = _native.PreferenceOutputs(F, None, None)
+    _refused(L.coup_sample_actions(ctypes.byref(d), F, F, F, None), b"rows")
+    _refused(L.coup_policy_loss(ctypes.byref(d), ctypes.byref(_terms()), ctypes.byref(out), F, 1 << 40, None), b"rows")
+    one, many = (_native.PreferenceTerms(F, 8, p, 0.1, 0.0) for p in (1, (1 << 28) + 1))
+    _refused(L.coup_preference_loss(ctypes.byref(d), ctypes.byref(one), ctypes.byref(po), F, 1 << 40, None), b"rows")
+    _refused(L.coup_preference_loss(ctypes.byref(_decisions()), ctypes.byref(many), ctypes.byref(po), F, 1 << 40, None), b"pairs")
+    w = _native.Window(F, F, F, F, None, 1, (1 << 30) + 1, 2, 0)
+    _refused(L.coup_advantages(ctypes.byref(w), 0.9, 0.9, F, F, None), b"lanes")
+
+
 def test_sample_refusals():
     L = _native.load()
     _refused(L.coup_sample_actions(None, F, F, F, None), b"null")
