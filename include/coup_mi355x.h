@@ -514,6 +514,7 @@ typedef struct {
   int64_t* count;   /* [1] decisions that count, or NULL */
   float* log_probs; /* [rows] log pi(action), 0 where the row does not count; or NULL */
   void* grad;       /* [rows][num_actions] of the logits, d loss / d logits; or NULL */
+  const float* grad_scale; /* [1] what the gradient is multiplied by before it is rounded; NULL: 1 */
 } coup_policy_outputs;
 size_t coup_policy_workspace(int64_t rows);
 int coup_policy_loss(const coup_decisions* d, const coup_policy_terms* terms, const coup_policy_outputs* out,
@@ -541,6 +542,7 @@ typedef struct {
   float* loss;    /* [1]; 0 for no pairs */
   float* rewards; /* [2 * pairs] or NULL */
   void* grad;     /* [rows][num_actions] of the logits, or NULL */
+  const float* grad_scale; /* as in coup_policy_outputs */
 } coup_preference_outputs;
 size_t coup_preference_workspace(int64_t rows, int64_t pairs);
 int coup_preference_loss(const coup_decisions* d, const coup_preference_terms* terms,

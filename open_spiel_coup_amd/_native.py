@@ -101,7 +101,7 @@ class PolicyTerms(ctypes.Structure):
 class PolicyOutputs(ctypes.Structure):
     """coup_policy_outputs."""
     _fields_ = [("loss", ctypes.c_void_p), ("stats", ctypes.c_void_p), ("count", ctypes.c_void_p),
-                ("log_probs", ctypes.c_void_p), ("grad", ctypes.c_void_p)]
+                ("log_probs", ctypes.c_void_p), ("grad", ctypes.c_void_p), ("grad_scale", ctypes.c_void_p)]
 
 
 class PreferenceTerms(ctypes.Structure):
@@ -112,7 +112,8 @@ class PreferenceTerms(ctypes.Structure):
 
 class PreferenceOutputs(ctypes.Structure):
     """coup_preference_outputs."""
-    _fields_ = [("loss", ctypes.c_void_p), ("rewards", ctypes.c_void_p), ("grad", ctypes.c_void_p)]
+    _fields_ = [("loss", ctypes.c_void_p), ("rewards", ctypes.c_void_p), ("grad", ctypes.c_void_p),
+                ("grad_scale", ctypes.c_void_p)]
 
 
 class CoupError(RuntimeError):

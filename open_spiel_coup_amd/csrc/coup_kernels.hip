@@ -4932,6 +4932,7 @@ int coup_policy_loss(const coup_decisions* d, const coup_policy_terms* terms, co
   q.ent = (float)terms->entropy_coef;
   q.log_probs = out->log_probs;
   q.grad = out->grad;
+  q.grad_scale = out->grad_scale;
   coup::policy::launch_policy(q, d->dtype, terms->kl_coef, terms->entropy_coef, out->loss, out->stats, out->count,
                               workspace, (hipStream_t)hip_stream);
   COUP_HIP_TRY(hipGetLastError());
@@ -4967,6 +4968,7 @@ int coup_preference_loss(const coup_decisions* d, const coup_preference_terms* t
   q.eps = terms->label_smoothing;
   q.rewards = out->rewards;
   q.grad = out->grad;
+  q.grad_scale = out->grad_scale;
   q.loss = out->loss;
   coup::policy::launch_preference(q, d->dtype, workspace, (hipStream_t)hip_stream);
   COUP_HIP_TRY(hipGetLastError());

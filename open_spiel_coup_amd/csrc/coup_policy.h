@@ -738,6 +738,7 @@ struct PolicyArgs {
   int few;  // ratios and log probabilities from 64-bit sums in every row (kFewRows)
   float* log_probs;  // null: not wanted
   void* grad;        // null: no gradient
+  const float* grad_scale;  // its factor; null: 1
   double* partial;   // [blocks][4] sums of the terms over a block's rows
   int32_t* decided;  // [blocks] its decisions
   float* counts;     // [count blocks] the call's decisions, for the gradient
@@ -798,8 +799,9 @@ __global__ __launch_bounds__(kRowThreads, AP <= 20 ? 4 : 2) void k_policy_loss(P
   const bool mine = (int)threadIdx.x < rows;
   // the decisions of the call: every wave adds the counting blocks' numbers
   // (as 32-bit floats: they scale the gradient)
-  float count = 0.0f;
+  float count = 0.0f, factor = 1.0f;
   if (q.grad) {
+    if (q.grad_scale) factor = *q.grad_scale;
 #pragma unroll
     for (int k = 0; k < kCountBlocks; k += 64) {
       const int at = k + ((int)threadIdx.x & 63);
@@ -824,7 +826,7 @@ __global__ __launch_bounds__(kRowThreads, AP <= 20 ? 4 : 2) void k_policy_loss(P
         rta = rs.t(one);
       },
       x, xa);
-  const float n = wave_sum(count), scale = 1.0f / (n > 0.0f ? n : 1.0f);
+  const float n = wave_sum(count), scale = factor / (n > 0.0f ? n : 1.0f);
   float surrogate = 0.0f, kl = 0.0f, entropy = 0.0f, clipped = 0.0f, logp = 0.0f, ga = 0.0f;
   if (legal) {
     // x becomes t
@@ -862,11 +864,13 @@ __global__ __launch_bounds__(kRowThreads, AP <= 20 ? 4 : 2) void k_policy_loss(P
       // p_b w_b, w_b = ent (l_b + H) + kl (d_b - K) - w, in which the lse's
       // cancel: (ent + kl) (t_b - E t) - kl (tr_b - E tr) - w
       const float w = (over || adv == 0.0f) ? 0.0f : -rho * adv;
-      const float share = inv * scale, ct = (REF ? q.ent + q.kl : q.ent) * share, cr = REF ? q.kl * share : 0.0f;
-      const float base = cr * (et - ed) - ct * et - w * share;
+      // (the factor, which has no bound, meets p_b and not the coefficients
+      // that kLowest is held for)
+      const float share = inv * scale, ct = REF ? q.ent + q.kl : q.ent, cr = REF ? q.kl : 0.0f;
+      const float base = cr * (et - ed) - ct * et - w;
 #pragma unroll
-      for (int a = 0; a < AP; ++a) x[a] = e[a] * (ct * x[a] + (REF ? base - cr * d[a] : base));
-      ga = s.e(xa) * (ct * s.t(xa) + (REF ? base - cr * rta : base)) + w * scale;
+      for (int a = 0; a < AP; ++a) x[a] = (e[a] * share) * (ct * x[a] + (REF ? base - cr * d[a] : base));
+      ga = (s.e(xa) * share) * (ct * s.t(xa) + (REF ? base - cr * rta : base)) + w * scale;
       if (!(fabsf(base) < 1e30f)) {  // else 0 times it is 0 at the actions outside the word
 #pragma unroll
         for (int a = 0; a < AP; ++a) x[a] = keep(legal, a, x[a], 0.0f);
@@ -961,6 +965,7 @@ struct PreferenceArgs {
   float* loss;
   float* rewards;   // [2 pairs] or null
   void* grad;       // or null
+  const float* grad_scale;  // its factor; null: 1
   double* partial;  // [blocks] a block's pairs' costs
   int group;        // the short form: pairs a block
   // the long form
@@ -991,7 +996,8 @@ __device__ __forceinline__ float pair_cost(const PreferenceArgs& q, int64_t pair
   const float x = (float)(chosen - rejected), size = fabsf(x), eps = (float)q.eps;
   const float y = exp_of(-size), part = __builtin_amdgcn_rcpf(1.0f + y);
   const float miss = x > 0.0f ? y * part : part;  // sigma(-x)
-  *coef = ok ? (eps - miss) * (float)(q.beta / (double)q.pairs) : NAN;
+  const float factor = q.grad_scale ? *q.grad_scale : 1.0f;
+  *coef = ok ? (eps - miss) * (float)(q.beta / (double)q.pairs) * factor : NAN;
   return ok ? log1p_of(y) + size * (x > 0.0f ? eps : 1.0f - eps) : NAN;
 }
 
@@ -1270,7 +1276,9 @@ __global__ __launch_bounds__(kFinishThreads) void k_preference_finish(const doub
 
 // A gradient for a loss's own derivative of 1, times the derivative that
 // came in: nothing is read or written where that is 1, as in loss.backward()
-// (1.9 us, a launch).
+// (1.9 us, a launch).  A second rounding, at most another half step; nothing
+// for a power of two, unless the first one was to a half's smallest steps,
+// which is what grad_scale is for.
 template <class T>
 __global__ __launch_bounds__(kRowThreads) void k_scale_grad(T* grad, int64_t n, const float* __restrict__ scale) {
   const float g = *scale;

@@ -21,7 +21,8 @@ reset or skipped (action -1), finished games and chance nodes give zeros,
 whatever the row holds besides; so do logits of actions outside the word.
 Logits are float32, float16 or bfloat16; arithmetic is in 32 bits or more,
 gradients have the logits' type.  Logits may be strided; the other arguments
-are made contiguous.
+are made contiguous.  Nothing but a loss is differentiable, and that in its
+logits.
 
 Everything runs on the tensors' device, on torch's current stream of it,
 without a synchronisation or a memory that outlives the call.  All calls may be
@@ -237,12 +238,15 @@ def advantages(rewards, step_type, players, values, bootstrap=None, gamma=1.0, l
 class _LossOf(torch.autograd.Function):
     """A loss whose call also wrote its gradient: backward hands that out,
     times the incoming derivative (one pass over it in place, or none where it
-    is 1).  A second backward over a retained graph makes the call again."""
+    is 1).  A second backward over a retained graph makes the call again, with
+    the derivative as the gradient's factor; so does the first of float16
+    logits, whose range a gradient over many rows needs the factor (a loss
+    scaler's) for before it is rounded."""
 
     @staticmethod
     def forward(ctx, logits, call, args):
-        out, grad = call(True, logits, *args)
-        # for a second backward, which reads them: torch checks their versions there
+        out, grad = call(logits.dtype != torch.float16, logits, *args)
+        # for a backward that calls again: torch checks their versions there
         ctx.save_for_backward(logits, *[t for t in args if isinstance(t, torch.Tensor)])
         ctx.call, ctx.grad = call, grad
         ctx.args = [None if isinstance(t, torch.Tensor) else (t,) for t in args]
@@ -259,7 +263,8 @@ class _LossOf(torch.autograd.Function):
         if grad is None:
             logits, *tensors = ctx.saved_tensors
             tensors = iter(tensors)
-            grad = ctx.call(True, logits, *[next(tensors) if a is None else a[0] for a in ctx.args])[1]
+            args = [next(tensors) if a is None else a[0] for a in ctx.args]
+            return ctx.call(True, logits, *args, grad_scale=incoming)[1], None, None
         scale = incoming.contiguous()
         _enqueue("coup_scale_grad", grad.device, grad.data_ptr(), _DTYPES[grad.dtype], grad.numel(), scale.data_ptr())
         return grad, None, None
@@ -277,13 +282,14 @@ def _loss(call, logits, *args):
 
 
 def _policy(want_grad, logits, actions, legal_mask, old_log_probs, advantages, ref_logits, active, clip_low, clip_high,
-            kl_coef, entropy_coef):
+            kl_coef, entropy_coef, grad_scale=None):
     """((loss, stats, count, log_probs), gradient or None)"""
     d, keep = _decisions(logits, legal_mask, actions, ref_logits)
     lead, device = logits.shape[:-1], logits.device
     old = _arg(old_log_probs, "old_log_probs", device, lead, _FLOAT32)
     adv = _arg(advantages, "advantages", device, lead, _FLOAT32)
     act = None if active is None else _arg(active, "active", device, lead, _BOOL)
+    factor = None if grad_scale is None else _arg(grad_scale, "grad_scale", device, (), _FLOAT32)
     clip_low, clip_high, kl_coef, entropy_coef = float(clip_low), float(clip_high), float(kl_coef), float(entropy_coef)
     if not (0.0 <= clip_low <= 1.0 and 0.0 <= clip_high < float("inf")):
         raise ValueError("clip_low must be in 0..1, clip_high finite and not negative")
@@ -299,7 +305,8 @@ def _policy(want_grad, logits, actions, legal_mask, old_log_probs, advantages, r
     nbytes = _native.load().coup_policy_workspace(d.rows)
     scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
     out = _native.PolicyOutputs(loss.data_ptr(), stats.data_ptr(), count.data_ptr(), log_probs.data_ptr(),
-                                None if grad is None else grad.data_ptr())
+                                None if grad is None else grad.data_ptr(),
+                                None if factor is None else factor.data_ptr())
     _enqueue("coup_policy_loss", device, ctypes.byref(d), ctypes.byref(terms), ctypes.byref(out), scratch.data_ptr(),
              nbytes)
     return (loss, stats, count, log_probs), grad
@@ -327,15 +334,18 @@ def policy_loss(logits, actions, legal_mask, old_log_probs, advantages, ref_logi
 
 
 def policy_loss_and_grad(logits, actions, legal_mask, old_log_probs, advantages, ref_logits=None, active=None,
-                         clip_low=0.2, clip_high=0.2, kl_coef=0.0, entropy_coef=0.0) -> PolicyLossAndGrad:
+                         clip_low=0.2, clip_high=0.2, kl_coef=0.0, entropy_coef=0.0,
+                         grad_scale=None) -> PolicyLossAndGrad:
     """policy_loss and its gradient in the logits in one pass, outside
-    autograd (hand the gradient on with logits.backward(grad))."""
+    autograd (hand the gradient on with logits.backward(grad)).  grad_scale
+    (0-d float32): what the gradient is multiplied by before it is rounded to
+    the logits' type (a loss scaler's factor)."""
     out, grad = _policy(True, logits, actions, legal_mask, old_log_probs, advantages, ref_logits, active, clip_low,
-                        clip_high, kl_coef, entropy_coef)
+                        clip_high, kl_coef, entropy_coef, grad_scale)
     return PolicyLossAndGrad(*out, grad)
 
 
-def _preference(want_grad, logits, actions, legal_mask, offsets, ref_logits, beta, label_smoothing):
+def _preference(want_grad, logits, actions, legal_mask, offsets, ref_logits, beta, label_smoothing, grad_scale=None):
     """((loss, rewards), gradient or None)"""
     if not isinstance(logits, torch.Tensor) or logits.dim() != 2:
         raise ValueError("logits must be [rows, A]: the sequences' decisions one after another")
@@ -344,6 +354,7 @@ def _preference(want_grad, logits, actions, legal_mask, offsets, ref_logits, bet
     if not isinstance(offsets, torch.Tensor) or offsets.dim() != 1 or offsets.numel() % 2 == 0:
         raise ValueError("offsets must be [2 * pairs + 1]")
     off = _arg(offsets, "offsets", device, offsets.shape, _OFFSET)
+    factor = None if grad_scale is None else _arg(grad_scale, "grad_scale", device, (), _FLOAT32)
     pairs = off.numel() // 2
     beta, label_smoothing = float(beta), float(label_smoothing)
     if beta - beta != 0.0:
@@ -356,7 +367,8 @@ def _preference(want_grad, logits, actions, legal_mask, offsets, ref_logits, bet
     grad = torch.empty(logits.shape, dtype=logits.dtype, device=device) if want_grad else None
     nbytes = _native.load().coup_preference_workspace(d.rows, pairs)
     scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    out = _native.PreferenceOutputs(loss.data_ptr(), rewards.data_ptr(), None if grad is None else grad.data_ptr())
+    out = _native.PreferenceOutputs(loss.data_ptr(), rewards.data_ptr(), None if grad is None else grad.data_ptr(),
+                                    None if factor is None else factor.data_ptr())
     _enqueue("coup_preference_loss", device, ctypes.byref(d), ctypes.byref(terms), ctypes.byref(out),
              scratch.data_ptr(), nbytes)
     return (loss, rewards), grad
@@ -381,9 +393,10 @@ def preference_loss(logits, actions, legal_mask, offsets, ref_logits=None, beta=
     return PreferenceLoss(*_loss(_preference, logits, actions, legal_mask, offsets, ref_logits, beta, label_smoothing))
 
 
-def preference_loss_and_grad(logits, actions, legal_mask, offsets, ref_logits=None, beta=0.1,
-                             label_smoothing=0.0) -> PreferenceLossAndGrad:
+def preference_loss_and_grad(logits, actions, legal_mask, offsets, ref_logits=None, beta=0.1, label_smoothing=0.0,
+                             grad_scale=None) -> PreferenceLossAndGrad:
     """preference_loss and its gradient in the logits in one call, outside
-    autograd (hand the gradient on with logits.backward(grad))."""
-    out, grad = _preference(True, logits, actions, legal_mask, offsets, ref_logits, beta, label_smoothing)
+    autograd (hand the gradient on with logits.backward(grad)).  grad_scale: as
+    in policy_loss_and_grad."""
+    out, grad = _preference(True, logits, actions, legal_mask, offsets, ref_logits, beta, label_smoothing, grad_scale)
     return PreferenceLossAndGrad(*out, grad)

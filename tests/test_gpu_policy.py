@@ -370,7 +370,10 @@ def test_policy_loss(n, A, with_ref, with_active, dtype):
     grad, = torch.autograd.grad(out.loss, leaf, retain_graph=True)
     assert torch.equal(grad, both.grad)
     again, = torch.autograd.grad(out.loss * -4.0, leaf)
-    assert torch.equal(again, (both.grad.float() * -4.0).to(dtype)) and torch.equal(grad, both.grad)
+    # rounded once, after the scale; a power of two commutes with that but at a type's smallest steps
+    assert torch.equal(again, policy.policy_loss_and_grad(*args, **kw, grad_scale=torch.tensor(-4.0, device=DEV)).grad)
+    usual = both.grad.abs() >= torch.finfo(dtype).smallest_normal
+    assert torch.equal(again[usual], (both.grad.float() * -4.0).to(dtype)[usual]) and torch.equal(grad, both.grad)
     with pytest.raises(RuntimeError, match="backward through the graph a second time|already been freed"):
         torch.autograd.grad(out.loss, leaf)
 
@@ -538,6 +541,63 @@ def test_arguments_held_constant_are_refused_beside_logits_with_a_gradient():
     assert leaf.grad is not None
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=lambda d: str(d)[6:])
+def test_a_scaled_losss_gradient_is_rounded_after_the_scale(dtype):
+    """4096 times the loss of 5000 rows: a gradient that was first rounded to a half's smallest steps (2^-24, entries of
+    about 2^-14) and then scaled would be off by up to 2^-13."""
+    n, A, scale = 5000, 18, 4096.0
+    x, mask, actions, ref, old, adv = _policy_inputs(11, n, A, dtype)
+    o = oracle.policy(_np(x), actions.numpy(), mask.numpy(), _np(old), _np(adv), _np(ref), None, 0.2, 0.2, 0.05, 0.01)
+    o.update(grad=scale * o["grad"], size=scale * o["size"])
+    lim = _grad_tol(o, _reach(x, mask), dtype)
+    kw = dict(ref_logits=ref.to(DEV), kl_coef=0.05, entropy_coef=0.01)
+    rest = [t.to(DEV) for t in (actions, mask, old, adv)]
+    factor = torch.tensor(scale, device=DEV)
+    leaf = x.to(DEV).requires_grad_()
+    loss = policy.policy_loss(leaf, *rest, **kw).loss
+    (loss * factor).backward(retain_graph=True)
+    _close(_np(leaf.grad), o["grad"], lim, "autograd")
+    leaf.grad = None
+    (loss * factor).backward()
+    _close(_np(leaf.grad), o["grad"], lim, "autograd again")
+    got = policy.policy_loss_and_grad(x.to(DEV), *rest, **kw, grad_scale=factor)
+    _close(_np(got.grad), o["grad"], lim, "grad_scale")
+    # the paired loss of 250 pairs
+    offsets = list(range(0, n + 1, 10))
+    o = oracle.preference(_np(x), actions.numpy(), mask.numpy(), offsets, _np(ref), 0.1, 0.1)
+    z = _reach(x, mask)
+    tol = 0.1 * 2 * (48 + 4 * z) * H * o["length"].max()
+    info = torch.finfo(dtype)
+    lim = (8 * (48 + 2 * z) * H + 2 * tol) * scale * o["size"] + info.eps / 2 * scale * np.abs(o["grad"])
+    lim = lim + info.smallest_normal * info.eps / 2
+    off = torch.tensor(offsets, device=DEV)
+    leaf = x.to(DEV).requires_grad_()
+    (policy.preference_loss(leaf, rest[0], rest[1], off, ref_logits=kw["ref_logits"], label_smoothing=0.1).loss * factor).backward()
+    _close(_np(leaf.grad), scale * o["grad"], lim, "preference autograd")
+    got = policy.preference_loss_and_grad(x.to(DEV), rest[0], rest[1], off, ref_logits=kw["ref_logits"], label_smoothing=0.1,
+                                          grad_scale=factor)
+    _close(_np(got.grad), scale * o["grad"], lim, "preference grad_scale")
+
+
+def test_a_scale_does_not_meet_the_coefficients():
+    """The largest coefficients, a large power of two for a scale, legal actions that neither policy takes: the gradient
+    is the unscaled one's multiple, to the bit."""
+    n, A = 300, 18
+    x, mask, actions, ref, old, adv = (t.to(DEV) for t in _policy_inputs(12, n, A, torch.float32))
+    for t in (x, ref):
+        t[torch.arange(n), torch.arange(n) % A] = -math.inf
+    taken = actions.long() == torch.arange(n, device=DEV) % A
+    actions = torch.where(taken, -1, actions).to(torch.int8)
+    kw = dict(ref_logits=ref, kl_coef=1e4, entropy_coef=1e4)
+    one = policy.policy_loss_and_grad(x, actions, mask, old, adv, **kw)
+    far = policy.policy_loss_and_grad(x, actions, mask, old, adv, **kw, grad_scale=torch.tensor(2.0**40, device=DEV))
+    assert torch.isfinite(far.grad).all() and far.grad.any()
+    big = one.grad.abs() > 1e-30
+    assert torch.equal(far.grad[big], one.grad[big] * 2.0**40)
+    with pytest.raises(ValueError, match="grad_scale"):
+        policy.policy_loss_and_grad(x, actions, mask, old, adv, grad_scale=torch.ones(1, device=DEV))
+
+
 # ------------------------------------------------------------ preference loss
 def _check_preference(got, o, x, mask, beta, dtype):
     z = _reach(x, mask)
@@ -580,7 +640,8 @@ def test_preference_loss(offsets, n, A, with_ref, eps, dtype):
     grad, = torch.autograd.grad(out.loss, leaf, retain_graph=True)
     assert torch.equal(grad, both.grad)
     again, = torch.autograd.grad(out.loss * 2.0, leaf)
-    assert torch.equal(again, (both.grad.float() * 2.0).to(dtype))
+    usual = both.grad.abs() >= torch.finfo(dtype).smallest_normal
+    assert torch.equal(again[usual], (both.grad.float() * 2.0).to(dtype)[usual])
 
 
 def test_preference_extreme_margins_and_bad_offsets():
