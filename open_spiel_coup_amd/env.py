@@ -455,6 +455,8 @@ class BatchedCoupEnv:
                 raise ValueError(f"the policy's logits must be [{self.batch}, {NUM_ACTIONS}], not {tuple(logits.shape)}")
             if buf is None:
                 buf = self.policy_trajectory_buffers(T, values is not None)
+            if ("values" in buf) != (values is not None):
+                raise ValueError("buf holds values where the policy returns them, and only there")
             uniform = torch.rand(self.batch, dtype=torch.float32, device=dev, generator=generator)
             word = now["legal_mask"].masked_fill(over, 0)
             actions, log_probs = ops.sample_actions(logits.detach(), word, uniform)

@@ -786,6 +786,15 @@ def test_policy_trajectory_is_the_steps_it_records(auto_reset):
         env.collect_policy_trajectory(1, lambda ts: table[:, :7])
 
 
+def test_policy_trajectory_values_need_their_buffer():
+    env = BatchedCoupEnv(8, seed=1, auto_reset=True, obs=False)
+    logits, values = torch.zeros(8, 18, device=DEV), torch.zeros(8, device=DEV)
+    with pytest.raises(ValueError, match="values"):
+        env.collect_policy_trajectory(2, lambda ts: (logits, values), env.policy_trajectory_buffers(2))
+    with pytest.raises(ValueError, match="values"):
+        env.collect_policy_trajectory(2, lambda ts: logits, env.policy_trajectory_buffers(2, values=True))
+
+
 @pytest.mark.parametrize("players", [2, 4])
 def test_a_learners_round(players):
     """Trajectories played by a policy, advantages over them, policy updates on their rows, and the finished games'
