@@ -461,9 +461,20 @@ __global__ __launch_bounds__(kRowThreads) void k_sample(Rows r, const float* __r
 // steps is one pair (f, g), z -> f z + g, per player, and stretches compose.
 // A factor of 0 (a cut) takes nothing of z, be it infinite or NaN.
 // A block holds L lanes; its NT / L threads of a lane take kStretch steps
-// each, latest first, all loaded before the first is used (the window is read
-// once); a scan over the stretches' pairs gives each its z, and the block
-// goes on to the next NT / L * kStretch steps.
+// each, latest first, all loaded before the first is used; a scan over the
+// stretches' pairs gives each its z, and the block goes on to the next round of
+// NT / L * kStretch steps.
+//
+// Where the lanes are too few to fill the chip, a long window is split over
+// blocks too (grid y).  A block finds z behind its part by reading on: it
+// composes the rounds that follow until no player's pair lets anything pass
+// (games end: mostly one or two rounds; else to the window's end) and stores
+// nothing there.  No block waits for another, and nothing is kept between two
+// launches.
+// 20 steps x 2^20 lanes of 6 players (390 MB) take 91 us, 4.2 TB/s, with 96
+// vector instructions a wave and step (50 us alone); 64 x 65,536 of 2 (67 MB)
+// 14.3 us, 4.7 TB/s; 4096 x 33, whose games end after some 25 steps, 8.5 us: a
+// round read, a round computed, each a latency.
 struct AdvantageArgs {
   const int8_t* rewards;  // [T][B][P]
   const uint8_t* step_type;
@@ -472,6 +483,7 @@ struct AdvantageArgs {
   const void* bootstrap;  // [B][P] or null
   float *adv, *target;
   int64_t T, B;
+  int64_t part;  // steps a block: a number of rounds
   int dtype;
   float gamma, gl, gv;  // gamma, gamma lam, gamma (1 - lam)
 };
@@ -511,8 +523,8 @@ struct Rewards {
 // A thread's steps in memory: step k of lane l is at uniform element `base[k]`
 // plus `off[k]`.  With one stretch a lane the step is the block's, so the
 // offset is the lane; with more, it is the lane and the stretch's steps from
-// the window's first: below 2^17 lanes x 32 steps, or 2^14 x 128, 2^11 x 512,
-// 2^7 x 4096, x 24 bytes of any array (launch_advantages_of).
+// the round's first: below 2^17 lanes x 32 steps, or 2^15 x 64, 2^14 x 128, 2^11
+// x 512, x 24 bytes of any array (launch_advantages_of).
 template <int C>
 struct Steps {
   int64_t base[C == 1 ? kStretch : 1];
@@ -558,96 +570,146 @@ __global__ __launch_bounds__(NT) void k_advantages(AdvantageArgs q) {
   constexpr int CW = L < 64 ? 64 / L : 1;  // of them in a wave
   constexpr int NW = C / CW;               // waves a lane's stretches span
   constexpr int LW = L < 64 ? L : 64;
+  constexpr int kSteps = C * kStretch;     // a round's
+  constexpr bool PARTS = L < 64;           // blocks that share a window
   static_assert(C == 1 || L <= 64, "a wave's threads are of one run of lanes");
   __shared__ float totals[C > 1 ? NW * LW * P * 2 : 1];
   const int64_t b0 = (int64_t)blockIdx.x * L;
   const int lanes = (int)(q.B - b0 < L ? q.B - b0 : L);
   const int l = (int)threadIdx.x % L, c = (int)threadIdx.x / L;
+  const int cw = c % CW, wave = c / CW;        // C > 1: this stretch in its wave
   const int lane = l < lanes ? l : lanes - 1;  // lanes past the last load its steps and store nothing
+
+  // This thread's steps of [first, end), at most kSteps: kStretch back from step first + top; ones before the first
+  // load it and are skipped.
+  struct Round {
+    Steps<C> at;
+    int st[kStretch], pl[kStretch], top;
+    Rewards<P> r[kStretch];
+    float v[kStretch];
+  };
+  const auto load = [&](Round& o, int64_t first, int64_t end) {
+    int top = (int)(end - first) - 1 - c * kStretch;
+    if (PARTS) asm volatile("" : "+v"(top));  // else every round's addresses are kept from the first: twice the registers
+    o.top = top;
+#pragma unroll
+    for (int k = 0; k < kStretch; ++k) {
+      const int rel = top - k > 0 ? top - k : 0;
+      if (C == 1) o.at.base[k < (int)(sizeof(o.at.base) / 8) ? k : 0] = (first + rel) * q.B + b0;
+      else o.at.off[k < (int)(sizeof(o.at.off) / 4) ? k : 0] = (uint32_t)rel * (uint32_t)q.B + lane;
+    }
+    if (C == 1) o.at.off[0] = lane;
+    else o.at.base[0] = first * q.B + b0;
+    uint32_t bits[kStretch];
+#pragma unroll
+    for (int k = 0; k < kStretch; ++k) {
+      o.st[k] = *o.at.at(q.step_type, k);
+      o.pl[k] = *o.at.at(q.players, k);
+      o.r[k].load(o.at.at(q.rewards, k, P));
+    }
+    if (q.dtype == COUP_DTYPE_F32) {
+#pragma unroll
+      for (int k = 0; k < kStretch; ++k) bits[k] = *o.at.at((const uint32_t*)q.values, k);
+    } else {
+#pragma unroll
+      for (int k = 0; k < kStretch; ++k) bits[k] = *o.at.at((const uint16_t*)q.values, k);
+    }
+#pragma unroll
+    for (int k = 0; k < kStretch; ++k) {
+      // FIRST 0 and LAST 2 cut, MID 1 and LAST 2 are steps; the rest is skipped, as 3
+      o.st[k] = k > top || o.st[k] > COUP_STEP_SKIPPED ? COUP_STEP_SKIPPED : o.st[k];
+      const bool step = o.st[k] == COUP_STEP_MID || o.st[k] == COUP_STEP_LAST;
+      o.r[k].lo = step ? o.r[k].lo : 0u;
+      o.r[k].hi = step ? o.r[k].hi : 0u;
+      o.pl[k] = step && o.pl[k] < P ? o.pl[k] : -1;
+      o.v[k] = o.pl[k] >= 0 ? widen_bits(bits[k], q.dtype) : 0.0f;
+    }
+  };
+  // Its stretch's pairs (f, g), composed with those before it in its wave; the waves' wholes go to `totals`.
+  const auto compose = [&](const Round& o, float (&f)[P], float (&g)[P]) {
+#pragma unroll
+    for (int p = 0; p < P; ++p) f[p] = 1.0f, g[p] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kStretch; ++k) {
+      const bool cut = !(o.st[k] & 1);
+      const float gvv = q.gv * o.v[k];
+#pragma unroll
+      for (int p = 0; p < P; ++p) {
+        const float here = (cut ? 0.0f : g[p]) + o.r[k].of(p), after = q.gl * here + gvv;
+        const bool acts = p == o.pl[k];
+        const float kept = cut ? 0.0f : f[p];
+        f[p] = acts ? q.gl * kept : kept;
+        g[p] = acts ? after : here;
+      }
+    }
+    // the wave's stretches up to each, a lower index (a later time) first
+#pragma unroll
+    for (int d = 1; d < CW; d *= 2) {
+#pragma unroll
+      for (int p = 0; p < P; ++p) {
+        const float f0 = __shfl_up(f[p], d * L, 64), g0 = __shfl_up(g[p], d * L, 64);
+        if (cw >= d) {
+          g[p] = join(f[p], g0, g[p]);
+          f[p] *= f0;
+        }
+      }
+    }
+    if (cw == CW - 1) {
+      float* mine = totals + (wave * LW + (l & (LW - 1))) * P * 2;
+#pragma unroll
+      for (int p = 0; p < P; ++p) mine[2 * p] = f[p], mine[2 * p + 1] = g[p];
+    }
+  };
+  const auto total = [&](int w, int p) { return totals + ((w * LW + (l & (LW - 1))) * P + p) * 2; };
+
   float z[P];
 #pragma unroll
   for (int p = 0; p < P; ++p)
     z[p] = q.bootstrap ? q.gamma * widen_bits(load_bits(q.bootstrap, (b0 + lane) * P + p, q.dtype), q.dtype) : 0.0f;
 
-  for (int64_t end = q.T; end > 0; end -= C * kStretch) {
-    // this thread's steps: kStretch back from the window's step `top`; ones before the first load it and are skipped
-    const int64_t first = end > C * kStretch ? end - C * kStretch : 0;
-    const int top = (int)(end - first) - 1 - c * kStretch;
-    const int steps = l < lanes ? top + 1 : 0;
-    Steps<C> at;
+  // this block's steps [last, begin)
+  const int64_t begin = PARTS ? q.T - (int64_t)blockIdx.y * q.part : q.T;
+  const int64_t last = PARTS && begin > q.part ? begin - q.part : 0;
+  if (PARTS && begin < q.T) {
+    // z behind them: the rounds after `begin` up to where nothing passes, or the window's end
+    float F[P], G[P];
 #pragma unroll
-    for (int k = 0; k < kStretch; ++k) {
-      const int rel = top - k > 0 ? top - k : 0;
-      if (C == 1) at.base[k < (int)(sizeof(at.base) / 8) ? k : 0] = (first + rel) * q.B + b0;
-      else at.off[k < (int)(sizeof(at.off) / 4) ? k : 0] = (uint32_t)rel * (uint32_t)q.B + lane;
+    for (int p = 0; p < P; ++p) F[p] = 1.0f, G[p] = 0.0f;
+    for (int64_t first = begin; first < q.T; first += kSteps) {
+      Round o;
+      float f[P], g[P];
+      load(o, first, first + kSteps);
+      compose(o, f, g);
+      __syncthreads();
+      bool passes = false;
+#pragma unroll
+      for (int p = 0; p < P; ++p) {
+        float a = 1.0f, b = 0.0f;
+        for (int w = 0; w < NW; ++w) {
+          const float* whole = total(w, p);
+          b = join(whole[0], b, whole[1]);
+          a *= whole[0];
+        }
+        G[p] = join(F[p], b, G[p]);
+        F[p] *= a;
+        passes |= F[p] != 0.0f;
+      }
+      if (!__syncthreads_or(passes)) break;
     }
-    if (C == 1) at.off[0] = lane;
-    else at.base[0] = first * q.B + b0;
-    int st[kStretch], pl[kStretch];
-    uint32_t bits[kStretch];
-    Rewards<P> r[kStretch];
 #pragma unroll
-    for (int k = 0; k < kStretch; ++k) {
-      st[k] = *at.at(q.step_type, k);
-      pl[k] = *at.at(q.players, k);
-      r[k].load(at.at(q.rewards, k, P));
-    }
-    if (q.dtype == COUP_DTYPE_F32) {
-#pragma unroll
-      for (int k = 0; k < kStretch; ++k) bits[k] = *at.at((const uint32_t*)q.values, k);
-    } else {
-#pragma unroll
-      for (int k = 0; k < kStretch; ++k) bits[k] = *at.at((const uint16_t*)q.values, k);
-    }
-    float v[kStretch];
-#pragma unroll
-    for (int k = 0; k < kStretch; ++k) {
-      // FIRST 0 and LAST 2 cut, MID 1 and LAST 2 are steps; the rest is skipped, as 3
-      st[k] = k > top || st[k] > COUP_STEP_SKIPPED ? COUP_STEP_SKIPPED : st[k];
-      const bool step = st[k] == COUP_STEP_MID || st[k] == COUP_STEP_LAST;
-      r[k].lo = step ? r[k].lo : 0u;
-      r[k].hi = step ? r[k].hi : 0u;
-      pl[k] = step && pl[k] < P ? pl[k] : -1;
-      v[k] = pl[k] >= 0 ? widen_bits(bits[k], q.dtype) : 0.0f;
-    }
+    for (int p = 0; p < P; ++p) z[p] = join(F[p], z[p], G[p]);
+  }
+
+  for (int64_t end = begin; end > last; end -= kSteps) {
+    Round o;
+    load(o, end > kSteps ? end - kSteps : 0, end);
+    const int steps = l < lanes ? o.top + 1 : 0;
     if (C == 1) {
-      advance<P, C>(q, at, st, pl, r, v, z, steps);
+      advance<P, C>(q, o.at, o.st, o.pl, o.r, o.v, z, steps);
     } else {
       float f[P], g[P];
-#pragma unroll
-      for (int p = 0; p < P; ++p) f[p] = 1.0f, g[p] = 0.0f;
-#pragma unroll
-      for (int k = 0; k < kStretch; ++k) {
-        const bool cut = !(st[k] & 1);
-        const float gvv = q.gv * v[k];
-#pragma unroll
-        for (int p = 0; p < P; ++p) {
-          const float here = (cut ? 0.0f : g[p]) + r[k].of(p), after = q.gl * here + gvv;
-          const bool acts = p == pl[k];
-          const float kept = cut ? 0.0f : f[p];
-          f[p] = acts ? q.gl * kept : kept;
-          g[p] = acts ? after : here;
-        }
-      }
-      // the wave's stretches up to each, a lower index (a later time) first
-      const int cw = c % CW, wave = c / CW;
-#pragma unroll
-      for (int d = 1; d < CW; d *= 2) {
-#pragma unroll
-        for (int p = 0; p < P; ++p) {
-          const float f0 = __shfl_up(f[p], d * L, 64), g0 = __shfl_up(g[p], d * L, 64);
-          if (cw >= d) {
-            g[p] = join(f[p], g0, g[p]);
-            f[p] *= f0;
-          }
-        }
-      }
-      // the wave's whole, then what stands before this stretch in its wave
-      float* mine = totals + (wave * LW + (l & (LW - 1))) * P * 2;
-      if (cw == CW - 1) {
-#pragma unroll
-        for (int p = 0; p < P; ++p) mine[2 * p] = f[p], mine[2 * p + 1] = g[p];
-      }
+      compose(o, f, g);
+      // what stands before this stretch in its wave
 #pragma unroll
       for (int p = 0; p < P; ++p) {
         f[p] = CW > 1 ? __shfl_up(f[p], L, 64) : 1.0f;
@@ -657,15 +719,15 @@ __global__ __launch_bounds__(NT) void k_advantages(AdvantageArgs q) {
       __syncthreads();
       float here[P];
       for (int w = 0; w < NW; ++w) {
-        const float* o = totals + (w * LW + (l & (LW - 1))) * P * 2;
 #pragma unroll
         for (int p = 0; p < P; ++p) {
+          const float* whole = total(w, p);
           if (w == wave) here[p] = join(f[p], z[p], g[p]);  // z runs through the waves: here it stands before this one
-          z[p] = join(o[2 * p], z[p], o[2 * p + 1]);
+          z[p] = join(whole[0], z[p], whole[1]);
         }
       }
-      __syncthreads();  // the next window writes the totals again
-      advance<P, C>(q, at, st, pl, r, v, here, steps);
+      __syncthreads();  // the next round writes the totals again
+      advance<P, C>(q, o.at, o.st, o.pl, o.r, o.v, here, steps);
     }
   }
 }
@@ -1335,21 +1397,42 @@ inline void launch_sample(const Rows& r, int dtype, const float* uniform, int8_t
   });
 }
 
-// How a window is split: C = 1, 4, 16, 64 or 512 of a lane's stretches at a
-// time, by the lanes there are to fill the chip with (few lanes a block read
-// short runs of memory), and no more of them than the window has.  Either side
-// of the borders, 2 players, us: 256 steps x 65,536 lanes C = 4 52, 1 77;
-// 256 x 131,072 C = 1 117, 4 122; 1024 x 16,384 C = 4 85, 16 109; 1024 x 4096
-// C = 16 33, 128 70; 256 x 1024 C = 64 5.9, 16 7.1; 4096 x 33 C = 512 17, 128 23.
+// How a window is split: L lanes a block and C of each one's stretches at a
+// time (few lanes a block read short runs of memory), by the lanes there are
+// to fill the chip with and with no more stretches than the window has; then
+// into parts, up to a block a CU (twice that: no faster), that look for their
+// z themselves.  Either side of the borders, 2 players, games of some 25 steps,
+// us, L x C: 256 steps x 65,536 lanes 64 x 4 52, 256 x 1 77; 256 x 131,072 256 x
+// 1 117, 64 x 4 122; 512 x 32,768 64 x 4 54, 64 x 8 67; 1024 x 16,384 64 x 8
+// 63, 64 x 4 86, 32 x 16 80; 512 x 8192 32 x 16 24.4, 64 x 8 29; 200 x 1500
+// 8 x 32 6.6, 32 x 16 9.2; 500 x 1500 8 x 64 12.3, 32 x 16 13.8, 500 x 2100
+// 17.0, 18.2; 4000 x 256 32 x 16 13.5, 8 x 32 17.7; 4000 x 130 15.9, 14.5.
+// Without parts 1024 x 2048 took 35 for 18, 4096 x 33 16.7 for 8.5.  A window
+// without one cut, whose parts all read on to its end, loses by them: 4096 x 33
+// 39, 1024 x 2048 29.
+constexpr int64_t kPartBlocks = 256;
+
+template <int P, int L, int NT>
+void launch_advantages_as(AdvantageArgs q, hipStream_t s) {
+  constexpr int64_t kSteps = NT / L * kStretch;
+  const int64_t groups = (q.B + L - 1) / L, rounds = (q.T + kSteps - 1) / kSteps;
+  int64_t parts = L < 64 && groups < kPartBlocks ? kPartBlocks / groups : 1;
+  if (parts > rounds) parts = rounds;
+  q.part = (rounds + parts - 1) / parts * kSteps;
+  const unsigned y = (unsigned)((q.T + q.part - 1) / q.part);
+  k_advantages<P, L, NT><<<dim3((unsigned)groups, y), NT, 0, s>>>(q);
+}
+
 template <int P>
 void launch_advantages_of(const AdvantageArgs& q, hipStream_t s) {
   const auto enough = [&](int c, int64_t lanes) { return q.B >= lanes || (int64_t)c * kStretch >= q.T; };
-  const auto grid = [&](int lanes) { return (unsigned)((q.B + lanes - 1) / lanes); };
-  if (enough(1, 1 << 17)) k_advantages<P, 256, 256><<<grid(256), 256, 0, s>>>(q);
-  else if (enough(4, 1 << 14)) k_advantages<P, 64, 256><<<grid(64), 256, 0, s>>>(q);
-  else if (enough(16, 1 << 11)) k_advantages<P, 32, 512><<<grid(32), 512, 0, s>>>(q);
-  else if (enough(64, 1 << 7)) k_advantages<P, 8, 512><<<grid(8), 512, 0, s>>>(q);
-  else k_advantages<P, 1, 512><<<grid(1), 512, 0, s>>>(q);
+  if (enough(1, 1 << 17)) launch_advantages_as<P, 256, 256>(q, s);
+  else if (enough(4, 1 << 15)) launch_advantages_as<P, 64, 256>(q, s);
+  else if (enough(8, 1 << 14)) launch_advantages_as<P, 64, 512>(q, s);
+  else if (enough(16, 1 << 11)) launch_advantages_as<P, 32, 512>(q, s);
+  else if (q.T > 32 * kStretch && q.T <= 64 * kStretch) launch_advantages_as<P, 8, 512>(q, s);
+  else if (q.T > 64 * kStretch && q.B >= 1 << 8) launch_advantages_as<P, 32, 512>(q, s);
+  else launch_advantages_as<P, 8, 256>(q, s);
 }
 
 inline void launch_advantages(const AdvantageArgs& q, int players, hipStream_t s) {

@@ -295,6 +295,29 @@ def test_advantages_no_ends_and_empty():
         assert a.shape == t.shape == (T, B)
 
 
+@pytest.mark.parametrize("ends", [0.1, 0.004, 0.0])
+@pytest.mark.parametrize("T,B,P,lam", [(2305, 9, 2, 0.95), (1000, 77, 3, 0.9), (700, 600, 6, 0.95), (257, 510, 2, 0.0),
+                                       (300, 2100, 2, 0.95), (129, 8000, 4, 0.8), (70, 16500, 2, 0.95)])
+def test_advantages_of_split_windows(T, B, P, lam, ends):
+    """Windows that several blocks share, each of which reads on for the cuts behind its part: games that end soon, games
+    that mostly outlast a part, and none that ends; some lanes against the oracle, tolerance as above with a chain's
+    terms decayed by gamma lam <= 0.95 (none further than 300 steps counts: 0.95^300 < 2^-22, of sums of 600 or less)."""
+    gen = torch.Generator().manual_seed(T + B + P)
+    r, st, pl, v, b = _window(gen, T, B, P, torch.float32, ends=0.0)
+    cut = torch.rand(T, B, generator=gen) < ends
+    st = torch.where(cut, 2, torch.where(st == 2, 1, st.long())).to(torch.uint8)
+    if not ends:
+        st[st == 0] = 3
+    v = torch.randn(T, B, generator=gen)
+    got = policy.advantages(*(t.to(DEV) for t in (r, st, pl, v, b)), gamma=0.95, lam=lam)
+    lanes = sorted({0, 1, 8, B // 2, B - 2, B - 1})
+    pick = [t[:, lanes].numpy() for t in (r, st, pl)]
+    want = oracle.advantages(*pick, _np(v[:, lanes]), _np(b[lanes]), 0.95, lam)
+    for g, w, name in zip(got, want, ("advantages", "targets")):
+        # a player's rewards are summed undecayed until its next decision: at most some 100 P steps
+        _close(g[:, lanes].cpu().numpy(), w, 4 * 300 * H * 25 * P * (P + 9), name)
+
+
 @pytest.mark.parametrize("T,B,P", [(6, 40, 2), (40, 20000, 2), (200, 3000, 3), (300, 300, 2), (700, 5, 6), (5000, 2, 2)])
 @pytest.mark.parametrize("junk", [math.nan, math.inf, -math.inf])
 def test_nothing_crosses_a_cut(T, B, P, junk):
