@@ -245,11 +245,9 @@ class _LossOf(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, call, args):
-        out, grad = call(logits.dtype != torch.float16, logits, *args)
-        # for a backward that calls again: torch checks their versions there
-        ctx.save_for_backward(logits, *[t for t in args if isinstance(t, torch.Tensor)])
-        ctx.call, ctx.grad = call, grad
-        ctx.args = [None if isinstance(t, torch.Tensor) else (t,) for t in args]
+        out, grad, again, read = call(logits.dtype != torch.float16, logits, *args)
+        ctx.save_for_backward(*read)  # for `again`, which reads them: torch checks their versions there
+        ctx.grad, ctx.again, ctx.at = grad, again, [t.data_ptr() for t in read]
         ctx.mark_non_differentiable(*out[1:])
         return out
 
@@ -261,10 +259,9 @@ class _LossOf(torch.autograd.Function):
                                "_and_grad form and hand the gradient on")
         grad, ctx.grad = ctx.grad, None
         if grad is None:
-            logits, *tensors = ctx.saved_tensors
-            tensors = iter(tensors)
-            args = [next(tensors) if a is None else a[0] for a in ctx.args]
-            return ctx.call(True, logits, *args, grad_scale=incoming)[1], None, None
+            if [t.data_ptr() for t in ctx.saved_tensors] != ctx.at:
+                raise RuntimeError("an argument of this loss was given other data since")
+            return ctx.again(incoming), None, None
         scale = incoming.contiguous()
         _enqueue("coup_scale_grad", grad.device, grad.data_ptr(), _DTYPES[grad.dtype], grad.numel(), scale.data_ptr())
         return grad, None, None
@@ -281,9 +278,23 @@ def _loss(call, logits, *args):
     return _LossOf.apply(logits, call, args)
 
 
+def _again(name, outputs, d, terms, nbytes, shape, dtype, device):
+    """The call `name` once more, for its gradient times a factor.  Holds no
+    tensor: those that d and terms point into are its caller's to keep."""
+    def call(factor):
+        grad = torch.empty(shape, dtype=dtype, device=device)
+        loss = torch.empty((), dtype=torch.float32, device=device)
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        out = outputs(loss=loss.data_ptr(), grad=grad.data_ptr(), grad_scale=factor.data_ptr())
+        _enqueue(name, device, ctypes.byref(d), ctypes.byref(terms), ctypes.byref(out), scratch.data_ptr(), nbytes)
+        return grad
+    return call
+
+
 def _policy(want_grad, logits, actions, legal_mask, old_log_probs, advantages, ref_logits, active, clip_low, clip_high,
             kl_coef, entropy_coef, grad_scale=None):
-    """((loss, stats, count, log_probs), gradient or None)"""
+    """((loss, stats, count, log_probs), gradient or None, the call for a
+    gradient with a factor alone, the tensors that it reads)"""
     d, keep = _decisions(logits, legal_mask, actions, ref_logits)
     lead, device = logits.shape[:-1], logits.device
     old = _arg(old_log_probs, "old_log_probs", device, lead, _FLOAT32)
@@ -309,7 +320,8 @@ def _policy(want_grad, logits, actions, legal_mask, old_log_probs, advantages, r
                                 None if factor is None else factor.data_ptr())
     _enqueue("coup_policy_loss", device, ctypes.byref(d), ctypes.byref(terms), ctypes.byref(out), scratch.data_ptr(),
              nbytes)
-    return (loss, stats, count, log_probs), grad
+    again = _again("coup_policy_loss", _native.PolicyOutputs, d, terms, nbytes, logits.shape, logits.dtype, device)
+    return (loss, stats, count, log_probs), grad, again, [t for t in (*keep, old, adv, act) if t is not None]
 
 
 def policy_loss(logits, actions, legal_mask, old_log_probs, advantages, ref_logits=None, active=None, clip_low=0.2,
@@ -340,13 +352,13 @@ def policy_loss_and_grad(logits, actions, legal_mask, old_log_probs, advantages,
     autograd (hand the gradient on with logits.backward(grad)).  grad_scale
     (0-d float32): what the gradient is multiplied by before it is rounded to
     the logits' type (a loss scaler's factor)."""
-    out, grad = _policy(True, logits, actions, legal_mask, old_log_probs, advantages, ref_logits, active, clip_low,
+    out, grad, *_ = _policy(True, logits, actions, legal_mask, old_log_probs, advantages, ref_logits, active, clip_low,
                         clip_high, kl_coef, entropy_coef, grad_scale)
     return PolicyLossAndGrad(*out, grad)
 
 
 def _preference(want_grad, logits, actions, legal_mask, offsets, ref_logits, beta, label_smoothing, grad_scale=None):
-    """((loss, rewards), gradient or None)"""
+    """((loss, rewards), gradient or None, and as _policy)"""
     if not isinstance(logits, torch.Tensor) or logits.dim() != 2:
         raise ValueError("logits must be [rows, A]: the sequences' decisions one after another")
     d, keep = _decisions(logits, legal_mask, actions, ref_logits)
@@ -371,7 +383,8 @@ def _preference(want_grad, logits, actions, legal_mask, offsets, ref_logits, bet
                                     None if factor is None else factor.data_ptr())
     _enqueue("coup_preference_loss", device, ctypes.byref(d), ctypes.byref(terms), ctypes.byref(out),
              scratch.data_ptr(), nbytes)
-    return (loss, rewards), grad
+    again = _again("coup_preference_loss", _native.PreferenceOutputs, d, terms, nbytes, logits.shape, logits.dtype, device)
+    return (loss, rewards), grad, again, [t for t in (*keep, off) if t is not None]
 
 
 def preference_loss(logits, actions, legal_mask, offsets, ref_logits=None, beta=0.1,
@@ -398,5 +411,5 @@ def preference_loss_and_grad(logits, actions, legal_mask, offsets, ref_logits=No
     """preference_loss and its gradient in the logits in one call, outside
     autograd (hand the gradient on with logits.backward(grad)).  grad_scale: as
     in policy_loss_and_grad."""
-    out, grad = _preference(True, logits, actions, legal_mask, offsets, ref_logits, beta, label_smoothing, grad_scale)
+    out, grad, *_ = _preference(True, logits, actions, legal_mask, offsets, ref_logits, beta, label_smoothing, grad_scale)
     return PreferenceLossAndGrad(*out, grad)

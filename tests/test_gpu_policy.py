@@ -733,6 +733,39 @@ def test_graph_replays_of_every_call():
             assert torch.equal(a.nan_to_num(3), b.nan_to_num(3)), (k, i)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16], ids=lambda d: str(d)[6:])
+def test_a_backward_that_calls_again_reads_what_the_forward_read(dtype):
+    """Strided logits and arguments, changed arguments and freed graphs: the second call's inputs are the first's or it
+    raises."""
+    n, A = 400, 18
+    x, mask, actions, ref, old, adv = (t.to(DEV) for t in _policy_inputs(4, n, A, dtype))
+    want = policy.policy_loss_and_grad(x, actions, mask, old, adv, ref_logits=ref, kl_coef=0.1).grad
+    wide = torch.zeros(n, 40, dtype=dtype, device=DEV)
+    wide[:, 3:21] = x
+    for leaf, view in ((x.clone().requires_grad_(), lambda t: t), (wide.clone().requires_grad_(), lambda t: t[:, 3:21]),
+                       (x.t().clone().requires_grad_(), lambda t: t.t())):
+        twice = [t.repeat_interleave(2) for t in (actions, mask, old, adv)]
+        out = policy.policy_loss(view(leaf), *[t[::2] for t in twice], ref_logits=ref, kl_coef=0.1)
+        for _ in range(2):
+            grad, = torch.autograd.grad(out.loss, leaf, retain_graph=True)
+            assert torch.equal(view(grad), want)
+        torch.autograd.grad(out.loss, leaf)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(out.loss, leaf)
+    leaf = x.clone().requires_grad_()
+    ours = adv.clone()
+    out = policy.policy_loss(leaf, actions, mask, old, ours)
+    torch.autograd.grad(out.loss, leaf, retain_graph=True)
+    ours.zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(out.loss, leaf, retain_graph=True)
+    out = policy.policy_loss(leaf, actions, mask, old, ours)
+    torch.autograd.grad(out.loss, leaf, retain_graph=True)
+    ours.data = ours.clone()
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(out.loss, leaf)
+
+
 def test_captured_autograd_is_refused():
     """A loss whose logits require a gradient raises under capture, before anything is enqueued."""
     n, A = 64, 18
