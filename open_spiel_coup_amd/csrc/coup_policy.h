@@ -13,7 +13,8 @@
 //
 // Arithmetic: logits are widened to 32 bits on load; the softmax statistics,
 // the log probabilities and the gradient are 32-bit; the losses' sums over
-// rows are 64-bit (a preference sequence's within one tile 32-bit).  A
+// rows are 64-bit (a preference sequence's within one tile 32-bit where rows
+// are many).  A
 // gradient is rounded once, to the logits' type, at its store.  Two
 // comparisons decide whole outputs and are repeated in 64 bits where 32-bit
 // rounding could turn them: which action a uniform number falls on, and which
@@ -750,6 +751,23 @@ __device__ __forceinline__ float wave_sum(float v) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double add_moved(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROWS, 0xf, true);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, ROWS, 0xf, true);
+  return v + __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// The same in 64 bits, in the last lane alone.
+__device__ __forceinline__ double wave_sum_last(double v) {
+  v = add_moved<0x111, 0xf>(v);
+  v = add_moved<0x112, 0xf>(v);
+  v = add_moved<0x114, 0xf>(v);
+  v = add_moved<0x118, 0xf>(v);
+  v = add_moved<0x142, 0xa>(v);
+  return add_moved<0x143, 0xc>(v);
+}
+
 // Four values summed over the wave at once, in 64 bits (a loss's terms nearly
 // cancel): the sum of value k is lane k's (7 exchanges for 24: each of the first two halves what a lane still holds).
 __device__ __forceinline__ double wave_sum_four(const float (&v)[4]) {
@@ -1055,8 +1073,13 @@ __device__ __forceinline__ float pair_cost(const PreferenceArgs& q, int64_t pair
   chosen *= q.beta, rejected *= q.beta;
   if (!ok) chosen = rejected = NAN;
   if (q.rewards) q.rewards[2 * pair] = (float)chosen, q.rewards[2 * pair + 1] = (float)rejected;
-  const float x = (float)(chosen - rejected), size = fabsf(x), eps = (float)q.eps;
-  const float y = exp_of(-size), part = __builtin_amdgcn_rcpf(1.0f + y);
+  const double whole = chosen - rejected;
+  const float x = (float)whole, size = fabsf(x), eps = (float)q.eps;
+  // what x lost to rounding: exp(-|x|) has its absolute error as a relative one
+  const float less = size < INFINITY ? (float)(fabs(whole) - (double)size) : 0.0f;
+  float y = exp_of(-size);
+  y -= y * less;
+  const float part = __builtin_amdgcn_rcpf(1.0f + y);
   const float miss = x > 0.0f ? y * part : part;  // sigma(-x)
   const float factor = q.grad_scale ? *q.grad_scale : 1.0f;
   *coef = ok ? (eps - miss) * (float)(q.beta / (double)q.pairs) * factor : NAN;
@@ -1156,16 +1179,19 @@ __global__ __launch_bounds__(kRowThreads, AP > 20 ? 2 : FEW ? 4 : sizeof(T) == 2
   const bool good = __syncthreads_and(ok);
   const int64_t begin = good ? edge[0] : 0, end = good ? edge[seqs] : 0;
 
-  // a tile's log ratios to its sequences' sums (32 bits within a tile, 64 across)
+  // a tile's log ratios to its sequences' sums (64 bits across tiles and, for
+  // calls of few rows, within one: one pair's cost of e^-x has x's absolute error)
+  using Sum = std::conditional_t<FEW, double, float>;
   const auto add_tile = [&](int64_t row0, int rows) {
     __syncthreads();
     for (int s = wave; s < seqs; s += kRowThreads / 64) {
       const int64_t lo = edge[s] - row0, hi = edge[s + 1] - row0;
       const int to = !good ? 0 : hi < rows ? (int)hi : rows;
-      float v = 0.0f;
-      for (int k = (lo > 0 ? (lo < rows ? (int)lo : rows) : 0) + ((int)threadIdx.x & 63); k < to; k += 64) v += ratio[k];
-      v = wave_sum(v);
-      if ((threadIdx.x & 63) == 0) sum[s] += (double)v;
+      Sum v = 0;
+      for (int k = (lo > 0 ? (lo < rows ? (int)lo : rows) : 0) + ((int)threadIdx.x & 63); k < to; k += 64) v += (Sum)ratio[k];
+      if constexpr (FEW) v = wave_sum_last(v);
+      else v = wave_sum(v);
+      if ((threadIdx.x & 63) == 63) sum[s] += (double)v;
     }
     __syncthreads();
   };

@@ -684,6 +684,26 @@ def test_preference_extreme_margins_and_bad_offsets():
         assert math.isnan(float(got.loss)), bad
 
 
+def test_a_sure_pairs_small_loss_keeps_its_digits():
+    """One pair 20 apart: its cost e^-20 has the absolute error of the difference of two sums of about 2000.  Every row's
+    log probability is its logit less log(1 + e^-20) < 2.1e-9, which 32 bits round off; the sums and their difference
+    are left to err, and the exponential by a few 2^-24."""
+    rows = 100
+    gen = torch.Generator().manual_seed(8)
+    depth = 20 + torch.rand(2 * rows, generator=gen)
+    depth[rows:] = depth[:rows] + 0.2 + 1e-3 * torch.rand(rows, generator=gen)
+    x = torch.zeros(2 * rows, 3)
+    x[:, 1] = -depth
+    mask, actions = torch.full((2 * rows,), 3, dtype=torch.int32), torch.ones(2 * rows, dtype=torch.int8)
+    want = oracle.preference(_np(x), actions.numpy(), mask.numpy(), [0, rows, 2 * rows], None, 1.0, 0.0)
+    assert 1e-10 < want["loss"] < 1e-8
+    off = torch.tensor([0, rows, 2 * rows], device=DEV)
+    got = policy.preference_loss_and_grad(x.to(DEV), actions.to(DEV), mask.to(DEV), off, beta=1.0)
+    assert abs(float(got.loss) / want["loss"] - 1) <= 2 * rows * 2.1e-9 + 16 * H
+    k = want["grad"] != 0
+    assert np.abs(_np(got.grad)[k] / want["grad"][k] - 1).max() <= 2 * rows * 2.1e-9 + 32 * H
+
+
 def test_preference_refusals():
     x = torch.zeros(6, 18, device=DEV)
     m, a = torch.zeros(6, dtype=torch.int32, device=DEV), torch.zeros(6, dtype=torch.int8, device=DEV)
