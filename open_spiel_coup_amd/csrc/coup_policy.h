@@ -831,7 +831,7 @@ struct PolicyArgs {
 // many rows the 32-bit roundings average out).  A call of 65,536 float rows
 // takes 14.0 us, one of 65,537 13.0.
 constexpr int64_t kFewRows = 65536;
-constexpr int kCountBlocks = 256, kCountThreads = 1024, kFinishThreads = 1024;
+constexpr int kCountBlocks = 256, kCountThreads = 1024, kFinishThreads = 512;
 
 // How many decisions there are: 6 bytes a row, four rows a thread at a time.
 // The gradient needs it before its first store, and a second pass over the
@@ -988,9 +988,11 @@ __global__ __launch_bounds__(kRowThreads, AP <= 20 ? 4 : 2) void k_policy_loss(P
 
 // The blocks' sums in a fixed order, in 64 bits: the loss and its terms'
 // means.  16,384 blocks (4 x 2^20 rows) leave 576 KiB, which one block takes
-// 13 us to read; so kFoldBlocks of them fold a stretch each, and the one that
-// is done last (by a ticket that the loss kernel reset) folds those, in 8 us.
-constexpr int kFoldBlocks = 64, kFoldStretch = 256;
+// 13 us to read; so from kFoldsFrom on up to kFoldBlocks of them fold a stretch
+// each, and the one that is done last (by a ticket that the loss kernel reset)
+// folds those, in 8 us.  1025 blocks: one block makes a call of 13.5 us, four
+// 15.5; 5120: twenty fold in 5.8 us, five in 6.5.
+constexpr int kFoldBlocks = 64, kFoldStretch = 256, kFoldsFrom = 2048;
 
 __global__ __launch_bounds__(kRowThreads) void k_policy_finish(const double* __restrict__ partial,
                                                                 const int32_t* __restrict__ decided, int64_t blocks,
@@ -1496,7 +1498,8 @@ inline void launch_policy(PolicyArgs q, int dtype, double kl, double ent, float*
       else k_policy_loss<T, AP, false><<<blocks, kRowThreads, 0, s>>>(q);
     });
   }
-  const unsigned folds = blocks / kFoldStretch < 1 ? 1 : blocks / kFoldStretch < kFoldBlocks ? blocks / kFoldStretch : kFoldBlocks;
+  const unsigned stretches = blocks < kFoldsFrom ? 1 : blocks / kFoldStretch;
+  const unsigned folds = stretches < kFoldBlocks ? stretches : kFoldBlocks;
   k_policy_finish<<<folds, kRowThreads, 0, s>>>(q.partial, q.decided, blocks, fold, q.ticket, kl, ent, loss, stats, count);
 }
 

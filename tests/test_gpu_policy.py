@@ -434,6 +434,34 @@ def test_losses_of_many_rows(A, with_ref, dtype):
         _check_preference((gp.loss, gp.rewards[seqs], gp.grad[rows]), part, x, mask, 0.1, dtype)
 
 
+@pytest.mark.parametrize("times", [750, 3003])
+def test_losses_of_more_rows_than_one_block_folds(times):
+    """The sums of 2050 and of 8212 blocks, folded by several, in a call of its own, again, and captured and replayed:
+    the 700's loss, and the same to the bit each time."""
+    n, A = 700, 5
+    x, mask, actions, ref, old, adv = _policy_inputs(21, n, A, torch.float32)
+    o = oracle.policy(_np(x), actions.numpy(), mask.numpy(), _np(old), _np(adv), _np(ref), None, 0.2, 0.2, 0.2, 0.05)
+    args = [t.to(DEV).repeat(times, *[1] * (t.dim() - 1)) for t in (x, actions, mask, old, adv)]
+    kw = dict(ref_logits=ref.to(DEV).repeat(times, 1), kl_coef=0.2, entropy_coef=0.05)
+    got = policy.policy_loss_and_grad(*args, **kw)
+    assert int(got.count) == times * o["count"]
+    part = {**o, "grad": o["grad"] / times, "size": o["size"] / times}
+    for k in (0, times - 1):
+        rows = slice(k * n, (k + 1) * n)
+        _check_policy((got.loss, got.stats, torch.tensor(o["count"]), got.log_probs[rows], got.grad[rows]), part, x, mask,
+                      torch.float32)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        held = policy.policy_loss_and_grad(*args, **kw)
+    for _ in range(4):
+        graph.replay()
+        again = policy.policy_loss_and_grad(*args, **kw)
+        torch.cuda.synchronize()
+        for a, b, c in zip(got, again, held):
+            assert torch.equal(a, b) and torch.equal(a, c)
+
+
 def test_a_large_ratio_overflows_to_infinity():
     """exp of more than 88, where it is not clipped (a negative advantage): an infinite loss, in calls of few rows and of many."""
     for n in (64, 70000):
