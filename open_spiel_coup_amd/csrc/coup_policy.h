@@ -1069,7 +1069,8 @@ __device__ __forceinline__ int64_t offset_at(const PreferenceArgs& q, int64_t s)
 // derivative in a chosen row's log ratio (a rejected row's is -coef).  NaN
 // where `ok` is false: its offsets do not ascend within the rows.  With
 // y = exp(-|x|), -log sigma(+-x) is log(1 + y) and for the wrong sign |x| more,
-// and sigma(-|x|) is y / (1 + y): 32 bits hold both to a few units.
+// and sigma(-|x|) is y / (1 + y): 32 bits hold both to a few units.  x is
+// infinite where one sequence holds an action of probability 0.
 __device__ __forceinline__ float pair_cost(const PreferenceArgs& q, int64_t pair, double chosen, double rejected, bool ok,
                                            float* coef) {
   chosen *= q.beta, rejected *= q.beta;
@@ -1085,7 +1086,8 @@ __device__ __forceinline__ float pair_cost(const PreferenceArgs& q, int64_t pair
   const float miss = x > 0.0f ? y * part : part;  // sigma(-x)
   const float factor = q.grad_scale ? *q.grad_scale : 1.0f;
   *coef = ok ? (eps - miss) * (float)(q.beta / (double)q.pairs) * factor : NAN;
-  return ok ? log1p_of(y) + size * (x > 0.0f ? eps : 1.0f - eps) : NAN;
+  const float wrong = x > 0.0f ? eps : 1.0f - eps;
+  return ok ? log1p_of(y) + (wrong != 0.0f ? wrong * size : 0.0f) : NAN;  // an infinite x costs nothing without a weight
 }
 
 __device__ __forceinline__ bool ascending(int64_t a, int64_t b, int64_t c, int64_t n) {
