@@ -500,7 +500,10 @@ int coup_advantages(const coup_window* w, double gamma, double lam, float* adv, 
  *   -min(rho adv, clip(rho, 1 - clip_low, 1 + clip_high) adv)
  *     + kl_coef KL(pi || pi_ref) - entropy_coef H(pi),
  * rho = exp(log pi(action) - old_log_probs); KL and H over the legal actions
- * (KL is 0 without ref_logits).  A ratio exactly on a border is not clipped. */
+ * (KL is 0 without ref_logits).  A ratio exactly on a border is not clipped.
+ * The KL is infinite where the reference's logit is -inf at a legal action
+ * that the policy gives a share (its logit within 745 of the row's largest);
+ * with kl_coef != 0 such a row's gradient is NaN at its legal actions. */
 typedef struct {
   const float* old_log_probs; /* [rows] */
   const float* advantages;    /* [rows] */

@@ -39,8 +39,9 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kRowThreads = 256;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
-// Stands for -inf in products with a 0 share.  Far below any logit's distance,
-// and 1e4 (the largest coefficient of the loss) times it is still finite.
+// Stands for -inf in products with a 0 share: 1e4 (the largest coefficient of
+// the loss) times it is still finite.  Rows where a reference's logit is that
+// far below its largest at an action with a share are taken again (far_row).
 constexpr float kLowest = -1e33f;
 
 template <class T>
@@ -826,6 +827,58 @@ struct PolicyArgs {
   int count_blocks;
 };
 
+// Whether a row's t_ref (its held logits less their largest, softmax) is
+// about kLowest at a legal action: the illegal ones alone add up to the rest.
+template <int AP>
+__device__ __forceinline__ bool is_far(const float (&t)[AP], uint32_t legal) {
+  float sum = 0.0f;
+#pragma unroll
+  for (int a = 0; a < AP; ++a) sum += t[a];
+  return sum < kLowest * ((float)(AP - __popc(legal)) + 0.5f);
+}
+
+// A row that is_far: one legal action's t_ref at least is below kLowest / 62.
+// Where the policy takes such an action (with a share above 0 in 64 bits), K and
+// the gradient (this thread's row of `tile`, if wanted) anew, in 64 bits and
+// from memory.  K is infinite where the reference's logit is -inf, and then has
+// no gradient: NaN at the legal actions.  Actions that both policies rule out
+// (-inf, or a type's lowest value, in both) leave the row as it is.
+template <class T, int AP>
+__device__ __forceinline__ void far_row(const Rows& r, int64_t i, uint32_t legal, int action, double m, double rm, double w,
+                                        double kl, double ent, double scale, bool grad, char* tile, float& K) {
+  const T* x = (const T*)r.logits + i * r.stride;
+  const T* ref = (const T*)r.ref + i * r.ref_stride;
+  bool taken = false;
+#pragma unroll 1
+  for (uint32_t b = legal; b; b &= b - 1) {
+    const int a = __builtin_ctz(b);
+    taken |= (double)widen(x[a]) - m > -745.0 && (double)widen(ref[a]) - rm < (double)kLowest / 64;
+  }
+  if (!taken) return;
+  double sum = 0.0, rsum = 0.0, et = 0.0, ed = 0.0;
+#pragma unroll 1
+  for (uint32_t b = legal; b; b &= b - 1) {
+    const int a = __builtin_ctz(b);
+    const double t = (double)widen(x[a]) - m, tr = (double)widen(ref[a]) - rm, e = exp(t);
+    sum += e;
+    rsum += exp(tr);
+    et += e > 0.0 ? e * t : 0.0;
+    ed += e > 0.0 ? e * (t - tr) : 0.0;
+  }
+  const double lse = log(sum), H = lse - et / sum, k = ed / sum - (lse - log(rsum));
+  K = (float)k;
+  if (!grad) return;
+#pragma unroll 1
+  for (uint32_t b = legal; b; b &= b - 1) {
+    const int a = __builtin_ctz(b);
+    const double t = (double)widen(x[a]) - m, tr = (double)widen(ref[a]) - rm, p = exp(t) / sum, l = t - lse;
+    double g = w * ((a == action ? 1.0 : 0.0) - p);
+    if (p > 0.0) g += p * (kl * (l - (tr - log(rsum)) - k) + ent * (l + H));
+    if (!(k < INFINITY)) g = NAN;
+    Tile<T, AP>::write_one(tile, r.A, a, (float)(g * scale));
+  }
+}
+
 // Up to this many rows every row's ratio is taken in 64 bits, not only those
 // by a border: a loss of few terms that nearly cancel keeps its digits (over
 // many rows the 32-bit roundings average out).  A call of 65,536 float rows
@@ -897,6 +950,7 @@ __global__ __launch_bounds__(kRowThreads, AP <= 20 ? 4 : 2) void k_policy_loss(P
     adv = q.adv[i];
   }
   float x[AP], d[AP], xa, rta = 0.0f;  // d: the reference's t, rta the action's
+  bool far = false;
   Softmax rs{0.0f, 1.0f, 0.0f};
   stage_rows<T, AP, REF>(
       tile, q.r, row0, rows, legal, action, d,
@@ -904,10 +958,11 @@ __global__ __launch_bounds__(kRowThreads, AP <= 20 ? 4 : 2) void k_policy_loss(P
         float unused[AP];
         rs = softmax<false, AP>(row, unused);
         rta = rs.t(one);
+        far = is_far<AP>(row, legal);
       },
       x, xa);
   const float n = wave_sum(count), scale = factor / (n > 0.0f ? n : 1.0f);
-  float surrogate = 0.0f, kl = 0.0f, entropy = 0.0f, clipped = 0.0f, logp = 0.0f, ga = 0.0f;
+  float surrogate = 0.0f, kl = 0.0f, entropy = 0.0f, clipped = 0.0f, logp = 0.0f, ga = 0.0f, m = 0.0f, w = 0.0f;
   if (legal) {
     // x becomes t
     float e[AP];
@@ -921,10 +976,8 @@ __global__ __launch_bounds__(kRowThreads, AP <= 20 ? 4 : 2) void k_policy_loss(P
     const float inv = __builtin_amdgcn_rcpf(s.sum), lse = log_of(s.sum);
     et *= inv, ed *= inv;
     entropy = lse - et;
-    if (REF) {
-      kl = ed - log_ratio(s.sum, rs.sum);
-      if (kl > 1e24f) kl = INFINITY;  // an action that the reference never takes
-    }
+    if (REF) kl = ed - log_ratio(s.sum, rs.sum);
+    m = s.m;
     logp = (xa - s.m) - lse;
     const float dl = logp - old, border = adv > 0.0f ? q.log_high : q.log_low;
     bool over = adv > 0.0f ? dl > border : dl < border;
@@ -943,7 +996,7 @@ __global__ __launch_bounds__(kRowThreads, AP <= 20 ? 4 : 2) void k_policy_loss(P
     if (q.grad) {
       // p_b w_b, w_b = ent (l_b + H) + kl (d_b - K) - w, in which the lse's
       // cancel: (ent + kl) (t_b - E t) - kl (tr_b - E tr) - w
-      const float w = (over || adv == 0.0f) ? 0.0f : -rho * adv;
+      w = (over || adv == 0.0f) ? 0.0f : -rho * adv;
       // (the factor, which has no bound, meets p_b and not the coefficients
       // that kLowest is held for)
       const float share = inv * scale, ct = REF ? q.ent + q.kl : q.ent, cr = REF ? q.kl : 0.0f;
@@ -964,6 +1017,9 @@ __global__ __launch_bounds__(kRowThreads, AP <= 20 ? 4 : 2) void k_policy_loss(P
   if (q.grad) {
     Tile<T, AP>::write(tile, q.r.A, x);
     if (legal) Tile<T, AP>::write_one(tile, q.r.A, action, ga);
+  }
+  if (REF && far) far_row<T, AP>(q.r, i, legal, action, m, rs.m, w, q.kl, q.ent, scale, q.grad && q.kl != 0.0f, tile, kl);
+  if (q.grad) {
     __syncthreads();
     Tile<T, AP>::copy_out(tile, (T*)q.grad, row0, rows, q.r.A);
   }

@@ -340,7 +340,9 @@ def policy_loss(logits, actions, legal_mask, old_log_probs, advantages, ref_logi
     (e.g. one player's; None: all).  Everything but logits is held constant.
     The loss is 0, with zero gradients, where nothing counts.  A ratio exactly
     on a border is not clipped.  A legal action that the reference gives no
-    probability makes the KL infinite."""
+    probability (a logit of -inf) and the policy some (a logit within 745 of
+    the row's largest) makes the KL infinite, and with a kl_coef its row's
+    gradient NaN."""
     return PolicyLoss(*_loss(_policy, logits, actions, legal_mask, old_log_probs, advantages, ref_logits, active,
                              clip_low, clip_high, kl_coef, entropy_coef))
 

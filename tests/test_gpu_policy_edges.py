@@ -45,3 +45,66 @@ def test_a_margin_of_plus_infinity_costs_nothing(pairs, each, eps):
     y = x.clone()
     y[0], y[each // 2] = x[each // 2], x[0]
     assert float(policy.preference_loss(y.to(DEV), *args, beta=0.25, label_smoothing=eps).loss) == math.inf
+
+
+# ------------------------------------------------------------ references without a share
+def _one_decision(x, ref, n):
+    """Row n // 2 of n like rows is the decision of logits x against ref; the others' KL is 0."""
+    A = x.numel()
+    rows, refs = torch.zeros(n, A, dtype=x.dtype), torch.zeros(n, A, dtype=x.dtype)
+    rows[n // 2], refs[n // 2] = x, ref
+    words = torch.full((n,), (1 << A) - 1, dtype=torch.int32)
+    return rows, refs, words, torch.ones(n, dtype=torch.int8), torch.full((n,), -math.log(A)), torch.ones(n)
+
+
+@pytest.mark.parametrize("dtype", base.DTYPES, ids=lambda d: str(d)[6:])
+@pytest.mark.parametrize("n", [5, 70001])
+@pytest.mark.parametrize("A", [3, 18, 24])
+def test_an_action_only_the_policy_takes_makes_the_kl_infinite(A, n, dtype):
+    """However small its share is (e^-25 to e^-700): the KL and the loss are infinite, and the row has no gradient.
+    Where the share is 0 (a logit of -inf, or 800 below), or the loss does not weigh the KL, all is finite."""
+    for gap in (1.0, 25.0, 60.0, 80.0, 150.0, 700.0):
+        x, ref = torch.zeros(A, dtype=dtype), torch.zeros(A, dtype=dtype)
+        x[A - 1], ref[A - 1] = -gap, -math.inf
+        rows, refs, words, acts, old, adv = (t.to(DEV) for t in _one_decision(x, ref, n))
+        got = policy.policy_loss_and_grad(rows, acts, words, old, adv, ref_logits=refs, kl_coef=0.1)
+        assert float(got.stats[1]) == math.inf and float(got.loss) == math.inf, gap
+        assert got.grad[n // 2].isnan().all() and int(got.grad.isnan().sum()) == A
+        assert float(policy.policy_loss(rows, acts, words, old, adv, ref_logits=refs, kl_coef=0.1).loss) == math.inf
+        free = policy.policy_loss_and_grad(rows, acts, words, old, adv, ref_logits=refs)
+        none = policy.policy_loss_and_grad(rows, acts, words, old, adv)
+        assert float(free.stats[1]) == math.inf and torch.equal(free.loss, none.loss) and torch.equal(free.grad, none.grad)
+    for gap in (800.0, math.inf):
+        x[A - 1] = -gap
+        rows, refs, words, acts, old, adv = (t.to(DEV) for t in _one_decision(x, ref, n))
+        got = policy.policy_loss_and_grad(rows, acts, words, old, adv, ref_logits=refs, kl_coef=0.1)
+        # both policies are uniform over the other A - 1 actions
+        assert abs(float(got.stats[1])) <= 100 * H and torch.isfinite(got.grad).all()
+        assert float(got.grad[n // 2, A - 1]) == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=lambda d: str(d)[6:])
+@pytest.mark.parametrize("n", [5, 70001])
+def test_a_references_lowest_values_have_a_finite_kl(n, dtype):
+    """Logits of the type's lowest value, -1e30 and -1e34 at actions the policy takes: finite distances, weighed as such.
+    64-bit sums, rounded: the KL is off by a rounding of the row's and one of the mean (2 H), a gradient entry by the
+    scale's, its own (2 H of its terms) and its type's."""
+    low = torch.finfo(dtype).min
+    # (logit, reference's) of an action; the first is acted
+    for far in ([(-1.0, low)], [(-30.0, low)], [(-1.0, low), (0.5, low / 4), (0.25, -1e30)], [(-60.0, -1e34)], [(0.0, -3e32)]):
+        x, ref = torch.zeros(9), torch.zeros(9)
+        x[1], ref[1], x[2], ref[2] = 0.75, -0.5, -1.5, 0.25
+        for k, (a, b) in enumerate(far):
+            x[4 + k], ref[4 + k] = a, b
+        rows, refs, words, acts, old, adv = _one_decision(x.to(dtype), ref.to(dtype), n)
+        one = [t[n // 2:n // 2 + 1] for t in (rows, acts, words, old, adv, refs)]
+        o = oracle.policy(_np(one[0]), one[1].numpy(), one[2].numpy(), _np(one[3]), _np(one[4]), _np(one[5]), None, 0.2, 0.2,
+                          0.25, 0.01)
+        got = policy.policy_loss_and_grad(*(t.to(DEV) for t in (rows, acts, words, old, adv)), ref_logits=refs.to(DEV),
+                                          kl_coef=0.25, entropy_coef=0.01)
+        kl = o["stats"][1] / n
+        # below kLowest / 2 the row is taken in 32 bits as every other: 9 terms, each a few roundings
+        _close(float(got.stats[1]), kl, 50 * H * abs(kl), "kl")
+        info = torch.finfo(dtype)
+        lim = 50 * H * o["size"] + info.eps / 2 * np.abs(o["grad"])
+        _close(_np(got.grad[n // 2]), o["grad"][0] / n, lim[0] / n, "grad")
