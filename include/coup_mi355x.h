@@ -532,8 +532,9 @@ int coup_policy_loss(const coup_decisions* d, const coup_policy_terms* terms, co
  * of -(1 - label_smoothing) log sigmoid(x) - label_smoothing log sigmoid(-x).
  * offsets: 2 * pairs + 1 of int32 or int64 (offset_bytes 4 or 8), ascending,
  * 0..rows; rows outside every sequence get zero gradients.  Offsets that do
- * not ascend make the loss NaN and leave the gradient undefined; none makes
- * the call read or write outside the rows. */
+ * not ascend make the loss NaN and leave the rewards and the gradient
+ * undefined; none makes the call read or write outside the rows, or walk more
+ * of them than a fixed number of times the call's. */
 typedef struct {
   const void* offsets;
   int32_t offset_bytes;

@@ -1121,6 +1121,30 @@ __device__ __forceinline__ int64_t raw_offset(const PreferenceArgs& q, int64_t s
 __device__ __forceinline__ int64_t held(int64_t o, int64_t n) { return o < 0 ? 0 : o > n ? n : o; }
 __device__ __forceinline__ int64_t offset_at(const PreferenceArgs& q, int64_t s) { return held(raw_offset(q, s), q.r.n); }
 
+// The sequence of row i: the last that starts at or before it (the non-empty
+// one where several start there); -1 before the first, 2 pairs behind the last.
+// Offsets that do not ascend give some sequence too, and a later row never an
+// earlier one: searches of two rows part where the earlier one goes left.
+__device__ __forceinline__ int64_t sequence_of(const PreferenceArgs& q, int64_t i) {
+  int64_t lo = 0, hi = 2 * q.pairs + 1;  // offsets[lo - 1] <= i < offsets[hi]
+  while (lo < hi) {
+    const int64_t mid = (lo + hi) >> 1;
+    if (offset_at(q, mid) <= i) lo = mid + 1;
+    else hi = mid;
+  }
+  return lo - 1;
+}
+
+// Whether rows [from, to) are sequences first..last's by that search.  Runs of
+// rows that are belong to different sequences where they do not meet, so those
+// that pass are together no more than the call's rows, whatever the offsets;
+// of ascending offsets every run passes.  Asked for long runs alone: it takes
+// some 20 loads one after another.
+__device__ __forceinline__ bool owned(const PreferenceArgs& q, int64_t from, int64_t to, int64_t first, int64_t last) {
+  return sequence_of(q, from) >= first && sequence_of(q, to - 1) <= last;
+}
+constexpr int kGroupTrusted = 1024, kSliceTrusted = 16384;  // rows of a run that is not asked for
+
 // A pair from its sequences' summed log ratios: its cost, and coef, the
 // derivative in a chosen row's log ratio (a rejected row's is -coef).  NaN
 // where `ok` is false: its offsets do not ascend within the rows.  With
@@ -1235,8 +1259,11 @@ __global__ __launch_bounds__(kRowThreads, AP > 20 ? 2 : FEW ? 4 : sizeof(T) == 2
     const int64_t* o = edge + 2 * threadIdx.x;
     ok = ascending(o[0], o[1], o[2], q.r.n);
   }
-  // a group of bad offsets is not walked: the groups' rows are never more than the call's
-  const bool good = __syncthreads_and(ok);
+  // a group of bad offsets is not walked, nor a long one that is not the rows' (offsets elsewhere do not ascend): the
+  // groups walk 13 times the call's rows and 32 a pair at most
+  bool good = __syncthreads_and(ok);
+  if (good && edge[seqs] - edge[0] > kGroupTrusted)
+    good = owned(q, edge[0], edge[seqs], 2 * pair0, 2 * pair0 + seqs - 1);
   const int64_t begin = good ? edge[0] : 0, end = good ? edge[seqs] : 0;
 
   // a tile's log ratios to its sequences' sums (64 bits across tiles and, for
@@ -1342,8 +1369,10 @@ __global__ __launch_bounds__(kRowThreads) void k_preference_sums(PreferenceArgs 
   const int slice = (int)((int64_t)blockIdx.x % q.slices);
   const int64_t lo = offset_at(q, seq), hi = offset_at(q, seq + 1), len = hi > lo ? hi - lo : 0;
   const int64_t from = lo + len / q.slices * slice + (len % q.slices) * slice / q.slices;
-  const int64_t to = lo + len / q.slices * (slice + 1) + (len % q.slices) * (slice + 1) / q.slices;
+  int64_t to = lo + len / q.slices * (slice + 1) + (len % q.slices) * (slice + 1) / q.slices;
   double s[1] = {0.0};
+  // offsets that do not ascend: the slices walk some 200 times the call's rows at most
+  if (to - from > kSliceTrusted && !owned(q, from, to, seq, seq)) to = from, s[0] = NAN;
 #pragma unroll 4
   for (int64_t i = from + threadIdx.x; i < to; i += kRowThreads) s[0] += (double)q.ratio[i];
   block_sum<kRowThreads, 1>(s, lds);
@@ -1390,14 +1419,8 @@ __global__ __launch_bounds__(kRowThreads) void k_preference_grad(PreferenceArgs 
   uint32_t legal = row_of(q.r, i, (int)threadIdx.x < rows, action);
   float coef = 0.0f;
   if (legal) {
-    // the last sequence that starts at or before row i (the non-empty one where several start there)
-    int64_t lo = 0, hi = 2 * q.pairs + 1;  // offsets[lo - 1] <= i < offsets[hi]
-    while (lo < hi) {
-      const int64_t mid = (lo + hi) >> 1;
-      if (offset_at(q, mid) <= i) lo = mid + 1;
-      else hi = mid;
-    }
-    if (lo >= 1 && lo <= 2 * q.pairs) coef = q.coef[lo - 1];
+    const int64_t seq = sequence_of(q, i);
+    if (seq >= 0 && seq < 2 * q.pairs) coef = q.coef[seq];
     else legal = 0;
   }
   stage<T, AP>(tile, q.r.logits, q.r.stride, row0, rows, q.r.A);

@@ -403,8 +403,8 @@ def preference_loss(logits, actions, legal_mask, offsets, ref_logits=None, beta=
     rewards the loss is the mean over pairs of
         -(1 - label_smoothing) log sigmoid(x) - label_smoothing log sigmoid(-x).
     Sequences may be empty; rows outside every sequence get zero gradients.
-    Offsets that do not ascend within 0..rows make the loss NaN and its
-    gradient undefined."""
+    Offsets that do not ascend within 0..rows make the loss NaN, and rewards
+    and gradient undefined."""
     return PreferenceLoss(*_loss(_preference, logits, actions, legal_mask, offsets, ref_logits, beta, label_smoothing))
 
 

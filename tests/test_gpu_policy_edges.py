@@ -108,3 +108,94 @@ def test_a_references_lowest_values_have_a_finite_kl(n, dtype):
         info = torch.finfo(dtype)
         lim = 50 * H * o["size"] + info.eps / 2 * np.abs(o["grad"])
         _close(_np(got.grad[n // 2]), o["grad"][0] / n, lim[0] / n, "grad")
+
+
+# ------------------------------------------------------------ many sequences
+def _preference64(x, actions, mask, offsets, ref, beta, eps):
+    """oracle.preference over many rows at once (torch, 64 bits), as a dict of the same names."""
+    n, A = x.shape
+    legal = ((mask[:, None] >> torch.arange(A)) & 1).bool() & (mask >= 0)[:, None]
+    a = actions.long()
+    real = (a >= 0) & (a < A) & legal.gather(1, a.clamp(0, A - 1)[:, None])[:, 0]
+    hot = (torch.arange(A) == a[:, None]) & real[:, None]
+
+    def logs(t):
+        return torch.log_softmax(t.double().masked_fill(~legal, -math.inf), 1).masked_fill(~legal | ~real[:, None], 0.0)
+
+    lp = logs(x)
+    ratio = (lp * hot).sum(1) - ((logs(ref) * hot).sum(1) if ref is not None else 0.0)
+    off = torch.as_tensor(offsets)
+    lens = off[1:] - off[:-1]
+    owner = torch.repeat_interleave(torch.arange(lens.numel()), lens)
+    inside = slice(int(off[0]), int(off[-1]))
+    rewards = beta * torch.zeros(lens.numel(), dtype=torch.float64).index_add(0, owner, ratio[inside])
+    m = rewards[0::2] - rewards[1::2]
+    pairs = m.numel()
+    loss = ((1 - eps) * torch.nn.functional.softplus(-m) + eps * torch.nn.functional.softplus(m)).mean()
+    c = (eps - torch.sigmoid(-m)) * beta / pairs
+    coef = torch.zeros(n, dtype=torch.float64)
+    coef[inside] = torch.stack((c, -c), 1).flatten()[owner]
+    p = lp.exp().masked_fill(~legal | ~real[:, None], 0.0)
+    length = torch.zeros(lens.numel(), dtype=torch.float64).index_add(0, owner, real[inside].double())
+    return dict(loss=float(loss), rewards=rewards.numpy(), grad=(coef[:, None] * (hot.double() - p)).numpy(),
+                size=(coef.abs()[:, None] * (hot.double() + p)).numpy(), length=length.numpy())
+
+
+def _many(seed, n, A, dtype, with_ref):
+    """base._table's kinds of rows, 660 of them over and over, with waste of their own."""
+    gen = torch.Generator().manual_seed(seed)
+    x, mask, actions = base._table(gen, 660, A, dtype)
+    k = (n + 659) // 660
+    x, mask, actions = (t.repeat(k, *[1] * (t.dim() - 1))[:n] for t in (x, mask, actions))
+    x = torch.where(torch.isfinite(x.float()), x.float() + torch.randn(n, A, generator=gen), x.float()).to(dtype)
+    ref = (x.float() + 0.5 * torch.randn(n, A, generator=gen)).to(dtype) if with_ref else None
+    return x, mask, actions, ref
+
+
+def test_the_vector_form_is_the_oracle():
+    x, mask, actions, ref = _many(3, 900, 7, torch.float32, True)
+    offsets = [2, 9, 9, 120, 400, 640, 899]
+    for r in (ref, None):
+        want = oracle.preference(_np(x), actions.numpy(), mask.numpy(), offsets, None if r is None else _np(r), 0.2, 0.1)
+        got = _preference64(x, actions, mask, offsets, r, 0.2, 0.1)
+        for k in want:
+            _close(got[k], want[k], 1e-12, k)
+
+
+@pytest.mark.parametrize("n,pairs", [(20000, 400), (70000, 150)], ids=["short", "long"])
+def test_one_long_sequence_among_many(n, pairs):
+    """A sequence of most of the call's rows, which the kernels ask the offsets for, among short ones and empty ones, at
+    the head, in the middle and at the end."""
+    x, mask, actions, ref = _many(n, n, 5, torch.float32, True)
+    short = [0, 3, 11, 0, 7]
+    for at in (0, pairs, 2 * pairs - 1):
+        lens = [short[k % 5] for k in range(2 * pairs)]
+        lens[at] = n - 50 - (sum(lens) - lens[at])
+        offsets = np.concatenate(([20], 20 + np.cumsum(lens)))
+        o = _preference64(x, actions, mask, offsets, ref, 0.01, 0.1)
+        got = policy.preference_loss_and_grad(*(t.to(DEV) for t in (x, actions, mask)), torch.tensor(offsets, device=DEV),
+                                              ref_logits=ref.to(DEV), beta=0.01, label_smoothing=0.1)
+        base._check_preference(got, o, x, mask, 0.01, torch.float32)
+
+
+@pytest.mark.parametrize("pairs", [30000, 24000], ids=["short", "long"])
+@pytest.mark.parametrize("wide", [False, True], ids=["int32", "int64"])
+def test_offsets_that_do_not_ascend_are_not_walked(pairs, wide):
+    """2^22 rows; every other pair is 0, n / 2, n, or every sequence all the rows, so that walking them all would be 10^10
+    rows and more: the loss is NaN, in about the time of a good call's."""
+    n, A = 1 << 22, 2
+    x = torch.zeros(n, A, dtype=torch.float16, device=DEV)
+    words = torch.full((n,), 3, dtype=torch.int32, device=DEV)
+    acts = torch.zeros(n, dtype=torch.int8, device=DEV)
+    good = torch.arange(2 * pairs + 1) * (n // (2 * pairs))
+    alternate = torch.tensor([0, n // 2, n, 0] * (pairs // 2) + [0])
+    whole = torch.tensor([0, n] * pairs + [0])
+    started, ended = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    for offsets in (good, good, alternate, whole, n - whole):
+        off = offsets.to(torch.int64 if wide else torch.int32).to(DEV)
+        started.record()
+        got = policy.preference_loss_and_grad(x, acts, words, off)
+        ended.record()
+        ended.synchronize()
+        assert math.isnan(float(got.loss)) == (offsets is not good)
+        assert started.elapsed_time(ended) < (1000 if offsets is good else 4)
