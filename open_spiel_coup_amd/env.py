@@ -432,6 +432,20 @@ class BatchedCoupEnv:
                 buf["decision_" + k] = torch.empty_like(buf[k])
         return buf
 
+    def _check_policy_buffers(self, buf, steps):
+        may_lack = {"actions", "rewards", *(() if not self.auto_reset else ("step_type",))}
+        for k in ("obs", "info_state"):
+            if k not in buf:  # not recorded: the policy gets them with the first step alone
+                may_lack |= {k, "decision_" + k}
+        for k, like in self.policy_trajectory_buffers(0, values="values" in buf).items():
+            t = buf.get(k)
+            if t is None and k in may_lack:
+                continue
+            if (not isinstance(t, torch.Tensor) or t.dtype != like.dtype or t.device != like.device or t.dim() != like.dim()
+                    or t.shape[0] < steps or t.shape[1:] != like.shape[1:] or (steps and not t[0].is_contiguous())):
+                raise ValueError(f"buf[{k!r}] must be {like.dtype} [{steps}, {', '.join(map(str, like.shape[1:]))}] on "
+                                 f"{like.device}, each step contiguous (policy_trajectory_buffers)")
+
     def collect_policy_trajectory(self, steps, policy, buf=None, generator=None):
         """`steps` env steps played by a policy (collect_trajectory plays the
         uniform one): before each step policy(time_step) gets a dict of
@@ -446,6 +460,8 @@ class BatchedCoupEnv:
         at a chance node (new_initial_state) are skipped: reset them first."""
         from . import policy as ops
         T, dev = int(steps), self.device
+        if buf is not None:
+            self._check_policy_buffers(buf, T)
         now = self.query(obs=self.obs is not None, info_state=self.info_state is not None)
         over = now["terminal"] != 0
         for t in range(T):
@@ -453,6 +469,8 @@ class BatchedCoupEnv:
             logits, values = given if isinstance(given, (tuple, list)) else (given, None)
             if tuple(logits.shape) != (self.batch, NUM_ACTIONS):
                 raise ValueError(f"the policy's logits must be [{self.batch}, {NUM_ACTIONS}], not {tuple(logits.shape)}")
+            if values is not None and tuple(values.shape) != (self.batch,):
+                raise ValueError(f"the policy's values must be [{self.batch}], not {tuple(values.shape)}")
             if buf is None:
                 buf = self.policy_trajectory_buffers(T, values is not None)
             if ("values" in buf) != (values is not None):

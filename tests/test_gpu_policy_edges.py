@@ -9,7 +9,7 @@ import numpy as np
 import pytest
 import torch
 
-from open_spiel_coup_amd import policy
+from open_spiel_coup_amd import BatchedCoupEnv, policy
 from tests import policy_oracle as oracle
 from tests import test_gpu_policy as base
 
@@ -199,3 +199,34 @@ def test_offsets_that_do_not_ascend_are_not_walked(pairs, wide):
         ended.synchronize()
         assert math.isnan(float(got.loss)) == (offsets is not good)
         assert started.elapsed_time(ended) < (1000 if offsets is good else 4)
+
+
+# ------------------------------------------------------------ trajectories
+def test_policy_trajectory_buffers_are_checked_before_a_step():
+    """Buffers that a step would write past, of another type or layout, or missing: refused, the env as it was; longer
+    buffers are filled as far as asked."""
+    B, T = 24, 3
+    env = BatchedCoupEnv(B, seed=6, auto_reset=True, obs=True)
+    logits, values = torch.zeros(B, 18, device=DEV), torch.zeros(B, device=DEV)
+    before = env.export_state().clone()
+    good = env.policy_trajectory_buffers(T)
+    bad = [dict(good, actions=good["actions"][:2]), dict(good, rewards=good["rewards"][:, :8].contiguous()),
+           dict(good, legal_mask=good["legal_mask"].long()), dict(good, obs=good["obs"].half()),
+           dict(good, step_type=good["step_type"].cpu()), dict(good, log_probs=good["log_probs"][0]),
+           dict(good, current_player=good["current_player"].t().contiguous().t()),
+           dict(good, decision_obs=good["obs"][:, :, :1]), {k: v for k, v in good.items() if k != "decision_player"},
+           dict(good, values=torch.zeros(T, B, dtype=torch.float64, device=DEV))]
+    for buf in bad:
+        with pytest.raises(ValueError, match="buf"):
+            env.collect_policy_trajectory(T, lambda ts: logits, buf)
+    for wrong in (values[:1], values[:, None], values.repeat(2)):
+        with pytest.raises(ValueError, match="values must be"):
+            env.collect_policy_trajectory(T, lambda ts: (logits, wrong))
+    assert torch.equal(env.export_state(), before)
+    longer = env.policy_trajectory_buffers(T + 2)
+    longer["actions"].fill_(99)
+    assert env.collect_policy_trajectory(T, lambda ts: logits, longer) is longer
+    assert (longer["actions"][:T] < 18).all() and (longer["actions"][T:] == 99).all()
+    few = {k: good[k] for k in ("legal_mask", "current_player", "decision_mask", "decision_player", "log_probs")}
+    env.collect_policy_trajectory(T, lambda ts: logits, few)  # what else a step writes need not be recorded
+    assert env.error_count() == 0
