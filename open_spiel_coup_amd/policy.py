@@ -22,7 +22,8 @@ whatever the row holds besides; so do logits of actions outside the word.
 Logits are float32, float16 or bfloat16; arithmetic is in 32 bits or more,
 gradients have the logits' type.  Logits may be strided; the other arguments
 are made contiguous.  Nothing but a loss is differentiable, and that in its
-logits.
+logits and in reverse mode: tensors that carry a forward-mode derivative are
+refused.
 
 Everything runs on the tensors' device, on torch's current stream of it,
 without a synchronisation or a memory that outlives the call.  All calls may be
@@ -35,6 +36,7 @@ import ctypes
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _native
@@ -99,6 +101,11 @@ def _enqueue(name, device, *args):
         _native.check(rc)
 
 
+def _is_dual(t):
+    """Whether t carries a forward-mode derivative (none does outside a dual level)."""
+    return forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None
+
+
 def _wrong(t, name, device, shape, dtypes):
     """What is wrong with an argument, as an exception."""
     if not isinstance(t, torch.Tensor):
@@ -115,7 +122,7 @@ def _wrong(t, name, device, shape, dtypes):
 def _arg(t, name, device, shape, dtypes):
     """`t` checked and contiguous."""
     if (not isinstance(t, torch.Tensor) or t.dtype not in dtypes or t.device != device or t.shape != shape
-            or (t.requires_grad and torch.is_grad_enabled())):
+            or (t.requires_grad and torch.is_grad_enabled()) or _is_dual(t)):
         raise _wrong(t, name, device, shape, dtypes)
     return t if t.is_contiguous() else t.contiguous()
 
@@ -126,6 +133,8 @@ def _table(t, name):
         raise ValueError(f"{name} must be a float32, float16 or bfloat16 tensor")
     if not t.is_cuda:
         raise ValueError(f"{name} must be on a HIP device")
+    if _is_dual(t):
+        raise ValueError(f"{name} carries a forward-mode derivative, which these calls do not pass on: detach() it")
     A = t.shape[-1] if t.dim() else 0
     if not 1 <= A <= _native.MAX_POLICY_ACTIONS:
         raise ValueError(f"{name} must have 1..{_native.MAX_POLICY_ACTIONS} actions in the last dimension")
@@ -167,7 +176,7 @@ def _decisions(logits, legal_mask, actions=None, ref_logits=None):
 def _arg_held(t, name, device):
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, not on {device}")
-    if t.requires_grad and torch.is_grad_enabled():
+    if (t.requires_grad and torch.is_grad_enabled()) or _is_dual(t):
         raise ValueError(f"{name} is held constant: detach() it")
 
 
@@ -257,6 +266,8 @@ class _LossOf(torch.autograd.Function):
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("the backward pass of this loss cannot be captured into a graph: capture its "
                                "_and_grad form and hand the gradient on")
+        if _is_dual(incoming):
+            raise ValueError("the loss's derivative carries a forward-mode one, which this backward pass does not pass on")
         grad, ctx.grad = ctx.grad, None
         if grad is None:
             if [t.data_ptr() for t in ctx.saved_tensors] != ctx.at:
@@ -270,8 +281,11 @@ class _LossOf(torch.autograd.Function):
 def _loss(call, logits, *args):
     if not (isinstance(logits, torch.Tensor) and logits.requires_grad and torch.is_grad_enabled()):
         return call(False, logits, *args)[0]
-    if any(isinstance(t, torch.Tensor) and t.requires_grad for t in args):  # unseen inside the function below
+    # unseen inside the function below
+    if any(isinstance(t, torch.Tensor) and (t.requires_grad or _is_dual(t)) for t in args):
         raise ValueError("every argument but logits is held constant: detach() those that require a gradient")
+    if _is_dual(logits):
+        raise ValueError("logits carry a forward-mode derivative, which a loss does not pass on: detach() them")
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError("a loss whose logits require a gradient cannot be captured into a graph: capture its "
                            "_and_grad form and hand the gradient on")

@@ -230,3 +230,41 @@ def test_policy_trajectory_buffers_are_checked_before_a_step():
     few = {k: good[k] for k in ("legal_mask", "current_player", "decision_mask", "decision_player", "log_probs")}
     env.collect_policy_trajectory(T, lambda ts: logits, few)  # what else a step writes need not be recorded
     assert env.error_count() == 0
+
+
+# ------------------------------------------------------------ derivatives
+def test_forward_mode_derivatives_are_refused():
+    """A dual tensor in any place raises, with and without logits that require a gradient, and so does a derivative that
+    comes in as one: their tangents would be lost without a word.  Detached, and outside the dual level, all is as ever."""
+    n, A = 16, 18
+    x, mask, actions, ref, old, adv = (t.to(DEV) for t in base._policy_inputs(2, n, A, torch.float32))
+    off, u = torch.tensor([0, 4, 16], device=DEV), torch.rand(n, device=DEV)
+    window = [t.to(DEV) for t in base._window(torch.Generator().manual_seed(1), 4, 5, 2, torch.float32)]
+    one = torch.ones((), device=DEV)
+    dual = lambda t: torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+    leaf = x.clone().requires_grad_()
+    with torch.autograd.forward_ad.dual_level():
+        for logits in (x, leaf):
+            for call in (lambda x: policy.policy_loss(x, actions, mask, old, adv),
+                         lambda x: policy.preference_loss(x, actions, mask, off)):
+                with pytest.raises(ValueError, match="forward-mode"):
+                    call(dual(logits))
+            for kw in (dict(old_log_probs=dual(old)), dict(advantages=dual(adv)), dict(ref_logits=dual(ref))):
+                with pytest.raises(ValueError, match="forward-mode|held constant"):
+                    policy.policy_loss(logits, actions, mask, **{**dict(old_log_probs=old, advantages=adv), **kw})
+            with pytest.raises(ValueError, match="forward-mode|held constant"):
+                policy.preference_loss(logits, actions, mask, off, ref_logits=dual(ref))
+        for call in (lambda: policy.sample_actions(dual(x), mask, u), lambda: policy.sample_actions(x, mask, dual(u)),
+                     lambda: policy.policy_loss_and_grad(dual(x), actions, mask, old, adv),
+                     lambda: policy.policy_loss_and_grad(x, actions, mask, old, adv, grad_scale=dual(one)),
+                     lambda: policy.preference_loss_and_grad(dual(x), actions, mask, off),
+                     lambda: policy.advantages(*window[:3], dual(window[3]), window[4]),
+                     lambda: policy.advantages(*window[:4], dual(window[4]))):
+            with pytest.raises(ValueError, match="forward-mode|held constant"):
+                call()
+        out = policy.policy_loss(leaf, actions, mask, old, adv)
+        with pytest.raises(ValueError, match="forward-mode"):
+            torch.autograd.grad(out.loss, leaf, dual(one))
+        inside = policy.policy_loss(dual(x).detach(), actions, mask, old, adv)
+        policy.policy_loss(leaf, actions, mask, old, adv, ref_logits=dual(ref).detach()).loss.backward()
+    assert torch.equal(inside.loss, policy.policy_loss(x, actions, mask, old, adv).loss) and leaf.grad is not None
