@@ -33,6 +33,7 @@ run inside a capture): capture the *_and_grad form and hand its gradient on
 (`logits.backward(grad)`).
 """
 import ctypes
+import weakref
 from typing import NamedTuple
 
 import torch
@@ -247,16 +248,18 @@ def advantages(rewards, step_type, players, values, bootstrap=None, gamma=1.0, l
 class _LossOf(torch.autograd.Function):
     """A loss whose call also wrote its gradient: backward hands that out,
     times the incoming derivative (one pass over it in place, or none where it
-    is 1).  A second backward over a retained graph makes the call again, with
-    the derivative as the gradient's factor; so does the first of float16
-    logits, whose range a gradient over many rows needs the factor (a loss
-    scaler's) for before it is rounded."""
+    is 1).  A second backward over a retained graph makes the call again, on
+    the saved arguments and with the derivative as the gradient's factor; so
+    does the first of float16 logits, whose range a gradient over many rows
+    needs the factor (a loss scaler's) for before it is rounded."""
 
     @staticmethod
     def forward(ctx, logits, call, args):
-        out, grad, again, read = call(logits.dtype != torch.float16, logits, *args)
-        ctx.save_for_backward(*read)  # for `again`, which reads them: torch checks their versions there
-        ctx.grad, ctx.again, ctx.at = grad, again, [t.data_ptr() for t in read]
+        out, ctx.grad = call(logits.dtype != torch.float16, logits, *args)
+        tensors = [logits, *(t for t in args if isinstance(t, torch.Tensor))]
+        ctx.save_for_backward(*tensors)
+        ctx.call, ctx.rest = call, [None if isinstance(t, torch.Tensor) else (t,) for t in args]
+        ctx.given = [(weakref.ref(t), t.data_ptr()) for t in tensors]
         ctx.mark_non_differentiable(*out[1:])
         return out
 
@@ -270,9 +273,13 @@ class _LossOf(torch.autograd.Function):
             raise ValueError("the loss's derivative carries a forward-mode one, which this backward pass does not pass on")
         grad, ctx.grad = ctx.grad, None
         if grad is None:
-            if [t.data_ptr() for t in ctx.saved_tensors] != ctx.at:
-                raise RuntimeError("an argument of this loss was given other data since")
-            return ctx.again(incoming), None, None
+            logits, *held = ctx.saved_tensors  # torch checks their versions; hooks may hand out equal ones instead
+            for t, (given, at) in zip((logits, *held), ctx.given):
+                if t is given() and t.data_ptr() != at:
+                    raise RuntimeError("an argument of this loss was given other data since")
+            held = iter(held)
+            args = [next(held) if c is None else c[0] for c in ctx.rest]
+            return ctx.call(True, logits, *args, grad_scale=incoming, alone=True)[1], None, None
         scale = incoming.contiguous()
         _enqueue("coup_scale_grad", grad.device, grad.data_ptr(), _DTYPES[grad.dtype], grad.numel(), scale.data_ptr())
         return grad, None, None
@@ -292,23 +299,9 @@ def _loss(call, logits, *args):
     return _LossOf.apply(logits, call, args)
 
 
-def _again(name, outputs, d, terms, nbytes, shape, dtype, device):
-    """The call `name` once more, for its gradient times a factor.  Holds no
-    tensor: those that d and terms point into are its caller's to keep."""
-    def call(factor):
-        grad = torch.empty(shape, dtype=dtype, device=device)
-        loss = torch.empty((), dtype=torch.float32, device=device)
-        scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        out = outputs(loss=loss.data_ptr(), grad=grad.data_ptr(), grad_scale=factor.data_ptr())
-        _enqueue(name, device, ctypes.byref(d), ctypes.byref(terms), ctypes.byref(out), scratch.data_ptr(), nbytes)
-        return grad
-    return call
-
-
 def _policy(want_grad, logits, actions, legal_mask, old_log_probs, advantages, ref_logits, active, clip_low, clip_high,
-            kl_coef, entropy_coef, grad_scale=None):
-    """((loss, stats, count, log_probs), gradient or None, the call for a
-    gradient with a factor alone, the tensors that it reads)"""
+            kl_coef, entropy_coef, grad_scale=None, alone=False):
+    """((loss, stats, count, log_probs), gradient or None); `alone`: the loss and the gradient only"""
     d, keep = _decisions(logits, legal_mask, actions, ref_logits)
     lead, device = logits.shape[:-1], logits.device
     old = _arg(old_log_probs, "old_log_probs", device, lead, _FLOAT32)
@@ -323,19 +316,16 @@ def _policy(want_grad, logits, actions, legal_mask, old_log_probs, advantages, r
     terms = _native.PolicyTerms(old.data_ptr(), adv.data_ptr(), None if act is None else act.data_ptr(), clip_low,
                                 clip_high, kl_coef, entropy_coef)
     loss = torch.empty((), dtype=torch.float32, device=device)
-    stats = torch.empty(4, dtype=torch.float32, device=device)
-    count = torch.empty((), dtype=torch.int64, device=device)
-    log_probs = torch.empty_like(old)
+    stats = None if alone else torch.empty(4, dtype=torch.float32, device=device)
+    count = None if alone else torch.empty((), dtype=torch.int64, device=device)
+    log_probs = None if alone else torch.empty_like(old)
     grad = torch.empty(logits.shape, dtype=logits.dtype, device=device) if want_grad else None
     nbytes = _native.load().coup_policy_workspace(d.rows)
     scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    out = _native.PolicyOutputs(loss.data_ptr(), stats.data_ptr(), count.data_ptr(), log_probs.data_ptr(),
-                                None if grad is None else grad.data_ptr(),
-                                None if factor is None else factor.data_ptr())
+    out = _native.PolicyOutputs(*[None if t is None else t.data_ptr() for t in (loss, stats, count, log_probs, grad, factor)])
     _enqueue("coup_policy_loss", device, ctypes.byref(d), ctypes.byref(terms), ctypes.byref(out), scratch.data_ptr(),
              nbytes)
-    again = _again("coup_policy_loss", _native.PolicyOutputs, d, terms, nbytes, logits.shape, logits.dtype, device)
-    return (loss, stats, count, log_probs), grad, again, [t for t in (*keep, old, adv, act) if t is not None]
+    return (loss, stats, count, log_probs), grad
 
 
 def policy_loss(logits, actions, legal_mask, old_log_probs, advantages, ref_logits=None, active=None, clip_low=0.2,
@@ -368,13 +358,14 @@ def policy_loss_and_grad(logits, actions, legal_mask, old_log_probs, advantages,
     autograd (hand the gradient on with logits.backward(grad)).  grad_scale
     (0-d float32): what the gradient is multiplied by before it is rounded to
     the logits' type (a loss scaler's factor)."""
-    out, grad, *_ = _policy(True, logits, actions, legal_mask, old_log_probs, advantages, ref_logits, active, clip_low,
+    out, grad = _policy(True, logits, actions, legal_mask, old_log_probs, advantages, ref_logits, active, clip_low,
                         clip_high, kl_coef, entropy_coef, grad_scale)
     return PolicyLossAndGrad(*out, grad)
 
 
-def _preference(want_grad, logits, actions, legal_mask, offsets, ref_logits, beta, label_smoothing, grad_scale=None):
-    """((loss, rewards), gradient or None, and as _policy)"""
+def _preference(want_grad, logits, actions, legal_mask, offsets, ref_logits, beta, label_smoothing, grad_scale=None,
+                alone=False):
+    """((loss, rewards), gradient or None), as _policy"""
     if not isinstance(logits, torch.Tensor) or logits.dim() != 2:
         raise ValueError("logits must be [rows, A]: the sequences' decisions one after another")
     d, keep = _decisions(logits, legal_mask, actions, ref_logits)
@@ -391,16 +382,14 @@ def _preference(want_grad, logits, actions, legal_mask, offsets, ref_logits, bet
         raise ValueError("label_smoothing must be in 0..0.5")
     terms = _native.PreferenceTerms(off.data_ptr(), off.element_size(), pairs, beta, label_smoothing)
     loss = torch.empty((), dtype=torch.float32, device=device)
-    rewards = torch.empty(2 * pairs, dtype=torch.float32, device=device)
+    rewards = None if alone else torch.empty(2 * pairs, dtype=torch.float32, device=device)
     grad = torch.empty(logits.shape, dtype=logits.dtype, device=device) if want_grad else None
     nbytes = _native.load().coup_preference_workspace(d.rows, pairs)
     scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    out = _native.PreferenceOutputs(loss.data_ptr(), rewards.data_ptr(), None if grad is None else grad.data_ptr(),
-                                    None if factor is None else factor.data_ptr())
+    out = _native.PreferenceOutputs(*[None if t is None else t.data_ptr() for t in (loss, rewards, grad, factor)])
     _enqueue("coup_preference_loss", device, ctypes.byref(d), ctypes.byref(terms), ctypes.byref(out),
              scratch.data_ptr(), nbytes)
-    again = _again("coup_preference_loss", _native.PreferenceOutputs, d, terms, nbytes, logits.shape, logits.dtype, device)
-    return (loss, rewards), grad, again, [t for t in (*keep, off) if t is not None]
+    return (loss, rewards), grad
 
 
 def preference_loss(logits, actions, legal_mask, offsets, ref_logits=None, beta=0.1,
@@ -427,5 +416,5 @@ def preference_loss_and_grad(logits, actions, legal_mask, offsets, ref_logits=No
     """preference_loss and its gradient in the logits in one call, outside
     autograd (hand the gradient on with logits.backward(grad)).  grad_scale: as
     in policy_loss_and_grad."""
-    out, grad, *_ = _preference(True, logits, actions, legal_mask, offsets, ref_logits, beta, label_smoothing, grad_scale)
+    out, grad = _preference(True, logits, actions, legal_mask, offsets, ref_logits, beta, label_smoothing, grad_scale)
     return PreferenceLossAndGrad(*out, grad)

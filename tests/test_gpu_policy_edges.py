@@ -8,6 +8,7 @@ import math
 import numpy as np
 import pytest
 import torch
+import torch.utils.checkpoint
 
 from open_spiel_coup_amd import BatchedCoupEnv, policy
 from tests import policy_oracle as oracle
@@ -268,3 +269,37 @@ def test_forward_mode_derivatives_are_refused():
         inside = policy.policy_loss(dual(x).detach(), actions, mask, old, adv)
         policy.policy_loss(leaf, actions, mask, old, adv, ref_logits=dual(ref).detach()).loss.backward()
     assert torch.equal(inside.loss, policy.policy_loss(x, actions, mask, old, adv).loss) and leaf.grad is not None
+
+
+@pytest.mark.parametrize("dtype", base.DTYPES, ids=lambda d: str(d)[6:])
+@pytest.mark.parametrize("hooks", ["save_on_cpu", "clone", "checkpoint"])
+def test_losses_under_saved_tensor_hooks(hooks, dtype):
+    """Hooks that hand out equal tensors at other addresses (and of other strides), and a checkpoint that computes them
+    again: the gradients without hooks, in the first backward pass and in a second one."""
+    n, A = 300, 18
+    x, mask, actions, ref, old, adv = (t.to(DEV) for t in base._policy_inputs(7, n, A, dtype))
+    off = torch.tensor([0, 30, 100, 180, 300], device=DEV)
+    wide = torch.zeros(n, 40, dtype=dtype, device=DEV)
+    wide[:, 3:21] = x
+    twice = [t.repeat_interleave(2)[::2] for t in (actions, mask, old, adv)]
+
+    def both(table):
+        logits = table[:, 3:21]
+        return (policy.policy_loss(logits, *twice, ref_logits=ref, kl_coef=0.1).loss
+                + policy.preference_loss(logits, twice[0], twice[1], off, ref_logits=ref).loss)
+
+    def gradients(call):
+        leaf = wide.clone().requires_grad_()
+        loss = call(leaf)
+        return [torch.autograd.grad(loss, leaf, retain_graph=True)[0] for _ in range(2)]
+
+    want = gradients(both)
+    assert want[0].any() and torch.equal(want[0], want[1])
+    if hooks == "checkpoint":
+        got = gradients(lambda t: torch.utils.checkpoint.checkpoint(both, t, use_reentrant=False))
+    else:
+        with (torch.autograd.graph.save_on_cpu() if hooks == "save_on_cpu" else
+              torch.autograd.graph.saved_tensors_hooks(torch.clone, torch.clone)):
+            got = gradients(both)
+    for g in got:
+        assert torch.equal(g, want[0])
