@@ -325,9 +325,13 @@ __device__ __forceinline__ float log_ratio(float a, float b) { return log1p_any(
 struct Softmax {
   float m;    // largest logit
   float sum;  // sum of e
-  float lse;  // log of the sum (precise only): log p_a = (x_a - m) - lse
+  float others;  // sum of the e's fractions, that is without the ones (PRECISE alone)
+  float lse;  // log of the sum (PRECISE alone): log p_a = (x_a - m) - lse
   __device__ __forceinline__ float e(float logit) const { return __builtin_amdgcn_exp2f((logit - m) * kLog2e); }
   __device__ __forceinline__ float t(float logit) const { return max_of(logit - m, kLowest); }
+  // The sum without one of the e's: 1 - p_a is rest / sum, which keeps its
+  // digits where p_a is nearly 1 (its e is 1 and the only one).  PRECISE alone.
+  __device__ __forceinline__ float rest(float one) const { return one == 1.0f && sum - others < 1.5f ? others : sum - one; }
 };
 
 template <int AP>
@@ -347,21 +351,21 @@ __device__ __forceinline__ float lse_of(float sum, float others) {
 
 // e = exp(x - m), and x becomes t = x - m held above -inf, so that e t is 0
 // where e is; a NaN or +inf logit makes the sum NaN.  The sum is at least 1,
-// the largest logit's own e.  PRECISE: also lse.
+// the largest logit's own e.  PRECISE: also others and lse.
 template <bool PRECISE, int AP>
 __device__ __forceinline__ Softmax softmax(float (&x)[AP], float (&e)[AP]) {
   Softmax s;
   s.m = row_max<AP>(x);
   s.sum = 0.0f;
-  float others = 0.0f;
+  s.others = 0.0f;
 #pragma unroll
   for (int a = 0; a < AP; ++a) {
     e[a] = s.e(x[a]);
     x[a] = s.t(x[a]);
     s.sum += e[a];
-    if (PRECISE) others += __builtin_amdgcn_fractf(e[a]);
+    if (PRECISE) s.others += __builtin_amdgcn_fractf(e[a]);
   }
-  s.lse = PRECISE ? lse_of(s.sum, others) : 0.0f;
+  s.lse = PRECISE ? lse_of(s.sum, s.others) : 0.0f;
   return s;
 }
 
@@ -951,7 +955,7 @@ __global__ __launch_bounds__(kRowThreads, AP <= 20 ? 4 : 2) void k_policy_loss(P
   }
   float x[AP], d[AP], xa, rta = 0.0f;  // d: the reference's t, rta the action's
   bool far = false;
-  Softmax rs{0.0f, 1.0f, 0.0f};
+  Softmax rs{0.0f, 1.0f, 0.0f, 0.0f};
   stage_rows<T, AP, REF>(
       tile, q.r, row0, rows, legal, action, d,
       [&](float(&row)[AP], float one) {
@@ -966,19 +970,19 @@ __global__ __launch_bounds__(kRowThreads, AP <= 20 ? 4 : 2) void k_policy_loss(P
   if (legal) {
     // x becomes t
     float e[AP];
-    const Softmax s = softmax<false, AP>(x, e);
+    const Softmax s = softmax<true, AP>(x, e);
     float et = 0.0f, ed = 0.0f;  // sums of e t and e (t - t_ref)
 #pragma unroll
     for (int a = 0; a < AP; ++a) {
       et += e[a] * x[a];
       if (REF) ed += e[a] * (x[a] - d[a]);
     }
-    const float inv = __builtin_amdgcn_rcpf(s.sum), lse = log_of(s.sum);
+    const float inv = __builtin_amdgcn_rcpf(s.sum);
     et *= inv, ed *= inv;
-    entropy = lse - et;
+    entropy = s.lse - et;
     if (REF) kl = ed - log_ratio(s.sum, rs.sum);
     m = s.m;
-    logp = (xa - s.m) - lse;
+    logp = (xa - s.m) - s.lse;
     const float dl = logp - old, border = adv > 0.0f ? q.log_high : q.log_low;
     bool over = adv > 0.0f ? dl > border : dl < border;
     float rho = exp_of(dl);
@@ -988,7 +992,8 @@ __global__ __launch_bounds__(kRowThreads, AP <= 20 ? 4 : 2) void k_policy_loss(P
       const double top = exp((double)xa - (double)s.m - (double)old);
       over = adv > 0.0f ? top > q.high * whole : top < q.low * whole;
       rho = (float)(top / whole);
-      if (q.few) logp = (xa - s.m) - lse_of((float)whole, (float)(whole - 1.0));
+      // (whole - 1 has an error of 2^-53: from 2^-32 down the fractions' sum is the better one)
+      if (q.few) logp = (xa - s.m) - (s.rest(1.0f) < 2.3283064e-10f ? s.lse : lse_of((float)whole, (float)(whole - 1.0)));
     }
     over = over && adv != 0.0f;
     surrogate = adv == 0.0f ? 0.0f : -(over ? (float)(adv > 0.0f ? q.high : q.low) : rho) * adv;
@@ -1000,10 +1005,12 @@ __global__ __launch_bounds__(kRowThreads, AP <= 20 ? 4 : 2) void k_policy_loss(P
       // (the factor, which has no bound, meets p_b and not the coefficients
       // that kLowest is held for)
       const float share = inv * scale, ct = REF ? q.ent + q.kl : q.ent, cr = REF ? q.kl : 0.0f;
-      const float base = cr * (et - ed) - ct * et - w;
+      const float held = cr * (et - ed) - ct * et, base = held - w;
 #pragma unroll
       for (int a = 0; a < AP; ++a) x[a] = (e[a] * share) * (ct * x[a] + (REF ? base - cr * d[a] : base));
-      ga = (s.e(xa) * share) * (ct * s.t(xa) + (REF ? base - cr * rta : base)) + w * scale;
+      // the action's own: w (1 - p_a) apart, of the other actions' e
+      const float ea = s.e(xa);
+      ga = (ea * share) * (ct * s.t(xa) + (REF ? held - cr * rta : held)) + (w * s.rest(ea)) * share;
       if (!(fabsf(base) < 1e30f)) {  // else 0 times it is 0 at the actions outside the word
 #pragma unroll
         for (int a = 0; a < AP; ++a) x[a] = keep(legal, a, x[a], 0.0f);
@@ -1174,13 +1181,13 @@ __device__ __forceinline__ bool ascending(int64_t a, int64_t b, int64_t c, int64
   return a >= 0 && b >= a && c >= b && c <= n;
 }
 
-// A tile's rows: this thread's log ratio, its e, the action's and their sum.
+// A tile's rows: this thread's log ratio, its e, their sum, and that without the action's.
 template <class T, int AP, bool REF, bool FEW>
 __device__ __forceinline__ float row_ratio(char* tile, const PreferenceArgs& q, int64_t row0, int rows, uint32_t legal,
-                                           int action, float (&e)[AP], float& ea, float& sum) {
+                                           int action, float (&e)[AP], float& rest, float& sum) {
   float x[AP], d[AP], xa, out = 0.0f, one = 0.0f;
   double whole = 1.0;
-  Softmax rs{0.0f, 1.0f, 0.0f};
+  Softmax rs{0.0f, 1.0f, 0.0f, 0.0f};
   stage_rows<T, AP, REF>(
       tile, q.r, row0, rows, legal, action, d,
       [&](float(&row)[AP], float taken) {
@@ -1191,9 +1198,9 @@ __device__ __forceinline__ float row_ratio(char* tile, const PreferenceArgs& q, 
       },
       x, xa);
   sum = 1.0f;
-  ea = 0.0f;
+  rest = 0.0f;
   if (legal) {
-    const Softmax s = softmax<false, AP>(x, e);
+    const Softmax s = softmax<true, AP>(x, e);
     // the two sums' logs as one, of a ratio near 1
     out = REF ? (xa - s.m) - (one - rs.m) : xa - s.m;
     if (FEW) {
@@ -1201,21 +1208,21 @@ __device__ __forceinline__ float row_ratio(char* tile, const PreferenceArgs& q, 
     } else {
       out -= REF ? log_ratio(s.sum, rs.sum) : log_of(s.sum);
     }
-    ea = s.e(xa);
+    rest = s.rest(s.e(xa));
     sum = s.sum;
   }
   return out;
 }
 
-// The gradient of a tile's rows: coef ([b = action] - e_b / sum).
+// The gradient of a tile's rows: coef ([b = action] - e_b / sum), the action's own as coef rest / sum.
 template <class T, int AP>
 __device__ __forceinline__ void row_grad(char* tile, const PreferenceArgs& q, int64_t row0, int rows, uint32_t legal,
-                                         int action, float (&e)[AP], float ea, float sum, float coef) {
+                                         int action, float (&e)[AP], float rest, float sum, float coef) {
   const float p = -coef / sum;
 #pragma unroll
   for (int a = 0; a < AP; ++a) e[a] = keep(legal, a, p * e[a], 0.0f);
   Tile<T, AP>::write(tile, q.r.A, e);
-  if (legal) Tile<T, AP>::write_one(tile, q.r.A, action, p * ea + coef);
+  if (legal) Tile<T, AP>::write_one(tile, q.r.A, action, -p * rest);
   __syncthreads();
   Tile<T, AP>::copy_out(tile, (T*)q.grad, row0, rows, q.r.A);
 }
@@ -1310,22 +1317,22 @@ __global__ __launch_bounds__(kRowThreads, AP > 20 ? 2 : FEW ? 4 : sizeof(T) == 2
     return lo < seqs ? coef[lo] : 0.0f;
   };
 
-  float e[AP], ea, total;
+  float e[AP], rest, total;
   int action;
   if (end - begin <= kRowThreads) {
     const int64_t i = begin + threadIdx.x;
     const int rows = end > begin ? (int)(end - begin) : 0;
     const uint32_t legal = row_of(q.r, i, (int)threadIdx.x < rows, action);
-    ratio[threadIdx.x] = row_ratio<T, AP, REF, FEW>(tile, q, begin, rows, legal, action, e, ea, total);
+    ratio[threadIdx.x] = row_ratio<T, AP, REF, FEW>(tile, q, begin, rows, legal, action, e, rest, total);
     add_tile(begin, rows);
     close_pairs();
-    if (q.grad) row_grad<T, AP>(tile, q, begin, rows, legal, action, e, ea, total, coef_of(i));
+    if (q.grad) row_grad<T, AP>(tile, q, begin, rows, legal, action, e, rest, total, coef_of(i));
     return;
   }
   for (int64_t row0 = begin; row0 < end; row0 += kRowThreads) {
     const int rows = (int)(end - row0 < kRowThreads ? end - row0 : kRowThreads);
     const uint32_t legal = row_of(q.r, row0 + threadIdx.x, (int)threadIdx.x < rows, action);
-    ratio[threadIdx.x] = row_ratio<T, AP, REF, FEW>(tile, q, row0, rows, legal, action, e, ea, total);
+    ratio[threadIdx.x] = row_ratio<T, AP, REF, FEW>(tile, q, row0, rows, legal, action, e, rest, total);
     add_tile(row0, rows);
   }
   close_pairs();
@@ -1339,8 +1346,8 @@ __global__ __launch_bounds__(kRowThreads, AP > 20 ? 2 : FEW ? 4 : sizeof(T) == 2
     float x[AP];
     Tile<T, AP>::read(tile, q.r.A, legal, x);
     const float xa = Tile<T, AP>::read_one(tile, q.r.A, action);
-    const Softmax sm = softmax<false, AP>(x, e);
-    row_grad<T, AP>(tile, q, row0, rows, legal, action, e, sm.e(xa), sm.sum, coef_of(i));
+    const Softmax sm = softmax<true, AP>(x, e);
+    row_grad<T, AP>(tile, q, row0, rows, legal, action, e, sm.rest(sm.e(xa)), sm.sum, coef_of(i));
     __syncthreads();
   }
 }
@@ -1358,8 +1365,8 @@ __global__ __launch_bounds__(kRowThreads) void k_preference_rows(PreferenceArgs 
   const bool mine = (int)threadIdx.x < rows;
   int action;
   const uint32_t legal = row_of(q.r, i, mine, action);
-  float e[AP], ea, total;
-  const float out = row_ratio<T, AP, REF, FEW>(tile, q, row0, rows, legal, action, e, ea, total);
+  float e[AP], rest, total;
+  const float out = row_ratio<T, AP, REF, FEW>(tile, q, row0, rows, legal, action, e, rest, total);
   if (mine) q.ratio[i] = out;
 }
 
@@ -1428,8 +1435,8 @@ __global__ __launch_bounds__(kRowThreads) void k_preference_grad(PreferenceArgs 
   float x[AP], e[AP];
   Tile<T, AP>::read(tile, q.r.A, legal, x);
   const float xa = Tile<T, AP>::read_one(tile, q.r.A, action);
-  const Softmax sm = softmax<false, AP>(x, e);
-  row_grad<T, AP>(tile, q, row0, rows, legal, action, e, sm.e(xa), sm.sum, coef);
+  const Softmax sm = softmax<true, AP>(x, e);
+  row_grad<T, AP>(tile, q, row0, rows, legal, action, e, sm.rest(sm.e(xa)), sm.sum, coef);
 }
 
 // The blocks' costs in a fixed order.

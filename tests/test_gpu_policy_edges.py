@@ -303,3 +303,57 @@ def test_losses_under_saved_tensor_hooks(hooks, dtype):
             got = gradients(both)
     for g in got:
         assert torch.equal(g, want[0])
+
+
+# ------------------------------------------------------------ nearly sure decisions
+def _sure(seed, n, A, dtype):
+    """Rows whose acted action is 10 to 20 above all others, two of them legal at least."""
+    gen = torch.Generator().manual_seed(seed)
+    actions = torch.randint(A, (n,), generator=gen)
+    legal = torch.rand(n, A, generator=gen) < 0.5
+    row = torch.arange(n)
+    legal[row, actions] = legal[row, (actions + 1) % A] = True
+    x = 3.0 - 10.0 - 10.0 * torch.rand(n, A, generator=gen)
+    x[row, actions] = 3.0
+    mask = (legal.long() << torch.arange(A)).sum(1).to(torch.int32)
+    return x.to(dtype), mask, actions.to(torch.int8)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=lambda d: str(d)[6:])
+@pytest.mark.parametrize("A", [4, 18, 31])
+@pytest.mark.parametrize("times", [1, 30, 170], ids=lambda k: f"{400 * k} rows")
+def test_nearly_sure_decisions_keep_their_digits(times, A, dtype):
+    """1 - p of 1e-3 to 1e-9: the log probability and every gradient entry, the acted action's too, to the softmax's
+    relative error (the logits' z = 20) of themselves.  Ratios of about 1 and a surrogate weight of either sign; pairs of
+    short sequences, and one pair of long ones."""
+    n, z = 400, 20
+    x, mask, actions = _sure(A, n, A, dtype)
+    old, adv = torch.full((n,), -0.01), torch.where(torch.arange(n) % 2 == 0, 1.0, -0.5)
+    o = oracle.policy(_np(x), actions.numpy(), mask.numpy(), _np(old), _np(adv), None, None, 0.2, 0.2, 0.0, 0.05)
+    assert -A * math.exp(-10) < o["log_probs"].min() and o["log_probs"].max() < 0  # A - 1 others of e^-10 at most
+    info, rel = torch.finfo(dtype), 8 * (48 + 2 * z) * H
+    many = lambda t: t.to(DEV).repeat(times, *[1] * (t.dim() - 1))  # noqa: E731
+    xm, am, mm = many(x), many(actions), many(mask)
+    got = policy.policy_loss_and_grad(xm, am, mm, many(old), many(adv), entropy_coef=0.05)
+    where = slice((times - 1) * n, times * n)
+    _close(got.log_probs[where].cpu().numpy(), o["log_probs"], rel * np.abs(o["log_probs"]), "log_probs")
+    want = o["grad"] / times
+    _close(_np(got.grad[where]), want, (rel + info.eps / 2) * np.abs(want) + info.smallest_normal * info.eps, "policy grad")
+    u = torch.full((n * times,), 0.5, device=DEV)
+    acts, lp = policy.sample_actions(xm, mm, u)
+    assert torch.equal(acts, am)
+    _close(lp[where].cpu().numpy(), o["log_probs"], rel * np.abs(o["log_probs"]), "sample's log_probs")
+    short = [n * k // 8 for k in range(9)]
+    for offsets in ([*(r * n + v for r in range(times) for v in short[:-1]), times * n], [0, times * n // 2, times * n]):
+        o = _preference64(x.repeat(times, 1), actions.repeat(times), mask.repeat(times), offsets, None, 0.1, 0.1)
+        got = policy.preference_loss_and_grad(xm, am, mm, torch.tensor(offsets, device=DEV), label_smoothing=0.1)
+        # 1 - p of the vector form's own log_softmax is good to 2^-53 of 1 only
+        p = x.repeat(times, 1).double().masked_fill(((mask.repeat(times)[:, None] >> torch.arange(A)) & 1) == 0, -math.inf)
+        p = torch.softmax(p, 1).numpy()
+        acted = np.arange(A) == actions.repeat(times).numpy()[:, None]
+        rest = np.where(acted, 0.0, p).sum(1)
+        want = np.where(acted, -(o["grad"] * ~acted).sum(1, keepdims=True), o["grad"])
+        assert (rest > 1e-10).all() and np.abs(want[acted]).min() > 0
+        # the pair's weight moves by its difference's error, beta * rows * 32-bit roundings of a log ratio near 0
+        lim = (rel + 0.1 * o["length"].max() * 8 * H + info.eps / 2) * np.abs(want) + info.smallest_normal * info.eps
+        _close(_np(got.grad), want, lim, "preference grad")
