@@ -39,6 +39,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kRowThreads = 256;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+constexpr float kLog2eLow = 1.925963033500576e-08f;  // what kLog2e rounds off
 // Stands for -inf in products with a 0 share: 1e4 (the largest coefficient of
 // the loss) times it is still finite.  Rows where a reference's logit is that
 // far below its largest at an action with a share are taken again (far_row).
@@ -306,8 +307,8 @@ __device__ __forceinline__ float max_of(float a, float b) { return __builtin_ele
 // The hardware's base-2 logarithm, exponential and reciprocal, each good to
 // a unit in the last place.
 __device__ __forceinline__ float log_of(float v) { return __builtin_amdgcn_logf(v) * kLn2; }  // v >= 1, or of a ratio
-__device__ __forceinline__ float exp_of(float v) {  // the product's rounding is made good
-  const float hi = v * kLog2e, lo = __builtin_fmaf(v, kLog2e, -hi);
+__device__ __forceinline__ float exp_of(float v) {  // the product's rounding, and the constant's, are made good
+  const float hi = v * kLog2e, lo = __builtin_fmaf(v, kLog2eLow, __builtin_fmaf(v, kLog2e, -hi));
   const float e = __builtin_amdgcn_exp2f(hi);
   return e < INFINITY && lo == lo ? __builtin_fmaf(e * lo, kLn2, e) : e;  // 0 and inf as they are
 }

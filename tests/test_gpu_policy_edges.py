@@ -357,3 +357,20 @@ def test_nearly_sure_decisions_keep_their_digits(times, A, dtype):
         # the pair's weight moves by its difference's error, beta * rows * 32-bit roundings of a log ratio near 0
         lim = (rel + 0.1 * o["length"].max() * 8 * H + info.eps / 2) * np.abs(want) + info.smallest_normal * info.eps
         _close(_np(got.grad), want, lim, "preference grad")
+
+
+def test_a_very_sure_pairs_small_loss():
+    """Pairs 40 to 85 apart, where the constant's part that log2(e) rounds off weighs 85 * 1.3e-8: e^-x to a few 2^-24.
+    The rows' other action is 40 below or more: its e leaves no trace in the log probabilities, which are then 32-bit
+    numbers, and their 64-bit sums are exact."""
+    depth = torch.tensor([40.0, 55.5, 70.25, 84.875])
+    x = torch.zeros(8, 2)
+    x[1::2, 1] = -depth  # the rejected row takes it; the chosen one is certain
+    actions = (torch.arange(8) % 2).to(torch.int8)
+    mask = torch.tensor([1, 3] * 4, dtype=torch.int32)
+    for k in range(4):
+        off = torch.tensor([2 * k, 2 * k + 1, 2 * k + 2], device=DEV)
+        got = policy.preference_loss_and_grad(x.to(DEV), actions.to(DEV), mask.to(DEV), off, beta=1.0)
+        want = math.exp(-float(depth[k]))
+        assert abs(float(got.loss) / want - 1) <= 8 * H
+        assert abs(float(got.grad[2 * k + 1, 1]) / want - 1) <= 16 * H
