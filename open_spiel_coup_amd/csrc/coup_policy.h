@@ -1012,7 +1012,7 @@ __global__ __launch_bounds__(kRowThreads, AP <= 20 ? 4 : 2) void k_policy_loss(P
       // the action's own: w (1 - p_a) apart, of the other actions' e
       const float ea = s.e(xa);
       ga = (ea * share) * (ct * s.t(xa) + (REF ? held - cr * rta : held)) + (w * s.rest(ea)) * share;
-      if (!(fabsf(base) < 1e30f)) {  // else 0 times it is 0 at the actions outside the word
+      if (!(fabsf(base) < 1e30f && fabsf(scale) < INFINITY)) {  // else 0 times them is 0 at the actions outside the word
 #pragma unroll
         for (int a = 0; a < AP; ++a) x[a] = keep(legal, a, x[a], 0.0f);
       }
@@ -1457,13 +1457,13 @@ __global__ __launch_bounds__(kFinishThreads) void k_preference_finish(const doub
 // came in: nothing is read or written where that is 1, as in loss.backward()
 // (1.9 us, a launch).  A second rounding, at most another half step; nothing
 // for a power of two, unless the first one was to a half's smallest steps,
-// which is what grad_scale is for.
+// which is what grad_scale is for.  What is 0 stays it, whatever came in.
 template <class T>
 __global__ __launch_bounds__(kRowThreads) void k_scale_grad(T* grad, int64_t n, const float* __restrict__ scale) {
   const float g = *scale;
   if (g == 1.0f) return;
   for (int64_t i = (int64_t)blockIdx.x * kRowThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kRowThreads)
-    grad[i] = (T)(g * (float)grad[i]);
+    if (const float v = (float)grad[i]; v != 0.0f) grad[i] = (T)(g * v);
 }
 
 // ---------------------------------------------------------------- launch

@@ -374,3 +374,28 @@ def test_a_very_sure_pairs_small_loss():
         want = math.exp(-float(depth[k]))
         assert abs(float(got.loss) / want - 1) <= 8 * H
         assert abs(float(got.grad[2 * k + 1, 1]) / want - 1) <= 16 * H
+
+
+@pytest.mark.parametrize("dtype", base.DTYPES, ids=lambda d: str(d)[6:])
+@pytest.mark.parametrize("scale", [math.inf, math.nan])
+def test_masked_entries_stay_zero_under_a_scale_without_bound(scale, dtype):
+    """A loss scaler's infinite factor, or a NaN that comes in: rows that do not count and actions outside the word get 0
+    all the same, the others something that is no number."""
+    n, A = 200, 18
+    x, mask, actions, ref, old, adv = (t.to(DEV) for t in base._policy_inputs(9, n, A, dtype))
+    x[0] = torch.arange(A, device=DEV) / 4  # a row of the loss whose every legal action has a share
+    mask[0], actions[0], old[0], adv[0], ref[0] = 0x155, 2, -1.5, 1.0, 0.0
+    off = torch.tensor([0, 20, 60, 90, 180], device=DEV)
+    factor = torch.tensor(scale, device=DEV)
+    kw = dict(ref_logits=ref, kl_coef=0.1, entropy_coef=0.01)
+    legal = ((mask[:, None] >> torch.arange(A, device=DEV)) & 1).bool() & (mask >= 0)[:, None]
+    counts = legal.gather(1, actions.long().clamp(0, A - 1)[:, None])[:, 0] & (actions >= 0) & (actions < A)
+    live = legal & counts[:, None]
+    leaf = x.clone().requires_grad_()
+    for loss, both in ((lambda t, **k: policy.policy_loss(t, actions, mask, old, adv, **kw),
+                        lambda t, **k: policy.policy_loss_and_grad(t, actions, mask, old, adv, **kw, **k)),
+                       (lambda t, **k: policy.preference_loss(t, actions, mask, off, ref_logits=ref),
+                        lambda t, **k: policy.preference_loss_and_grad(t, actions, mask, off, ref_logits=ref, **k))):
+        first = torch.autograd.grad(loss(leaf).loss, leaf, factor)[0]
+        for g in (first, both(x, grad_scale=factor).grad):
+            assert not g[~live].any() and not torch.isfinite(g[0][live[0]]).any()
