@@ -102,6 +102,14 @@ def _enqueue(name, device, *args):
         _native.check(rc)
 
 
+def _capturing(device):
+    """Whether torch's current stream of `device` (which need not be the current one) is being captured."""
+    if device.index == torch._C._cuda_getDevice():
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(device):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def _is_dual(t):
     """Whether t carries a forward-mode derivative (none does outside a dual level)."""
     return forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None
@@ -266,7 +274,7 @@ class _LossOf(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, incoming, *_):
-        if torch.cuda.is_current_stream_capturing():
+        if _capturing(incoming.device):
             raise RuntimeError("the backward pass of this loss cannot be captured into a graph: capture its "
                                "_and_grad form and hand the gradient on")
         if _is_dual(incoming):
@@ -293,7 +301,7 @@ def _loss(call, logits, *args):
         raise ValueError("every argument but logits is held constant: detach() those that require a gradient")
     if _is_dual(logits):
         raise ValueError("logits carry a forward-mode derivative, which a loss does not pass on: detach() them")
-    if torch.cuda.is_current_stream_capturing():
+    if logits.is_cuda and _capturing(logits.device):
         raise RuntimeError("a loss whose logits require a gradient cannot be captured into a graph: capture its "
                            "_and_grad form and hand the gradient on")
     return _LossOf.apply(logits, call, args)

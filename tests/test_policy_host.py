@@ -204,3 +204,26 @@ def test_python_refuses_host_tensors():
     with pytest.raises(ValueError, match="HIP device"):
         policy.advantages(torch.zeros(2, 3, 2, dtype=torch.int8), torch.zeros(2, 3, dtype=torch.uint8),
                           torch.zeros(2, 3, dtype=torch.int8), torch.zeros(2, 3))
+
+
+def test_a_capture_is_looked_for_on_the_tensors_device(monkeypatch):
+    """The stream that counts is the current one of the logits' device, also where another device is current."""
+    current, captured = [0], {1}
+
+    class Guard:
+        def __init__(self, device):
+            self.index = device.index
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.index
+
+        def __exit__(self, *_):
+            current[0] = self.before
+
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: current[0], raising=False)
+    monkeypatch.setattr(torch.cuda, "device", Guard)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: current[0] in captured)
+    assert policy._capturing(torch.device("cuda", 1)) and not policy._capturing(torch.device("cuda", 0))
+    current[0] = 1
+    assert policy._capturing(torch.device("cuda", 1)) and not policy._capturing(torch.device("cuda", 0))
+    assert current[0] == 1
