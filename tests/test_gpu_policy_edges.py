@@ -399,3 +399,60 @@ def test_masked_entries_stay_zero_under_a_scale_without_bound(scale, dtype):
         first = torch.autograd.grad(loss(leaf).loss, leaf, factor)[0]
         for g in (first, both(x, grad_scale=factor).grad):
             assert not g[~live].any() and not torch.isfinite(g[0][live[0]]).any()
+
+
+# ------------------------------------------------------------ forms that larger calls take
+@pytest.mark.parametrize("dtype", base.DTYPES, ids=lambda d: str(d)[6:])
+@pytest.mark.parametrize("A", [5, 16, 18, 31])
+@pytest.mark.parametrize("with_ref", [True, False], ids=["ref", "none"])
+def test_short_sequences_of_many_rows(with_ref, A, dtype):
+    """More than 16,384 rows in short sequences (32-bit sums within a tile): groups of one tile and of several, empty
+    sequences, rows outside every one; the loss alone, with its gradient and through autograd."""
+    pairs = 300
+    x, mask, actions, ref = _many(A, 18003, A, dtype, with_ref)
+    gen = torch.Generator().manual_seed(A)
+    lens = torch.randint(0, 55, (2 * pairs,), generator=gen)
+    lens[100], lens[301], lens[302], lens[7:12] = 300, 700, 520, 0
+    offsets = (11 + torch.cat((torch.zeros(1, dtype=torch.int64), lens.cumsum(0)))).tolist()
+    assert 16384 < offsets[-1] < 18000 and 18003 // pairs <= 160
+    o = _preference64(x, actions, mask, offsets, ref, 0.05, 0.1)
+    args = [t.to(DEV) for t in (actions, mask)] + [torch.tensor(offsets, device=DEV)]
+    kw = dict(ref_logits=None if ref is None else ref.to(DEV), beta=0.05, label_smoothing=0.1)
+    got = policy.preference_loss_and_grad(x.to(DEV), *args, **kw)
+    base._check_preference(got, o, x, mask, 0.05, dtype)
+    assert not got.grad[:11].any() and not got.grad[offsets[-1]:].any()
+    leaf = x.to(DEV).requires_grad_()
+    out = policy.preference_loss(leaf, *args, **kw)
+    grad, = torch.autograd.grad(out.loss, leaf)
+    only = policy.preference_loss(x.to(DEV), *args, **kw)
+    for a, b in zip((out.loss, out.rewards, grad, only.loss, only.rewards), (*got, got.loss, got.rewards)):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("cuts", [0, 1, 3])
+@pytest.mark.parametrize("T,B,P", [(2305, 9, 2), (5000, 130, 2), (700, 250, 6), (500, 1500, 2), (300, 5, 3), (1000, 600, 6),
+                                   (257, 2100, 2), (130, 8000, 4), (4000, 300, 2), (70, 33000, 2), (200, 16500, 3),
+                                   (9, 140000, 2), (40, 140000, 2)])
+def test_what_lies_far_behind_reaches_every_step(T, B, P, cuts):
+    """gamma = lam = 1: an advantage is every reward up to the lane's next cut (or the bootstrap) less the value, however
+    many rounds behind a block's part they lie.  Whole rewards, values in eighths: every sum is exact in 32 bits
+    (3 T + 4 < 2^17), so is the comparison."""
+    gen = torch.Generator().manual_seed(T + B + cuts)
+    st = torch.ones(T, B, dtype=torch.uint8)
+    lane = torch.arange(B)
+    for k in range(cuts):
+        st[torch.randint(0, T, (B,), generator=gen), lane] = 2 if k != 1 else 0
+    pl = torch.randint(0, P, (T, B), generator=gen).to(torch.int8)
+    r = torch.randint(-3, 4, (T, B, P), generator=gen).to(torch.int8)
+    v = torch.randint(-32, 33, (T, B), generator=gen).float() / 8
+    b = torch.randint(-32, 33, (B, P), generator=gen).float() / 8
+    togo, want = b.clone(), torch.zeros(T, B)
+    for t in range(T - 1, -1, -1):
+        togo[st[t] != 1] = 0
+        togo += r[t] * (st[t] != 0)[:, None]
+        want[t] = torch.where(st[t] != 0, togo[lane, pl[t].long()], 0.0)
+    for dtype in (torch.float32, torch.bfloat16):
+        adv, target = policy.advantages(r.to(DEV), st.to(DEV), pl.to(DEV), v.to(dtype).to(DEV), b.to(dtype).to(DEV),
+                                        gamma=1.0, lam=1.0)
+        assert torch.equal(target.cpu(), want)
+        assert torch.equal(adv.cpu(), torch.where(st != 0, want - v, 0.0))
