@@ -219,7 +219,8 @@ def advantages(rewards, step_type, players, values, bootstrap=None, gamma=1.0, l
     acts in step t (the current player before it); values [T, B] (float32,
     float16 or bfloat16): that player's value of the state it acts in;
     bootstrap [B, P], values' type: each player's value of the state behind
-    the window (None: 0).  Each player's decisions are one chain: its rewards
+    the window, e.g. a critic's of the last step's obs [B, P, ...] (None: 0,
+    which takes games that are still open there to be worth nothing).  Each player's decisions are one chain: its rewards
     up to its next decision, that one's value discounted by gamma, advantages
     decayed by gamma * lam; a LAST step ends every chain, a FIRST step cuts.
     Returns (advantages, targets = advantages + values), float32 [T, B], 0 at

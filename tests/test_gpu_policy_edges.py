@@ -456,3 +456,42 @@ def test_what_lies_far_behind_reaches_every_step(T, B, P, cuts):
                                         gamma=1.0, lam=1.0)
         assert torch.equal(target.cpu(), want)
         assert torch.equal(adv.cpu(), torch.where(st != 0, want - v, 0.0))
+
+
+# ------------------------------------------------------------ the documented round
+@pytest.mark.parametrize("auto_reset", [True, False])
+def test_a_round_with_open_games(auto_reset):
+    """The guide's policy update: acting seats' observations, and the last step's as each seat's bootstrap for the games
+    left open; advantages and loss against the oracle."""
+    B, T = 40, 30
+    env = BatchedCoupEnv(B, seed=5, auto_reset=auto_reset, obs=True, num_players=3)
+    torch.manual_seed(1)
+    model = torch.nn.Linear(env.obs_size, 18 + 1, device=DEV)
+
+    def act(ts):
+        seat = ts["current_player"].long().clamp(min=0)
+        out = model(ts["obs"][torch.arange(env.batch, device=env.device), seat]).detach()
+        return out[:, :18], out[:, 18]
+
+    buf = env.collect_policy_trajectory(T, act)
+    bootstrap = model(buf["obs"][-1])[..., 18].detach()
+    assert bootstrap.shape == (B, 3)
+    given = (buf["rewards"], buf["step_type"], buf["decision_player"], buf["values"])
+    adv, target = policy.advantages(*given, bootstrap, gamma=0.99)
+    want, _ = oracle.advantages(*(t.cpu().numpy() for t in given[:3]), _np(buf["values"]), _np(bootstrap), 0.99, 0.95)
+    # sums of at most T terms, below T (3 + 2 * 4) in size, 4 roundings a term
+    _close(adv.cpu().numpy(), want, 4 * T * H * T * 11, "advantages")
+    unopened = policy.advantages(*given, gamma=0.99)[0]
+    still = buf["step_type"][-1] == 1
+    assert still.any() and (unopened - adv)[-1][still].abs().max() > 0.01
+    seat = buf["decision_player"].long().clamp(min=0)[:, :, None, None].expand(-1, -1, 1, env.obs_size)
+    logits = model(buf["decision_obs"].gather(2, seat)[:, :, 0])[..., :18]
+    kw = dict(kl_coef=0.05, ref_logits=logits.detach() * 0.9, active=buf["decision_player"] == 0)
+    out = policy.policy_loss(logits, buf["actions"], buf["decision_mask"], buf["log_probs"], adv, **kw)
+    out.loss.backward()
+    flat = lambda t: _np(t).reshape(T * B, -1).squeeze()  # noqa: E731
+    o = oracle.policy(flat(logits), flat(buf["actions"]), buf["decision_mask"].flatten().cpu().numpy(), flat(buf["log_probs"]),
+                      flat(adv), flat(kw["ref_logits"]), flat(kw["active"]) > 0, 0.2, 0.2, 0.05, 0.0)
+    assert int(out.count) == o["count"] > 0 and torch.isfinite(model.weight.grad).all() and model.weight.grad.any()
+    z = base._reach(logits.detach().reshape(T * B, 18).cpu(), buf["decision_mask"].flatten().cpu())
+    assert abs(float(out.loss.detach()) - o["loss"]) <= 8 * (48 + 2 * z) * H * (o["mass"].sum() + 3 * z)
