@@ -495,3 +495,60 @@ def test_a_round_with_open_games(auto_reset):
     assert int(out.count) == o["count"] > 0 and torch.isfinite(model.weight.grad).all() and model.weight.grad.any()
     z = base._reach(logits.detach().reshape(T * B, 18).cpu(), buf["decision_mask"].flatten().cpu())
     assert abs(float(out.loss.detach()) - o["loss"]) <= 8 * (48 + 2 * z) * H * (o["mass"].sum() + 3 * z)
+
+
+@pytest.mark.parametrize("auto_reset", [True, False])
+def test_policy_trajectory_of_information_states(auto_reset):
+    """An env that writes information states: each decision's is the state's before the step, and what the policy got; a
+    lane whose logits are no numbers is skipped."""
+    B, T = 50, 12
+    kw = dict(seed=3, auto_reset=auto_reset, obs=False, info_state=True, history=True)
+    env, ref = BatchedCoupEnv(B, **kw), BatchedCoupEnv(B, **kw)
+    seen = []
+
+    def act(ts):
+        assert "obs" not in ts
+        seen.append(ts["info_state"].clone())
+        logits = torch.zeros(B, 18, device=DEV)
+        logits[7] = math.nan
+        return logits
+
+    buf = env.collect_policy_trajectory(T, act, generator=torch.Generator(DEV).manual_seed(1))
+    now = ref.query(obs=False, info_state=True)
+    for t in range(T):
+        assert torch.equal(buf["decision_info_state"][t], now["info_state"]) and torch.equal(seen[t], now["info_state"])
+        over = now["terminal"].bool()
+        ref.step(buf["actions"][t].masked_fill(over, 0))
+        now = ref.query(obs=False, info_state=True)
+    assert (buf["actions"][:, 7] == -1).all() and (buf["step_type"][:, 7] == 3).all() and buf["log_probs"][:, 7].isnan().all()
+    assert torch.equal(env.export_state(), ref.export_state()) and env.error_count() == 0
+
+
+@pytest.mark.parametrize("dtype", base.DTYPES, ids=lambda d: str(d)[6:])
+def test_excluded_actions_in_strided_tables_and_graphs(dtype):
+    """Rows whose reference excludes an action the policy takes, in strided tables, captured and replayed: the contiguous,
+    eager call's results."""
+    n, A = 700, 18
+    x, mask, actions, ref, old, adv = (t.to(DEV) for t in base._policy_inputs(13, n, A, dtype))
+    rows = torch.arange(n, device=DEV)
+    ref[rows[::3], rows[::3] % A] = -math.inf
+    ref[rows[1::3], rows[1::3] % A] = torch.finfo(dtype).min
+    wide = torch.zeros(n, 2, 41, dtype=dtype, device=DEV)
+    wide[:, 0, 5:23], wide[:, 1, 3:21] = x, ref
+    kw = dict(kl_coef=0.1, entropy_coef=0.01)
+    want = policy.policy_loss_and_grad(x, actions, mask, old, adv, ref_logits=ref, **kw)
+    # a row whose one legal action the reference excludes has no reference at all: NaN, and so is the mean
+    assert math.isnan(float(want.loss)) and want.grad.isnan().any() and (want.grad == 0).any()
+    strided = lambda: policy.policy_loss_and_grad(wide[:, 0, 5:23], actions, mask, old, adv,  # noqa: E731
+                                                  ref_logits=wide[:, 1, 3:21], **kw)
+    held = [strided()]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held.append(strided())
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        for got in held:
+            for a, b in zip(got, want):
+                assert torch.equal(a.nan_to_num(5), b.nan_to_num(5))
