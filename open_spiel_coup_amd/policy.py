@@ -110,9 +110,11 @@ def _capturing(device):
         return torch.cuda.is_current_stream_capturing()
 
 
-def _is_dual(t):
-    """Whether t carries a forward-mode derivative (none does outside a dual level)."""
-    return forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None
+def _refuse_duals(*args):
+    """Raise where an argument carries a forward-mode derivative (asked for inside a dual level alone)."""
+    for t in args:
+        if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+            raise ValueError("a tensor carries a forward-mode derivative, which these calls do not pass on: detach() it")
 
 
 def _wrong(t, name, device, shape, dtypes):
@@ -131,7 +133,7 @@ def _wrong(t, name, device, shape, dtypes):
 def _arg(t, name, device, shape, dtypes):
     """`t` checked and contiguous."""
     if (not isinstance(t, torch.Tensor) or t.dtype not in dtypes or t.device != device or t.shape != shape
-            or (t.requires_grad and torch.is_grad_enabled()) or _is_dual(t)):
+            or (t.requires_grad and torch.is_grad_enabled())):
         raise _wrong(t, name, device, shape, dtypes)
     return t if t.is_contiguous() else t.contiguous()
 
@@ -142,8 +144,6 @@ def _table(t, name):
         raise ValueError(f"{name} must be a float32, float16 or bfloat16 tensor")
     if not t.is_cuda:
         raise ValueError(f"{name} must be on a HIP device")
-    if _is_dual(t):
-        raise ValueError(f"{name} carries a forward-mode derivative, which these calls do not pass on: detach() it")
     A = t.shape[-1] if t.dim() else 0
     if not 1 <= A <= _native.MAX_POLICY_ACTIONS:
         raise ValueError(f"{name} must have 1..{_native.MAX_POLICY_ACTIONS} actions in the last dimension")
@@ -185,7 +185,7 @@ def _decisions(logits, legal_mask, actions=None, ref_logits=None):
 def _arg_held(t, name, device):
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, not on {device}")
-    if (t.requires_grad and torch.is_grad_enabled()) or _is_dual(t):
+    if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} is held constant: detach() it")
 
 
@@ -200,6 +200,8 @@ def sample_actions(logits, legal_mask, uniform):
     (actions int8 [...], log_probs float32 [...]).  A row without a legal
     action gives -1 (which `BatchedCoupEnv.step` skips) and 0; one with a NaN
     or +inf logit at a legal action, or only -inf ones, gives -1 and NaN."""
+    if forward_ad._current_level >= 0:
+        _refuse_duals(logits, legal_mask, uniform)
     d, keep = _decisions(logits, legal_mask)
     device = logits.device
     u = _arg(uniform, "uniform", device, logits.shape[:-1], _FLOAT32)
@@ -230,6 +232,8 @@ def advantages(rewards, step_type, players, values, bootstrap=None, gamma=1.0, l
     device = values.device
     if device.type != "cuda":
         raise ValueError("values must be on a HIP device")
+    if forward_ad._current_level >= 0:
+        _refuse_duals(rewards, step_type, players, values, bootstrap)
     _arg_held(values, "values", device)
     if values.dim() != 2:
         raise ValueError("values must be [T, B]")
@@ -263,54 +267,73 @@ class _LossOf(torch.autograd.Function):
     needs the factor (a loss scaler's) for before it is rounded."""
 
     @staticmethod
-    def forward(ctx, logits, call, args):
-        out, ctx.grad = call(logits.dtype != torch.float16, logits, *args)
-        tensors = [logits, *(t for t in args if isinstance(t, torch.Tensor))]
-        ctx.save_for_backward(*tensors)
-        ctx.call, ctx.rest = call, [None if isinstance(t, torch.Tensor) else (t,) for t in args]
-        ctx.given = [(weakref.ref(t), t.data_ptr()) for t in tensors]
+    def forward(ctx, logits, call, tensors, numbers):
+        out, ctx.grad, again, read = call(logits.dtype != torch.float16, logits, *tensors, *numbers)
+        ctx.save_for_backward(logits, *tensors)
+        given = [(weakref.ref(t), t.data_ptr()) for t in (logits, *tensors) if t is not None]
+        # a call to come for sure may take this one's addresses, where these are the arguments' own and still hold
+        as_given = ctx.grad is None and {t.data_ptr() for t in read} <= {at for _, at in given}
+        ctx.later = call, numbers, given, again if as_given else None
         ctx.mark_non_differentiable(*out[1:])
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, incoming, *_):
-        if _capturing(incoming.device):
+        if torch.cuda.is_current_stream_capturing():  # this thread's device is the incoming derivative's
             raise RuntimeError("the backward pass of this loss cannot be captured into a graph: capture its "
                                "_and_grad form and hand the gradient on")
-        if _is_dual(incoming):
-            raise ValueError("the loss's derivative carries a forward-mode one, which this backward pass does not pass on")
+        if forward_ad._current_level >= 0:
+            _refuse_duals(incoming)
         grad, ctx.grad = ctx.grad, None
-        if grad is None:
-            logits, *held = ctx.saved_tensors  # torch checks their versions; hooks may hand out equal ones instead
-            for t, (given, at) in zip((logits, *held), ctx.given):
-                if t is given() and t.data_ptr() != at:
-                    raise RuntimeError("an argument of this loss was given other data since")
-            held = iter(held)
-            args = [next(held) if c is None else c[0] for c in ctx.rest]
-            return ctx.call(True, logits, *args, grad_scale=incoming, alone=True)[1], None, None
-        scale = incoming.contiguous()
-        _enqueue("coup_scale_grad", grad.device, grad.data_ptr(), _DTYPES[grad.dtype], grad.numel(), scale.data_ptr())
-        return grad, None, None
+        if grad is not None:
+            scale = incoming.contiguous()
+            _enqueue("coup_scale_grad", grad.device, grad.data_ptr(), _DTYPES[grad.dtype], grad.numel(), scale.data_ptr())
+            return grad, None, None, None
+        call, numbers, given, again = ctx.later
+        saved = ctx.saved_tensors  # torch checks their versions
+        for t, (one, at) in zip([t for t in saved if t is not None], given):
+            if t is not one():
+                again = None  # a hook's equal one
+            elif t.data_ptr() != at:
+                raise RuntimeError("an argument of this loss was given other data since")
+        grad = again(incoming) if again is not None else call(True, *saved, *numbers, grad_scale=incoming)[1]
+        return grad, None, None, None
 
 
-def _loss(call, logits, *args):
+def _loss(call, logits, tensors, numbers):
+    if forward_ad._current_level >= 0:
+        _refuse_duals(logits, *tensors)
     if not (isinstance(logits, torch.Tensor) and logits.requires_grad and torch.is_grad_enabled()):
-        return call(False, logits, *args)[0]
-    # unseen inside the function below
-    if any(isinstance(t, torch.Tensor) and (t.requires_grad or _is_dual(t)) for t in args):
-        raise ValueError("every argument but logits is held constant: detach() those that require a gradient")
-    if _is_dual(logits):
-        raise ValueError("logits carry a forward-mode derivative, which a loss does not pass on: detach() them")
+        return call(False, logits, *tensors, *numbers)[0]
+    for t in tensors:  # unseen inside the function below
+        if isinstance(t, torch.Tensor) and t.requires_grad:
+            raise ValueError("every argument but logits is held constant: detach() those that require a gradient")
     if logits.is_cuda and _capturing(logits.device):
         raise RuntimeError("a loss whose logits require a gradient cannot be captured into a graph: capture its "
                            "_and_grad form and hand the gradient on")
-    return _LossOf.apply(logits, call, args)
+    return _LossOf.apply(logits, call, tensors, numbers)
+
+
+def _again(name, outputs, d, terms, nbytes, logits):
+    """The call `name` once more, for its gradient times a factor.  Holds no
+    tensor: those that d and terms point into are its caller's to keep."""
+    shape, dtype, device = logits.shape, logits.dtype, logits.device
+
+    def call(factor):
+        grad = torch.empty(shape, dtype=dtype, device=device)
+        loss = torch.empty((), dtype=torch.float32, device=device)
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        out = outputs(loss=loss.data_ptr(), grad=grad.data_ptr(), grad_scale=factor.data_ptr())
+        _enqueue(name, device, ctypes.byref(d), ctypes.byref(terms), ctypes.byref(out), scratch.data_ptr(), nbytes)
+        return grad
+    return call
 
 
 def _policy(want_grad, logits, actions, legal_mask, old_log_probs, advantages, ref_logits, active, clip_low, clip_high,
-            kl_coef, entropy_coef, grad_scale=None, alone=False):
-    """((loss, stats, count, log_probs), gradient or None); `alone`: the loss and the gradient only"""
+            kl_coef, entropy_coef, grad_scale=None):
+    """((loss, stats, count, log_probs), gradient or None, the call for a
+    gradient with a factor alone, the tensors that it reads)"""
     d, keep = _decisions(logits, legal_mask, actions, ref_logits)
     lead, device = logits.shape[:-1], logits.device
     old = _arg(old_log_probs, "old_log_probs", device, lead, _FLOAT32)
@@ -325,16 +348,17 @@ def _policy(want_grad, logits, actions, legal_mask, old_log_probs, advantages, r
     terms = _native.PolicyTerms(old.data_ptr(), adv.data_ptr(), None if act is None else act.data_ptr(), clip_low,
                                 clip_high, kl_coef, entropy_coef)
     loss = torch.empty((), dtype=torch.float32, device=device)
-    stats = None if alone else torch.empty(4, dtype=torch.float32, device=device)
-    count = None if alone else torch.empty((), dtype=torch.int64, device=device)
-    log_probs = None if alone else torch.empty_like(old)
+    stats = torch.empty(4, dtype=torch.float32, device=device)
+    count = torch.empty((), dtype=torch.int64, device=device)
+    log_probs = torch.empty_like(old)
     grad = torch.empty(logits.shape, dtype=logits.dtype, device=device) if want_grad else None
     nbytes = _native.load().coup_policy_workspace(d.rows)
     scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
     out = _native.PolicyOutputs(*[None if t is None else t.data_ptr() for t in (loss, stats, count, log_probs, grad, factor)])
     _enqueue("coup_policy_loss", device, ctypes.byref(d), ctypes.byref(terms), ctypes.byref(out), scratch.data_ptr(),
              nbytes)
-    return (loss, stats, count, log_probs), grad
+    again = _again("coup_policy_loss", _native.PolicyOutputs, d, terms, nbytes, logits)
+    return (loss, stats, count, log_probs), grad, again, [t for t in (*keep, old, adv, act) if t is not None]
 
 
 def policy_loss(logits, actions, legal_mask, old_log_probs, advantages, ref_logits=None, active=None, clip_low=0.2,
@@ -356,8 +380,8 @@ def policy_loss(logits, actions, legal_mask, old_log_probs, advantages, ref_logi
     probability (a logit of -inf) and the policy some (a logit within 745 of
     the row's largest) makes the KL infinite, and with a kl_coef its row's
     gradient NaN."""
-    return PolicyLoss(*_loss(_policy, logits, actions, legal_mask, old_log_probs, advantages, ref_logits, active,
-                             clip_low, clip_high, kl_coef, entropy_coef))
+    return PolicyLoss(*_loss(_policy, logits, (actions, legal_mask, old_log_probs, advantages, ref_logits, active),
+                             (float(clip_low), float(clip_high), float(kl_coef), float(entropy_coef))))
 
 
 def policy_loss_and_grad(logits, actions, legal_mask, old_log_probs, advantages, ref_logits=None, active=None,
@@ -367,14 +391,15 @@ def policy_loss_and_grad(logits, actions, legal_mask, old_log_probs, advantages,
     autograd (hand the gradient on with logits.backward(grad)).  grad_scale
     (0-d float32): what the gradient is multiplied by before it is rounded to
     the logits' type (a loss scaler's factor)."""
-    out, grad = _policy(True, logits, actions, legal_mask, old_log_probs, advantages, ref_logits, active, clip_low,
+    if forward_ad._current_level >= 0:
+        _refuse_duals(logits, old_log_probs, advantages, ref_logits, grad_scale)
+    out, grad, *_ = _policy(True, logits, actions, legal_mask, old_log_probs, advantages, ref_logits, active, clip_low,
                         clip_high, kl_coef, entropy_coef, grad_scale)
     return PolicyLossAndGrad(*out, grad)
 
 
-def _preference(want_grad, logits, actions, legal_mask, offsets, ref_logits, beta, label_smoothing, grad_scale=None,
-                alone=False):
-    """((loss, rewards), gradient or None), as _policy"""
+def _preference(want_grad, logits, actions, legal_mask, offsets, ref_logits, beta, label_smoothing, grad_scale=None):
+    """((loss, rewards), gradient or None, and as _policy)"""
     if not isinstance(logits, torch.Tensor) or logits.dim() != 2:
         raise ValueError("logits must be [rows, A]: the sequences' decisions one after another")
     d, keep = _decisions(logits, legal_mask, actions, ref_logits)
@@ -391,14 +416,15 @@ def _preference(want_grad, logits, actions, legal_mask, offsets, ref_logits, bet
         raise ValueError("label_smoothing must be in 0..0.5")
     terms = _native.PreferenceTerms(off.data_ptr(), off.element_size(), pairs, beta, label_smoothing)
     loss = torch.empty((), dtype=torch.float32, device=device)
-    rewards = None if alone else torch.empty(2 * pairs, dtype=torch.float32, device=device)
+    rewards = torch.empty(2 * pairs, dtype=torch.float32, device=device)
     grad = torch.empty(logits.shape, dtype=logits.dtype, device=device) if want_grad else None
     nbytes = _native.load().coup_preference_workspace(d.rows, pairs)
     scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
     out = _native.PreferenceOutputs(*[None if t is None else t.data_ptr() for t in (loss, rewards, grad, factor)])
     _enqueue("coup_preference_loss", device, ctypes.byref(d), ctypes.byref(terms), ctypes.byref(out),
              scratch.data_ptr(), nbytes)
-    return (loss, rewards), grad
+    again = _again("coup_preference_loss", _native.PreferenceOutputs, d, terms, nbytes, logits)
+    return (loss, rewards), grad, again, [t for t in (*keep, off) if t is not None]
 
 
 def preference_loss(logits, actions, legal_mask, offsets, ref_logits=None, beta=0.1,
@@ -417,7 +443,8 @@ def preference_loss(logits, actions, legal_mask, offsets, ref_logits=None, beta=
     Sequences may be empty; rows outside every sequence get zero gradients.
     Offsets that do not ascend within 0..rows make the loss NaN, and rewards
     and gradient undefined."""
-    return PreferenceLoss(*_loss(_preference, logits, actions, legal_mask, offsets, ref_logits, beta, label_smoothing))
+    return PreferenceLoss(*_loss(_preference, logits, (actions, legal_mask, offsets, ref_logits),
+                                 (float(beta), float(label_smoothing))))
 
 
 def preference_loss_and_grad(logits, actions, legal_mask, offsets, ref_logits=None, beta=0.1, label_smoothing=0.0,
@@ -425,5 +452,7 @@ def preference_loss_and_grad(logits, actions, legal_mask, offsets, ref_logits=No
     """preference_loss and its gradient in the logits in one call, outside
     autograd (hand the gradient on with logits.backward(grad)).  grad_scale: as
     in policy_loss_and_grad."""
-    out, grad = _preference(True, logits, actions, legal_mask, offsets, ref_logits, beta, label_smoothing, grad_scale)
+    if forward_ad._current_level >= 0:
+        _refuse_duals(logits, ref_logits, grad_scale)
+    out, grad, *_ = _preference(True, logits, actions, legal_mask, offsets, ref_logits, beta, label_smoothing, grad_scale)
     return PreferenceLossAndGrad(*out, grad)
