@@ -887,7 +887,7 @@ __device__ __forceinline__ void far_row(const Rows& r, int64_t i, uint32_t legal
 // Up to this many rows every row's ratio is taken in 64 bits, not only those
 // by a border: a loss of few terms that nearly cancel keeps its digits (over
 // many rows the 32-bit roundings average out).  A call of 65,536 float rows
-// takes 14.0 us, one of 65,537 13.0.
+// takes 14.6 us, one of 65,537 13.4.
 constexpr int64_t kFewRows = 65536;
 constexpr int kCountBlocks = 256, kCountThreads = 1024, kFinishThreads = 512;
 
@@ -923,8 +923,8 @@ __global__ __launch_bounds__(kCountThreads) void k_policy_count(PolicyArgs q) {
 
 // Loss and gradient in one pass, a tile a block: the tables are read once and
 // the gradient written once.  4 x 2^20 float rows with a reference (961 MB)
-// take 177 us, 5.4 TB/s; 1.3 M bf16 rows (165 MB) 39.7 us, 4.2 TB/s, bound by
-// what four blocks a CU keep in flight (864 vector instructions a wave are 30
+// take 177 us, 5.4 TB/s; 1.3 M bf16 rows (165 MB) 42 us, 3.9 TB/s, bound by
+// what four blocks a CU keep in flight (970 vector instructions a wave are 32
 // us of it).  Four is what up to 128 registers allow; held to five the compiler
 // spills, and 1.3 M rows took 65 us for 52 a call.
 template <class T, int AP, bool REF>
@@ -1234,7 +1234,7 @@ __device__ __forceinline__ void row_grad(char* tile, const PreferenceArgs& q, in
 // costs follow, and the gradient is written from the e still in registers.
 // A group of more rows goes through its tiles twice.  Blocks past the groups
 // write the zero gradients of the rows outside every sequence.
-// 8192 pairs over 327,680 bf16 rows (37 MB) take 23.5 us, bound by a block's
+// 8192 pairs over 327,680 bf16 rows (37 MB) take 24.6 us, bound by a block's
 // latency: its steps wait for one another.  Groups of 120, 160 and 200 rows
 // come to the same.
 constexpr int kMaxGroup = 32, kZeroBlocks = 64;
@@ -1356,8 +1356,8 @@ __global__ __launch_bounds__(kRowThreads, AP > 20 ? 2 : FEW ? 4 : sizeof(T) == 2
 // Long sequences: every row's log ratio to memory, the sequences' sums from
 // slices of them, the pairs, then the gradient with the logits read again
 // (A sizeof(T) of a row's 3 A sizeof(T) + 5 bytes).  8 pairs over 1.5 M float
-// rows: 34.9 us for the rows (229 MB, 6.5 TB/s, partly cached), 6.8 and 4.6 for
-// the sums and pairs, 34.1 for the gradient (223 MB).
+// rows: 35.0 us for the rows (229 MB, 6.5 TB/s, partly cached), 6.7 and 4.6 for
+// the sums and pairs, 34.0 for the gradient (223 MB).
 template <class T, int AP, bool REF, bool FEW>
 __global__ __launch_bounds__(kRowThreads) void k_preference_rows(PreferenceArgs q) {
   __shared__ __align__(16) char tile[Tile<T, AP>::kBytes];
@@ -1597,14 +1597,15 @@ inline void launch_policy(PolicyArgs q, int dtype, double kl, double ent, float*
 // groups spill into a second; else a sequence's sum takes a block per 4096
 // rows of the average one.
 // Few rows' sums are taken in 64 bits, as the policy loss's (kFewRows): the
-// short form's up to a quarter of them (16,384 rows 18.3 us, 16,385 13.8; at
-// 65,536 it would be 22 for 15), the long form's up to all (19.6, 17.2).
+// short form's up to a quarter of them (16,384 rows 18.6 us, 16,385 13.8; at
+// 65,536 it would be 21 for 15), the long form's up to all (20.2, 17.5).
 // A short block has 32 pairs or 81 rows and more on average, a long sequence
 // more than 80, so the calls the entries take (COUP_MAX_DECISIONS,
 // COUP_MAX_PAIRS) launch fewer than 2^32 threads.  One sequence far longer than
-// its call's average keeps one block busy, 256 of its rows at a time.
-// On either side of kShortRows, 2^19 bf16 rows, us: 40 rows a pair short 34,
-// long 66; 150 41, 44; 300 39, 40; 1000 98, 37.
+// its call's average keeps one block busy, 256 of its rows at a time (2^20
+// rows, 8192 pairs: 53 us; with one sequence of 65,536 rows 1290).
+// On either side of kShortRows, 2^19 bf16 rows, us: 40 rows a pair short 35,
+// long 66; 150 43, 44; 165 41, 43; 300 44, 40; 1000 103, 37.
 constexpr int kShortRows = 160;
 
 struct PreferencePlan {

@@ -222,9 +222,10 @@ def advantages(rewards, step_type, players, values, bootstrap=None, gamma=1.0, l
     float16 or bfloat16): that player's value of the state it acts in;
     bootstrap [B, P], values' type: each player's value of the state behind
     the window, e.g. a critic's of the last step's obs [B, P, ...] (None: 0,
-    which takes games that are still open there to be worth nothing).  Each player's decisions are one chain: its rewards
-    up to its next decision, that one's value discounted by gamma, advantages
-    decayed by gamma * lam; a LAST step ends every chain, a FIRST step cuts.
+    which takes games that are still open there to be worth nothing).  Each
+    player's decisions are one chain: its rewards up to its next decision, that
+    one's value discounted by gamma, advantages decayed by gamma * lam; a LAST
+    step ends every chain, a FIRST step cuts.
     Returns (advantages, targets = advantages + values), float32 [T, B], 0 at
     steps that are no decision (FIRST, SKIPPED, no acting player)."""
     if not isinstance(values, torch.Tensor) or values.dtype not in _DTYPES:
@@ -373,8 +374,9 @@ def policy_loss(logits, actions, legal_mask, old_log_probs, advantages, ref_logi
     logits [..., A]; actions int8 [...] and legal_mask int32 [...]: the action
     taken and the legal-action word it was taken under; old_log_probs,
     advantages float32 [...]; ref_logits [..., A]: the reference policy's, in
-    the logits' type (None: the KL is 0, whatever kl_coef); active bool [...]: which rows to train on
-    (e.g. one player's; None: all).  Everything but logits is held constant.
+    the logits' type (None: the KL is 0, whatever kl_coef); active bool [...]:
+    which rows to train on (e.g. one player's; None: all).  Everything but
+    logits is held constant.
     The loss is 0, with zero gradients, where nothing counts.  A ratio exactly
     on a border is not clipped.  A legal action that the reference gives no
     probability (a logit of -inf) and the policy some (a logit within 745 of
