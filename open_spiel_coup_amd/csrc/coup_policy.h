@@ -310,7 +310,7 @@ __device__ __forceinline__ float log_of(float v) { return __builtin_amdgcn_logf(
 __device__ __forceinline__ float exp_of(float v) {  // the product's rounding, and the constant's, are made good
   const float hi = v * kLog2e, lo = __builtin_fmaf(v, kLog2eLow, __builtin_fmaf(v, kLog2e, -hi));
   const float e = __builtin_amdgcn_exp2f(hi);
-  return e < INFINITY && lo == lo ? __builtin_fmaf(e * lo, kLn2, e) : e;  // 0 and inf as they are
+  return e > 0.0f && e < INFINITY ? __builtin_fmaf(e * lo, kLn2, e) : e;  // 0 and inf as they are, whatever lo is
 }
 // log(1 + v), v > -1 / 2: the rounding of w = 1 + v is made good by v / (w - 1),
 // along which log(w) / (w - 1) hardly changes.

@@ -552,3 +552,32 @@ def test_excluded_actions_in_strided_tables_and_graphs(dtype):
         for got in held:
             for a, b in zip(got, want):
                 assert torch.equal(a.nan_to_num(5), b.nan_to_num(5))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=lambda d: str(d)[6:])
+@pytest.mark.parametrize("n", [64, 70000])
+def test_decisions_of_a_types_lowest_logit(n, dtype):
+    """An acted action of the type's lowest logit, 3.4e38 below the others: its ratio is 0 (clipped for a negative
+    advantage), without a gradient; a rejected sequence that holds one costs nothing, a chosen one 3.4e38, in calls of few
+    rows and of many."""
+    low = torch.finfo(dtype).min
+    x = torch.zeros(n, 3, dtype=dtype, device=DEV)
+    x[:, 1] = low
+    words = torch.full((n,), 7, dtype=torch.int32, device=DEV)
+    acts = torch.ones(n, dtype=torch.int8, device=DEV)
+    old = torch.full((n,), -1.0, device=DEV)
+    for adv, loss in ((1.0, 0.0), (-1.0, 0.8)):
+        got = policy.policy_loss_and_grad(x, acts, words, old, torch.full((n,), adv, device=DEV))
+        assert abs(float(got.loss) - loss) <= 4 * H and not got.grad.any()
+        assert (got.log_probs == float(low)).all()
+    for each in (1, n // 2):  # short sequences, and (of 70,000 rows) long ones
+        taken = torch.zeros(n, dtype=torch.int8, device=DEV)
+        off = torch.arange(0, n + 1, each, device=DEV)
+        taken[each] = 1  # the first rejected row
+        got = policy.preference_loss_and_grad(x, taken, words, off, beta=1.0)
+        pairs = n // each // 2
+        assert abs(float(got.loss) - (pairs - 1) * math.log(2) / pairs) <= 16 * H and torch.isfinite(got.grad).all()
+        taken[each], taken[0] = 0, 1
+        got = policy.preference_loss_and_grad(x, taken, words, off, beta=1.0)
+        _close(float(got.loss), -low / pairs, 4 * H * -low / pairs, "loss")
+        assert torch.isfinite(got.grad).all()
