@@ -13,10 +13,8 @@
 //
 // Arithmetic: logits are widened to 32 bits on load; the softmax statistics,
 // the log probabilities and the gradient are 32-bit; the losses' sums over
-// rows are 64-bit (a preference sequence's within one tile 32-bit where rows
-// are many).  A
-// gradient is rounded once, to the logits' type, at its store.  Two
-// comparisons decide whole outputs and are repeated in 64 bits where 32-bit
+// rows are 64-bit.  A gradient is rounded once, to the logits' type, at its
+// store.  Two comparisons decide whole outputs and are repeated in 64 bits where 32-bit
 // rounding could turn them: which action a uniform number falls on, and which
 // side of the clip border a ratio is on.
 //
@@ -1234,7 +1232,7 @@ __device__ __forceinline__ void row_grad(char* tile, const PreferenceArgs& q, in
 // costs follow, and the gradient is written from the e still in registers.
 // A group of more rows goes through its tiles twice.  Blocks past the groups
 // write the zero gradients of the rows outside every sequence.
-// 8192 pairs over 327,680 bf16 rows (37 MB) take 24.6 us, bound by a block's
+// 8192 pairs over 327,680 bf16 rows (37 MB) take 24.7 us, bound by a block's
 // latency: its steps wait for one another.  Groups of 120, 160 and 200 rows
 // come to the same.
 constexpr int kMaxGroup = 32, kZeroBlocks = 64;
@@ -1274,19 +1272,17 @@ __global__ __launch_bounds__(kRowThreads, AP > 20 ? 2 : FEW ? 4 : sizeof(T) == 2
     good = owned(q, edge[0], edge[seqs], 2 * pair0, 2 * pair0 + seqs - 1);
   const int64_t begin = good ? edge[0] : 0, end = good ? edge[seqs] : 0;
 
-  // a tile's log ratios to its sequences' sums (64 bits across tiles and, for
-  // calls of few rows, within one: one pair's cost of e^-x has x's absolute error)
-  using Sum = std::conditional_t<FEW, double, float>;
+  // a tile's log ratios to its sequences' sums, in 64 bits (one pair's cost of e^-x has x's absolute error, and two
+  // log ratios of a type's lowest logits pass 32 bits' range; 32-bit sums: 8192 bf16 pairs 24.6 us for 24.7)
   const auto add_tile = [&](int64_t row0, int rows) {
     __syncthreads();
     for (int s = wave; s < seqs; s += kRowThreads / 64) {
       const int64_t lo = edge[s] - row0, hi = edge[s + 1] - row0;
       const int to = !good ? 0 : hi < rows ? (int)hi : rows;
-      Sum v = 0;
-      for (int k = (lo > 0 ? (lo < rows ? (int)lo : rows) : 0) + ((int)threadIdx.x & 63); k < to; k += 64) v += (Sum)ratio[k];
-      if constexpr (FEW) v = wave_sum_last(v);
-      else v = wave_sum(v);
-      if ((threadIdx.x & 63) == 63) sum[s] += (double)v;
+      double v = 0.0;
+      for (int k = (lo > 0 ? (lo < rows ? (int)lo : rows) : 0) + ((int)threadIdx.x & 63); k < to; k += 64) v += (double)ratio[k];
+      v = wave_sum_last(v);
+      if ((threadIdx.x & 63) == 63) sum[s] += v;
     }
     __syncthreads();
   };

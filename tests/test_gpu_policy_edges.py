@@ -581,3 +581,19 @@ def test_decisions_of_a_types_lowest_logit(n, dtype):
         got = policy.preference_loss_and_grad(x, taken, words, off, beta=1.0)
         _close(float(got.loss), -low / pairs, 4 * H * -low / pairs, "loss")
         assert torch.isfinite(got.grad).all()
+
+
+@pytest.mark.parametrize("pairs,each", [(4, 50), (600, 50), (200, 400)], ids=["short-few", "short", "long"])
+def test_sums_of_lowest_logits_keep_their_range(pairs, each):
+    """Two acted actions of float32's lowest logit in each of a pair's sequences: sums of -6.8e38, past 32 bits' range,
+    whose difference is 0; 0.1 of them is a reward within it."""
+    n, low = pairs * each, torch.finfo(torch.float32).min
+    x = torch.zeros(n, 3, device=DEV)
+    x[:, 1] = low
+    words = torch.full((n,), 7, dtype=torch.int32, device=DEV)
+    taken = torch.zeros(n, dtype=torch.int8, device=DEV)
+    taken[[0, 1, each // 2, each // 2 + 1]] = 1
+    off = torch.arange(0, n + 1, each // 2, device=DEV)
+    got = policy.preference_loss_and_grad(x, taken, words, off, beta=0.1)
+    _close(got.rewards[:2].cpu().numpy(), np.full(2, 0.2 * low), 2 * H * 0.2 * -low, "rewards")
+    assert abs(float(got.loss) - math.log(2)) <= 16 * H and torch.isfinite(got.grad).all()
